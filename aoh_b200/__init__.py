@@ -10,7 +10,10 @@ behind the C ABI of include/aoh.h.
 from .attention import aoh_attention, rope_qk
 from .cache import AoHKVCache, pages_needed
 from .classifier import AoHClassifier, compute_all_eff_ranks, compute_eff_rank, label_margins
+from .eviction import KeyWeights, evict, key_weights, select_keys
 from .io import load_results, save_results
+from .logits import TokenHistory, penalize_logits
+from .rotary import rope_axes_qk
 
 
 def __getattr__(name):
@@ -24,14 +27,21 @@ def __getattr__(name):
 __all__ = [
     "AoHClassifier",
     "AoHKVCache",
+    "KeyWeights",
+    "TokenHistory",
     "aoh_attention",
     "rope_qk",
     "compute_all_eff_ranks",
     "compute_eff_rank",
+    "evict",
+    "key_weights",
     "label_margins",
     "patch_aoh_model",
     "ModelDecodeGraph",
     "load_results",
     "pages_needed",
+    "penalize_logits",
+    "rope_axes_qk",
     "save_results",
+    "select_keys",
 ]

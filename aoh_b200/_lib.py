@@ -79,6 +79,16 @@ _SIGNATURES = {
     "aoh_diag_exp2_poly": (C.c_int, [_vp, _vp, _i32, _vp]),
     "aoh_rope_qk": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
                               _vp]),
+    "aoh_rope_axes_qk": (C.c_int, [_vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _i32, _vp, _i32, C.POINTER(_i64), _vp,
+                                   C.POINTER(_i32), _i32, _i32, _vp, _vp, C.c_float, C.c_float, _i32, _i32, _i32, _i32,
+                                   _i32, _vp, _vp, _vp]),
+    "aoh_key_weights_workspace_bytes": (C.c_size_t, [_vp, _i32, _i32, _i32]),
+    "aoh_key_weights": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _vp, C.c_size_t, _vp]),
+    "aoh_select_keys": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "aoh_kv_evict": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _i32, _vp]),
+    "aoh_history_add": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _vp]),
+    "aoh_logits_penalize": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, C.c_float, _vp, C.c_float, _vp,
+                                      C.c_float, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _vp]),
 }
 IPC_HANDLE_BYTES = 64
 
@@ -131,3 +141,13 @@ def stream_handle(stream=None) -> int:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def launch(device, fn, what: str, *args) -> None:
+    """fn(*args, stream) with ``device`` current and on its current stream."""
+    import torch
+    if device.index is None or device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream), what)

@@ -96,6 +96,7 @@ class AoHKVCache:
         self.n_ret = [int((labels[i] >= 0.5).sum()) for i in range(self.num_layers)]
         self.n_str = [self.num_kv_heads - n for n in self.n_ret]
         self.kv_seq_len = 0
+        self.evicted = 0  # tokens seen that the retrieval heads hold no more (eviction.evict)
         # While True, decode calls read the device-resident length (set with
         # aoh_kv_set_length, advanced by aoh_kv_advance) instead of kv_seq_len and
         # leave kv_seq_len alone: how a captured decode step is recorded.
@@ -140,6 +141,12 @@ class AoHKVCache:
 
     def get_max_cache_shape(self):
         return None
+
+    @property
+    def tokens_seen(self) -> int:
+        """Tokens this cache has seen: the next token's position.  Equal to
+        ``kv_seq_len`` unless keys were evicted."""
+        return self.kv_seq_len + self.evicted
 
     # -- paging ----------------------------------------------------------------
     def reserve(self, n_tokens: int) -> None:

@@ -903,7 +903,7 @@ static int plan_and_launch(aoh_kv_cache* c, int layer, int past_len, const void*
   }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = launch_config(grid, cluster, st, attr, true);
-  a.prefetch = c->last_write_layer != layer ? 1 : 0;
+  a.prefetch = c->may_prefetch(layer) ? 1 : 0;
   a.append = c->decode_append ? 1 : 0;
   if (a.append) c->last_write_layer = layer;  // the kernel appends the new token to this layer
   return cuda_check(cluster == kClusterBig ? cudaLaunchKernelEx(&cfg, decode_bf16_kernel<kClusterBig>, a, plan)

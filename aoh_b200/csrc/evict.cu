@@ -1,0 +1,415 @@
+// Eviction by accumulated attention weight: which keys a retrieval head keeps,
+// and the copy of the kept rows into another cache.
+//
+// select: of each row of n weights the first `sink` and the last `recent` keys
+// and the largest of the keys between them, `keep` in all, in ascending order
+// of their positions; of equal weights the lower position first.  NaN ranks
+// like -inf, -0 like +0.
+//   A cluster of 1 to 8 CTAs takes a row, each CTA a contiguous part of the
+//   middle, which it reads from memory once and holds in shared memory as
+//   32-bit keys in the order of the weights.  Three passes over 11, 11 and 10
+//   bits find the exact bits of the smallest kept weight: every CTA counts its
+//   part, and all of them add up the cluster's histograms.  A count of larger
+//   and of equal keys per warp, summed over warps and CTAs, then gives every
+//   kept key its place, so the output needs no sorting.
+//   Bound: HBM (4 bytes a key in, 8 bytes a kept key out) and the latency of
+//   the passes; a part that does not fit shared memory is read again by each
+//   pass.
+//
+// evict: retrieval units' kept rows go to positions 0..keep-1 of the other
+// cache; a streaming unit's sink rows keep their place and the rows of its
+// ring go to the slots of their new positions (keep - T lower).  Source and
+// destination are different caches, so every row moves independently.
+//   Bound: HBM, 2 x 512 bytes a row (bf16).  A warp copies 8 rows: eight lanes
+//   resolve the rows' pages side by side, then each 16-byte chunk of the 8
+//   rows is in flight at once.
+#include "common.cuh"
+#include "internal.h"
+#include "page_layout.cuh"
+
+namespace aoh {
+namespace {
+
+// ---------------------------------------------------------------------------
+// select
+// ---------------------------------------------------------------------------
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kSelMaxCluster = 8;
+constexpr int kSelResident = 48 * 1024;  // keys of a part held in shared memory (192 KB)
+
+struct SelectArgs {
+  const float* w;
+  long long w_stride;
+  int n, sink, recent, take;  // take: keys chosen from the middle
+  int keep;
+  int cluster, part;  // CTAs of a row, keys of a part (a multiple of 32)
+  int resident;       // the part is held in shared memory
+  int32_t* kept;
+  float* kept_w;
+};
+
+// Order-preserving bits of a weight: larger weight, larger key.
+__device__ __forceinline__ uint32_t weight_key(float x) {
+  if (x != x) x = -INFINITY;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct SelectShared {
+  uint32_t hist[kBins];
+  uint32_t scan[kSelWarps];
+  uint32_t gt[kSelWarps], eq[kSelWarps];  // keys above / equal to the threshold, by warp
+  uint32_t total[2];                      // of this CTA
+  uint32_t bin, above;
+};
+
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ SelectArgs a) {
+  extern __shared__ uint32_t keys[];
+  __shared__ SelectShared s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = a.cluster > 1 ? (int)cluster_ctarank() : 0;
+  const long long row = blockIdx.x / a.cluster;
+  const float* w = a.w + row * a.w_stride;
+  const int mid = a.n - a.sink - a.recent;
+  const int lo = rank * a.part, cnt = max(0, min(a.part, mid - lo));
+  const float* wm = w + a.sink + lo;
+  int32_t* kept = a.kept + row * a.keep;
+  float* kept_w = a.kept_w ? a.kept_w + row * a.keep : nullptr;
+
+  // the first and the last keys are kept as they are
+  for (int i = rank * kSelThreads + tid; i < a.sink + a.recent; i += a.cluster * kSelThreads) {
+    const int at = i < a.sink ? i : a.keep - a.sink - a.recent + i;
+    const int p = i < a.sink ? i : a.n - a.sink - a.recent + i;
+    kept[at] = p;
+    if (kept_w) kept_w[at] = w[p];
+  }
+  if (a.take == 0) return;  // the same for every CTA of the cluster
+
+  if (a.resident)
+    for (int i = tid; i < cnt; i += kSelThreads) keys[i] = weight_key(wm[i]);
+  auto key = [&](int i) { return a.resident ? keys[i] : weight_key(wm[i]); };
+
+  uint32_t prefix = 0, left = (uint32_t)a.take;  // the threshold's leading bits, keys still to take
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int bins = pass == 2 ? 1024 : kBins;
+    for (int i = tid; i < kBins; i += kSelThreads) s.hist[i] = 0;
+    __syncthreads();
+    for (int i0 = warp * 32; i0 < cnt; i0 += kSelThreads) {
+      const int i = i0 + lane;
+      const uint32_t k = i < cnt ? key(i) : 0;
+      // digits above this one agree with the threshold
+      const bool in = i < cnt && (pass == 0 || k >> (shift + (pass == 2 ? 10 : 11)) == prefix);
+      const uint32_t b = k >> shift & (uint32_t)(bins - 1);
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      if (m == 0) continue;
+      // many equal weights (zeros) would be added one by one to one address
+      const uint32_t b0 = __shfl_sync(0xffffffffu, b, __ffs(m) - 1);
+      const unsigned same = __ballot_sync(0xffffffffu, in && b == b0);
+      if (lane == __ffs(m) - 1)
+        atomicAdd(&s.hist[b0], (uint32_t)__popc(same));
+      else if (in && b != b0)
+        atomicAdd(&s.hist[b], 1u);
+    }
+    if (a.cluster > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    // thread t sums bins [4t, 4t + 4) counted from the top over the cluster
+    uint32_t c[4] = {0, 0, 0, 0};
+    const int per = kBins / kSelThreads;
+#pragma unroll
+    for (int j = 0; j < per; ++j) {
+      const int b = kBins - 1 - (tid * per + j);
+      if (a.cluster > 1) {
+        for (int r = 0; r < a.cluster; ++r) c[j] += ld_dsmem_u32(mapa_shared(&s.hist[b], r));
+      } else {
+        c[j] = s.hist[b];
+      }
+    }
+    const uint32_t mine = c[0] + c[1] + c[2] + c[3];
+    uint32_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += v;
+    }
+    if (lane == 31) s.scan[warp] = incl;
+    __syncthreads();
+    uint32_t before = incl - mine;
+    for (int i = 0; i < warp; ++i) before += s.scan[i];
+    if (before < left && before + mine >= left) {
+#pragma unroll
+      for (int j = 0; j < per; ++j) {
+        if (before < left && before + c[j] >= left) {
+          s.bin = (uint32_t)(kBins - 1 - (tid * per + j));
+          s.above = before;
+        }
+        before += c[j];
+      }
+    }
+    // every CTA has read the histograms before any is cleared
+    if (a.cluster > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+    prefix = pass == 0 ? s.bin : pass == 1 ? prefix << 11 | s.bin : prefix << 10 | s.bin;
+    left -= s.above;
+  }
+  // prefix: the threshold's bits; `left` of the keys equal to it are taken
+  const uint32_t thr = prefix;
+
+  // keys of warp w: a contiguous range of whole 32-key groups
+  const int groups = (cnt + 31) / 32, per_warp = (groups + kSelWarps - 1) / kSelWarps;
+  const int g0 = min(groups, warp * per_warp), g1 = min(groups, g0 + per_warp);
+  uint32_t gt = 0, eq = 0;
+  for (int g = g0; g < g1; ++g) {
+    const int i = g * 32 + lane;
+    const uint32_t k = i < cnt ? key(i) : 0;
+    gt += __popc(__ballot_sync(0xffffffffu, i < cnt && k > thr));
+    eq += __popc(__ballot_sync(0xffffffffu, i < cnt && k == thr));
+  }
+  if (lane == 0) {
+    s.gt[warp] = gt;
+    s.eq[warp] = eq;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t tg = 0, te = 0;
+    for (int i = 0; i < kSelWarps; ++i) {
+      tg += s.gt[i];
+      te += s.eq[i];
+    }
+    s.total[0] = tg;
+    s.total[1] = te;
+  }
+  if (a.cluster > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  uint32_t bg = 0, be = 0;  // larger / equal keys before this warp's range
+  for (int r = 0; r < rank; ++r) {
+    bg += ld_dsmem_u32(mapa_shared(&s.total[0], r));
+    be += ld_dsmem_u32(mapa_shared(&s.total[1], r));
+  }
+  for (int i = 0; i < warp; ++i) {
+    bg += s.gt[i];
+    be += s.eq[i];
+  }
+  const unsigned below = (1u << lane) - 1u;
+  for (int g = g0; g < g1; ++g) {
+    const int i = g * 32 + lane;
+    const uint32_t k = i < cnt ? key(i) : 0;
+    const bool is_gt = i < cnt && k > thr, is_eq = i < cnt && k == thr;
+    const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+    const uint32_t rank_eq = be + __popc(me & below);
+    if (is_gt || (is_eq && rank_eq < left)) {
+      const int at = a.sink + (int)(bg + __popc(mg & below) + min(rank_eq, left));
+      kept[at] = a.sink + lo + i;
+      if (kept_w) kept_w[at] = wm[i];
+    }
+    bg += __popc(mg);
+    be += __popc(me);
+  }
+  // no CTA leaves while another may still read its totals
+  if (a.cluster > 1) cluster_sync_all();
+}
+
+// ---------------------------------------------------------------------------
+// evict
+// ---------------------------------------------------------------------------
+constexpr int kEvictWarps = 8, kEvictRows = 8;  // warps of a CTA, rows of a warp
+
+// Table entry (page index within the unit) and slot of position p in a unit that holds it.
+__device__ __forceinline__ void place(const CacheGeom& g, bool retrieval, int p, int& entry, int& slot) {
+  if (retrieval || p < g.sink) {
+    entry = p / kPage;
+    slot = p % kPage;
+  } else {
+    const int r = (p - g.sink) % g.ring_cap;
+    entry = g.sink_pages + r / kPage;
+    slot = r % kPage;
+  }
+}
+
+__device__ __forceinline__ int page_of(const CacheGeom& g, int unit, int entry) {
+  const int at = g.unit_offset[unit] + entry;
+  if (at >= g.unit_offset[unit + 1]) return -1;
+  const int p = g.block_table[at];
+  return p >= 0 && p < g.num_pages ? p : -1;
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kEvictWarps * 32)
+    evict_kernel(CacheGeom src, CacheGeom dst, const int32_t* unit_row, const int32_t* kept, long long kept_stride,
+                 int keep, int len, int chunks) {
+  const int unit = blockIdx.x / chunks;
+  if (dst.unit_offset[unit + 1] == dst.unit_offset[unit]) return;  // not stored here
+  const int row = unit_row[unit];
+  const bool retrieval = row >= 0;
+  // a streaming unit holds its sink and, behind it, the latest ring_cap positions
+  const int sink = min(dst.sink, keep), held = max(0, min(dst.ring_cap, keep - dst.sink));
+  const int rows = retrieval ? keep : sink + held;
+  const int lane = threadIdx.x & 31;
+  const int r0 = ((blockIdx.x % chunks) * kEvictWarps + (threadIdx.x >> 5)) * kEvictRows;
+  if (r0 >= rows) return;
+  // lane j resolves row r0 + j
+  int from = -1, to = -1;  // page * 16 + slot
+  if (lane < kEvictRows && r0 + lane < rows) {
+    const int i = r0 + lane;
+    const int p_dst = retrieval || i < sink ? i : keep - held + (i - sink);
+    const int p_src = retrieval ? kept[row * kept_stride + i] : i < sink ? i : p_dst + len - keep;
+    if (p_src >= 0 && p_src < len) {
+      int e, sl;
+      place(src, retrieval, p_src, e, sl);
+      const int ps = page_of(src, unit, e);
+      if (ps >= 0) from = ps * kPage + sl;
+      place(dst, retrieval, p_dst, e, sl);
+      const int pd = page_of(dst, unit, e);
+      if (pd >= 0) to = pd * kPage + sl;
+    }
+    if (from < 0 || to < 0) {
+      atomicOr(dst.err, kErrBadPage);
+      to = -1;
+    }
+  }
+  const char* sp = static_cast<const char*>(src.pool);
+  char* dp = static_cast<char*>(dst.pool);
+  constexpr int kRowChunks = kBf16 ? 32 : 64;  // 16-byte chunks of a row's K and V
+#pragma unroll
+  for (int c0 = 0; c0 < kRowChunks; c0 += 32) {
+    uint4 v[kEvictRows];
+    const int c = c0 + lane;
+#pragma unroll
+    for (int j = 0; j < kEvictRows; ++j) {
+      const int f = __shfl_sync(0xffffffffu, from, j), t = __shfl_sync(0xffffffffu, to, j);
+      if (t < 0) continue;
+      const long long page = f / kPage;
+      const int slot = f % kPage;
+      v[j] = kBf16 ? *reinterpret_cast<const uint4*>(sp + page * kPageBf16Bytes + bf16_chunk_offset(c >> 4, slot, c & 15))
+                   : *reinterpret_cast<const uint4*>(sp + page * kPageF32Bytes + ((c >> 5) * kPage + slot) * 512 +
+                                                     (c & 31) * 16);
+    }
+#pragma unroll
+    for (int j = 0; j < kEvictRows; ++j) {
+      const int t = __shfl_sync(0xffffffffu, to, j);
+      if (t < 0) continue;
+      const long long page = t / kPage;
+      const int slot = t % kPage;
+      char* o = kBf16 ? dp + page * kPageBf16Bytes + bf16_chunk_offset(c >> 4, slot, c & 15)
+                      : dp + page * kPageF32Bytes + ((c >> 5) * kPage + slot) * 512 + (c & 31) * 16;
+      *reinterpret_cast<uint4*>(o) = v[j];
+    }
+  }
+}
+
+}  // namespace
+}  // namespace aoh
+
+using namespace aoh;
+
+extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t rows, int32_t n, int32_t keep,
+                               int32_t sink, int32_t recent, int32_t* kept, float* kept_weights, aoh_stream stream) {
+  const char* who = "aoh_select_keys";
+  if (rows < 0 || n < 0 || sink < 0 || recent < 0) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: negative size", who);
+  if (keep < 0 || keep > n) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: keep %d of %d keys", who, keep, n);
+  if ((int64_t)sink + recent > keep)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: sink %d and recent %d exceed keep %d", who, sink, recent, keep);
+  if (rows == 0 || keep == 0) return AOH_OK;
+  if (!weights || !kept) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
+  if (rows > (1 << 27)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  static PerDeviceOnce once;
+  rc = once.run(dev, [&] {
+    return cuda_check(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelResident * 4),
+                      "aoh_select_keys shared memory");
+  });
+  if (rc) return rc;
+  SelectArgs a{};
+  a.w = weights;
+  a.w_stride = row_stride;
+  a.n = n;
+  a.sink = sink;
+  a.recent = recent;
+  a.keep = keep;
+  a.take = keep - sink - recent;
+  const int mid = n - sink - recent;
+  // a CTA for every 4096 keys of a row, 8 at most: below that the passes' barriers cost more than their loads
+  a.cluster = 1;
+  while (a.cluster < kSelMaxCluster && a.cluster * 4096 < mid) a.cluster *= 2;
+  a.part = ((mid + a.cluster - 1) / a.cluster + 31) / 32 * 32;
+  a.resident = a.part <= kSelResident;
+  a.kept = kept;
+  a.kept_w = kept_weights;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * a.cluster));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = a.resident ? (size_t)a.part * 4 : 0;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, select_kernel, a), "aoh_select_keys launch");
+}
+
+extern "C" int aoh_kv_evict(aoh_kv_cache* src, aoh_kv_cache* dst, int32_t past_len, const int32_t* kept,
+                            int64_t kept_stride, int32_t keep, aoh_stream stream) {
+  const char* who = "aoh_kv_evict";
+  if (!src || !dst) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null cache", who);
+  if (src == dst) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: source and destination are the same cache", who);
+  const aoh_kv_config &a = src->cfg, &b = dst->cfg;
+  if (a.num_layers != b.num_layers || a.batch != b.batch || a.num_kv_heads != b.num_kv_heads || a.dtype != b.dtype ||
+      a.sink_size != b.sink_size || a.recent_size != b.recent_size || src->labels != dst->labels ||
+      src->owned != dst->owned)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the caches differ in more than their length", who);
+  if (keep < 0 || past_len < 0 || keep > past_len)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: keep %d of %d positions", who, keep, past_len);
+  bool any_retrieval = false, any_streaming = false;
+  for (uint8_t v : src->labels) (v ? any_retrieval : any_streaming) = true;
+  // a streaming head attends to its sink and window after the eviction as before
+  if (any_streaming && keep < past_len && (int64_t)a.sink_size + a.recent_size > keep)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: keep %d is less than the streaming heads' sink %d + recent %d", who, keep,
+                a.sink_size, a.recent_size);
+  if (any_retrieval && keep > 0 && !kept) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
+  if (!src->bound || !dst->bound) return fail(AOH_ERR_STATE, "%s: cache is not bound to device memory", who);
+  if (src->device != dst->device) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the caches are on different devices", who);
+  if (src->dirty_hi > src->dirty_lo || dst->dirty_hi > dst->dirty_lo)
+    return fail(AOH_ERR_STATE, "%s: block tables changed since the last aoh_kv_sync", who);
+  const int need_src = (past_len + kPage - 1) / kPage, need_dst = (keep + kPage - 1) / kPage;
+  for (int u = 0; u < src->n_units; ++u) {
+    const int l = u / (a.batch * a.num_kv_heads), g = u % a.num_kv_heads;
+    if (!src->owned[u] || !src->retrieval(l, g)) continue;
+    if (src->unit_npages[u] < need_src || dst->unit_npages[u] < need_dst)
+      return fail(AOH_ERR_OUT_OF_PAGES, "%s: positions < %d (source) and < %d (destination) are not reserved", who,
+                  past_len, keep);
+  }
+  if (keep == 0) return AOH_OK;
+  const int rows = std::max(any_retrieval ? keep : 0, any_streaming ? a.sink_size + dst->ring_cap : 0);
+  if (rows == 0) return AOH_OK;
+  const int chunks = (rows + kEvictWarps * kEvictRows - 1) / (kEvictWarps * kEvictRows);
+  const long long blocks = (long long)src->n_units * chunks;
+  if (blocks > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const CacheGeom gs = src->geom(), gd = dst->geom();
+  if (a.dtype == AOH_BF16)
+    evict_kernel<true><<<(unsigned)blocks, kEvictWarps * 32, 0, st>>>(gs, gd, src->dev_unit_row, kept, kept_stride, keep,
+                                                                      past_len, chunks);
+  else
+    evict_kernel<false><<<(unsigned)blocks, kEvictWarps * 32, 0, st>>>(gs, gd, src->dev_unit_row, kept, kept_stride, keep,
+                                                                       past_len, chunks);
+  dst->last_write_layer = kEveryLayer;
+  return cuda_check(cudaGetLastError(), "aoh_kv_evict launch");
+}

@@ -19,6 +19,7 @@ constexpr int kHeadDim = 128;
 constexpr int kPage = 16;
 constexpr int kMaxRanks = 8;     // GPUs of one node taking part in an output gather
 constexpr int kMaxDevices = 64;  // device ordinals with per-device state
+constexpr int kEveryLayer = -2;  // aoh_kv_cache::last_write_layer after a kernel that wrote pages of all layers
 
 // Device check word bits (written with atomicOr by the kernels, read and
 // cleared by aoh_kv_device_status).
@@ -84,6 +85,7 @@ struct aoh_kv_cache {
   int32_t* dev_unit_offset = nullptr;
   int32_t* dev_table = nullptr;
   int32_t* dev_err = nullptr;   // [0] check word, [1] device-resident sequence length
+  int32_t* dev_unit_row = nullptr;  // per unit: its index among the retrieval units (stored here or not), -1: streaming
   int32_t len_hint = 0;          // host copy of the device length (plans kernels in device mode)
   bool bound = false;
   int device = -1;
@@ -100,7 +102,9 @@ struct aoh_kv_cache {
   // layer whose pages the last stream-ordered write kernel (prefill or decode
   // with its append, append) touched; a following kernel on another layer may
   // prefetch its pages before waiting for that kernel
-  int last_write_layer = -1;
+  int last_write_layer = -1;  // -1: none, kEveryLayer: all of them
+  // whether a kernel on `layer` may read its pages before its dependency wait
+  bool may_prefetch(int layer) const { return last_write_layer != layer && last_write_layer != aoh::kEveryLayer; }
   bool decode_append = true;  // false: decode calls attend without appending (aoh_kv_set_decode_append)
   // prefill scratch owned by the cache (grow-only; freed on destroy):
   // [prefill_cnt_cap ticket counters, padded to 256 B][split partials]; the

@@ -1,0 +1,325 @@
+// Attention weight by key: for a layer's retrieval units
+//
+//   W[j] (+)= sum over queries i and heads h of the unit's group of
+//             softmax over j' <= past_len + i of (q_ih . k_j' / sqrt(128))  at j
+//
+// i.e. the column sums of the softmax matrix whose product with V the
+// attention entry points compute.  A weight needs its row's maximum and sum
+// over all keys first, so two passes over K: one for every query row's (m, l),
+// by key ranges that fill the GPU, one that adds up exp(s - lse) per key.  Each
+// key is summed by one CTA in a fixed order, so results do not depend on timing.
+//
+// This file holds the entry point and the kernels for any type: 64 rows x 64
+// keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.
+#include "common.cuh"
+#include "internal.h"
+#include "key_weights.h"
+#include "page_layout.cuh"
+
+namespace aoh {
+namespace {
+
+constexpr int kTile = 64;                 // query rows and keys of a tile
+constexpr int kStride = kHeadDim + 4;     // floats of a row in shared memory: 16-byte rows on distinct banks
+constexpr int kSmem = 2 * kTile * kStride * 4;
+
+template <typename T>
+__device__ __forceinline__ void load_queries(const KeyWeightsArgs& a, int b, int g, int row0, int rows, float* sm) {
+  for (int e = threadIdx.x; e < kTile * (kHeadDim / 4); e += 256) {
+    const int r = e / (kHeadDim / 4), c = e % (kHeadDim / 4) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row0 + r < rows) {
+      const int tok = (row0 + r) / a.g.grp, h = g * a.g.grp + (row0 + r) % a.g.grp;
+      const T* p = static_cast<const T*>(a.q) + (((long long)b * a.q_len + tok) * a.g.Hq + h) * kHeadDim + c;
+      if constexpr (sizeof(T) == 4) {
+        v = *reinterpret_cast<const float4*>(p);
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        v = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+      }
+    }
+    *reinterpret_cast<float4*>(sm + r * kStride + c) = v;
+  }
+}
+
+// Keys [j0, j0 + 64) of a unit; rows that are not stored are zero.
+template <typename T>
+__device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int j0, int len, float* sm) {
+  const int base = a.g.unit_offset[unit], n_pages = a.g.unit_offset[unit + 1] - base;
+  for (int e = threadIdx.x; e < kTile * (kHeadDim / 4); e += 256) {
+    const int r = e / (kHeadDim / 4), c = e % (kHeadDim / 4) * 4;
+    const int j = j0 + r, slot = j % kPage;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j < len && j / kPage < n_pages) {
+      const int page = a.g.block_table[base + j / kPage];
+      if (page >= 0 && page < a.g.num_pages) {
+        if constexpr (sizeof(T) == 4) {
+          v = *reinterpret_cast<const float4*>(static_cast<const char*>(a.g.pool) + (long long)page * kPageF32Bytes +
+                                               4 * f32_elem_offset(0, slot, c));
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const char*>(a.g.pool) +
+                                                          (long long)page * kPageBf16Bytes + 2 * bf16_elem_offset(0, slot, c));
+          v = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
+        }
+      } else if (c == 0) {
+        atomicOr(a.g.err, kErrBadPage);
+      }
+    }
+    *reinterpret_cast<float4*>(sm + r * kStride + c) = v;
+  }
+}
+
+// s[i][j]: row 4 ty + i, key tx + 16 j, in the log2 domain
+__device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < kHeadDim; d += 4) {
+    float4 q[4], k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(qs + (4 * ty + i) * kStride + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStride + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(q[i].x, k[j].x, s[i][j]);
+        s[i][j] = fmaf(q[i].y, k[j].y, s[i][j]);
+        s[i][j] = fmaf(q[i].z, k[j].z, s[i][j]);
+        s[i][j] = fmaf(q[i].w, k[j].w, s[i][j]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] *= kScoreScale;
+}
+
+// Keys a row may see: j <= past + token.
+__device__ __forceinline__ int last_key(const KeyWeightsArgs& a, int past, int row) { return past + row / a.g.grp; }
+
+// (m, l) of 64 query rows over one range of keys.
+template <typename T>
+__global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ KeyWeightsArgs a) {
+  extern __shared__ float sm[];
+  const int unit = a.unit0 + blockIdx.y, r = a.unit_row[unit];
+  if (r < 0 || a.g.unit_offset[unit] == a.g.unit_offset[unit + 1]) return;
+  const int past = key_weights_past(a);
+  const int rows = a.q_len * a.g.grp, row0 = blockIdx.x * kTile;
+  const int b = blockIdx.y / a.g.G, g = blockIdx.y % a.g.G;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  float *qs = sm, *ks = sm + kTile * kStride;
+  load_queries<T>(a, b, g, row0, rows, qs);
+  // key tiles up to the last one that any row of the tile sees, split evenly
+  const int len = last_key(a, past, min(row0 + kTile, rows) - 1) + 1;
+  const int tiles = (len + kTile - 1) / kTile;
+  const int t0 = (int)((long long)tiles * blockIdx.z / a.splits), t1 = (int)((long long)tiles * (blockIdx.z + 1) / a.splits);
+  float m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();
+    load_keys<T>(a, unit, t * kTile, len, ks);
+    __syncthreads();
+    float s[4][4];
+    tile_scores(qs, ks, ty, tx, s);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int last = last_key(a, past, row0 + 4 * ty + i);
+      float mt = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (t * kTile + tx + 16 * j > last) s[i][j] = -INFINITY;
+        mt = fmaxf(mt, s[i][j]);
+      }
+      if (mt > m[i]) {
+        l[i] *= fast_exp2(m[i] - mt);
+        m[i] = mt;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (s[i][j] > -INFINITY) l[i] += fast_exp2(s[i][j] - m[i]);
+    }
+  }
+  // the 16 threads of a row
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float mm = m[i];
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+    float ll = mm > -INFINITY ? l[i] * fast_exp2(m[i] - mm) : 0.f;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+    const int row = row0 + 4 * ty + i;
+    if (tx == 0 && row < rows)
+      a.part[blockIdx.z * a.rows_total + (long long)(r - a.row0) * rows + row] = make_float2(mm, ll);
+  }
+}
+
+// The weights of 64 keys, summed over every query row of the unit.
+template <typename T>
+__global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a) {
+  extern __shared__ float sm[];
+  __shared__ float lse[kTile];
+  const int unit = a.unit0 + blockIdx.y, r = a.unit_row[unit];
+  if (r < 0) return;
+  const int past = key_weights_past(a);
+  const int len = past + a.q_len, rows = a.q_len * a.g.grp;
+  const int j0 = blockIdx.x * kTile;
+  if (j0 >= len) return;
+  const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
+  const int b = blockIdx.y / a.g.G, g = blockIdx.y % a.g.G;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  float *qs = sm, *ks = sm + kTile * kStride;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  if (stored) {
+    load_keys<T>(a, unit, j0, len, ks);
+    // the first token that sees key j0
+    const int tok0 = max(0, j0 - past);
+    for (int row0 = tok0 * a.g.grp; row0 < rows; row0 += kTile) {
+      __syncthreads();
+      load_queries<T>(a, b, g, row0, rows, qs);
+      if (threadIdx.x < kTile && row0 + threadIdx.x < rows) {
+        const float2* p = a.part + (long long)(r - a.row0) * rows + row0 + threadIdx.x;
+        float mm = -INFINITY, ll = 0.f;
+        for (int i = 0; i < a.splits; ++i) mm = fmaxf(mm, p[i * a.rows_total].x);
+        for (int i = 0; i < a.splits; ++i) {
+          const float2 v = p[i * a.rows_total];
+          if (v.y > 0.f) ll += v.y * fast_exp2(v.x - mm);
+        }
+        lse[threadIdx.x] = mm + log2f(ll);
+      }
+      __syncthreads();
+      float s[4][4];
+      tile_scores(qs, ks, ty, tx, s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row0 + 4 * ty + i;
+        if (row >= rows) continue;
+        const int last = last_key(a, past, row);
+        const float e = lse[4 * ty + i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j0 + tx + 16 * j <= last) w[j] += fast_exp2(s[i][j] - e);
+      }
+    }
+  }
+  // over the 16 groups of rows, in their order
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) qs[ty * kTile + tx + 16 * j] = w[j];
+  __syncthreads();
+  if (threadIdx.x < kTile && j0 + threadIdx.x < len) {
+    float x = 0.f;
+    for (int i = 0; i < 16; ++i) x += qs[i * kTile + threadIdx.x];
+    float* o = a.out + (r - a.row0) * a.out_stride + j0 + threadIdx.x;
+    *o = a.accumulate ? *o + x : x;
+  }
+}
+
+template <typename T>
+int launch_generic(const KeyWeightsArgs& a, int row_tiles, cudaStream_t st) {
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  static PerDeviceOnce once;
+  rc = once.run(dev, [] {
+    int e = cuda_check(cudaFuncSetAttribute(key_lse_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                       "key_lse shared memory");
+    return e ? e : cuda_check(cudaFuncSetAttribute(key_sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+                              "key_sum shared memory");
+  });
+  if (rc) return rc;
+  const int key_tiles = (a.max_len + kTile - 1) / kTile;
+  key_lse_kernel<T><<<dim3(row_tiles, a.units, a.splits), 256, kSmem, st>>>(a);
+  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSmem, st>>>(a);
+  return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+}
+
+int retrieval_heads(const aoh_kv_cache* c, int layer) {
+  int n = 0;
+  for (int g = 0; g < c->cfg.num_kv_heads; ++g) n += c->retrieval(layer, g);
+  return n;
+}
+
+// The plan of a call: query-row tiles and the key ranges of each.
+struct Plan {
+  int n_units, row_tiles, splits;
+  size_t workspace;
+};
+
+Plan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
+  Plan p;
+  p.n_units = c->cfg.batch * retrieval_heads(c, layer);
+  const long long rows = (long long)q_len * (c->cfg.num_q_heads / c->cfg.num_kv_heads);
+  p.row_tiles = (int)((rows + kTile - 1) / kTile);
+  const int key_tiles = (max_len + kTile - 1) / kTile;
+  // enough CTAs for three per SM
+  const long long ctas = std::max(1LL, (long long)p.n_units * p.row_tiles);
+  p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles), (3LL * std::max(1, c->num_sms) + ctas - 1) / ctas));
+  p.workspace = (size_t)p.splits * p.n_units * rows * sizeof(float2);
+  return p;
+}
+
+// Keys a call covers: with the device's length, every position the cache may come to hold.
+int most_keys(const aoh_kv_cache* c, int32_t past_len, int32_t q_len) {
+  return past_len == AOH_PAST_LEN_DEVICE ? c->cfg.max_context : past_len + q_len;
+}
+
+}  // namespace
+}  // namespace aoh
+
+using namespace aoh;
+
+extern "C" size_t aoh_key_weights_workspace_bytes(const aoh_kv_cache* c, int32_t layer, int32_t past_len, int32_t q_len) {
+  if (!c || layer < 0 || layer >= c->cfg.num_layers || past_len < AOH_PAST_LEN_DEVICE || q_len <= 0 ||
+      (int64_t)past_len + q_len > c->cfg.max_context)
+    return 0;
+  return plan(c, layer, most_keys(c, past_len, q_len), q_len).workspace;
+}
+
+extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len, int32_t q_len, const void* q, float* out,
+                               int64_t out_stride, int32_t accumulate, void* workspace, size_t workspace_bytes,
+                               aoh_stream stream) {
+  const char* who = "aoh_key_weights";
+  if (!c) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null cache", who);
+  const bool device_len = past_len == AOH_PAST_LEN_DEVICE;
+  const int rc = check_common(c, layer, device_len ? 0 : past_len, q_len, q, q, q, nullptr, who);
+  if (rc) return rc;
+  const int n_ret = retrieval_heads(c, layer);
+  if (n_ret == 0 || q_len == 0) return AOH_OK;
+  const int max_len = most_keys(c, past_len, q_len);
+  if (!out) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
+  if (out_stride < max_len)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: rows of %lld weights for %d keys", who, (long long)out_stride, max_len);
+  KeyWeightsArgs a{};
+  a.g = c->geom();
+  a.units = c->cfg.batch * c->cfg.num_kv_heads;
+  if (a.units > 65535) return fail(AOH_ERR_UNSUPPORTED, "%s: too many units", who);
+  if ((long long)q_len * a.g.grp > (1 << 30)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many queries", who);
+  const Plan p = plan(c, layer, max_len, q_len);
+  if (!workspace || workspace_bytes < p.workspace)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.workspace);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
+  a.unit_row = c->dev_unit_row;
+  a.unit0 = c->unit(layer, 0, 0);
+  for (int l = 0; l < layer; ++l) a.row0 += c->cfg.batch * retrieval_heads(c, l);
+  a.past_len = past_len;
+  a.past_len_dev = device_len ? c->dev_err + 1 : nullptr;
+  a.max_len = max_len;
+  a.q_len = q_len;
+  a.q = q;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.accumulate = accumulate;
+  a.part = static_cast<float2*>(workspace);
+  a.rows_total = (long long)p.n_units * q_len * a.g.grp;
+  a.splits = p.splits;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return c->cfg.dtype == AOH_BF16 ? launch_generic<__nv_bfloat16>(a, p.row_tiles, st)
+                                  : launch_generic<float>(a, p.row_tiles, st);
+}

@@ -1169,7 +1169,7 @@ int launch_prefill_bf16(aoh_kv_cache* c, int layer, int past_len, int q_len, con
   // next kernel launches only after all of them have started)
   a.coop = n_split > 1 && heavy_live * n_split + light <= sms ? 1 : 0;
   a.append = all_causal ? 0 : 1;
-  a.prefetch = c->last_write_layer != layer ? 1 : 0;
+  a.prefetch = c->may_prefetch(layer) ? 1 : 0;
   c->last_write_layer = layer;  // the kernel appends this call's rows to the layer's pages
   // Scratch: ticket counters -- one per (sequence, KV head) for the streaming
   // units' ring append, then two per retrieval slot when split (arrivals and

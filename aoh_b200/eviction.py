@@ -1,0 +1,180 @@
+"""Eviction by accumulated attention weight.
+
+The reference's retrieval heads keep every token; these operators bound them.
+``key_weights`` sums the attention that each cached key of a layer's retrieval
+heads received, ``select_keys`` picks the keys to keep by it, and ``evict``
+copies their rows -- and the streaming heads' sink and window -- into another,
+shorter cache, in which decoding goes on.  ``KeyWeights`` holds the sums of a
+whole cache:
+
+    sums = KeyWeights(cache)
+    for layer in range(L):                      # a prefill chunk or a decode step
+        past = cache.kv_seq_len
+        out = aoh_attention(cache, layer, q, k, v)
+        sums.add(layer, q, past_len=past)
+    small = AoHKVCache(labels, num_q_heads, max_context=8192 + 1024, ...)
+    sums = sums.evict(8192, into=small)         # small.tokens_seen goes on counting
+
+A kept key's RoPE position stays what it was: after an eviction, rotate new
+tokens by ``tokens_seen``, not by ``kv_seq_len``.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .attention import _check_q
+from .cache import AoHKVCache
+
+
+def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len: int | None = None,
+                out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
+    """The attention weight that each key received from the queries ``q``.
+
+    q (B, C, Hq, D): the post-RoPE queries of the tokens at positions past_len..
+    past_len + C - 1, whose keys the cache holds already (call it after
+    :func:`aoh_attention` of the layer).  ``past_len`` defaults to
+    ``cache.kv_seq_len``, which moves after the last layer only.  Returns (B,
+    n_ret, T = past_len + C) float32: for each of the layer's retrieval heads in
+    ascending order the softmax probabilities of its group's heads, summed over
+    heads and queries.  ``out``: a float32 tensor (B, n_ret, >= T) whose rows are
+    contiguous and evenly spaced (a slice of a larger buffer); its first T columns
+    are written, or with ``accumulate`` added to.  A cache in device-length mode
+    takes single tokens and ``out`` of max_context columns or more.
+    """
+    if not 0 <= layer_idx < cache.num_layers:
+        raise ValueError(f"layer_idx {layer_idx} out of range")
+    if q.dim() != 4:
+        raise ValueError("q must be (B, C, Hq, D)")
+    n = q.shape[1]
+    _check_q(cache, q, n)
+    if cache.device_length:
+        if n != 1 or past_len is not None or out is None:
+            raise ValueError("a cache in device-length mode takes single tokens (q_len 1), no past_len, and an out")
+        past, total = _lib.PAST_LEN_DEVICE, cache.max_context
+    else:
+        past = cache.kv_seq_len if past_len is None else int(past_len)
+        if past < 0:
+            raise ValueError("past_len must be non-negative")
+        total = past + n
+    B, R = cache.batch, cache.n_ret[layer_idx]
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs an out to add to")
+        out = torch.empty((B, R, total), dtype=torch.float32, device=cache.device)
+    elif (out.dim() != 3 or out.shape[0] != B or out.shape[1] != R or out.shape[2] < total
+          or out.dtype != torch.float32 or out.device != cache.device):
+        raise ValueError(f"out must be float32 (batch, n_ret, >= keys) = {(B, R, total)} on {cache.device}, "
+                         f"got {out.dtype} {tuple(out.shape)}")
+    if R == 0 or n == 0:
+        if not accumulate:
+            out[:, :, :total].zero_()
+        return out
+    stride = out.stride(1) if R > 1 else out.stride(0) if B > 1 else max(out.shape[2], total)
+    if out.stride(2) != 1 or stride < total or (B > 1 and out.stride(0) != R * stride):
+        raise ValueError("out's rows must be contiguous and evenly spaced over (batch, n_ret)")
+    L = cache._L
+    ws = torch.empty(int(L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n)), dtype=torch.uint8,
+                     device=cache.device)
+    _lib.launch(cache.device, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
+                out.data_ptr(), stride, bool(accumulate), ws.data_ptr(), ws.numel())
+    return out
+
+
+def select_keys(weights: torch.Tensor, keep: int, *, sink: int = 0, recent: int = 0
+                ) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys to keep by their weights.
+
+    weights (..., n) float32, n contiguous.  Keeps, per row, the first ``sink``
+    and the last ``recent`` keys and the largest weights between them, ``keep``
+    keys in all; the lower position first among equal weights, NaN like -inf.
+    Returns (positions (..., keep) int32, ascending, and their weights)."""
+    if weights.dim() < 1 or weights.dtype != torch.float32 or not weights.is_cuda:
+        raise ValueError("weights must be a float32 CUDA tensor (..., n)")
+    n = weights.shape[-1]
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if not 0 <= keep <= n:
+        raise ValueError(f"keep {keep} of {n} keys")
+    if sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError(f"sink {sink} and recent {recent} must be non-negative and fit keep {keep}")
+    lead = weights.shape[:-1]
+    rows = lead.numel()
+    kept = torch.empty((*lead, keep), dtype=torch.int32, device=weights.device)
+    kept_w = torch.empty((*lead, keep), dtype=torch.float32, device=weights.device)
+    if rows == 0 or keep == 0:
+        return kept, kept_w
+    w = weights.reshape(rows, n)  # a view, or a copy where the rows are not evenly spaced
+    if n > 1 and w.stride(1) != 1:
+        raise ValueError("the last dimension of weights must be contiguous")
+    _lib.launch(weights.device, _lib.lib().aoh_select_keys, "aoh_select_keys", w.data_ptr(), w.stride(0), rows, n, keep,
+                sink, recent, kept.data_ptr(), kept_w.data_ptr())
+    return kept, kept_w
+
+
+def evict(cache: AoHKVCache, kept: torch.Tensor, into: AoHKVCache) -> AoHKVCache:
+    """Copy the rows that stay of every layer into another cache.
+
+    kept (R, keep) int32, rows contiguous: the positions to keep of each
+    retrieval unit, in (layer, sequence, KV head) order, R = batch * sum(n_ret).
+    Position kept[r, i] becomes position i; streaming heads keep their sink and
+    their latest rows.  ``into``: a different cache with the same labels, batch,
+    windows and dtype and room for keep tokens; what it held is given up.  It then
+    holds keep tokens (``kv_seq_len``) of ``tokens_seen`` seen.  With streaming
+    heads, keep must reach sink + recent (or kv_seq_len)."""
+    if into is cache:
+        raise ValueError("into must be another cache")
+    if cache.device_length or into.device_length:
+        raise ValueError("a cache in device-length mode cannot be evicted")
+    R = cache.batch * sum(cache.n_ret)
+    if kept.dim() != 2 or kept.shape[0] != R or kept.dtype != torch.int32 or kept.device != cache.device:
+        raise ValueError(f"kept must be int32 ({R}, keep) on {cache.device}, got {kept.dtype} {tuple(kept.shape)}")
+    keep = kept.shape[1]
+    if keep > 1 and kept.stride(1) != 1:
+        raise ValueError("the rows of kept must be contiguous")
+    if into.device != cache.device:
+        raise ValueError(f"the caches are on {cache.device} and {into.device}")
+    if keep > cache.kv_seq_len:
+        raise ValueError(f"keep {keep} of {cache.kv_seq_len} tokens")
+    if keep > into.max_context:
+        raise ValueError(f"keep {keep} exceeds the destination's max_context {into.max_context}")
+    into.reserve(keep)
+    _lib.launch(cache.device, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, cache.kv_seq_len,
+                kept.data_ptr(), kept.stride(0), keep)
+    into.kv_seq_len = keep
+    into.evicted = cache.tokens_seen - keep
+    return into
+
+
+class KeyWeights:
+    """The attention weight of every cached key of every retrieval unit.
+
+    ``rows`` (R, max_context) float32, zero at the start, R = batch *
+    sum(n_ret) rows in (layer, sequence, KV head) order; column j belongs to the
+    key at cache position j."""
+
+    def __init__(self, cache: AoHKVCache):
+        self.cache = cache
+        self.rows = torch.zeros((cache.batch * sum(cache.n_ret), cache.max_context), dtype=torch.float32,
+                                device=cache.device)
+        self._first = [cache.batch * sum(cache.n_ret[:i]) for i in range(cache.num_layers + 1)]
+
+    def layer(self, layer_idx: int) -> torch.Tensor:
+        """(batch, n_ret, max_context) of one layer, a view."""
+        lo, hi = self._first[layer_idx], self._first[layer_idx + 1]
+        return self.rows[lo:hi].view(self.cache.batch, self.cache.n_ret[layer_idx], -1)
+
+    def add(self, layer_idx: int, q: torch.Tensor, past_len: int | None = None) -> None:
+        """Add what the queries q gave (see :func:`key_weights`)."""
+        key_weights(self.cache, layer_idx, q, past_len=past_len, out=self.layer(layer_idx), accumulate=True)
+
+    def evict(self, keep: int, into: AoHKVCache, *, sink: int | None = None, recent: int | None = None) -> "KeyWeights":
+        """Keep ``keep`` keys of every retrieval unit -- the first ``sink`` and the
+        last ``recent`` (default: the cache's window) among them -- and copy them
+        into ``into``.  Returns its KeyWeights, with the kept keys' sums."""
+        c = self.cache
+        kept, weights = select_keys(self.rows[:, :c.kv_seq_len], keep, sink=c.sink_size if sink is None else sink,
+                                    recent=c.recent_size if recent is None else recent)
+        evict(c, kept, into)
+        new = KeyWeights(into)
+        new.rows[:, :keep] = weights
+        return new

@@ -244,10 +244,119 @@ AOH_API int aoh_rope_qk(const void* q, const void* k, const void* cos, const voi
                         const void* k_norm_weight, float eps, int32_t batch, int32_t q_len, int32_t num_q_heads,
                         int32_t num_kv_heads, int32_t head_dim, void* q_out, void* k_out, aoh_stream stream);
 
+/* Rotary embedding by positions with several axes (images and video: time,
+ * height, width; one axis: the ordinary rotary embedding), with optional
+ * per-head RMSNorm, computed in fp32 from the positions (angles in fp64) and
+ * rounded once; no counterpart in the reference, whose models take cos / sin
+ * (aoh_rope_qk).  q (batch, q_len, num_q_heads, head_dim) and k (...,
+ * num_kv_heads, head_dim) of `dtype`: any strides q_strides / k_strides =
+ * {batch, token, head} in elements, head_dim contiguous, even and <= 256.
+ * positions (n_axes, batch, q_len): int64 if positions_64, else int32, strides
+ * {axis, batch, token}.  sections[n_axes] (host): how many of the half =
+ * sum(sections) <= head_dim / 2 frequencies take each axis's position, axis by
+ * axis, or, if interleaved, frequency i takes axis a = i mod n_axes while i <
+ * n_axes * sections[a], else axis 0.  inv_freq (half) fp32.  With angle a_i =
+ * positions[axis(i)] * inv_freq[i]: out[i] = scaling * (x[i] cos a_i - x[i +
+ * half] sin a_i), out[i + half] = scaling * (x[i + half] cos a_i + x[i] sin
+ * a_i), dimensions from 2 * half on are copied.  q_norm_weight / k_norm_weight
+ * (head_dim, `dtype`) or both NULL.  q_out / k_out: contiguous, not aliasing
+ * the inputs. */
+AOH_API int aoh_rope_axes_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                             int32_t dtype, const void* positions, int32_t positions_64,
+                             const int64_t* position_strides, const float* inv_freq, const int32_t* sections,
+                             int32_t n_axes, int32_t interleaved, const void* q_norm_weight, const void* k_norm_weight,
+                             float eps, float scaling, int32_t batch, int32_t q_len, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, void* q_out, void* k_out, aoh_stream stream);
+
 /* AoHKVCache.append_layer alone (benchmark_llama31.py:171-184): write q_len
  * new tokens at positions past_len.. into every unit of `layer`. */
 AOH_API int aoh_kv_append(aoh_kv_cache* cache, int32_t layer, int32_t past_len, int32_t q_len,
                   const void* k_new, const void* v_new, aoh_stream stream);
+
+/* ------------------------------------------------------------------------- */
+/* Eviction by accumulated attention weight (no counterpart in the           */
+/* reference, whose retrieval heads keep every token): the weight each key   */
+/* of a retrieval head received, the keys to keep by it, and the copy of     */
+/* their rows into another, shorter cache.  Streaming heads keep their sink  */
+/* and window.  "Retrieval rows" below are the (layer, sequence, KV head)    */
+/* units with label 1 in that order, owned here or not.                      */
+/* ------------------------------------------------------------------------- */
+
+/* out[r * out_stride + j] (+)= the attention weight of key j: the softmax
+ * probabilities of this call's q_len queries (all heads of r's group) over
+ * the keys each of them sees (j <= past_len + its index), summed.  r counts the
+ * retrieval rows of `layer` (batch x its retrieval heads).  Call it after the
+ * attention entry point has appended the same tokens: positions < past_len +
+ * q_len must be cached; out_stride >= past_len + q_len.  past_len may be
+ * AOH_PAST_LEN_DEVICE; out_stride must then reach max_context.  accumulate: add
+ * to out instead of writing it.  Units not stored here get (add) zeros.
+ * q (batch, q_len, num_q_heads, 128) as for aoh_attn_prefill.  workspace:
+ * 16-byte aligned device memory of aoh_key_weights_workspace_bytes() for the
+ * same lengths, of any contents, not shared by calls that overlap.  Scores are
+ * fp32 and sums are made in a fixed order. */
+AOH_API size_t aoh_key_weights_workspace_bytes(const aoh_kv_cache* cache, int32_t layer, int32_t past_len,
+                                               int32_t q_len);
+AOH_API int aoh_key_weights(aoh_kv_cache* cache, int32_t layer, int32_t past_len, int32_t q_len, const void* q,
+                            float* out, int64_t out_stride, int32_t accumulate, void* workspace,
+                            size_t workspace_bytes, aoh_stream stream);
+
+/* For each of `rows` rows of n fp32 weights (row_stride elements apart): the
+ * `keep` keys to keep -- the first `sink`, the last `recent` and the largest
+ * weights between them, lower position first among equal ones (NaN ranks like
+ * -inf) -- ascending, to kept (rows, keep) int32, and their weights to
+ * kept_weights (rows, keep) unless NULL. */
+AOH_API int aoh_select_keys(const float* weights, int64_t row_stride, int32_t rows, int32_t n, int32_t keep,
+                            int32_t sink, int32_t recent, int32_t* kept, float* kept_weights, aoh_stream stream);
+
+/* Copy the rows that stay of `src` (past_len positions cached) into `dst`, a
+ * different cache of the same layers, batch, heads, labels, owned units, dtype
+ * and windows, with positions [0, keep) reserved: retrieval row r's position
+ * kept[r * kept_stride + i] becomes position i; a streaming unit's sink stays
+ * and its latest rows get the positions up to keep.  With streaming heads keep
+ * must reach sink_size + recent_size (or past_len).  kept: device, for all
+ * retrieval rows of all layers; a position outside [0, past_len) is not
+ * copied and sets bit 1 of dst's device check word.  Rows of dst behind keep
+ * stay as they are. */
+AOH_API int aoh_kv_evict(aoh_kv_cache* src, aoh_kv_cache* dst, int32_t past_len, const int32_t* kept,
+                         int64_t kept_stride, int32_t keep, aoh_stream stream);
+
+/* ------------------------------------------------------------------------- */
+/* Logits (no counterpart in the reference): penalties for repeated tokens,  */
+/* biases and a grammar's mask, and the greedy token.                        */
+/* ------------------------------------------------------------------------- */
+
+/* A history is counts (rows, vocab) int32 -- bits 0..30: occurrences in the
+ * output, bit 31: in the prompt -- and seen (rows, ceil(vocab / 32)) int32, bit
+ * t % 32 of word t / 32 set where counts[t] is not 0; both zero at the start.
+ * Adds ids[row * id_stride + i], i < per_row (and < lengths[row] unless
+ * lengths is NULL): one occurrence each, or the prompt's mark if `prompt`.
+ * ids: device, int64 if ids_64, else int32; ids outside [0, vocab) are left
+ * out. */
+AOH_API int aoh_history_add(int32_t* counts, int32_t* seen, int32_t rows, int32_t vocab, const void* ids,
+                            int32_t ids_64, int64_t id_stride, int32_t per_row, const int32_t* lengths, int32_t prompt,
+                            aoh_stream stream);
+
+/* Per row of logits (rows, vocab; AOH_BF16 or AOH_F32, row_stride elements
+ * apart), in this order, each step rounded to fp32:
+ *   x > 0 ? x / repetition : x * repetition   for tokens of the prompt or output,
+ *   x - frequency * count, then x - presence  for tokens of the output,
+ *   x + the sum of its biases                 (bias_ids, bias (rows, n_bias); ids outside [0, vocab) are left out),
+ *   -inf                                      where bit t % 32 of word t / 32 of the row's mask is 0.
+ * repetition / presence / frequency: device fp32 (rows), or NULL for the
+ * scalar.  counts / seen: the history, or both NULL (no penalties).  allowed
+ * (n_allowed, ceil(vocab / 32)) int32 or NULL; row n's mask is allowed[n], or
+ * allowed[allowed_rows[n]] with allowed_rows (rows) int32, an index outside
+ * [0, n_allowed) meaning no mask.  out (out_dtype, out_stride) may be the
+ * logits themselves.  greedy (rows) int64 or NULL: the token of the largest
+ * fp32 result, the lowest of equal ones (NaN above every number; 0 where
+ * nothing is allowed). */
+AOH_API int aoh_logits_penalize(const void* logits, int64_t row_stride, int32_t dtype, int32_t rows, int32_t vocab,
+                                const int32_t* counts, const int32_t* seen, const float* repetition,
+                                float repetition_scalar, const float* presence, float presence_scalar,
+                                const float* frequency, float frequency_scalar, const int32_t* bias_ids,
+                                const float* bias, int32_t n_bias, const int32_t* allowed, const int32_t* allowed_rows,
+                                int32_t n_allowed, void* out, int64_t out_stride, int32_t out_dtype, int64_t* greedy,
+                                aoh_stream stream);
 
 /* ------------------------------------------------------------------------- */
 /* Effective-rank classifier                                                 */
