@@ -86,6 +86,7 @@ struct aoh_kv_cache {
   int32_t* dev_table = nullptr;
   int32_t* dev_err = nullptr;   // [0] check word, [1] device-resident sequence length
   int32_t* dev_unit_row = nullptr;  // per unit: its index among the retrieval units (stored here or not), -1: streaming
+  int32_t* dev_row_unit = nullptr;  // per retrieval unit in that order: its unit
   int32_t len_hint = 0;          // host copy of the device length (plans kernels in device mode)
   bool bound = false;
   int device = -1;

@@ -10,7 +10,9 @@
 // key is summed by one CTA in a fixed order, so results do not depend on timing.
 //
 // This file holds the entry point and the kernels for any type: 64 rows x 64
-// keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.
+// keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.  bf16
+// caches run those of key_weights_sm100.cu: one pass over K for few query rows
+// (single tokens), tensor cores for more.
 #include "common.cuh"
 #include "internal.h"
 #include "key_weights.h"
@@ -103,20 +105,21 @@ __device__ __forceinline__ int last_key(const KeyWeightsArgs& a, int past, int r
 
 // (m, l) of 64 query rows over one range of keys.
 template <typename T>
-__global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ KeyWeightsArgs a) {
+__global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
-  const int unit = a.unit0 + blockIdx.y, r = a.unit_row[unit];
-  if (r < 0 || a.g.unit_offset[unit] == a.g.unit_offset[unit + 1]) return;
+  const int r = blockIdx.y, unit = a.row_unit[r];
+  if (a.g.unit_offset[unit] == a.g.unit_offset[unit + 1]) return;
   const int past = key_weights_past(a);
   const int rows = a.q_len * a.g.grp, row0 = blockIdx.x * kTile;
-  const int b = blockIdx.y / a.g.G, g = blockIdx.y % a.g.G;
+  const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
+  const long long rows_total = (long long)a.units * rows;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   float *qs = sm, *ks = sm + kTile * kStride;
   load_queries<T>(a, b, g, row0, rows, qs);
   // key tiles up to the last one that any row of the tile sees, split evenly
   const int len = last_key(a, past, min(row0 + kTile, rows) - 1) + 1;
   const int tiles = (len + kTile - 1) / kTile;
-  const int t0 = (int)((long long)tiles * blockIdx.z / a.splits), t1 = (int)((long long)tiles * (blockIdx.z + 1) / a.splits);
+  const int t0 = (int)((long long)tiles * blockIdx.z / splits), t1 = (int)((long long)tiles * (blockIdx.z + 1) / splits);
   float m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
@@ -155,23 +158,23 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
     for (int off = 8; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
     const int row = row0 + 4 * ty + i;
     if (tx == 0 && row < rows)
-      a.part[blockIdx.z * a.rows_total + (long long)(r - a.row0) * rows + row] = make_float2(mm, ll);
+      part[blockIdx.z * rows_total + (long long)r * rows + row] = make_float2(mm, ll);
   }
 }
 
 // The weights of 64 keys, summed over every query row of the unit.
 template <typename T>
-__global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a) {
+__global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
   __shared__ float lse[kTile];
-  const int unit = a.unit0 + blockIdx.y, r = a.unit_row[unit];
-  if (r < 0) return;
+  const int r = blockIdx.y, unit = a.row_unit[r];
   const int past = key_weights_past(a);
   const int len = past + a.q_len, rows = a.q_len * a.g.grp;
   const int j0 = blockIdx.x * kTile;
   if (j0 >= len) return;
   const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
-  const int b = blockIdx.y / a.g.G, g = blockIdx.y % a.g.G;
+  const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
+  const long long rows_total = (long long)a.units * rows;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   float *qs = sm, *ks = sm + kTile * kStride;
   float w[4] = {0.f, 0.f, 0.f, 0.f};
@@ -183,11 +186,11 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
       __syncthreads();
       load_queries<T>(a, b, g, row0, rows, qs);
       if (threadIdx.x < kTile && row0 + threadIdx.x < rows) {
-        const float2* p = a.part + (long long)(r - a.row0) * rows + row0 + threadIdx.x;
+        const float2* p = part + (long long)r * rows + row0 + threadIdx.x;
         float mm = -INFINITY, ll = 0.f;
-        for (int i = 0; i < a.splits; ++i) mm = fmaxf(mm, p[i * a.rows_total].x);
-        for (int i = 0; i < a.splits; ++i) {
-          const float2 v = p[i * a.rows_total];
+        for (int i = 0; i < splits; ++i) mm = fmaxf(mm, p[i * rows_total].x);
+        for (int i = 0; i < splits; ++i) {
+          const float2 v = p[i * rows_total];
           if (v.y > 0.f) ll += v.y * fast_exp2(v.x - mm);
         }
         lse[threadIdx.x] = mm + log2f(ll);
@@ -215,13 +218,13 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
   if (threadIdx.x < kTile && j0 + threadIdx.x < len) {
     float x = 0.f;
     for (int i = 0; i < 16; ++i) x += qs[i * kTile + threadIdx.x];
-    float* o = a.out + (r - a.row0) * a.out_stride + j0 + threadIdx.x;
+    float* o = a.out + r * a.out_stride + j0 + threadIdx.x;
     *o = a.accumulate ? *o + x : x;
   }
 }
 
 template <typename T>
-int launch_generic(const KeyWeightsArgs& a, int row_tiles, cudaStream_t st) {
+int launch_any(const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws, cudaStream_t st) {
   int dev = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
@@ -234,8 +237,9 @@ int launch_generic(const KeyWeightsArgs& a, int row_tiles, cudaStream_t st) {
   });
   if (rc) return rc;
   const int key_tiles = (a.max_len + kTile - 1) / kTile;
-  key_lse_kernel<T><<<dim3(row_tiles, a.units, a.splits), 256, kSmem, st>>>(a);
-  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSmem, st>>>(a);
+  float2* part = reinterpret_cast<float2*>(ws + p.part);
+  key_lse_kernel<T><<<dim3(p.row_tiles, a.units, p.splits), 256, kSmem, st>>>(a, part, p.splits);
+  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSmem, st>>>(a, part, p.splits);
   return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
 }
 
@@ -245,22 +249,22 @@ int retrieval_heads(const aoh_kv_cache* c, int layer) {
   return n;
 }
 
-// The plan of a call: query-row tiles and the key ranges of each.
-struct Plan {
-  int n_units, row_tiles, splits;
-  size_t workspace;
-};
-
-Plan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
-  Plan p;
-  p.n_units = c->cfg.batch * retrieval_heads(c, layer);
-  const long long rows = (long long)q_len * (c->cfg.num_q_heads / c->cfg.num_kv_heads);
-  p.row_tiles = (int)((rows + kTile - 1) / kTile);
-  const int key_tiles = (max_len + kTile - 1) / kTile;
-  // enough CTAs for three per SM
-  const long long ctas = std::max(1LL, (long long)p.n_units * p.row_tiles);
-  p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles), (3LL * std::max(1, c->num_sms) + ctas - 1) / ctas));
-  p.workspace = (size_t)p.splits * p.n_units * rows * sizeof(float2);
+KeyWeightsPlan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
+  KeyWeightsPlan p;
+  const int units = c->cfg.batch * retrieval_heads(c, layer), grp = c->cfg.num_q_heads / c->cfg.num_kv_heads;
+  p.rows = q_len * grp;
+  if (c->cfg.dtype == AOH_BF16 && p.rows <= kFewRows) {
+    plan_key_weights_few(c, units, max_len, p);
+  } else if (c->cfg.dtype == AOH_BF16 && grp <= 128) {
+    plan_key_weights_tensor(c, units, max_len, q_len, p);
+  } else {
+    p.row_tiles = (p.rows + kTile - 1) / kTile;
+    const int key_tiles = (max_len + kTile - 1) / kTile;
+    // enough CTAs for three per SM
+    const long long ctas = std::max(1LL, (long long)units * p.row_tiles);
+    p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles), (3LL * std::max(1, c->num_sms) + ctas - 1) / ctas));
+    p.bytes = (size_t)p.splits * units * p.rows * sizeof(float2);
+  }
   return p;
 }
 
@@ -278,7 +282,7 @@ extern "C" size_t aoh_key_weights_workspace_bytes(const aoh_kv_cache* c, int32_t
   if (!c || layer < 0 || layer >= c->cfg.num_layers || past_len < AOH_PAST_LEN_DEVICE || q_len <= 0 ||
       (int64_t)past_len + q_len > c->cfg.max_context)
     return 0;
-  return plan(c, layer, most_keys(c, past_len, q_len), q_len).workspace;
+  return plan(c, layer, most_keys(c, past_len, q_len), q_len).bytes;
 }
 
 extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len, int32_t q_len, const void* q, float* out,
@@ -297,17 +301,18 @@ extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len,
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: rows of %lld weights for %d keys", who, (long long)out_stride, max_len);
   KeyWeightsArgs a{};
   a.g = c->geom();
-  a.units = c->cfg.batch * c->cfg.num_kv_heads;
+  a.units = c->cfg.batch * n_ret;
   if (a.units > 65535) return fail(AOH_ERR_UNSUPPORTED, "%s: too many units", who);
   if ((long long)q_len * a.g.grp > (1 << 30)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many queries", who);
-  const Plan p = plan(c, layer, max_len, q_len);
-  if (!workspace || workspace_bytes < p.workspace)
-    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.workspace);
+  const KeyWeightsPlan p = plan(c, layer, max_len, q_len);
+  if (!workspace || workspace_bytes < p.bytes)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
-  a.unit_row = c->dev_unit_row;
+  int row0 = 0;
+  for (int l = 0; l < layer; ++l) row0 += c->cfg.batch * retrieval_heads(c, l);
+  a.row_unit = c->dev_row_unit + row0;
   a.unit0 = c->unit(layer, 0, 0);
-  for (int l = 0; l < layer; ++l) a.row0 += c->cfg.batch * retrieval_heads(c, l);
   a.past_len = past_len;
   a.past_len_dev = device_len ? c->dev_err + 1 : nullptr;
   a.max_len = max_len;
@@ -316,10 +321,12 @@ extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len,
   a.out = out;
   a.out_stride = out_stride;
   a.accumulate = accumulate;
-  a.part = static_cast<float2*>(workspace);
-  a.rows_total = (long long)p.n_units * q_len * a.g.grp;
-  a.splits = p.splits;
+  char* ws = static_cast<char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return c->cfg.dtype == AOH_BF16 ? launch_generic<__nv_bfloat16>(a, p.row_tiles, st)
-                                  : launch_generic<float>(a, p.row_tiles, st);
+  switch (p.kind) {
+    case KeyWeightsKind::few: return launch_key_weights_few(c, a, p, ws, st);
+    case KeyWeightsKind::tensor: return launch_key_weights_tensor(c, a, p, ws, st);
+    default:
+      return c->cfg.dtype == AOH_BF16 ? launch_any<__nv_bfloat16>(a, p, ws, st) : launch_any<float>(a, p, ws, st);
+  }
 }

@@ -10,9 +10,9 @@ namespace aoh {
 // row = token * grp + head.
 struct KeyWeightsArgs {
   CacheGeom g;
-  const int32_t* unit_row;  // per unit: index among the retrieval units, -1: streaming
-  int unit0, row0;          // first unit of the layer, first retrieval row of the layer
-  int units;                // B * G units of the layer
+  const int32_t* row_unit;  // per retrieval row of this layer: its unit
+  int unit0;                // first unit of the layer
+  int units;                // retrieval rows of the layer: B * n_ret
   int past_len;             // keys cached before these queries
   const int* past_len_dev;  // read instead of past_len when not null
   int max_len;              // keys that `out` and the plan have room for
@@ -21,10 +21,34 @@ struct KeyWeightsArgs {
   float* out;               // retrieval row r, key j: out[r * out_stride + j]
   long long out_stride;
   int accumulate;
-  float2* part;             // (m, l) of a query row over one key range: part[(split * n_rows_total + row)]
-  int splits;
-  long long rows_total;     // query rows of all retrieval units
 };
+
+// How a call is run and where its workspace's parts begin (bytes).
+//   any:     (m, l) of every query row by key range, then the sums
+//   few:     scores of every (key, query row) and (m, l) by key range, then the sums
+//   tensor:  (m, l) by key range, the rows' -lse, the sums by row range
+enum class KeyWeightsKind { any, few, tensor };
+struct KeyWeightsPlan {
+  KeyWeightsKind kind = KeyWeightsKind::any;
+  int rows = 0;            // query rows of a unit
+  int row_tiles = 0;
+  int tile_tokens = 0;     // tensor: tokens of a row tile
+  int splits = 1;          // key ranges
+  int row_splits = 1;      // tensor: row ranges of the sums
+  size_t part = 0, score = 0, lse = 0, sums = 0, bytes = 0;
+};
+
+// Launchers of the bf16 kernels (key_weights_sm100.cu).
+void plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p);
+void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int q_len, KeyWeightsPlan& p);
+int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
+                           cudaStream_t st);
+int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
+                              cudaStream_t st);
+
+constexpr int kFewRows = 32;  // query rows of a unit that the few-rows kernel takes
+
+inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 #ifdef __CUDACC__
 // Keys cached before the queries.  A device length beyond what the caller

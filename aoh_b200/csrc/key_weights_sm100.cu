@@ -1,0 +1,716 @@
+// Attention weight by key over a bf16 cache (see key_weights.cu for what is
+// computed).
+//
+// Few query rows (single tokens and a few more): bound by reading K once, 256
+// bytes a key.  few_scores_kernel keeps the rows of Q as mma fragments and
+// streams the pages of a key range from global memory straight into A
+// fragments: the product does not depend on the order of the 128 dimensions,
+// so a lane takes whole 16-byte chunks and Q is laid out to match.  It writes
+// the scores (4 bytes a key and row, which stay in L2) and the range's (m, l);
+// few_sum_kernel turns them into weights.
+//
+// More rows: tensor_pass_kernel<kLse> and <kSums>, the same product with its
+// operands exchanged.  A CTA keeps two 128-row tiles of one operand in shared
+// memory (two tiles of query rows, or two tiles of keys) and streams 128-row
+// tiles of the other; each 128 x 128 product goes to tensor memory (two
+// buffers per resident tile), where a warpgroup per resident tile reads it,
+// thread = row.  With query rows as rows a thread keeps its row's running
+// maximum and sum; with keys as rows it adds up exp(s - lse) over the columns,
+// so neither pass exchanges anything between threads.  Query rows are packed
+// (token, head) pairs, so a chunk of a few tokens still fills a tile.
+#include <type_traits>
+
+#include "common.cuh"
+#include "fast_math.cuh"
+#include "internal.h"
+#include "key_weights.h"
+#include "page_layout.cuh"
+
+namespace aoh {
+namespace {
+
+// ---------------------------------------------------------------------------
+// few query rows
+// ---------------------------------------------------------------------------
+constexpr int kFewWarps = 8;
+
+struct FewArgs {
+  KeyWeightsArgs a;
+  float2* part;   // [split][unit row][row]
+  float* score;   // [unit row][key][rows_even], log2 domain, -inf where a row does not see the key
+  int rows, rows_even, splits;
+  long long score_unit;  // floats of a unit's scores
+};
+
+template <int NT>  // tiles of 8 query rows
+__global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_kernel(const __grid_constant__ FewArgs f) {
+  __shared__ float2 red[kFewWarps][NT * 8];
+  const KeyWeightsArgs& a = f.a;
+  griddep_launch_dependents();  // the sums wait for this grid to finish
+  const int r = blockIdx.y, unit = a.row_unit[r];
+  const int base = a.g.unit_offset[unit], held = a.g.unit_offset[unit + 1] - base;
+  if (held == 0) return;
+  const int past = key_weights_past(a), len = past + a.q_len;
+  const int n_pages = (len + kPage - 1) / kPage;
+  const int b = (unit - a.unit0) / a.g.G, kvh = (unit - a.unit0) % a.g.G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
+  const int p0 = (int)((long long)n_pages * blockIdx.x / f.splits), p1 = (int)((long long)n_pages * (blockIdx.x + 1) / f.splits);
+
+  uint4 qf[NT][4];
+  int last[NT][2];  // last key that the lane's two query rows see (-1: no such row)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = n * 8 + gq;
+    const uint4* src = nullptr;
+    if (row < f.rows)
+      src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) +
+                                           (((long long)b * a.q_len + row / a.g.grp) * a.g.Hq + kvh * a.g.grp + row % a.g.grp) *
+                                               kHeadDim);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qf[n][i] = src ? src[4 * i + tq] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = n * 8 + 2 * tq + e;
+      last[n][e] = col < f.rows ? past + col / a.g.grp : -1;
+    }
+  }
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f;
+
+  const char* pool = static_cast<const char*>(a.g.pool);
+  // page ids of the warp's next 32 pages, one a lane
+  int ids = -1, ids_at = -32;
+  auto page_id = [&](int i) {  // i: the warp's i-th page
+    if (i - ids_at >= 32) {
+      ids_at = i;
+      const int p = p0 + warp + (i + lane) * kFewWarps;
+      ids = p < p1 && p < held ? a.g.block_table[base + p] : -1;
+      if (p < p1 && (ids < 0 || ids >= a.g.num_pages)) {
+        atomicOr(a.g.err, kErrBadPage);
+        ids = -1;
+      }
+    }
+    return __shfl_sync(0xffffffffu, ids, i - ids_at);
+  };
+  // chunk 4 i + t of rows g and g + 8
+  auto load_page = [&](int id, uint4 (&k)[4][2]) {
+    const char* src = pool + (long long)id * kPageBf16Bytes + gq * 128;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        k[i][h] = id < 0 ? make_uint4(0u, 0u, 0u, 0u)
+                         : __ldcs(reinterpret_cast<const uint4*>(src + (i >> 1) * kHalfBytes + h * 1024 +
+                                                                 (((4 * (i & 1) + tq) ^ gq) << 4)));
+  };
+  const int mine = p1 - p0 > warp ? (p1 - p0 - warp + kFewWarps - 1) / kFewWarps : 0;
+  uint4 cur[4][2], nxt[4][2];
+  if (mine > 0) load_page(page_id(0), cur);
+  for (int i = 0; i < mine; ++i) {
+    if (i + 1 < mine) load_page(page_id(i + 1), nxt);
+    float c[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t a0[4] = {cur[k][0].x, cur[k][1].x, cur[k][0].y, cur[k][1].y};
+        mma_bf16_16816(c[n], a0, qf[n][k].x, qf[n][k].y);
+        const uint32_t a1[4] = {cur[k][0].z, cur[k][1].z, cur[k][0].w, cur[k][1].w};
+        mma_bf16_16816(c[n], a1, qf[n][k].z, qf[n][k].w);
+      }
+    }
+    const int j0 = (p0 + warp + i * kFewWarps) * kPage + gq;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float s[2][2];  // [key j0, j0 + 8][column]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s[h][e] = j0 + 8 * h <= last[n][e] ? c[n][2 * h + e] * kScoreScale : -INFINITY;
+      const int col = n * 8 + 2 * tq;
+      if (col < f.rows_even) {
+        float* o = f.score + r * f.score_unit + (long long)j0 * f.rows_even + col;
+        *reinterpret_cast<float2*>(o) = make_float2(s[0][0], s[0][1]);
+        *reinterpret_cast<float2*>(o + 8 * f.rows_even) = make_float2(s[1][0], s[1][1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float mt = fmaxf(s[0][e], s[1][e]);
+        if (mt > m[n][e]) {
+          l[n][e] *= fast_exp2(m[n][e] - mt);
+          m[n][e] = mt;
+        }
+        if (m[n][e] > -INFINITY) l[n][e] += fast_exp2(s[0][e] - m[n][e]) + fast_exp2(s[1][e] - m[n][e]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) cur[k][0] = nxt[k][0], cur[k][1] = nxt[k][1];
+  }
+  // over the 8 lanes of a column, then over the warps
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mm = m[n][e];
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+      float ll = mm > -INFINITY ? l[n][e] * fast_exp2(m[n][e] - mm) : 0.f;
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+      if (gq == 0) red[warp][n * 8 + 2 * tq + e] = make_float2(mm, ll);
+    }
+  __syncthreads();
+  if (threadIdx.x < f.rows) {
+    float mm = -INFINITY, ll = 0.f;
+    for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, red[w][threadIdx.x].x);
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float2 v = red[w][threadIdx.x];
+      if (v.y > 0.f) ll += v.y * fast_exp2(v.x - mm);
+    }
+    f.part[((long long)blockIdx.x * a.units + r) * f.rows + threadIdx.x] = make_float2(mm, ll);
+  }
+}
+
+// Weights of 256 keys from their scores.
+__global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
+  __shared__ float lse[kFewRows];
+  const KeyWeightsArgs& a = f.a;
+  const int r = blockIdx.y, unit = a.row_unit[r];
+  const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
+  const int len = key_weights_past(a) + a.q_len;
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  griddep_wait();
+  if (blockIdx.x * 256 >= len) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (stored) {
+    for (int row = warp; row < f.rows; row += 8) {
+      float m = -INFINITY, l = 0.f;
+      for (int i = lane; i < f.splits; i += 32) {
+        const float2 v = f.part[((long long)i * a.units + r) * f.rows + row];
+        if (v.x > m) {
+          l *= fast_exp2(m - v.x);
+          m = v.x;
+        }
+        if (v.y > 0.f) l += v.y * fast_exp2(v.x - m);
+      }
+      float mm = m;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+      l = m > -INFINITY ? l * fast_exp2(m - mm) : 0.f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      if (lane == 0) lse[row] = mm + log2f(l);
+    }
+  }
+  __syncthreads();
+  if (j >= len) return;
+  float w = 0.f;
+  if (stored) {
+    const float* s = f.score + r * f.score_unit + (long long)j * f.rows_even;
+    for (int row = 0; row < f.rows; row += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(s + row);
+      w += fast_exp2(v.x - lse[row]);
+      if (row + 1 < f.rows) w += fast_exp2(v.y - lse[row + 1]);
+    }
+  }
+  float* o = a.out + r * a.out_stride + j;
+  *o = a.accumulate ? *o + w : w;
+}
+
+// ---------------------------------------------------------------------------
+// tensor cores
+// ---------------------------------------------------------------------------
+constexpr int kTcThreads = 384;  // warp 0 loads, warp 1 issues, warps 4..11: one warpgroup per resident tile
+constexpr int kStages = 3;
+constexpr int kTileRows = 128;
+constexpr int kHalfTile = kTileRows * 128;   // 64 dimensions of 128 rows
+constexpr int kTileBytes = 2 * kHalfTile;    // 32 KB
+constexpr int kLseBytes = kTileRows * 4;
+// Slots of the columns' -lse.  A warpgroup hands a product's buffer back before
+// it has read that tile's slot, so the products may be two tiles ahead of it
+// and the loads kStages ahead of those: a slot must outlive kStages + 2 tiles.
+constexpr int kLseSlots = 8;
+static_assert(kLseSlots > kStages + 2, "a slot of -lse would be loaded over while it is read");
+constexpr int kTcSmem = (2 + kStages) * kTileBytes + kLseSlots * kLseBytes + 1024;  // + alignment
+constexpr int kTmemCols = 512;
+
+enum { kLse = 0, kSums = 1 };
+
+struct TcArgs {
+  KeyWeightsArgs a;
+  float2* part;    // [split][unit row][row tile * 128 + row]: (m, l), kLse with several key ranges
+  float* neg_lse;  // [unit row][row tile * 128 + row]: -lse, -inf for rows that hold no query
+  float* sums;     // [row split][unit row][key], kSums with several row ranges
+  int row_tiles, tile_tokens;
+  int pairs;       // pairs of resident tiles of a unit
+  int splits;      // ranges of the streamed tiles
+  long long sums_unit;
+};
+
+template <int kPass>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tensor_pass_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ TcArgs t) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bar_a, bar_final, bar_full[kStages], bar_empty[kStages], bar_s_full[2][2], bar_s_empty[2][2],
+      bar_lse[kLseSlots];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  const KeyWeightsArgs& a = t.a;
+  const CacheGeom& G = a.g;
+  uint8_t* sA = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
+  uint8_t* sB = sA + 2 * kTileBytes;
+  float* sLse = reinterpret_cast<float*>(sB + kStages * kTileBytes);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+
+  // this CTA's resident pair and range of streamed tiles
+  const int split = blockIdx.x % t.splits;
+  const int item = blockIdx.x / t.splits;
+  const int r = item % a.units;
+  // causal: late query rows see more keys, early keys are seen by more rows -- the long items first
+  const int pair = kPass == kLse ? t.pairs - 1 - item / a.units : item / a.units;
+  const int unit = a.row_unit[r];
+  const int base = G.unit_offset[unit], held = G.unit_offset[unit + 1] - base;
+  const int past = key_weights_past(a), len = past + a.q_len;
+  const int b = (unit - a.unit0) / G.G, kvh = (unit - a.unit0) % G.G;
+  const int tt = t.tile_tokens;
+  const int key_tiles = (len + kTileRows - 1) / kTileRows;
+  const int resident = kPass == kLse ? t.row_tiles : key_tiles;
+  const int na = min(2, resident - 2 * pair);  // resident tiles (a device length may leave none)
+  if (na <= 0) return;
+  if (held == 0) {  // not stored here: no weight
+    if (kPass == kSums && split == 0 && tid < 256) {
+      const int j = 2 * pair * kTileRows + tid;
+      if (j < len) {
+        float* o = a.out + r * a.out_stride + j;
+        if (t.splits > 1)
+          for (int i = 0; i < t.splits; ++i) t.sums[((long long)i * a.units + r) * t.sums_unit + j] = 0.f;
+        else if (!a.accumulate)
+          *o = 0.f;
+      }
+    }
+    return;
+  }
+  int first, end;  // streamed tiles that any resident row needs
+  if (kPass == kLse) {
+    const int tok_end = min(a.q_len, (2 * pair + na) * tt);
+    first = 0;
+    end = (past + tok_end + kTileRows - 1) / kTileRows;
+  } else {
+    first = max(0, 2 * pair * kTileRows - past) / tt;
+    end = t.row_tiles;
+  }
+  const int t0 = first + (int)((long long)(end - first) * split / t.splits);
+  const int n = first + (int)((long long)(end - first) * (split + 1) / t.splits) - t0;
+
+  if (warp == 1) {
+    tmem_alloc(&s_tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    mbar_init(&bar_a, 1);
+    mbar_init(&bar_final, 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bar_full[s], 1);
+      mbar_init(&bar_empty[s], 1);
+    }
+    for (int s = 0; s < kLseSlots; ++s) mbar_init(&bar_lse[s], 1);
+    for (int w = 0; w < 2; ++w)
+      for (int u = 0; u < 2; ++u) {
+        mbar_init(&bar_s_full[w][u], 1);
+        mbar_init(&bar_s_empty[w][u], 128);
+      }
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  // rows of a query tile that no load writes: zero scores, which -lse = -inf turns to nothing
+  const int q_rows = tt * G.grp;
+  if (kPass == kSums)
+    for (int i = tid; i < kStages * 2 * (kTileRows - q_rows) * 8; i += kTcThreads) {
+      const int row = q_rows + (i / 8) % (kTileRows - q_rows), sh = i / 8 / (kTileRows - q_rows);
+      reinterpret_cast<uint4*>(sB + sh * kHalfTile + row * 128)[i % 8] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 0) {
+    // ============================ loads ============================
+    const int32_t* bt = G.block_table + base;
+    const uint8_t* pool = static_cast<const uint8_t*>(G.pool);
+    const uint32_t q_bytes = (uint32_t)q_rows * 256;
+    // K rows of 128 keys: lane = (page, 64-dim half), 2 KB each
+    auto key_id = [&](int tile) {
+      const int p = tile * 8 + (lane >> 1);
+      return lane < 16 && p * kPage < len && p < held ? bt[p] : -1;
+    };
+    auto load_keys = [&](int tile, int id, uint8_t* dst, uint64_t* bar, bool arrive) {
+      const bool want = lane < 16 && (tile * 8 + (lane >> 1)) * kPage < len;
+      const bool ok = want && id >= 0 && id < G.num_pages;
+      if (want && !ok) atomicOr(G.err, kErrBadPage);
+      const uint32_t okm = __ballot_sync(0xffffffffu, ok);
+      if (arrive && lane == 0) {
+        if (okm)
+          mbar_arrive_expect_tx(bar, __popc(okm) * kBlockBytes);
+        else
+          mbar_arrive(bar);
+      }
+      __syncwarp();
+      if (ok)
+        bulk_load(dst + (lane & 1) * kHalfTile + (lane >> 1) * kBlockBytes,
+                  pool + (size_t)id * kPageBf16Bytes + (lane & 1) * kHalfBytes, kBlockBytes, bar);
+      return okm;
+    };
+    auto load_queries = [&](int tile, uint8_t* dst, uint64_t* bar) {
+      tma_load_4d(dst, &tm_q, bar, 0, kvh * G.grp, tile * tt, b);
+      tma_load_4d(dst + kHalfTile, &tm_q, bar, 64, kvh * G.grp, tile * tt, b);
+    };
+    if (kPass == kLse) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bar_a, na * q_bytes);
+        for (int w = 0; w < na; ++w) load_queries(2 * pair + w, sA + w * kTileBytes, &bar_a);
+      }
+    } else {
+      // both tiles complete one phase: the copies' bytes are counted before any is issued
+      const int id0 = key_id(2 * pair), id1 = na > 1 ? key_id(2 * pair + 1) : -1;
+      const uint32_t ok0 = __ballot_sync(0xffffffffu, id0 >= 0 && id0 < G.num_pages);
+      const uint32_t ok1 = __ballot_sync(0xffffffffu, id1 >= 0 && id1 < G.num_pages);
+      if (lane == 0) {
+        const uint32_t bytes = (__popc(ok0) + __popc(ok1)) * kBlockBytes;
+        if (bytes)
+          mbar_arrive_expect_tx(&bar_a, bytes);
+        else
+          mbar_arrive(&bar_a);
+      }
+      __syncwarp();
+      load_keys(2 * pair, id0, sA, &bar_a, false);
+      if (na > 1) load_keys(2 * pair + 1, id1, sA + kTileBytes, &bar_a, false);
+    }
+    int issued = 0;
+    int id_next = kPass == kLse && n > 0 ? key_id(t0) : -1;
+    for (int i = 0; i < n; ++i) {
+      const int s = i % kStages;
+      const int id = id_next;
+      if (kPass == kLse && i + 1 < n) id_next = key_id(t0 + i + 1);
+      if (lane == 0 && i >= kStages && !s_abort) {
+        if (!mbar_wait(&bar_empty[s], (i / kStages - 1) & 1, G.err)) s_abort = 1;
+      }
+      __syncwarp();
+      if (s_abort) break;
+      uint8_t* dst = sB + s * kTileBytes;
+      if (kPass == kLse) {
+        load_keys(t0 + i, id, dst, &bar_full[s], true);
+      } else if (lane == 0) {
+        const int slot = i % kLseSlots;
+        mbar_arrive_expect_tx(&bar_full[s], q_bytes);
+        load_queries(t0 + i, dst, &bar_full[s]);
+        mbar_arrive_expect_tx(&bar_lse[slot], kLseBytes);
+        bulk_load(sLse + slot * kTileRows, t.neg_lse + ((long long)r * t.row_tiles + t0 + i) * kTileRows, kLseBytes,
+                  &bar_lse[slot]);
+      }
+      issued = i + 1;
+      __syncwarp();
+    }
+    // nothing this CTA issued may still be landing when it exits
+    if (lane == 0) {
+      mbar_wait(&bar_a, 0, G.err);
+      for (int i = max(0, issued - kStages); i < issued; ++i) {
+        mbar_wait(&bar_full[i % kStages], (i / kStages) & 1, G.err);
+        if (kPass == kSums) mbar_wait(&bar_lse[i % kLseSlots], (i / kLseSlots) & 1, G.err);
+      }
+    }
+  } else if (warp == 1) {
+    // ============================ products ============================
+    constexpr uint32_t kIdesc = idesc_bf16(kTileRows, kTileRows, 0, 0);
+    bool ok = mbar_wait_warp(&bar_a, 0, G.err);
+    if (!ok) s_abort = 1;
+    tc_fence_after();
+    for (int i = 0; i < n && ok && !s_abort; ++i) {
+      const int s = i % kStages, buf = i & 1;
+      if (!(ok = mbar_wait_warp(&bar_full[s], (i / kStages) & 1, G.err))) break;
+      for (int w = 0; w < na && ok; ++w) {
+        if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[w][buf], ((i >> 1) - 1) & 1, G.err))) break;
+        tc_fence_after();
+        const uint32_t a_addr = smem_u32(sA + w * kTileBytes), b_addr = smem_u32(sB + s * kTileBytes);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32;
+          mma_ss(tmem + (w * 2 + buf) * kTileRows, smem_desc_sw128(a_addr + off, 16, 1024),
+                 smem_desc_sw128(b_addr + off, 16, 1024), kIdesc, k > 0 ? 1u : 0u);
+        }
+        mma_commit(&bar_s_full[w][buf]);
+      }
+      if (ok) mma_commit(&bar_empty[s]);
+    }
+    if (!ok) s_abort = 1;
+    __syncwarp();
+    mma_commit(&bar_final);  // fires once every product issued above has completed
+  } else if (warp >= 4 && (warp - 4) / 4 < na) {
+    // ============================ exponentials ============================
+    const int w = (warp - 4) / 4, row = 32 * (warp & 3) + lane;
+    const uint32_t s_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + w * 2 * kTileRows;
+    const int tile = 2 * pair + w;
+    // kLse: last key the row's query sees.  kSums: the key, and the first token that sees it
+    const int tok = tile * tt + row / G.grp;
+    const int last = past + tok;
+    const int key = tile * kTileRows + row;
+    float m = -INFINITY;
+    uint64_t acc[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = f2_pack(0.f, 0.f);
+    const uint64_t scale2 = f2_pack(kScoreScale, kScoreScale);
+    for (int i = 0; i < n; ++i) {
+      const int buf = i & 1, slot = i % kLseSlots;
+      if (s_abort || !mbar_wait(&bar_s_full[w][buf], (i >> 1) & 1, G.err)) {
+        s_abort = 1;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sv[kTileRows];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_base + buf * kTileRows + 32 * c, sv + 32 * c);
+      tc_wait_ld();
+      tc_fence_before();
+      mbar_arrive(&bar_s_empty[w][buf]);
+      if (kPass == kLse) {
+        const int j0 = (t0 + i) * kTileRows;
+        if (j0 + kTileRows - 1 > past + tile * tt) {  // some row does not see all of the tile
+#pragma unroll
+          for (int e = 0; e < kTileRows; ++e)
+            if (j0 + e > last) sv[e] = __float_as_uint(-INFINITY);
+        }
+        float mx[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx[k] = fmaxf(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
+#pragma unroll
+        for (int e = 16; e < kTileRows; e += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mx[k] = fmax3(mx[k], __uint_as_float(sv[e + 2 * k]), __uint_as_float(sv[e + 2 * k + 1]));
+        const float mt = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * kScoreScale;
+        if (mt > m) {
+          const float f = fast_exp2(m - mt);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] = f2_fma(acc[k], f2_pack(f, f), f2_pack(0.f, 0.f));
+          m = mt;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const uint64_t nm2 = f2_pack(nm, nm);
+#pragma unroll
+        for (int e = 0; e < kTileRows; e += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), scale2, nm2), x0, x1);
+          acc[e / 2 & 3] = f2_add(acc[e / 2 & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
+        }
+      } else {
+        if (!mbar_wait(&bar_lse[slot], (i / kLseSlots) & 1, G.err)) {
+          s_abort = 1;
+          break;
+        }
+        const float4* nl = reinterpret_cast<const float4*>(sLse + slot * kTileRows);
+        const int tok0 = (t0 + i) * tt;
+        if (tile * kTileRows + kTileRows - 1 > past + tok0) {  // some key is not seen by the tile's first token
+          const int c_min = min(kTileRows, max(0, key - past - tok0) * G.grp);
+#pragma unroll
+          for (int e = 0; e < kTileRows; ++e)
+            if (e < c_min) sv[e] = __float_as_uint(-INFINITY);
+        }
+#pragma unroll
+        for (int e = 0; e < kTileRows; e += 4) {
+          const float4 v = nl[e / 4];
+          float x0, x1, x2, x3;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), scale2, f2_pack(v.x, v.y)), x0, x1);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), scale2, f2_pack(v.z, v.w)), x2,
+                    x3);
+          acc[e / 2 & 3] = f2_add(acc[e / 2 & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
+          acc[(e / 2 + 1) & 3] = f2_add(acc[(e / 2 + 1) & 3], f2_pack(fast_exp2(x2), fast_exp2(x3)));
+        }
+      }
+    }
+    float u[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f2_unpack(acc[k], u[2 * k], u[2 * k + 1]);
+    const float sum = ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
+    if (kPass == kLse) {
+      const long long at = ((long long)r * t.row_tiles + tile) * kTileRows + row;
+      const bool live = row < q_rows && tok < a.q_len;
+      if (t.splits > 1)
+        t.part[(long long)split * a.units * t.row_tiles * kTileRows + at] = live ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
+      else
+        t.neg_lse[at] = live ? -(m + log2f(sum)) : -INFINITY;
+    } else if (key < len) {
+      if (t.splits > 1) {
+        t.sums[((long long)split * a.units + r) * t.sums_unit + key] = sum;
+      } else {
+        float* o = a.out + r * a.out_stride + key;
+        *o = a.accumulate ? *o + sum : sum;
+      }
+    }
+  }
+
+  // ============================ teardown ============================
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0) mbar_wait(&bar_final, 0, G.err);  // every product has completed
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// -lse of every row from its key ranges.
+__global__ void __launch_bounds__(256) combine_lse_kernel(const float2* part, float* neg_lse, long long rows, int splits) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows) return;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, part[s * rows + i].x);
+  for (int s = 0; s < splits; ++s) {
+    const float2 v = part[s * rows + i];
+    if (v.y > 0.f) l += v.y * fast_exp2(v.x - m);
+  }
+  neg_lse[i] = l > 0.f ? -(m + log2f(l)) : -INFINITY;  // a row that holds no query adds nothing
+}
+
+// The row ranges' sums, in their order.
+__global__ void __launch_bounds__(256) combine_sums_kernel(const __grid_constant__ TcArgs t) {
+  const KeyWeightsArgs& a = t.a;
+  const int j = blockIdx.x * 256 + threadIdx.x, r = blockIdx.y;
+  if (j >= key_weights_past(a) + a.q_len) return;
+  float x = 0.f;
+  for (int s = 0; s < t.splits; ++s) x += t.sums[((long long)s * a.units + r) * t.sums_unit + j];
+  float* o = a.out + r * a.out_stride + j;
+  *o = a.accumulate ? *o + x : x;
+}
+
+int encode_queries(CUtensorMap* map, const KeyWeightsArgs& a, int tile_tokens) {
+  typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr);
+    return e == cudaSuccess && qr == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+  }();
+  if (!fn) return fail(AOH_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  // (B, C, Hq, 128): a box is 64 dimensions of one group's heads of tile_tokens tokens; tokens behind the last read as zeros
+  const cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)a.g.Hq, (cuuint64_t)a.q_len, (cuuint64_t)a.g.B};
+  const cuuint64_t strides[3] = {(cuuint64_t)kHeadDim * 2, (cuuint64_t)a.g.Hq * kHeadDim * 2,
+                                 (cuuint64_t)a.q_len * a.g.Hq * kHeadDim * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)a.g.grp, (cuuint32_t)tile_tokens, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a.q), dims, strides, box, es,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? AOH_OK : fail(AOH_ERR_CUDA, "cuTensorMapEncodeTiled (queries) failed (%d)", (int)r);
+}
+
+int key_pairs(int max_len) { return ((max_len + kTileRows - 1) / kTileRows + 1) / 2; }
+
+}  // namespace
+
+void plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p) {
+  p.kind = KeyWeightsKind::few;
+  const int pages = (max_len + kPage - 1) / kPage;
+  // two CTAs per SM in one wave, at least two pages for each of a CTA's warps
+  p.splits = std::max(1, std::min(2 * std::max(1, c->num_sms) / std::max(1, units), pages / (2 * kFewWarps)));
+  const size_t rows_even = (p.rows + 1) / 2 * 2;
+  p.part = 0;
+  p.score = align256((size_t)p.splits * units * p.rows * sizeof(float2));
+  p.bytes = p.score + (size_t)units * pages * kPage * rows_even * sizeof(float);
+}
+
+int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
+                           cudaStream_t st) {
+  FewArgs f;
+  f.a = a;
+  f.part = reinterpret_cast<float2*>(ws + p.part);
+  f.score = reinterpret_cast<float*>(ws + p.score);
+  f.rows = p.rows;
+  f.rows_even = (p.rows + 1) / 2 * 2;
+  f.splits = p.splits;
+  f.score_unit = (long long)((a.max_len + kPage - 1) / kPage) * kPage * f.rows_even;
+  const dim3 grid(p.splits, a.units);
+  if (p.rows <= 8)
+    few_scores_kernel<1><<<grid, kFewWarps * 32, 0, st>>>(f);
+  else if (p.rows <= 16)
+    few_scores_kernel<2><<<grid, kFewWarps * 32, 0, st>>>(f);
+  else
+    few_scores_kernel<4><<<grid, kFewWarps * 32, 0, st>>>(f);
+  int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.max_len + 255) / 256, a.units);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, few_sum_kernel, f), "aoh_key_weights sums launch");
+}
+
+void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int q_len, KeyWeightsPlan& p) {
+  p.kind = KeyWeightsKind::tensor;
+  const int grp = c->cfg.num_q_heads / c->cfg.num_kv_heads, sms = std::max(1, c->num_sms);
+  p.tile_tokens = std::min(kTileRows / grp, q_len);
+  p.row_tiles = (q_len + p.tile_tokens - 1) / p.tile_tokens;
+  // four CTAs per SM, each with at least four streamed tiles
+  const long long lse_items = (long long)units * ((p.row_tiles + 1) / 2), sum_items = (long long)units * key_pairs(max_len);
+  const int key_tiles = (max_len + kTileRows - 1) / kTileRows;
+  p.splits = (int)std::max(1LL, std::min<long long>((4LL * sms + lse_items - 1) / std::max(1LL, lse_items), key_tiles / 4));
+  p.row_splits = (int)std::max(1LL, std::min<long long>((4LL * sms + sum_items - 1) / std::max(1LL, sum_items), p.row_tiles / 4));
+  const size_t rows = (size_t)units * p.row_tiles * kTileRows;
+  p.lse = 0;
+  p.part = align256(rows * sizeof(float));
+  p.sums = p.part + (p.splits > 1 ? align256(rows * p.splits * sizeof(float2)) : 0);
+  p.bytes = p.sums + (p.row_splits > 1 ? (size_t)p.row_splits * units * max_len * sizeof(float) : 0);
+}
+
+int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
+                              cudaStream_t st) {
+  static PerDeviceOnce once;
+  int rc = once.run(c->device, [] {
+    int e = cuda_check(cudaFuncSetAttribute(tensor_pass_kernel<kLse>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem),
+                       "key weights shared memory");
+    return e ? e : cuda_check(cudaFuncSetAttribute(tensor_pass_kernel<kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kTcSmem),
+                              "key weights shared memory");
+  });
+  if (rc) return rc;
+  CUtensorMap tm;
+  rc = encode_queries(&tm, a, p.tile_tokens);
+  if (rc) return rc;
+  TcArgs t;
+  t.a = a;
+  t.neg_lse = reinterpret_cast<float*>(ws + p.lse);
+  t.part = reinterpret_cast<float2*>(ws + p.part);
+  t.sums = reinterpret_cast<float*>(ws + p.sums);
+  t.row_tiles = p.row_tiles;
+  t.tile_tokens = p.tile_tokens;
+  t.sums_unit = a.max_len;
+  t.pairs = (p.row_tiles + 1) / 2;
+  t.splits = p.splits;
+  const long long g1 = (long long)a.units * t.pairs * p.splits, g2 = (long long)a.units * key_pairs(a.max_len) * p.row_splits;
+  if (g1 > 0x7fffffffLL || g2 > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "aoh_key_weights: too many tiles");
+  tensor_pass_kernel<kLse><<<(unsigned)g1, kTcThreads, kTcSmem, st>>>(tm, t);
+  if (p.splits > 1) {
+    const long long rows = (long long)a.units * p.row_tiles * kTileRows;
+    combine_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(t.part, t.neg_lse, rows, p.splits);
+  }
+  t.pairs = key_pairs(a.max_len);
+  t.splits = p.row_splits;
+  tensor_pass_kernel<kSums><<<(unsigned)g2, kTcThreads, kTcSmem, st>>>(tm, t);
+  if (p.row_splits > 1)
+    combine_sums_kernel<<<dim3((a.max_len + 255) / 256, a.units), 256, 0, st>>>(t);
+  return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+}
+
+}  // namespace aoh
