@@ -10,6 +10,7 @@ state and CUDA errors).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -79,18 +80,20 @@ _SIGNATURES = {
     "aoh_diag_exp2_poly": (C.c_int, [_vp, _vp, _i32, _vp]),
     "aoh_rope_qk": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
                               _vp]),
-    "aoh_rope_axes_qk": (C.c_int, [_vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _i32, _vp, _i32, C.POINTER(_i64), _vp,
-                                   C.POINTER(_i32), _i32, _i32, _vp, _vp, C.c_float, C.c_float, _i32, _i32, _i32, _i32,
-                                   _i32, _vp, _vp, _vp]),
+    "aoh_rope_axes_qk": (C.c_int, [C.c_char_p, _vp]),  # the packed aoh_rope_axes_args
     "aoh_key_weights_workspace_bytes": (C.c_size_t, [_vp, _i32, _i32, _i32]),
     "aoh_key_weights": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _vp, C.c_size_t, _vp]),
     "aoh_select_keys": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "aoh_kv_evict": (C.c_int, [_vp, _vp, _i32, _vp, _i64, _i32, _vp]),
     "aoh_history_add": (C.c_int, [_vp, _vp, _i32, _i32, _vp, _i32, _i64, _i32, _vp, _i32, _vp]),
-    "aoh_logits_penalize": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, C.c_float, _vp, C.c_float, _vp,
-                                      C.c_float, _vp, _vp, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _vp]),
+    "aoh_logits_penalize": (C.c_int, [C.c_char_p, _vp]),  # the packed aoh_logits_args
 }
 IPC_HANDLE_BYTES = 64
+
+# The argument structures of include/aoh.h, packed in one go (converting as many
+# single arguments costs several microseconds a call); 0 stands for NULL.
+pack_rope_axes = struct.Struct("@8Q9q8i9i2fi").pack
+pack_logits = struct.Struct("@12Q2q6i3fi").pack
 
 _lib = None
 _lock = threading.Lock()
@@ -144,10 +147,18 @@ def stream_handle(stream=None) -> int:
 
 
 def launch(device, fn, what: str, *args) -> None:
-    """fn(*args, stream) with ``device`` current and on its current stream."""
+    """fn(*args, stream) with ``device`` (a tensor's) current, on its current stream."""
     import torch
-    if device.index is None or device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+            rc = fn(*args, _raw_stream(device.index))
+    if rc:
+        check(rc, what)
+
+
+def _raw_stream(index: int) -> int:
+    # the handle alone: building a torch.cuda.Stream object for it takes 3 us
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)

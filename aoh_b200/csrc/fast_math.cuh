@@ -61,4 +61,25 @@ __device__ __forceinline__ void exp2_poly2(uint64_t x2, float& p0, float& p1) {
   p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
 }
 
+// exp2_poly2 to fp32 accuracy: a degree-5 polynomial for 2^f, fitted the same
+// way (7.5e-8 exactly, 2.1e-7 with fp32 roundings -- that of ex2.approx).
+__device__ __forceinline__ uint64_t exp2_poly2_f32(uint64_t x2) {
+  float x0, x1;
+  f2_unpack(x2, x0, x1);
+  const uint64_t x = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t magic = f2_pack(12582912.f, 12582912.f);
+  const uint64_t t = f2_add(x, magic);
+  const uint64_t f = f2_sub(x, f2_sub(t, magic));
+  uint64_t p = f2_fma(f, f2_pack(1.32764608e-3f, 1.32764608e-3f), f2_pack(9.67554189e-3f, 9.67554189e-3f));
+  p = f2_fma(p, f, f2_pack(0.0555071346f, 0.0555071346f));
+  p = f2_fma(p, f, f2_pack(0.240221202f, 0.240221202f));
+  p = f2_fma(p, f, f2_pack(0.693146944f, 0.693146944f));
+  p = f2_fma(p, f, f2_pack(1.00000012f, 1.00000012f));
+  float q0, q1, t0, t1;
+  f2_unpack(p, q0, q1);
+  f2_unpack(t, t0, t1);
+  return f2_pack(__int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23)),
+                 __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23)));
+}
+
 }  // namespace aoh

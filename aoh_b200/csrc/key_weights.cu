@@ -25,50 +25,70 @@ constexpr int kTile = 64;                 // query rows and keys of a tile
 constexpr int kStride = kHeadDim + 4;     // floats of a row in shared memory: 16-byte rows on distinct banks
 constexpr int kSmem = 2 * kTile * kStride * 4;
 
+// Four dimensions of a stored row, as loaded and as floats.
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+  float4 v;
+  __device__ float4 get() const { return v; }
+};
+template <>
+struct Raw4<__nv_bfloat16> {
+  uint2 v;
+  __device__ float4 get() const { return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)); }
+};
+
+constexpr int kLoads = kTile * (kHeadDim / 4) / 256;  // of a thread for a tile: row 8 i + warp, dimensions 4 lane ..
+
+// The loads of a tile are all issued before any is stored: a thread's eight
+// would otherwise each wait for memory in turn.
 template <typename T>
 __device__ __forceinline__ void load_queries(const KeyWeightsArgs& a, int b, int g, int row0, int rows, float* sm) {
-  for (int e = threadIdx.x; e < kTile * (kHeadDim / 4); e += 256) {
-    const int r = e / (kHeadDim / 4), c = e % (kHeadDim / 4) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row0 + r < rows) {
-      const int tok = (row0 + r) / a.g.grp, h = g * a.g.grp + (row0 + r) % a.g.grp;
-      const T* p = static_cast<const T*>(a.q) + (((long long)b * a.q_len + tok) * a.g.Hq + h) * kHeadDim + c;
-      if constexpr (sizeof(T) == 4) {
-        v = *reinterpret_cast<const float4*>(p);
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        v = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
-      }
+  const int r0 = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
+  Raw4<T> v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = row0 + r0 + 8 * i;
+    v[i] = Raw4<T>{};
+    if (row < rows) {
+      const int tok = row / a.g.grp, h = g * a.g.grp + row % a.g.grp;
+      v[i] = *reinterpret_cast<const Raw4<T>*>(static_cast<const T*>(a.q) +
+                                               (((long long)b * a.q_len + tok) * a.g.Hq + h) * kHeadDim + c);
     }
-    *reinterpret_cast<float4*>(sm + r * kStride + c) = v;
   }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
 // Keys [j0, j0 + 64) of a unit; rows that are not stored are zero.
 template <typename T>
 __device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int j0, int len, float* sm) {
   const int base = a.g.unit_offset[unit], n_pages = a.g.unit_offset[unit + 1] - base;
-  for (int e = threadIdx.x; e < kTile * (kHeadDim / 4); e += 256) {
-    const int r = e / (kHeadDim / 4), c = e % (kHeadDim / 4) * 4;
-    const int j = j0 + r, slot = j % kPage;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (j < len && j / kPage < n_pages) {
-      const int page = a.g.block_table[base + j / kPage];
-      if (page >= 0 && page < a.g.num_pages) {
-        if constexpr (sizeof(T) == 4) {
-          v = *reinterpret_cast<const float4*>(static_cast<const char*>(a.g.pool) + (long long)page * kPageF32Bytes +
-                                               4 * f32_elem_offset(0, slot, c));
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const char*>(a.g.pool) +
-                                                          (long long)page * kPageBf16Bytes + 2 * bf16_elem_offset(0, slot, c));
-          v = make_float4(bf16_lo(u.x), bf16_hi(u.x), bf16_lo(u.y), bf16_hi(u.y));
-        }
-      } else if (c == 0) {
-        atomicOr(a.g.err, kErrBadPage);
-      }
-    }
-    *reinterpret_cast<float4*>(sm + r * kStride + c) = v;
+  const int r0 = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
+  int pages[kTile / kPage];
+#pragma unroll
+  for (int i = 0; i < kTile / kPage; ++i) {
+    const int p = j0 / kPage + i;
+    pages[i] = p * kPage < len && p < n_pages ? a.g.block_table[base + p] : -1;
+    if (pages[i] >= a.g.num_pages) pages[i] = -1;
+    if (pages[i] < 0 && p * kPage < len && threadIdx.x == 0) atomicOr(a.g.err, kErrBadPage);
   }
+  Raw4<T> v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = r0 + 8 * i, slot = r % kPage;
+    const int page = pages[8 * i / kPage];  // r0 < 8: row r is in page 8 i / 16
+    v[i] = Raw4<T>{};
+    if (page >= 0 && j0 + r < len) {
+      const char* p = static_cast<const char*>(a.g.pool);
+      p += sizeof(T) == 4 ? (long long)page * kPageF32Bytes + 4 * f32_elem_offset(0, slot, c)
+                          : (long long)page * kPageBf16Bytes + 2 * bf16_elem_offset(0, slot, c);
+      v[i] = *reinterpret_cast<const Raw4<T>*>(p);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
 // s[i][j]: row 4 ty + i, key tx + 16 j, in the log2 domain

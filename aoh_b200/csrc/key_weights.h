@@ -35,6 +35,7 @@ struct KeyWeightsPlan {
   int tile_tokens = 0;     // tensor: tokens of a row tile
   int splits = 1;          // key ranges
   int row_splits = 1;      // tensor: row ranges of the sums
+  bool stream = false;     // tensor: the query rows stay resident in the second pass too
   size_t part = 0, score = 0, lse = 0, sums = 0, bytes = 0;
 };
 

@@ -18,8 +18,6 @@
 // maximum and sum; with keys as rows it adds up exp(s - lse) over the columns,
 // so neither pass exchanges anything between threads.  Query rows are packed
 // (token, head) pairs, so a chunk of a few tokens still fills a tile.
-#include <type_traits>
-
 #include "common.cuh"
 #include "fast_math.cuh"
 #include "internal.h"
@@ -175,27 +173,34 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
   }
 }
 
-// Weights of 256 keys from their scores.
+// Weights of 1024 keys from their scores, four keys a thread.
+constexpr int kFewKeys = 4;
 __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
   __shared__ float lse[kFewRows];
   const KeyWeightsArgs& a = f.a;
   const int r = blockIdx.y, unit = a.row_unit[r];
   const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
   const int len = key_weights_past(a) + a.q_len;
-  const int j = blockIdx.x * 256 + threadIdx.x;
+  const int j0 = blockIdx.x * 256 * kFewKeys + threadIdx.x;
   griddep_wait();
-  if (blockIdx.x * 256 >= len) return;
+  if (blockIdx.x * 256 * kFewKeys >= len) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the first two rows' scores are on their way while the ranges are combined
+  const float* s = f.score + r * f.score_unit;
+  float2 v[kFewKeys];
+#pragma unroll
+  for (int k = 0; k < kFewKeys; ++k)
+    v[k] = stored && j0 + 256 * k < len ? *reinterpret_cast<const float2*>(s + (long long)(j0 + 256 * k) * f.rows_even)
+                                        : make_float2(-INFINITY, -INFINITY);
   if (stored) {
     for (int row = warp; row < f.rows; row += 8) {
       float m = -INFINITY, l = 0.f;
+#pragma unroll 4
       for (int i = lane; i < f.splits; i += 32) {
-        const float2 v = f.part[((long long)i * a.units + r) * f.rows + row];
-        if (v.x > m) {
-          l *= fast_exp2(m - v.x);
-          m = v.x;
-        }
-        if (v.y > 0.f) l += v.y * fast_exp2(v.x - m);
+        const float2 p = f.part[((long long)i * a.units + r) * f.rows + row];
+        const float mm = fmaxf(m, p.x);
+        if (mm > -INFINITY) l = l * fast_exp2(m - mm) + p.y * fast_exp2(p.x - mm);
+        m = mm;
       }
       float mm = m;
 #pragma unroll
@@ -207,64 +212,110 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
     }
   }
   __syncthreads();
-  if (j >= len) return;
-  float w = 0.f;
+  float w[kFewKeys] = {0.f, 0.f, 0.f, 0.f};
   if (stored) {
-    const float* s = f.score + r * f.score_unit + (long long)j * f.rows_even;
     for (int row = 0; row < f.rows; row += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(s + row);
-      w += fast_exp2(v.x - lse[row]);
-      if (row + 1 < f.rows) w += fast_exp2(v.y - lse[row + 1]);
+#pragma unroll
+      for (int k = 0; k < kFewKeys; ++k) {
+        if (j0 + 256 * k >= len) continue;
+        if (row > 0) v[k] = *reinterpret_cast<const float2*>(s + (long long)(j0 + 256 * k) * f.rows_even + row);
+        w[k] += fast_exp2(v[k].x - lse[row]);
+        if (row + 1 < f.rows) w[k] += fast_exp2(v[k].y - lse[row + 1]);
+      }
     }
   }
-  float* o = a.out + r * a.out_stride + j;
-  *o = a.accumulate ? *o + w : w;
+#pragma unroll
+  for (int k = 0; k < kFewKeys; ++k) {
+    if (j0 + 256 * k >= len) continue;
+    float* o = a.out + r * a.out_stride + j0 + 256 * k;
+    *o = a.accumulate ? *o + w[k] : w[k];
+  }
 }
 
 // ---------------------------------------------------------------------------
 // tensor cores
 // ---------------------------------------------------------------------------
-constexpr int kTcThreads = 384;  // warp 0 loads, warp 1 issues, warps 4..11: one warpgroup per resident tile
+constexpr int kTcThreads = 640;  // warp 0 loads, warp 1 issues, warps 4..19: a warpgroup per product buffer
 constexpr int kStages = 3;
 constexpr int kTileRows = 128;
 constexpr int kHalfTile = kTileRows * 128;   // 64 dimensions of 128 rows
 constexpr int kTileBytes = 2 * kHalfTile;    // 32 KB
 constexpr int kLseBytes = kTileRows * 4;
-// Slots of the columns' -lse.  A warpgroup hands a product's buffer back before
-// it has read that tile's slot, so the products may be two tiles ahead of it
-// and the loads kStages ahead of those: a slot must outlive kStages + 2 tiles.
+// Slots of the streamed columns' -lse.  A warpgroup hands a product's buffer
+// back before it has read that tile's slot, so the products may be two tiles
+// ahead of it and the loads kStages ahead of those: a slot must outlive
+// kStages + 2 tiles.
 constexpr int kLseSlots = 8;
 static_assert(kLseSlots > kStages + 2, "a slot of -lse would be loaded over while it is read");
 constexpr int kTcSmem = (2 + kStages) * kTileBytes + kLseSlots * kLseBytes + 1024;  // + alignment
 constexpr int kTmemCols = 512;
 
-enum { kLse = 0, kSums = 1 };
+enum { kLse = 0, kSums = 1, kStream = 2 };
 
 struct TcArgs {
   KeyWeightsArgs a;
-  float2* part;    // [split][unit row][row tile * 128 + row]: (m, l), kLse with several key ranges
-  float* neg_lse;  // [unit row][row tile * 128 + row]: -lse, -inf for rows that hold no query
+  float2* part;    // [split][unit row][row tile * 128 + row]: (m, l) by key range (kLse; kStream reads them)
+  float* neg_lse;  // [unit row][row tile * 128 + row]: -lse, -inf for rows that hold no query (kSums)
   float* sums;     // [row split][unit row][key], kSums with several row ranges
   int row_tiles, tile_tokens;
   int pairs;       // pairs of resident tiles of a unit
   int splits;      // ranges of the streamed tiles
+  int lse_splits;  // ranges that part holds
   long long sums_unit;
 };
+
+// Exponentials of 64 scores, added to acc: 2^(s * scale + b), b per column
+// pair.  Three pairs in eight take the FMA pipe; a masked tile's scores (-inf,
+// whose power must be exactly 0) all take the MUFU.
+template <bool kPoly, class B>
+__device__ __forceinline__ void add_exp2(const uint32_t* sv, B&& b, uint64_t (&acc)[4]) {
+  const uint64_t scale2 = f2_pack(kScoreScale, kScoreScale);
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, b(e));
+    if (kPoly && (e & 7) >= 5) {
+      acc[e & 3] = f2_add(acc[e & 3], exp2_poly2_f32(x2));
+    } else {
+      float x0, x1;
+      f2_unpack(x2, x0, x1);
+      acc[e & 3] = f2_add(acc[e & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
+    }
+  }
+}
+
+__device__ __forceinline__ float total(const uint64_t (&acc)[4]) {
+  float u[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f2_unpack(acc[k], u[2 * k], u[2 * k + 1]);
+  return ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
+}
+
+// (m, l) of two disjoint sets of keys as one.
+__device__ __forceinline__ float2 merge_ml(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x);
+  const float la = a.y > 0.f ? a.y * fast_exp2(a.x - m) : 0.f, lb = b.y > 0.f ? b.y * fast_exp2(b.x - m) : 0.f;
+  return make_float2(m, la + lb);
+}
 
 template <int kPass>
 __global__ void __launch_bounds__(kTcThreads, 1)
     tensor_pass_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ TcArgs t) {
+  constexpr bool kKeysStreamed = kPass != kSums;    // otherwise the query rows are
+  constexpr bool kQueriesResident = kPass != kSums;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar_a, bar_final, bar_full[kStages], bar_empty[kStages], bar_s_full[2][2], bar_s_empty[2][2],
-      bar_lse[kLseSlots];
+  __shared__ uint64_t bar_a, bar_final, bar_full[kStages], bar_empty[kStages], bar_s_full[4], bar_s_empty[4],
+      bar_lse[kLseSlots], bar_part_full[2][2], bar_part_empty[2][2];
+  __shared__ float2 s_row[2][kTileRows];    // kLse, kSums: what the second buffer's warpgroups found
+  __shared__ float s_part[2][2][kTileRows];  // kStream: sums of the second tile of query rows, [buffer][slot][key]
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   const KeyWeightsArgs& a = t.a;
   const CacheGeom& G = a.g;
-  uint8_t* sA = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
-  uint8_t* sB = sA + 2 * kTileBytes;
+  uint8_t* sA = smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024;  // resident tiles
+  uint8_t* sB = sA + 2 * kTileBytes;                                     // ring of streamed tiles
   float* sLse = reinterpret_cast<float*>(sB + kStages * kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  if (kPass != kSums || t.splits > 1) griddep_launch_dependents();
 
   // this CTA's resident pair and range of streamed tiles
   const int split = blockIdx.x % t.splits;
@@ -278,33 +329,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int b = (unit - a.unit0) / G.G, kvh = (unit - a.unit0) % G.G;
   const int tt = t.tile_tokens;
   const int key_tiles = (len + kTileRows - 1) / kTileRows;
-  const int resident = kPass == kLse ? t.row_tiles : key_tiles;
-  const int na = min(2, resident - 2 * pair);  // resident tiles (a device length may leave none)
+  const int na = min(2, (kQueriesResident ? t.row_tiles : key_tiles) - 2 * pair);  // a device length may leave none
   if (na <= 0) return;
-  if (held == 0) {  // not stored here: no weight
-    if (kPass == kSums && split == 0 && tid < 256) {
-      const int j = 2 * pair * kTileRows + tid;
-      if (j < len) {
-        float* o = a.out + r * a.out_stride + j;
-        if (t.splits > 1)
-          for (int i = 0; i < t.splits; ++i) t.sums[((long long)i * a.units + r) * t.sums_unit + j] = 0.f;
-        else if (!a.accumulate)
-          *o = 0.f;
-      }
-    }
-    return;
-  }
-  int first, end;  // streamed tiles that any resident row needs
-  if (kPass == kLse) {
-    const int tok_end = min(a.q_len, (2 * pair + na) * tt);
-    first = 0;
-    end = (past + tok_end + kTileRows - 1) / kTileRows;
-  } else {
+  int first = 0, end;  // streamed tiles that any resident row needs
+  if (kPass == kSums) {
     first = max(0, 2 * pair * kTileRows - past) / tt;
     end = t.row_tiles;
+  } else {
+    end = (past + min(a.q_len, (2 * pair + na) * tt) + kTileRows - 1) / kTileRows;
   }
   const int t0 = first + (int)((long long)(end - first) * split / t.splits);
   const int n = first + (int)((long long)(end - first) * (split + 1) / t.splits) - t0;
+  if (held == 0) {  // not stored here: no weight
+    if (kPass == kLse) return;
+    const int lo = kPass == kSums ? 2 * pair * kTileRows : t0 * kTileRows;
+    const int hi = min(len, kPass == kSums ? lo + 2 * kTileRows : (t0 + n) * kTileRows);
+    for (int j = lo + tid; j < hi; j += kTcThreads) {
+      if (kPass == kSums && t.splits > 1)
+        t.sums[((long long)split * a.units + r) * t.sums_unit + j] = 0.f;
+      else if (!a.accumulate)
+        a.out[r * a.out_stride + j] = 0.f;
+    }
+    return;
+  }
 
   if (warp == 1) {
     tmem_alloc(&s_tmem, kTmemCols);
@@ -318,26 +365,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&bar_empty[s], 1);
     }
     for (int s = 0; s < kLseSlots; ++s) mbar_init(&bar_lse[s], 1);
-    for (int w = 0; w < 2; ++w)
-      for (int u = 0; u < 2; ++u) {
-        mbar_init(&bar_s_full[w][u], 1);
-        mbar_init(&bar_s_empty[w][u], 128);
+    for (int u = 0; u < 4; ++u) {
+      mbar_init(&bar_s_full[u], 1);
+      mbar_init(&bar_s_empty[u], 128);
+    }
+    for (int u = 0; u < 2; ++u)
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&bar_part_full[u][k], 128);
+        mbar_init(&bar_part_empty[u][k], 128);
       }
     s_abort = 0;
     fence_mbar_init();
   }
-  // rows of a query tile that no load writes: zero scores, which -lse = -inf turns to nothing
+  // rows of a tile of queries that no load writes: zero scores, which -lse = -inf turns to nothing
   const int q_rows = tt * G.grp;
-  if (kPass == kSums)
-    for (int i = tid; i < kStages * 2 * (kTileRows - q_rows) * 8; i += kTcThreads) {
-      const int row = q_rows + (i / 8) % (kTileRows - q_rows), sh = i / 8 / (kTileRows - q_rows);
-      reinterpret_cast<uint4*>(sB + sh * kHalfTile + row * 128)[i % 8] = make_uint4(0u, 0u, 0u, 0u);
+  if (kPass != kLse) {
+    uint8_t* tiles = kPass == kSums ? sB : sA;
+    const int halves = kPass == kSums ? 2 * kStages : 4, tail = kTileRows - q_rows;
+    for (int i = tid; i < halves * tail * 8; i += kTcThreads) {
+      const int row = q_rows + (i / 8) % tail, h = i / 8 / tail;
+      reinterpret_cast<uint4*>(tiles + h * kHalfTile + row * 128)[i % 8] = make_uint4(0u, 0u, 0u, 0u);
     }
+  }
+  if (kPass == kStream) {
+    // -lse of the resident query rows from their key ranges
+    griddep_wait();
+    const long long rows = (long long)a.units * t.row_tiles * kTileRows;
+    if (tid < na * kTileRows) {
+      const float2* p = t.part + ((long long)r * t.row_tiles + 2 * pair) * kTileRows + tid;
+      float2 ml = make_float2(-INFINITY, 0.f);
+#pragma unroll 8
+      for (int s = 0; s < t.lse_splits; ++s) ml = merge_ml(ml, p[s * rows]);
+      sLse[tid] = ml.y > 0.f ? -(ml.x + log2f(ml.y)) : -INFINITY;
+    }
+  }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  float m = -INFINITY, sum = 0.f;  // of this thread's row, where it has one
 
   if (warp == 0) {
     // ============================ loads ============================
@@ -347,64 +414,58 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // K rows of 128 keys: lane = (page, 64-dim half), 2 KB each
     auto key_id = [&](int tile) {
       const int p = tile * 8 + (lane >> 1);
-      return lane < 16 && p * kPage < len && p < held ? bt[p] : -1;
+      if (lane >= 16 || p * kPage >= len) return -1;
+      const int id = p < held ? bt[p] : -1;
+      if (id >= 0 && id < G.num_pages) return id;
+      atomicOr(G.err, kErrBadPage);
+      return -1;
     };
-    auto load_keys = [&](int tile, int id, uint8_t* dst, uint64_t* bar, bool arrive) {
-      const bool want = lane < 16 && (tile * 8 + (lane >> 1)) * kPage < len;
-      const bool ok = want && id >= 0 && id < G.num_pages;
-      if (want && !ok) atomicOr(G.err, kErrBadPage);
-      const uint32_t okm = __ballot_sync(0xffffffffu, ok);
-      if (arrive && lane == 0) {
-        if (okm)
-          mbar_arrive_expect_tx(bar, __popc(okm) * kBlockBytes);
+    auto copy_keys = [&](int id, uint8_t* dst, uint64_t* bar) {
+      if (id >= 0)
+        bulk_load(dst + (lane & 1) * kHalfTile + (lane >> 1) * kBlockBytes,
+                  pool + (size_t)id * kPageBf16Bytes + (lane & 1) * kHalfBytes, kBlockBytes, bar);
+    };
+    // one arrival for `blocks` copies of 2 KB
+    auto expect_blocks = [&](uint64_t* bar, int blocks) {
+      if (lane == 0) {
+        if (blocks)
+          mbar_arrive_expect_tx(bar, blocks * kBlockBytes);
         else
           mbar_arrive(bar);
       }
       __syncwarp();
-      if (ok)
-        bulk_load(dst + (lane & 1) * kHalfTile + (lane >> 1) * kBlockBytes,
-                  pool + (size_t)id * kPageBf16Bytes + (lane & 1) * kHalfBytes, kBlockBytes, bar);
-      return okm;
     };
     auto load_queries = [&](int tile, uint8_t* dst, uint64_t* bar) {
       tma_load_4d(dst, &tm_q, bar, 0, kvh * G.grp, tile * tt, b);
       tma_load_4d(dst + kHalfTile, &tm_q, bar, 64, kvh * G.grp, tile * tt, b);
     };
-    if (kPass == kLse) {
+    if (kQueriesResident) {
       if (lane == 0) {
         mbar_arrive_expect_tx(&bar_a, na * q_bytes);
         for (int w = 0; w < na; ++w) load_queries(2 * pair + w, sA + w * kTileBytes, &bar_a);
       }
     } else {
-      // both tiles complete one phase: the copies' bytes are counted before any is issued
       const int id0 = key_id(2 * pair), id1 = na > 1 ? key_id(2 * pair + 1) : -1;
-      const uint32_t ok0 = __ballot_sync(0xffffffffu, id0 >= 0 && id0 < G.num_pages);
-      const uint32_t ok1 = __ballot_sync(0xffffffffu, id1 >= 0 && id1 < G.num_pages);
-      if (lane == 0) {
-        const uint32_t bytes = (__popc(ok0) + __popc(ok1)) * kBlockBytes;
-        if (bytes)
-          mbar_arrive_expect_tx(&bar_a, bytes);
-        else
-          mbar_arrive(&bar_a);
-      }
-      __syncwarp();
-      load_keys(2 * pair, id0, sA, &bar_a, false);
-      if (na > 1) load_keys(2 * pair + 1, id1, sA + kTileBytes, &bar_a, false);
+      expect_blocks(&bar_a, __popc(__ballot_sync(0xffffffffu, id0 >= 0)) + __popc(__ballot_sync(0xffffffffu, id1 >= 0)));
+      copy_keys(id0, sA, &bar_a);
+      copy_keys(id1, sA + kTileBytes, &bar_a);
+      griddep_wait();  // the lse that the first pass found
     }
     int issued = 0;
-    int id_next = kPass == kLse && n > 0 ? key_id(t0) : -1;
+    int id_next = kKeysStreamed && n > 0 ? key_id(t0) : -1;
     for (int i = 0; i < n; ++i) {
       const int s = i % kStages;
       const int id = id_next;
-      if (kPass == kLse && i + 1 < n) id_next = key_id(t0 + i + 1);
+      if (kKeysStreamed && i + 1 < n) id_next = key_id(t0 + i + 1);
       if (lane == 0 && i >= kStages && !s_abort) {
         if (!mbar_wait(&bar_empty[s], (i / kStages - 1) & 1, G.err)) s_abort = 1;
       }
       __syncwarp();
       if (s_abort) break;
       uint8_t* dst = sB + s * kTileBytes;
-      if (kPass == kLse) {
-        load_keys(t0 + i, id, dst, &bar_full[s], true);
+      if (kKeysStreamed) {
+        expect_blocks(&bar_full[s], __popc(__ballot_sync(0xffffffffu, id >= 0)));
+        copy_keys(id, dst, &bar_full[s]);
       } else if (lane == 0) {
         const int slot = i % kLseSlots;
         mbar_arrive_expect_tx(&bar_full[s], q_bytes);
@@ -427,135 +488,174 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == 1) {
     // ============================ products ============================
     constexpr uint32_t kIdesc = idesc_bf16(kTileRows, kTileRows, 0, 0);
+    if (kPass == kSums) griddep_wait();  // the bounded waits time this grid, not the one before
     bool ok = mbar_wait_warp(&bar_a, 0, G.err);
-    if (!ok) s_abort = 1;
     tc_fence_after();
     for (int i = 0; i < n && ok && !s_abort; ++i) {
-      const int s = i % kStages, buf = i & 1;
+      const int s = i % kStages;
       if (!(ok = mbar_wait_warp(&bar_full[s], (i / kStages) & 1, G.err))) break;
       for (int w = 0; w < na && ok; ++w) {
-        if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[w][buf], ((i >> 1) - 1) & 1, G.err))) break;
+        const int u = (i & 1) * 2 + w;  // buffer and warpgroup of this product
+        if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[u], ((i >> 1) - 1) & 1, G.err))) break;
         tc_fence_after();
-        const uint32_t a_addr = smem_u32(sA + w * kTileBytes), b_addr = smem_u32(sB + s * kTileBytes);
+        const uint32_t res = smem_u32(sA + w * kTileBytes), str = smem_u32(sB + s * kTileBytes);
+        const uint32_t rows = kPass == kStream ? str : res, cols = kPass == kStream ? res : str;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32;
-          mma_ss(tmem + (w * 2 + buf) * kTileRows, smem_desc_sw128(a_addr + off, 16, 1024),
-                 smem_desc_sw128(b_addr + off, 16, 1024), kIdesc, k > 0 ? 1u : 0u);
+          mma_ss(tmem + u * kTileRows, smem_desc_sw128(rows + off, 16, 1024), smem_desc_sw128(cols + off, 16, 1024), kIdesc,
+                 k > 0 ? 1u : 0u);
         }
-        mma_commit(&bar_s_full[w][buf]);
+        mma_commit(&bar_s_full[u]);
       }
       if (ok) mma_commit(&bar_empty[s]);
     }
     if (!ok) s_abort = 1;
     __syncwarp();
     mma_commit(&bar_final);  // fires once every product issued above has completed
-  } else if (warp >= 4 && (warp - 4) / 4 < na) {
+  } else if (warp >= 4 && ((warp - 4) / 4 & 1) < na) {
     // ============================ exponentials ============================
-    const int w = (warp - 4) / 4, row = 32 * (warp & 3) + lane;
-    const uint32_t s_base = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + w * 2 * kTileRows;
+    const int u = (warp - 4) / 4, w = u & 1, buf = u >> 1;  // every second streamed tile against resident tile w
+    const int row = 32 * (warp & 3) + lane;
+    const uint32_t s_col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + u * kTileRows;
     const int tile = 2 * pair + w;
-    // kLse: last key the row's query sees.  kSums: the key, and the first token that sees it
-    const int tok = tile * tt + row / G.grp;
-    const int last = past + tok;
-    const int key = tile * kTileRows + row;
-    float m = -INFINITY;
+    const int last = past + tile * tt + row / G.grp;  // kLse: last key the row's query sees
+    if (kPass == kSums) griddep_wait();
     uint64_t acc[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] = f2_pack(0.f, 0.f);
-    const uint64_t scale2 = f2_pack(kScoreScale, kScoreScale);
-    for (int i = 0; i < n; ++i) {
-      const int buf = i & 1, slot = i % kLseSlots;
-      if (s_abort || !mbar_wait(&bar_s_full[w][buf], (i >> 1) & 1, G.err)) {
+    for (int k = 0; k < 4; ++k) acc[k] = 0;
+    for (int i = buf; i < n; i += 2) {
+      const int slot = i % kLseSlots;
+      // the tile of keys and the first token of the tile of queries of this product
+      const int key0 = (kKeysStreamed ? t0 + i : tile) * kTileRows, tok0 = (kQueriesResident ? tile : t0 + i) * tt;
+      const bool full = key0 + kTileRows - 1 <= past + tok0;  // every token sees every key
+      if (kPass == kSums && !s_abort && !mbar_wait(&bar_lse[slot], (i / kLseSlots) & 1, G.err)) s_abort = 1;
+      if (s_abort || !mbar_wait(&bar_s_full[u], (i >> 1) & 1, G.err)) {
         s_abort = 1;
         break;
       }
       tc_fence_after();
-      uint32_t sv[kTileRows];
+      // rows = keys: columns from the first token that sees the row's key on
+      const int c_min = kPass == kLse ? 0 : min(kTileRows, max(0, key0 + row - past - tok0) * G.grp);
+      if (kPass == kStream) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_base + buf * kTileRows + 32 * c, sv + 32 * c);
-      tc_wait_ld();
-      tc_fence_before();
-      mbar_arrive(&bar_s_empty[w][buf]);
-      if (kPass == kLse) {
-        const int j0 = (t0 + i) * kTileRows;
-        if (j0 + kTileRows - 1 > past + tile * tt) {  // some row does not see all of the tile
+        for (int k = 0; k < 4; ++k) acc[k] = 0;
+      }
 #pragma unroll
-          for (int e = 0; e < kTileRows; ++e)
-            if (j0 + e > last) sv[e] = __float_as_uint(-INFINITY);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sv[64];
+        tmem_ld32(s_col + 64 * h, sv);
+        tmem_ld32(s_col + 64 * h + 32, sv + 32);
+        tc_wait_ld();
+        if (h == 1) {
+          tc_fence_before();
+          mbar_arrive(&bar_s_empty[u]);
         }
-        float mx[8];
+        if (!full) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx[k] = fmaxf(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
-#pragma unroll
-        for (int e = 16; e < kTileRows; e += 16)
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mx[k] = fmax3(mx[k], __uint_as_float(sv[e + 2 * k]), __uint_as_float(sv[e + 2 * k + 1]));
-        const float mt = fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * kScoreScale;
-        if (mt > m) {
-          const float f = fast_exp2(m - mt);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[k] = f2_fma(acc[k], f2_pack(f, f), f2_pack(0.f, 0.f));
-          m = mt;
+          for (int e = 0; e < 64; ++e) {
+            const int c = 64 * h + e;
+            if (kPass == kLse ? key0 + c > last : c < c_min) sv[e] = __float_as_uint(-INFINITY);
+          }
         }
-        const float nm = m == -INFINITY ? 0.f : -m;
-        const uint64_t nm2 = f2_pack(nm, nm);
+        if (kPass == kLse) {
+          float mx[4];
 #pragma unroll
-        for (int e = 0; e < kTileRows; e += 2) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), scale2, nm2), x0, x1);
-          acc[e / 2 & 3] = f2_add(acc[e / 2 & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
-        }
-      } else {
-        if (!mbar_wait(&bar_lse[slot], (i / kLseSlots) & 1, G.err)) {
-          s_abort = 1;
-          break;
-        }
-        const float4* nl = reinterpret_cast<const float4*>(sLse + slot * kTileRows);
-        const int tok0 = (t0 + i) * tt;
-        if (tile * kTileRows + kTileRows - 1 > past + tok0) {  // some key is not seen by the tile's first token
-          const int c_min = min(kTileRows, max(0, key - past - tok0) * G.grp);
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
 #pragma unroll
-          for (int e = 0; e < kTileRows; ++e)
-            if (e < c_min) sv[e] = __float_as_uint(-INFINITY);
-        }
+          for (int e = 8; e < 64; e += 8)
 #pragma unroll
-        for (int e = 0; e < kTileRows; e += 4) {
-          const float4 v = nl[e / 4];
-          float x0, x1, x2, x3;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), scale2, f2_pack(v.x, v.y)), x0, x1);
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3])), scale2, f2_pack(v.z, v.w)), x2,
-                    x3);
-          acc[e / 2 & 3] = f2_add(acc[e / 2 & 3], f2_pack(fast_exp2(x0), fast_exp2(x1)));
-          acc[(e / 2 + 1) & 3] = f2_add(acc[(e / 2 + 1) & 3], f2_pack(fast_exp2(x2), fast_exp2(x3)));
+            for (int k = 0; k < 4; ++k)
+              mx[k] = fmax3(mx[k], __uint_as_float(sv[e + 2 * k]), __uint_as_float(sv[e + 2 * k + 1]));
+          const float mt = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * kScoreScale;
+          if (mt > m) {
+            const float f = fast_exp2(m - mt);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] = f2_fma(acc[k], f2_pack(f, f), 0);
+            m = mt;
+          }
+          const float nm = m == -INFINITY ? 0.f : -m;
+          const uint64_t nm2 = f2_pack(nm, nm);
+          if (full)
+            add_exp2<true>(sv, [&](int) { return nm2; }, acc);
+          else
+            add_exp2<false>(sv, [&](int) { return nm2; }, acc);
+        } else {
+          const ulonglong2* nl =
+              reinterpret_cast<const ulonglong2*>(sLse + (kPass == kSums ? slot : w) * kTileRows + 64 * h);
+          ulonglong2 v = make_ulonglong2(0, 0);
+          auto column = [&](int e) {
+            if (e % 2 == 0) v = nl[e / 2];
+            return e % 2 == 0 ? v.x : v.y;
+          };
+          if (full)
+            add_exp2<true>(sv, column, acc);
+          else
+            add_exp2<false>(sv, column, acc);
+        }
+      }
+      if (kPass == kStream) {
+        // this buffer's k-th tile; the second tile of query rows hands its sums to the first's warpgroup
+        sum = total(acc);
+        const int k = i >> 1, key = key0 + row;
+        uint64_t *filled = &bar_part_full[buf][k & 1], *read = &bar_part_empty[buf][k & 1];
+        if (w == 1) {
+          if (k >= 2 && !mbar_wait(read, (k >> 1 & 1) ^ 1, G.err)) {
+            s_abort = 1;
+            break;
+          }
+          s_part[buf][k & 1][row] = sum;
+          mbar_arrive(filled);
+        } else {
+          if (na > 1) {
+            if (!mbar_wait(filled, k >> 1 & 1, G.err)) {
+              s_abort = 1;
+              break;
+            }
+            sum += s_part[buf][k & 1][row];
+            mbar_arrive(read);
+          }
+          if (key < len) {
+            float* o = a.out + r * a.out_stride + key;
+            *o = a.accumulate ? *o + sum : sum;
+          }
         }
       }
     }
-    float u[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f2_unpack(acc[k], u[2 * k], u[2 * k + 1]);
-    const float sum = ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
-    if (kPass == kLse) {
-      const long long at = ((long long)r * t.row_tiles + tile) * kTileRows + row;
-      const bool live = row < q_rows && tok < a.q_len;
-      if (t.splits > 1)
-        t.part[(long long)split * a.units * t.row_tiles * kTileRows + at] = live ? make_float2(m, sum) : make_float2(-INFINITY, 0.f);
-      else
-        t.neg_lse[at] = live ? -(m + log2f(sum)) : -INFINITY;
-    } else if (key < len) {
-      if (t.splits > 1) {
-        t.sums[((long long)split * a.units + r) * t.sums_unit + key] = sum;
-      } else {
-        float* o = a.out + r * a.out_stride + key;
-        *o = a.accumulate ? *o + sum : sum;
-      }
+    if (kPass != kStream) {
+      sum = total(acc);
+      if (buf == 1) s_row[w][row] = make_float2(m, sum);
     }
   }
 
   // ============================ teardown ============================
   tc_fence_before();
   __syncthreads();
+  if (kPass != kStream && warp >= 4 && warp < 12 && (warp - 4) / 4 < na) {
+    // the first buffer's warpgroups add what the second's found
+    const int w = (warp - 4) / 4, row = 32 * (warp & 3) + lane, tile = 2 * pair + w;
+    const float2 other = s_row[w][row];
+    if (kPass == kLse) {
+      const float2 ml = merge_ml(make_float2(m, sum), other);
+      const long long at = ((long long)r * t.row_tiles + tile) * kTileRows + row;
+      const bool live = row < q_rows && tile * tt + row / G.grp < a.q_len;
+      if (t.part)
+        t.part[(long long)split * a.units * t.row_tiles * kTileRows + at] = live ? ml : make_float2(-INFINITY, 0.f);
+      else
+        t.neg_lse[at] = live ? -(ml.x + log2f(ml.y)) : -INFINITY;
+    } else {
+      const int key = tile * kTileRows + row;
+      const float x = sum + other.y;
+      if (key < len) {
+        if (t.splits > 1) {
+          t.sums[((long long)split * a.units + r) * t.sums_unit + key] = x;
+        } else {
+          float* o = a.out + r * a.out_stride + key;
+          *o = a.accumulate ? *o + x : x;
+        }
+      }
+    }
+  }
   if (warp == 1) {
     if (lane == 0) mbar_wait(&bar_final, 0, G.err);  // every product has completed
     __syncwarp();
@@ -564,23 +664,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-// -lse of every row from its key ranges.
+// -lse of every row from its key ranges: a CTA takes 32 rows, eight threads each.
 __global__ void __launch_bounds__(256) combine_lse_kernel(const float2* part, float* neg_lse, long long rows, int splits) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows) return;
-  float m = -INFINITY, l = 0.f;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, part[s * rows + i].x);
-  for (int s = 0; s < splits; ++s) {
-    const float2 v = part[s * rows + i];
-    if (v.y > 0.f) l += v.y * fast_exp2(v.x - m);
+  __shared__ float2 s_ml[8][32];
+  const int row = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const long long i = (long long)blockIdx.x * 32 + row;  // rows is a multiple of 128
+  griddep_wait();
+  float2 ml = make_float2(-INFINITY, 0.f);
+  for (int s = sub; s < splits; s += 8) ml = merge_ml(ml, part[s * rows + i]);
+  s_ml[sub][row] = ml;
+  __syncthreads();
+  if (sub == 0) {
+    for (int k = 1; k < 8; ++k) ml = merge_ml(ml, s_ml[k][row]);
+    neg_lse[i] = ml.y > 0.f ? -(ml.x + log2f(ml.y)) : -INFINITY;  // a row that holds no query adds nothing
   }
-  neg_lse[i] = l > 0.f ? -(m + log2f(l)) : -INFINITY;  // a row that holds no query adds nothing
 }
 
 // The row ranges' sums, in their order.
 __global__ void __launch_bounds__(256) combine_sums_kernel(const __grid_constant__ TcArgs t) {
   const KeyWeightsArgs& a = t.a;
   const int j = blockIdx.x * 256 + threadIdx.x, r = blockIdx.y;
+  griddep_wait();
   if (j >= key_weights_past(a) + a.q_len) return;
   float x = 0.f;
   for (int s = 0; s < t.splits; ++s) x += t.sums[((long long)s * a.units + r) * t.sums_unit + j];
@@ -613,6 +717,42 @@ int encode_queries(CUtensorMap* map, const KeyWeightsArgs& a, int tile_tokens) {
 
 int key_pairs(int max_len) { return ((max_len + kTileRows - 1) / kTileRows + 1) / 2; }
 
+// Launch that may start while the kernel before it finishes (it waits for that kernel itself).
+template <class F, class... A>
+int launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
+// Ranges that `items` CTAs' lists of `tiles` tiles are cut into, one CTA per
+// SM: the fewest tile periods, a range costing its tiles and about four for a
+// CTA's start and end.  Candidates: a few ranges, and what fills 1 to 4 waves.
+int plan_ranges(long long items, int tiles, int sms) {
+  int best = 1;
+  double least = 1e300;
+  for (int k = 1; k <= 12; ++k) {
+    const long long s = k <= 8 ? k : (k - 8) * (long long)sms / items;
+    if (s < 1 || s > std::min(tiles, 256)) continue;
+    const double ctas = (double)items * s / sms;
+    // several waves overlap at their ends: half a range is lost, not a whole one
+    const double cost = (ctas > 1 ? ctas + 0.5 : 1.0) * ((tiles + s - 1) / s + 4);
+    if (cost < least * 0.98) {
+      best = (int)s;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 void plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p) {
@@ -643,18 +783,10 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
     few_scores_kernel<2><<<grid, kFewWarps * 32, 0, st>>>(f);
   else
     few_scores_kernel<4><<<grid, kFewWarps * 32, 0, st>>>(f);
-  int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
-  if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.max_len + 255) / 256, a.units);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, few_sum_kernel, f), "aoh_key_weights sums launch");
+  const int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
+  return rc ? rc
+            : launch_dependent(few_sum_kernel, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 256, 0, st,
+                               "aoh_key_weights sums launch", f);
 }
 
 void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int q_len, KeyWeightsPlan& p) {
@@ -662,27 +794,31 @@ void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int 
   const int grp = c->cfg.num_q_heads / c->cfg.num_kv_heads, sms = std::max(1, c->num_sms);
   p.tile_tokens = std::min(kTileRows / grp, q_len);
   p.row_tiles = (q_len + p.tile_tokens - 1) / p.tile_tokens;
-  // four CTAs per SM, each with at least four streamed tiles
   const long long lse_items = (long long)units * ((p.row_tiles + 1) / 2), sum_items = (long long)units * key_pairs(max_len);
-  const int key_tiles = (max_len + kTileRows - 1) / kTileRows;
-  p.splits = (int)std::max(1LL, std::min<long long>((4LL * sms + lse_items - 1) / std::max(1LL, lse_items), key_tiles / 4));
-  p.row_splits = (int)std::max(1LL, std::min<long long>((4LL * sms + sum_items - 1) / std::max(1LL, sum_items), p.row_tiles / 4));
+  p.splits = plan_ranges(lse_items, (max_len + kTileRows - 1) / kTileRows, sms);
+  // up to two tiles of query rows stay resident in the second pass too, which then needs the ranges alone
+  p.stream = p.row_tiles <= 2;
+  p.row_splits = p.stream ? p.splits : plan_ranges(sum_items, p.row_tiles, sms);
   const size_t rows = (size_t)units * p.row_tiles * kTileRows;
-  p.lse = 0;
-  p.part = align256(rows * sizeof(float));
-  p.sums = p.part + (p.splits > 1 ? align256(rows * p.splits * sizeof(float2)) : 0);
-  p.bytes = p.sums + (p.row_splits > 1 ? (size_t)p.row_splits * units * max_len * sizeof(float) : 0);
+  p.part = 0;
+  p.lse = p.stream || p.splits > 1 ? align256(rows * p.splits * sizeof(float2)) : 0;
+  p.sums = p.lse + (p.stream ? 0 : align256(rows * sizeof(float)));
+  p.bytes = p.sums + (!p.stream && p.row_splits > 1 ? (size_t)p.row_splits * units * max_len * sizeof(float) : 0);
 }
 
 int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
                               cudaStream_t st) {
   static PerDeviceOnce once;
   int rc = once.run(c->device, [] {
-    int e = cuda_check(cudaFuncSetAttribute(tensor_pass_kernel<kLse>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem),
+    const void* kernels[3] = {reinterpret_cast<const void*>(tensor_pass_kernel<kLse>),
+                              reinterpret_cast<const void*>(tensor_pass_kernel<kSums>),
+                              reinterpret_cast<const void*>(tensor_pass_kernel<kStream>)};
+    int e = AOH_OK;
+    for (const void* k : kernels)
+      if (e == AOH_OK)
+        e = cuda_check(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem),
                        "key weights shared memory");
-    return e ? e : cuda_check(cudaFuncSetAttribute(tensor_pass_kernel<kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kTcSmem),
-                              "key weights shared memory");
+    return e;
   });
   if (rc) return rc;
   CUtensorMap tm;
@@ -690,27 +826,36 @@ int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, co
   if (rc) return rc;
   TcArgs t;
   t.a = a;
+  t.part = p.stream || p.splits > 1 ? reinterpret_cast<float2*>(ws + p.part) : nullptr;
   t.neg_lse = reinterpret_cast<float*>(ws + p.lse);
-  t.part = reinterpret_cast<float2*>(ws + p.part);
   t.sums = reinterpret_cast<float*>(ws + p.sums);
   t.row_tiles = p.row_tiles;
   t.tile_tokens = p.tile_tokens;
   t.sums_unit = a.max_len;
   t.pairs = (p.row_tiles + 1) / 2;
-  t.splits = p.splits;
-  const long long g1 = (long long)a.units * t.pairs * p.splits, g2 = (long long)a.units * key_pairs(a.max_len) * p.row_splits;
+  t.splits = t.lse_splits = p.splits;
+  const long long g1 = (long long)a.units * t.pairs * p.splits;
+  const long long g2 = p.stream ? g1 : (long long)a.units * key_pairs(a.max_len) * p.row_splits;
   if (g1 > 0x7fffffffLL || g2 > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "aoh_key_weights: too many tiles");
   tensor_pass_kernel<kLse><<<(unsigned)g1, kTcThreads, kTcSmem, st>>>(tm, t);
+  rc = cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+  if (rc) return rc;
+  if (p.stream)
+    return launch_dependent(tensor_pass_kernel<kStream>, dim3((unsigned)g2), kTcThreads, kTcSmem, st,
+                            "aoh_key_weights sums launch", tm, t);
   if (p.splits > 1) {
     const long long rows = (long long)a.units * p.row_tiles * kTileRows;
-    combine_lse_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(t.part, t.neg_lse, rows, p.splits);
+    rc = launch_dependent(combine_lse_kernel, dim3((unsigned)(rows / 32)), 256, 0, st, "aoh_key_weights combine launch",
+                          (const float2*)t.part, t.neg_lse, rows, p.splits);
+    if (rc) return rc;
   }
   t.pairs = key_pairs(a.max_len);
   t.splits = p.row_splits;
-  tensor_pass_kernel<kSums><<<(unsigned)g2, kTcThreads, kTcSmem, st>>>(tm, t);
-  if (p.row_splits > 1)
-    combine_sums_kernel<<<dim3((a.max_len + 255) / 256, a.units), 256, 0, st>>>(t);
-  return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+  rc = launch_dependent(tensor_pass_kernel<kSums>, dim3((unsigned)g2), kTcThreads, kTcSmem, st,
+                        "aoh_key_weights sums launch", tm, t);
+  if (rc || p.row_splits == 1) return rc;
+  return launch_dependent(combine_sums_kernel, dim3((a.max_len + 255) / 256, a.units), 256, 0, st,
+                          "aoh_key_weights combine launch", t);
 }
 
 }  // namespace aoh

@@ -257,59 +257,56 @@ int launch(const LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
 
 using namespace aoh;
 
-extern "C" int aoh_logits_penalize(const void* logits, int64_t row_stride, int32_t dtype, int32_t rows, int32_t vocab,
-                                   const int32_t* counts, const int32_t* seen, const float* repetition,
-                                   float repetition_scalar, const float* presence, float presence_scalar,
-                                   const float* frequency, float frequency_scalar, const int32_t* bias_ids,
-                                   const float* bias, int32_t n_bias, const int32_t* allowed,
-                                   const int32_t* allowed_rows, int32_t n_allowed, void* out, int64_t out_stride,
-                                   int32_t out_dtype, int64_t* greedy, aoh_stream stream) {
+extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream stream) {
   const char* who = "aoh_logits_penalize";
-  if (rows < 0 || vocab < 1 || n_bias < 0 || n_allowed < 0) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
-  if (!logits || !out) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
-  if ((dtype != AOH_BF16 && dtype != AOH_F32) || (out_dtype != AOH_BF16 && out_dtype != AOH_F32))
+  if (!args) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null argument", who);
+  const aoh_logits_args& p = *args;
+  if (p.rows < 0 || p.vocab < 1 || p.n_bias < 0 || p.n_allowed < 0)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
+  if (p.rows > 0 && (!p.logits || !p.out)) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
+  if ((p.dtype != AOH_BF16 && p.dtype != AOH_F32) || (p.out_dtype != AOH_BF16 && p.out_dtype != AOH_F32))
     return fail(AOH_ERR_UNSUPPORTED, "%s: bad dtype", who);
-  if ((counts == nullptr) != (seen == nullptr))
+  if ((p.counts == nullptr) != (p.seen == nullptr))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: a history is counts and their bitmap", who);
-  if (n_bias > 0 && (!bias_ids || !bias)) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null biases", who);
-  if (allowed && !allowed_rows && n_allowed < rows)
-    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: %d mask rows for %d rows", who, n_allowed, rows);
-  if (logits == out && (dtype != out_dtype || (rows > 1 && row_stride != out_stride)))
+  if (p.n_bias > 0 && (!p.bias_ids || !p.bias)) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null biases", who);
+  if (p.allowed && !p.allowed_rows && p.n_allowed < p.rows)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: %d mask rows for %d rows", who, p.n_allowed, p.rows);
+  if (p.logits == p.out && (p.dtype != p.out_dtype || (p.rows > 1 && p.row_stride != p.out_stride)))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: in place needs the same type and strides", who);
-  if (vocab > (1 << 23)) return fail(AOH_ERR_UNSUPPORTED, "%s: vocabulary of %d", who, vocab);
-  if (rows > (1 << 27)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
-  if (rows == 0) return AOH_OK;
+  if (p.vocab > (1 << 23)) return fail(AOH_ERR_UNSUPPORTED, "%s: vocabulary of %d", who, p.vocab);
+  if (p.rows > (1 << 27)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
+  if (p.rows == 0) return AOH_OK;
   LogitsArgs a{};
-  a.logits = logits;
-  a.row_stride = row_stride;
-  a.vocab = vocab;
-  a.slice = ((vocab + kCluster - 1) / kCluster + 255) / 256 * 256;
-  a.counts = reinterpret_cast<const uint32_t*>(counts);
-  a.seen = reinterpret_cast<const uint32_t*>(seen);
-  a.repetition = repetition;
-  a.presence = presence;
-  a.frequency = frequency;
-  a.repetition_s = repetition_scalar;
-  a.presence_s = presence_scalar;
-  a.frequency_s = frequency_scalar;
-  a.bias_ids = bias_ids;
-  a.bias = bias;
-  a.n_bias = n_bias;
-  a.allowed = reinterpret_cast<const uint32_t*>(allowed);
-  a.allowed_rows = allowed_rows;
-  a.n_allowed = n_allowed;
-  a.out = out;
-  a.out_stride = out_stride;
-  a.greedy = reinterpret_cast<long long*>(greedy);
-  const int vin = dtype == AOH_BF16 ? 8 : 4, vout = out_dtype == AOH_BF16 ? 8 : 4;
-  const bool wide = vocab % 8 == 0 && (rows == 1 || (row_stride % vin == 0 && out_stride % vout == 0)) &&
-                    reinterpret_cast<uintptr_t>(logits) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  a.logits = p.logits;
+  a.row_stride = p.row_stride;
+  a.vocab = p.vocab;
+  a.slice = ((p.vocab + kCluster - 1) / kCluster + 255) / 256 * 256;
+  a.counts = reinterpret_cast<const uint32_t*>(p.counts);
+  a.seen = reinterpret_cast<const uint32_t*>(p.seen);
+  a.repetition = p.repetition;
+  a.presence = p.presence;
+  a.frequency = p.frequency;
+  a.repetition_s = p.repetition_scalar;
+  a.presence_s = p.presence_scalar;
+  a.frequency_s = p.frequency_scalar;
+  a.bias_ids = p.bias_ids;
+  a.bias = p.bias;
+  a.n_bias = p.n_bias;
+  a.allowed = reinterpret_cast<const uint32_t*>(p.allowed);
+  a.allowed_rows = p.allowed_rows;
+  a.n_allowed = p.n_allowed;
+  a.out = p.out;
+  a.out_stride = p.out_stride;
+  a.greedy = reinterpret_cast<long long*>(p.greedy);
+  const int vin = p.dtype == AOH_BF16 ? 8 : 4, vout = p.out_dtype == AOH_BF16 ? 8 : 4;
+  const bool wide = p.vocab % 8 == 0 && (p.rows == 1 || (p.row_stride % vin == 0 && p.out_stride % vout == 0)) &&
+                    reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == AOH_BF16)
-    return out_dtype == AOH_BF16 ? launch<__nv_bfloat16, __nv_bfloat16>(a, rows, wide, st)
-                                 : launch<__nv_bfloat16, float>(a, rows, wide, st);
-  return out_dtype == AOH_BF16 ? launch<float, __nv_bfloat16>(a, rows, wide, st)
-                               : launch<float, float>(a, rows, wide, st);
+  if (p.dtype == AOH_BF16)
+    return p.out_dtype == AOH_BF16 ? launch<__nv_bfloat16, __nv_bfloat16>(a, p.rows, wide, st)
+                                   : launch<__nv_bfloat16, float>(a, p.rows, wide, st);
+  return p.out_dtype == AOH_BF16 ? launch<float, __nv_bfloat16>(a, p.rows, wide, st)
+                                 : launch<float, float>(a, p.rows, wide, st);
 }
 
 extern "C" int aoh_history_add(int32_t* counts, int32_t* seen, int32_t rows, int32_t vocab, const void* ids,

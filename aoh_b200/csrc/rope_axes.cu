@@ -28,7 +28,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;  // rotary_dim <= head_dim <= 256
-constexpr int kMaxAxes = 8;
 constexpr int kMaxTokens = 4;  // tokens of one CTA
 
 struct RopeAxesArgs {
@@ -254,36 +253,33 @@ int launch(RopeAxesArgs& a, int num_sms, cudaStream_t st) {
 
 using namespace aoh;
 
-extern "C" int aoh_rope_axes_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                                int32_t dtype, const void* positions, int32_t positions_64,
-                                const int64_t* position_strides, const float* inv_freq, const int32_t* sections,
-                                int32_t n_axes, int32_t interleaved, const void* q_norm_weight,
-                                const void* k_norm_weight, float eps, float scaling, int32_t batch, int32_t q_len,
-                                int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, void* q_out, void* k_out,
-                                aoh_stream stream) {
+extern "C" int aoh_rope_axes_qk(const aoh_rope_axes_args* args, aoh_stream stream) {
   const char* who = "aoh_rope_axes_qk";
-  if (!q || !k || !q_strides || !k_strides || !positions || !position_strides || !inv_freq || !sections || !q_out ||
-      !k_out)
-    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null argument", who);
-  if (dtype != AOH_BF16 && dtype != AOH_F32) return fail(AOH_ERR_UNSUPPORTED, "%s: bad dtype %d", who, dtype);
-  if (batch < 0 || q_len < 0 || num_q_heads <= 0 || num_kv_heads <= 0)
+  if (!args) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null argument", who);
+  const aoh_rope_axes_args& p = *args;
+  if (!p.q || !p.k || !p.positions || !p.inv_freq || !p.q_out || !p.k_out)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: null tensor", who);
+  if (p.dtype != AOH_BF16 && p.dtype != AOH_F32) return fail(AOH_ERR_UNSUPPORTED, "%s: bad dtype %d", who, p.dtype);
+  if (p.batch < 0 || p.q_len < 0 || p.num_q_heads <= 0 || p.num_kv_heads <= 0)
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: bad sizes", who);
-  if (head_dim <= 0 || head_dim > 2 * kMaxHalf || head_dim % 2)
-    return fail(AOH_ERR_UNSUPPORTED, "%s: head_dim must be even and at most %d (got %d)", who, 2 * kMaxHalf, head_dim);
-  if (n_axes < 1 || n_axes > kMaxAxes)
-    return fail(AOH_ERR_UNSUPPORTED, "%s: 1 to %d position axes (got %d)", who, kMaxAxes, n_axes);
-  if ((q_norm_weight == nullptr) != (k_norm_weight == nullptr))
+  if (p.head_dim <= 0 || p.head_dim > 2 * kMaxHalf || p.head_dim % 2)
+    return fail(AOH_ERR_UNSUPPORTED, "%s: head_dim must be even and at most %d (got %d)", who, 2 * kMaxHalf, p.head_dim);
+  if (p.n_axes < 1 || p.n_axes > AOH_ROPE_MAX_AXES)
+    return fail(AOH_ERR_UNSUPPORTED, "%s: 1 to %d position axes (got %d)", who, AOH_ROPE_MAX_AXES, p.n_axes);
+  if ((p.q_norm_weight == nullptr) != (p.k_norm_weight == nullptr))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: give both norm weights or neither", who);
-  if (q == q_out || k == k_out) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: outputs must not alias inputs", who);
+  if (p.q == p.q_out || p.k == p.k_out) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: outputs must not alias inputs", who);
+  const int n_axes = p.n_axes;
+  const int32_t* sections = p.sections;
   long long half = 0;
   for (int i = 0; i < n_axes; ++i) {
     if (sections[i] < 0) return fail(AOH_ERR_INVALID_ARGUMENT, "%s: negative section", who);
     half += sections[i];
   }
-  if (half < 1 || 2 * half > head_dim)
-    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the sections sum to %lld, not to 1..%d", who, half, head_dim / 2);
+  if (half < 1 || 2 * half > p.head_dim)
+    return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the sections sum to %lld, not to 1..%d", who, half, p.head_dim / 2);
   RopeAxesArgs a{};
-  if (interleaved) {
+  if (p.interleaved) {
     for (int i = 0; i < half; ++i) {
       const int ax = i % n_axes;
       a.axis[i] = (uint8_t)(i < n_axes * (long long)sections[ax] ? ax : 0);
@@ -296,42 +292,42 @@ extern "C" int aoh_rope_axes_qk(const void* q, const int64_t* q_strides, const v
     for (int ax = 0; ax < n_axes; ++ax)
       for (int j = 0; j < sections[ax]; ++j) a.axis[i++] = (uint8_t)ax;
   }
-  a.n_tokens = (long long)batch * q_len;
+  a.n_tokens = (long long)p.batch * p.q_len;
   if (a.n_tokens == 0) return AOH_OK;
   int dev = 0, sms = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
   rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
   if (rc) return rc;
-  a.q = q;
-  a.k = k;
-  a.qw = q_norm_weight;
-  a.kw = k_norm_weight;
-  a.q_out = q_out;
-  a.k_out = k_out;
-  a.pos = positions;
-  a.pos64 = positions_64 != 0;
-  a.inv_freq = inv_freq;
+  a.q = p.q;
+  a.k = p.k;
+  a.qw = p.q_norm_weight;
+  a.kw = p.k_norm_weight;
+  a.q_out = p.q_out;
+  a.k_out = p.k_out;
+  a.pos = p.positions;
+  a.pos64 = p.positions_64 != 0;
+  a.inv_freq = p.inv_freq;
   for (int i = 0; i < 3; ++i) {
-    a.qs[i] = q_strides[i];
-    a.ks[i] = k_strides[i];
-    a.ps[i] = position_strides[i];
+    a.qs[i] = p.q_strides[i];
+    a.ks[i] = p.k_strides[i];
+    a.ps[i] = p.position_strides[i];
   }
-  a.q_len = q_len;
-  a.hq = num_q_heads;
-  a.g = num_kv_heads;
-  a.d = head_dim;
+  a.q_len = p.q_len;
+  a.hq = p.num_q_heads;
+  a.g = p.num_kv_heads;
+  a.d = p.head_dim;
   a.half = (int)half;
-  a.eps = eps;
-  a.scaling = scaling;
+  a.eps = p.eps;
+  a.scaling = p.scaling;
   // 16-byte accesses where every row, both halves and the weights allow them
-  const int es = dtype == AOH_BF16 ? 2 : 4, vec = 16 / es;
-  bool wide = half % vec == 0 && head_dim % vec == 0;
-  const void* ptrs[6] = {q, k, q_norm_weight, k_norm_weight, q_out, k_out};
-  for (const void* p : ptrs) wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  for (int i = 0; i < 3; ++i) wide = wide && q_strides[i] % vec == 0 && k_strides[i] % vec == 0;
+  const int es = p.dtype == AOH_BF16 ? 2 : 4, vec = 16 / es;
+  bool wide = half % vec == 0 && p.head_dim % vec == 0;
+  const void* ptrs[6] = {p.q, p.k, p.q_norm_weight, p.k_norm_weight, p.q_out, p.k_out};
+  for (const void* x : ptrs) wide = wide && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int i = 0; i < 3; ++i) wide = wide && p.q_strides[i] % vec == 0 && p.k_strides[i] % vec == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == AOH_BF16)
+  if (p.dtype == AOH_BF16)
     return wide ? launch<__nv_bfloat16, 8>(a, sms, st) : launch<__nv_bfloat16, 1>(a, sms, st);
   return wide ? launch<float, 4>(a, sms, st) : launch<float, 1>(a, sms, st);
 }

@@ -61,7 +61,7 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs an out to add to")
-        out = torch.empty((B, R, total), dtype=torch.float32, device=cache.device)
+        out = q.new_empty((B, R, total), dtype=torch.float32)
     elif (out.dim() != 3 or out.shape[0] != B or out.shape[1] != R or out.shape[2] < total
           or out.dtype != torch.float32 or out.device != cache.device):
         raise ValueError(f"out must be float32 (batch, n_ret, >= keys) = {(B, R, total)} on {cache.device}, "
@@ -74,9 +74,8 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
     if out.stride(2) != 1 or stride < total or (B > 1 and out.stride(0) != R * stride):
         raise ValueError("out's rows must be contiguous and evenly spaced over (batch, n_ret)")
     L = cache._L
-    ws = torch.empty(int(L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n)), dtype=torch.uint8,
-                     device=cache.device)
-    _lib.launch(cache.device, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
+    ws = q.new_empty(L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n), dtype=torch.uint8)
+    _lib.launch(q.device, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
                 out.data_ptr(), stride, bool(accumulate), ws.data_ptr(), ws.numel())
     return out
 
@@ -99,8 +98,8 @@ def select_keys(weights: torch.Tensor, keep: int, *, sink: int = 0, recent: int 
         raise ValueError(f"sink {sink} and recent {recent} must be non-negative and fit keep {keep}")
     lead = weights.shape[:-1]
     rows = lead.numel()
-    kept = torch.empty((*lead, keep), dtype=torch.int32, device=weights.device)
-    kept_w = torch.empty((*lead, keep), dtype=torch.float32, device=weights.device)
+    kept = weights.new_empty((*lead, keep), dtype=torch.int32)
+    kept_w = weights.new_empty((*lead, keep))
     if rows == 0 or keep == 0:
         return kept, kept_w
     w = weights.reshape(rows, n)  # a view, or a copy where the rows are not evenly spaced
@@ -138,7 +137,7 @@ def evict(cache: AoHKVCache, kept: torch.Tensor, into: AoHKVCache) -> AoHKVCache
     if keep > into.max_context:
         raise ValueError(f"keep {keep} exceeds the destination's max_context {into.max_context}")
     into.reserve(keep)
-    _lib.launch(cache.device, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, cache.kv_seq_len,
+    _lib.launch(kept.device, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, cache.kv_seq_len,
                 kept.data_ptr(), kept.stride(0), keep)
     into.kv_seq_len = keep
     into.evicted = cache.tokens_seen - keep

@@ -57,15 +57,19 @@ class TokenHistory:
                     ids.shape[1], None if lengths is None else lengths.data_ptr(), prompt)
 
 
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _per_row(x, name: str, rows: int, device, neutral: float):
-    """(pointer or None, scalar) of a penalty given as a float, a (rows,) tensor or None."""
+    """(pointer or 0, scalar) of a penalty given as a number, a (rows,) tensor or None."""
     if x is None:
-        return None, neutral
+        return 0, neutral
     if isinstance(x, torch.Tensor):
-        if x.dtype != torch.float32 or tuple(x.shape) != (rows,) or x.device != device or not x.is_contiguous():
+        if x.dtype != torch.float32 or x.shape != (rows,) or x.device != device or not x.is_contiguous():
             raise ValueError(f"{name} must be a number or a contiguous float32 tensor ({rows},) on {device}")
         return x.data_ptr(), neutral
-    return None, float(x)
+    return 0, float(x)
 
 
 def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *, repetition=None, presence=None,
@@ -109,8 +113,8 @@ def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *
     if bias is not None:
         ids, values = bias
         K = ids.shape[1] if ids.dim() == 2 else -1
-        if ids.dtype != torch.int32 or values.dtype != torch.float32 or tuple(ids.shape) != (N, K) \
-                or tuple(values.shape) != (N, K) or ids.device != dev or values.device != dev \
+        if ids.dtype != torch.int32 or values.dtype != torch.float32 or ids.shape != (N, K) \
+                or values.shape != (N, K) or ids.device != dev or values.device != dev \
                 or not ids.is_contiguous() or not values.is_contiguous():
             raise ValueError(f"bias must be contiguous int32 ids and float32 values of one shape ({N}, K) on {dev}")
     M = 0
@@ -122,22 +126,20 @@ def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *
         if allowed_rows is None and M != N:
             raise ValueError(f"{M} mask rows for {N} rows of logits need allowed_rows")
     if allowed_rows is not None and (allowed is None or allowed_rows.dtype != torch.int32
-                                     or tuple(allowed_rows.shape) != (N,) or allowed_rows.device != dev
+                                     or allowed_rows.shape != (N,) or allowed_rows.device != dev
                                      or not allowed_rows.is_contiguous()):
         raise ValueError(f"allowed_rows must be contiguous int32 ({N},) on {dev}, with allowed")
     if out is None:
-        out = torch.empty((N, V), dtype=torch.float32, device=dev)
-    elif tuple(out.shape) != (N, V) or out.device != dev or (V > 1 and out.stride(1) != 1) \
+        out = logits.new_empty((N, V), dtype=torch.float32)
+    elif out.shape != (N, V) or out.device != dev or (V > 1 and out.stride(1) != 1) \
             or (N > 1 and out.stride(0) < V):
         raise ValueError(f"out must be ({N}, {V}) on {dev}, its vocabulary contiguous and its rows apart")
     out_code = _dtype_code(out.dtype)
-    best = torch.empty((N,), dtype=torch.int64, device=dev) if greedy else None
+    best = logits.new_empty((N,), dtype=torch.int64) if greedy else None
     if N:
-        _lib.launch(dev, _lib.lib().aoh_logits_penalize, "aoh_logits_penalize", logits.data_ptr(), logits.stride(0),
-                    code, N, V, None if history is None else history.counts.data_ptr(),
-                    None if history is None else history.seen.data_ptr(), rep, rep_s, pres, pres_s, freq, freq_s,
-                    None if ids is None else ids.data_ptr(), None if values is None else values.data_ptr(), K,
-                    None if allowed is None else allowed.data_ptr(),
-                    None if allowed_rows is None else allowed_rows.data_ptr(), M, out.data_ptr(), out.stride(0),
-                    out_code, None if best is None else best.data_ptr())
+        args = _lib.pack_logits(
+            logits.data_ptr(), out.data_ptr(), _ptr(best), _ptr(history and history.counts),
+            _ptr(history and history.seen), rep, pres, freq, _ptr(ids), _ptr(values), _ptr(allowed), _ptr(allowed_rows),
+            logits.stride(0), out.stride(0), N, V, code, out_code, K, M, rep_s, pres_s, freq_s, 0)
+        _lib.launch(dev, _lib.lib().aoh_logits_penalize, "aoh_logits_penalize", args)
     return (out, best) if greedy else out

@@ -8,7 +8,6 @@ indices: after an eviction they go on counting (``AoHKVCache.tokens_seen``).
 """
 from __future__ import annotations
 
-import ctypes as C
 import functools
 
 import torch
@@ -16,12 +15,17 @@ import torch
 from . import _lib
 from .cache import _dtype_code
 
-_Strides = C.c_int64 * 3
-
-
 @functools.lru_cache(maxsize=64)
 def _sections(sections: tuple[int, ...]):
-    return (C.c_int32 * len(sections))(*sections), len(sections), sum(sections)
+    if not 1 <= len(sections) <= 8:
+        raise ValueError(f"1 to 8 sections, got {len(sections)}")
+    if max(map(abs, sections)) > 1 << 20:
+        raise ValueError(f"bad sections {sections}")
+    return sections + (0,) * (8 - len(sections)), len(sections), sum(sections)
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections, *,
@@ -44,20 +48,21 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         raise ValueError("q must be (B, C, Hq, D) and k (B, C, G, D)")
     B, n, Hq, D = q.shape
     G = k.shape[2]
+    qs, ks = q.stride(), k.stride()
     if k.shape[0] != B or k.shape[1] != n or k.shape[3] != D:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in all but their heads")
     dt, dev = q.dtype, q.device
     code = _dtype_code(dt)
     if not q.is_cuda or k.dtype != dt or k.device != dev:
         raise ValueError("q and k must be CUDA tensors of one dtype on one device")
-    if q.stride(3) != 1 or k.stride(3) != 1:
+    if qs[3] != 1 or ks[3] != 1:
         raise ValueError("the head dimension of q and k must be contiguous")
     secs, A, half = _sections(tuple(int(s) for s in sections))
-    if tuple(positions.shape) != (A, B, n):
+    if positions.shape != (A, B, n):
         raise ValueError(f"positions must have shape (axes, B, C) = {(A, B, n)}, got {tuple(positions.shape)}")
     if positions.dtype not in (torch.int64, torch.int32) or positions.device != dev:
         raise ValueError("positions must be int64 or int32 on q's device")
-    if inv_freq.dtype != torch.float32 or inv_freq.device != dev or tuple(inv_freq.shape) != (half,) \
+    if inv_freq.dtype != torch.float32 or inv_freq.device != dev or inv_freq.shape != (half,) \
             or not inv_freq.is_contiguous():
         raise ValueError(f"inv_freq must be a contiguous float32 tensor of sum(sections) = {half} on q's device")
     if (q_norm_weight is None) != (k_norm_weight is None):
@@ -65,17 +70,18 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     ws = [None, None]
     if q_norm_weight is not None:
         for i, w in enumerate((q_norm_weight, k_norm_weight)):
-            if tuple(w.shape) != (D,) or w.device != dev:
+            if w.shape != (D,) or w.device != dev:
                 raise ValueError(f"norm weights must be ({D},) on q's device")
             ws[i] = w.to(dt).contiguous()
-    q_out = torch.empty((B, n, Hq, D), dtype=dt, device=dev)
-    k_out = torch.empty((B, n, G, D), dtype=dt, device=dev)
-    if q_out.numel() == 0 and k_out.numel() == 0:
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if B == 0 or n == 0:
         return q_out, k_out
-    _lib.launch(dev, _lib.lib().aoh_rope_axes_qk, "aoh_rope_axes_qk", q.data_ptr(), _Strides(*q.stride()[:3]),
-                k.data_ptr(), _Strides(*k.stride()[:3]), code, positions.data_ptr(),
-                positions.dtype == torch.int64, _Strides(*positions.stride()), inv_freq.data_ptr(), secs, A,
-                bool(interleaved), None if ws[0] is None else ws[0].data_ptr(),
-                None if ws[1] is None else ws[1].data_ptr(), float(eps), float(scaling), B, n, Hq, G, D,
-                q_out.data_ptr(), k_out.data_ptr())
+    if D == 0 or Hq == 0 or G == 0:
+        raise ValueError("q and k must have heads and dimensions")
+    args = _lib.pack_rope_axes(
+        q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), _ptr(ws[0]), _ptr(ws[1]),
+        q_out.data_ptr(), k_out.data_ptr(), *qs[:3], *ks[:3], *positions.stride(), *secs, A, bool(interleaved), code,
+        positions.dtype == torch.int64, B, n, Hq, G, D, eps, scaling, 0)
+    _lib.launch(dev, _lib.lib().aoh_rope_axes_qk, "aoh_rope_axes_qk", args)
     return q_out, k_out

@@ -248,25 +248,39 @@ AOH_API int aoh_rope_qk(const void* q, const void* k, const void* cos, const voi
  * height, width; one axis: the ordinary rotary embedding), with optional
  * per-head RMSNorm, computed in fp32 from the positions (angles in fp64) and
  * rounded once; no counterpart in the reference, whose models take cos / sin
- * (aoh_rope_qk).  q (batch, q_len, num_q_heads, head_dim) and k (...,
- * num_kv_heads, head_dim) of `dtype`: any strides q_strides / k_strides =
- * {batch, token, head} in elements, head_dim contiguous, even and <= 256.
- * positions (n_axes, batch, q_len): int64 if positions_64, else int32, strides
- * {axis, batch, token}.  sections[n_axes] (host): how many of the half =
- * sum(sections) <= head_dim / 2 frequencies take each axis's position, axis by
- * axis, or, if interleaved, frequency i takes axis a = i mod n_axes while i <
- * n_axes * sections[a], else axis 0.  inv_freq (half) fp32.  With angle a_i =
- * positions[axis(i)] * inv_freq[i]: out[i] = scaling * (x[i] cos a_i - x[i +
- * half] sin a_i), out[i + half] = scaling * (x[i + half] cos a_i + x[i] sin
- * a_i), dimensions from 2 * half on are copied.  q_norm_weight / k_norm_weight
- * (head_dim, `dtype`) or both NULL.  q_out / k_out: contiguous, not aliasing
- * the inputs. */
-AOH_API int aoh_rope_axes_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                             int32_t dtype, const void* positions, int32_t positions_64,
-                             const int64_t* position_strides, const float* inv_freq, const int32_t* sections,
-                             int32_t n_axes, int32_t interleaved, const void* q_norm_weight, const void* k_norm_weight,
-                             float eps, float scaling, int32_t batch, int32_t q_len, int32_t num_q_heads,
-                             int32_t num_kv_heads, int32_t head_dim, void* q_out, void* k_out, aoh_stream stream);
+ * (aoh_rope_qk).  With angle a_i = positions[axis(i)] * inv_freq[i] and half =
+ * the sum of the sections: out[i] = scaling * (x[i] cos a_i - x[i + half] sin
+ * a_i), out[i + half] = scaling * (x[i + half] cos a_i + x[i] sin a_i),
+ * dimensions from 2 * half on are copied. */
+#define AOH_ROPE_MAX_AXES 8
+typedef struct {
+  const void* q;             /* (batch, q_len, num_q_heads, head_dim) of dtype, head_dim contiguous */
+  const void* k;             /* (batch, q_len, num_kv_heads, head_dim) */
+  const void* positions;     /* (n_axes, batch, q_len) int64 if positions_64, else int32 */
+  const float* inv_freq;     /* (half) */
+  const void* q_norm_weight; /* (head_dim) of dtype, or both NULL: no norm */
+  const void* k_norm_weight;
+  void* q_out;               /* contiguous, not aliasing the inputs */
+  void* k_out;
+  int64_t q_strides[3];      /* elements: batch, token, head */
+  int64_t k_strides[3];
+  int64_t position_strides[3]; /* axis, batch, token */
+  int32_t sections[AOH_ROPE_MAX_AXES]; /* frequencies of each axis, axis by axis; interleaved: frequency i takes
+                                          axis a = i mod n_axes while i < n_axes * sections[a], else axis 0 */
+  int32_t n_axes;
+  int32_t interleaved;
+  int32_t dtype;             /* aoh_dtype */
+  int32_t positions_64;
+  int32_t batch;
+  int32_t q_len;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;          /* even, <= 256 */
+  float eps;
+  float scaling;
+  int32_t reserved;          /* 0 */
+} aoh_rope_axes_args;
+AOH_API int aoh_rope_axes_qk(const aoh_rope_axes_args* args, aoh_stream stream);
 
 /* AoHKVCache.append_layer alone (benchmark_llama31.py:171-184): write q_len
  * new tokens at positions past_len.. into every unit of `layer`. */
@@ -336,27 +350,39 @@ AOH_API int aoh_history_add(int32_t* counts, int32_t* seen, int32_t rows, int32_
                             int32_t ids_64, int64_t id_stride, int32_t per_row, const int32_t* lengths, int32_t prompt,
                             aoh_stream stream);
 
-/* Per row of logits (rows, vocab; AOH_BF16 or AOH_F32, row_stride elements
- * apart), in this order, each step rounded to fp32:
+/* Per row of logits, in this order, each step rounded to fp32:
  *   x > 0 ? x / repetition : x * repetition   for tokens of the prompt or output,
  *   x - frequency * count, then x - presence  for tokens of the output,
- *   x + the sum of its biases                 (bias_ids, bias (rows, n_bias); ids outside [0, vocab) are left out),
- *   -inf                                      where bit t % 32 of word t / 32 of the row's mask is 0.
- * repetition / presence / frequency: device fp32 (rows), or NULL for the
- * scalar.  counts / seen: the history, or both NULL (no penalties).  allowed
- * (n_allowed, ceil(vocab / 32)) int32 or NULL; row n's mask is allowed[n], or
- * allowed[allowed_rows[n]] with allowed_rows (rows) int32, an index outside
- * [0, n_allowed) meaning no mask.  out (out_dtype, out_stride) may be the
- * logits themselves.  greedy (rows) int64 or NULL: the token of the largest
- * fp32 result, the lowest of equal ones (NaN above every number; 0 where
- * nothing is allowed). */
-AOH_API int aoh_logits_penalize(const void* logits, int64_t row_stride, int32_t dtype, int32_t rows, int32_t vocab,
-                                const int32_t* counts, const int32_t* seen, const float* repetition,
-                                float repetition_scalar, const float* presence, float presence_scalar,
-                                const float* frequency, float frequency_scalar, const int32_t* bias_ids,
-                                const float* bias, int32_t n_bias, const int32_t* allowed, const int32_t* allowed_rows,
-                                int32_t n_allowed, void* out, int64_t out_stride, int32_t out_dtype, int64_t* greedy,
-                                aoh_stream stream);
+ *   x + the sum of its biases,
+ *   -inf                                      where bit t % 32 of word t / 32 of the row's mask is 0. */
+typedef struct {
+  const void* logits;      /* (rows, vocab) of dtype, rows row_stride elements apart */
+  void* out;               /* (rows, vocab) of out_dtype, rows out_stride apart; may be the logits themselves */
+  int64_t* greedy;         /* (rows) or NULL: the token of the largest fp32 result, the lowest of equal ones (NaN
+                              above every number; 0 where nothing is allowed) */
+  const int32_t* counts;   /* the history, or both NULL: no penalties */
+  const int32_t* seen;
+  const float* repetition; /* (rows), or NULL: the scalar */
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_ids; /* (rows, n_bias); ids outside [0, vocab) are left out, repeated ones add up */
+  const float* bias;       /* (rows, n_bias) */
+  const int32_t* allowed;  /* (n_allowed, ceil(vocab / 32)) or NULL: no mask */
+  const int32_t* allowed_rows; /* (rows) or NULL: row n has mask n; an index outside [0, n_allowed) means no mask */
+  int64_t row_stride;
+  int64_t out_stride;
+  int32_t rows;
+  int32_t vocab;
+  int32_t dtype;           /* aoh_dtype */
+  int32_t out_dtype;
+  int32_t n_bias;
+  int32_t n_allowed;
+  float repetition_scalar;
+  float presence_scalar;
+  float frequency_scalar;
+  int32_t reserved;        /* 0 */
+} aoh_logits_args;
+AOH_API int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream stream);
 
 /* ------------------------------------------------------------------------- */
 /* Effective-rank classifier                                                 */
