@@ -9,15 +9,23 @@
 // the scores (4 bytes a key and row, which stay in L2) and the range's (m, l);
 // few_sum_kernel turns them into weights.
 //
-// More rows: tensor_pass_kernel<kLse> and <kSums>, the same product with its
-// operands exchanged.  A CTA keeps two 128-row tiles of one operand in shared
-// memory (two tiles of query rows, or two tiles of keys) and streams 128-row
+// More rows: tensor_pass_kernel, the same product three ways.  A CTA keeps up
+// to two 128-row tiles of one operand in shared memory and streams 128-row
 // tiles of the other; each 128 x 128 product goes to tensor memory (two
-// buffers per resident tile), where a warpgroup per resident tile reads it,
-// thread = row.  With query rows as rows a thread keeps its row's running
-// maximum and sum; with keys as rows it adds up exp(s - lse) over the columns,
-// so neither pass exchanges anything between threads.  Query rows are packed
-// (token, head) pairs, so a chunk of a few tokens still fills a tile.
+// buffers per resident tile) and is read by two warpgroups, thread = row of
+// the product, half of the columns each, while the other buffer is filled.
+//   kLse     query rows resident, keys streamed, rows = query rows: a thread
+//            keeps its row's running maximum and sum.
+//   kSums    keys resident, query rows streamed, rows = keys: a thread adds up
+//            exp(s - lse) over its columns.
+//   kStream  at most two tiles of query rows, resident, keys streamed, rows =
+//            keys: the sums of a key tile are complete with it.
+// So no pass exchanges anything between threads per element.  Query rows are
+// packed (token, head) pairs, so a chunk of a few tokens still fills a tile.
+// Bound: the exponentials, two a (query, key) pair, against 512 flops: the
+// MUFU alone would take 1024 cycles an SM for a product that the tensor cores
+// do in 512.  Four warpgroups keep it fed, and one pair in eight goes to a
+// polynomial of the same accuracy on the FMA pipe.
 #include "common.cuh"
 #include "fast_math.cuh"
 #include "internal.h"
@@ -235,7 +243,7 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
 // ---------------------------------------------------------------------------
 // tensor cores
 // ---------------------------------------------------------------------------
-constexpr int kTcThreads = 640;  // warp 0 loads, warp 1 issues, warps 4..19: a warpgroup per product buffer
+constexpr int kTcThreads = 640;  // warp 0 loads, warp 1 issues, warps 4..19: two warpgroups per resident tile
 constexpr int kStages = 3;
 constexpr int kTileRows = 128;
 constexpr int kHalfTile = kTileRows * 128;   // 64 dimensions of 128 rows
@@ -264,16 +272,30 @@ struct TcArgs {
   long long sums_unit;
 };
 
-// Exponentials of 64 scores, added to acc: 2^(s * scale + b), b per column
-// pair.  Three pairs in eight take the FMA pipe; a masked tile's scores (-inf,
-// whose power must be exactly 0) all take the MUFU.
+// Waits for this thread's tensor-memory loads.  The registers pass through, so
+// that nothing the compiler does with them moves before the wait.
+__device__ __forceinline__ void tc_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), 
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), 
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), 
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// Exponentials of 32 scores, added to acc: 2^(s * scale + b), b per column
+// pair.  One pair in eight takes the FMA pipe (none: 313 us for a pass over
+// 4096 x 16K keys of 4 units, one or two: 294, three: 314, four: 339 -- the
+// polynomial's twelve instructions soon cost more than the MUFU's wait); a
+// masked tile's scores (-inf, whose power must be exactly 0) all take the MUFU.
 template <bool kPoly, class B>
-__device__ __forceinline__ void add_exp2(const uint32_t* sv, B&& b, uint64_t (&acc)[4]) {
+__device__ __forceinline__ void add_exp2(const uint32_t (&sv)[32], B&& b, uint64_t (&acc)[4]) {
   const uint64_t scale2 = f2_pack(kScoreScale, kScoreScale);
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
+  for (int e = 0; e < 16; ++e) {
     const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale2, b(e));
-    if (kPoly && (e & 7) >= 5) {
+    if (kPoly && (e & 7) == 7) {
       acc[e & 3] = f2_add(acc[e & 3], exp2_poly2_f32(x2));
     } else {
       float x0, x1;
@@ -290,6 +312,29 @@ __device__ __forceinline__ float total(const uint64_t (&acc)[4]) {
   return ((u[0] + u[1]) + (u[2] + u[3])) + ((u[4] + u[5]) + (u[6] + u[7]));
 }
 
+// One 128 x 128 product over 128 dimensions: eight instructions of 16
+// dimensions, four in each 64-dim half.  The descriptors differ from the first
+// one's by their address fields (units of 16 bytes) alone, so stepping them is
+// one addition each: the issuing warp shares its scheduler with four busy
+// warps, and with descriptors built one by one it was late with the products.
+__device__ __forceinline__ void mma_tile(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred l, no, yes;\n\t.reg .u32 lid;\n\t.reg .b64 x, y;\n\t"
+      "mov.u32 lid, %%laneid;\n\tsetp.eq.u32 l, lid, 0;\n\tsetp.ne.u32 no, 0, 0;\n\tsetp.eq.u32 yes, 0, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, no;\n\t"
+      "add.s64 x, %1, 2;\n\tadd.s64 y, %2, 2;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 4;\n\tadd.s64 y, %2, 4;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 6;\n\tadd.s64 y, %2, 6;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 1024;\n\tadd.s64 y, %2, 1024;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 1026;\n\tadd.s64 y, %2, 1026;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 1028;\n\tadd.s64 y, %2, 1028;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "add.s64 x, %1, 1030;\n\tadd.s64 y, %2, 1030;\n\t@l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, yes;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc)
+      : "memory");
+}
+static_assert(kHalfTile / 16 == 1024, "descriptor step between the halves");
+
 // (m, l) of two disjoint sets of keys as one.
 __device__ __forceinline__ float2 merge_ml(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
@@ -303,10 +348,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr bool kKeysStreamed = kPass != kSums;    // otherwise the query rows are
   constexpr bool kQueriesResident = kPass != kSums;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bar_a, bar_final, bar_full[kStages], bar_empty[kStages], bar_s_full[4], bar_s_empty[4],
-      bar_lse[kLseSlots], bar_part_full[2][2], bar_part_empty[2][2];
-  __shared__ float2 s_row[2][kTileRows];    // kLse, kSums: what the second buffer's warpgroups found
-  __shared__ float s_part[2][2][kTileRows];  // kStream: sums of the second tile of query rows, [buffer][slot][key]
+  __shared__ uint64_t bar_a, bar_final, bar_full[kStages], bar_empty[kStages], bar_s_full[2][2], bar_s_empty[2][2],
+      bar_lse[kLseSlots], bar_part_full[2], bar_part_empty[2];
+  __shared__ float2 s_row[2][kTileRows];     // kLse, kSums: what the second half's warpgroups found
+  __shared__ float s_part[2][3][kTileRows];  // kStream: sums of all but the first warpgroup, [slot][warpgroup - 1][key]
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   const KeyWeightsArgs& a = t.a;
@@ -365,15 +410,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&bar_empty[s], 1);
     }
     for (int s = 0; s < kLseSlots; ++s) mbar_init(&bar_lse[s], 1);
-    for (int u = 0; u < 4; ++u) {
-      mbar_init(&bar_s_full[u], 1);
-      mbar_init(&bar_s_empty[u], 128);
-    }
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
       for (int k = 0; k < 2; ++k) {
-        mbar_init(&bar_part_full[u][k], 128);
-        mbar_init(&bar_part_empty[u][k], 128);
+        mbar_init(&bar_s_full[u][k], 1);
+        mbar_init(&bar_s_empty[u][k], 256);
       }
+      mbar_init(&bar_part_full[u], (2 * na - 1) * 128);
+      mbar_init(&bar_part_empty[u], 128);
+    }
     s_abort = 0;
     fence_mbar_init();
   }
@@ -491,130 +535,128 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (kPass == kSums) griddep_wait();  // the bounded waits time this grid, not the one before
     bool ok = mbar_wait_warp(&bar_a, 0, G.err);
     tc_fence_after();
+    const uint64_t res = smem_desc_sw128(smem_u32(sA), 16, 1024), str0 = smem_desc_sw128(smem_u32(sB), 16, 1024);
+    uint64_t str = str0;
+    int s = 0;
+    uint32_t round = 0;  // of the ring: parity of bar_full[s]
     for (int i = 0; i < n && ok && !s_abort; ++i) {
-      const int s = i % kStages;
-      if (!(ok = mbar_wait_warp(&bar_full[s], (i / kStages) & 1, G.err))) break;
+      if (!(ok = mbar_wait_warp(&bar_full[s], round & 1, G.err))) break;
+      const int buf = i & 1;
       for (int w = 0; w < na && ok; ++w) {
-        const int u = (i & 1) * 2 + w;  // buffer and warpgroup of this product
-        if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[u], ((i >> 1) - 1) & 1, G.err))) break;
+        if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[w][buf], ((i >> 1) - 1) & 1, G.err))) break;
         tc_fence_after();
-        const uint32_t res = smem_u32(sA + w * kTileBytes), str = smem_u32(sB + s * kTileBytes);
-        const uint32_t rows = kPass == kStream ? str : res, cols = kPass == kStream ? res : str;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kHalfTile + (k & 3) * 32;
-          mma_ss(tmem + u * kTileRows, smem_desc_sw128(rows + off, 16, 1024), smem_desc_sw128(cols + off, 16, 1024), kIdesc,
-                 k > 0 ? 1u : 0u);
-        }
-        mma_commit(&bar_s_full[u]);
+        const uint64_t tile = res + w * (kTileBytes / 16);
+        mma_tile(tmem + (w * 2 + buf) * kTileRows, kPass == kStream ? str : tile, kPass == kStream ? tile : str, kIdesc);
+        mma_commit(&bar_s_full[w][buf]);
       }
       if (ok) mma_commit(&bar_empty[s]);
+      str += kTileBytes / 16;
+      if (++s == kStages) {
+        s = 0;
+        str = str0;
+        ++round;
+      }
     }
     if (!ok) s_abort = 1;
     __syncwarp();
     mma_commit(&bar_final);  // fires once every product issued above has completed
-  } else if (warp >= 4 && ((warp - 4) / 4 & 1) < na) {
+  } else if (warp >= 4 && (warp - 4) / 8 < na) {
     // ============================ exponentials ============================
-    const int u = (warp - 4) / 4, w = u & 1, buf = u >> 1;  // every second streamed tile against resident tile w
+    const int u = (warp - 4) / 4, w = u >> 1, h = u & 1;  // half h of the columns of resident tile w's products
     const int row = 32 * (warp & 3) + lane;
-    const uint32_t s_col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + u * kTileRows;
+    const uint32_t s_col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + w * 2 * kTileRows + 64 * h;
     const int tile = 2 * pair + w;
     const int last = past + tile * tt + row / G.grp;  // kLse: last key the row's query sees
     if (kPass == kSums) griddep_wait();
     uint64_t acc[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = 0;
-    for (int i = buf; i < n; i += 2) {
-      const int slot = i % kLseSlots;
+    // 32 scores of product i, from column 64 h + c0 on, are added up
+    auto add_scores = [&](int i, int c0, uint32_t (&sv)[32]) {
       // the tile of keys and the first token of the tile of queries of this product
       const int key0 = (kKeysStreamed ? t0 + i : tile) * kTileRows, tok0 = (kQueriesResident ? tile : t0 + i) * tt;
       const bool full = key0 + kTileRows - 1 <= past + tok0;  // every token sees every key
-      if (kPass == kSums && !s_abort && !mbar_wait(&bar_lse[slot], (i / kLseSlots) & 1, G.err)) s_abort = 1;
-      if (s_abort || !mbar_wait(&bar_s_full[u], (i >> 1) & 1, G.err)) {
-        s_abort = 1;
-        break;
+      if (!full) {
+        // rows = keys: columns from the first token that sees the row's key on
+        const int c_min = max(0, key0 + row - past - tok0) * G.grp - 64 * h - c0, k_max = last - key0 - 64 * h - c0;
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (kPass == kLse ? e > k_max : e < c_min) sv[e] = __float_as_uint(-INFINITY);
       }
+      if (kPass == kLse) {
+        float mx[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
+#pragma unroll
+        for (int e = 8; e < 32; e += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mx[k] = fmax3(mx[k], __uint_as_float(sv[e + 2 * k]), __uint_as_float(sv[e + 2 * k + 1]));
+        const float mt = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * kScoreScale;
+        if (mt > m) {
+          const float f = fast_exp2(m - mt);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] = f2_fma(acc[k], f2_pack(f, f), 0);
+          m = mt;
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const uint64_t nm2 = f2_pack(nm, nm);
+        if (full)
+          add_exp2<true>(sv, [&](int) { return nm2; }, acc);
+        else
+          add_exp2<false>(sv, [&](int) { return nm2; }, acc);
+      } else {
+        const ulonglong2* nl =
+            reinterpret_cast<const ulonglong2*>(sLse + (kPass == kSums ? i % kLseSlots : w) * kTileRows + 64 * h + c0);
+        ulonglong2 v = make_ulonglong2(0, 0);
+        auto column = [&](int e) {
+          if (e % 2 == 0) v = nl[e / 2];
+          return e % 2 == 0 ? v.x : v.y;
+        };
+        if (full)
+          add_exp2<true>(sv, column, acc);
+        else
+          add_exp2<false>(sv, column, acc);
+      }
+    };
+    // Each 32 columns are on their way from tensor memory while the 32 before
+    // them are worked on.
+    auto arrived = [&](int i) {  // product i (and its columns' -lse)
+      if (kPass == kSums && !mbar_wait(&bar_lse[i % kLseSlots], (i / kLseSlots) & 1, G.err)) return false;
+      if (!mbar_wait(&bar_s_full[w][i & 1], (i >> 1) & 1, G.err)) return false;
       tc_fence_after();
-      // rows = keys: columns from the first token that sees the row's key on
-      const int c_min = kPass == kLse ? 0 : min(kTileRows, max(0, key0 + row - past - tok0) * G.grp);
+      return true;
+    };
+    uint32_t lo[32], hi[32];
+    bool ok = n > 0 && arrived(0);
+    if (ok) tmem_ld32(s_col, lo);
+    for (int i = 0; i < n && ok; ++i) {
+      const int buf = i & 1;
+      tc_wait_ld32(lo);
+      tmem_ld32(s_col + buf * kTileRows + 32, hi);
+      add_scores(i, 0, lo);
+      tc_wait_ld32(hi);
+      tc_fence_before();
+      mbar_arrive(&bar_s_empty[w][buf]);
+      if (i + 1 < n) {
+        ok = arrived(i + 1);
+        if (ok) tmem_ld32(s_col + (buf ^ 1) * kTileRows, lo);
+      }
+      add_scores(i, 32, hi);
       if (kPass == kStream) {
+        // the other warpgroups hand their columns' sums of this tile of keys to the first
+        sum = total(acc);
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = 0;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t sv[64];
-        tmem_ld32(s_col + 64 * h, sv);
-        tmem_ld32(s_col + 64 * h + 32, sv + 32);
-        tc_wait_ld();
-        if (h == 1) {
-          tc_fence_before();
-          mbar_arrive(&bar_s_empty[u]);
-        }
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            const int c = 64 * h + e;
-            if (kPass == kLse ? key0 + c > last : c < c_min) sv[e] = __float_as_uint(-INFINITY);
-          }
-        }
-        if (kPass == kLse) {
-          float mx[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
-#pragma unroll
-          for (int e = 8; e < 64; e += 8)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mx[k] = fmax3(mx[k], __uint_as_float(sv[e + 2 * k]), __uint_as_float(sv[e + 2 * k + 1]));
-          const float mt = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * kScoreScale;
-          if (mt > m) {
-            const float f = fast_exp2(m - mt);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] = f2_fma(acc[k], f2_pack(f, f), 0);
-            m = mt;
-          }
-          const float nm = m == -INFINITY ? 0.f : -m;
-          const uint64_t nm2 = f2_pack(nm, nm);
-          if (full)
-            add_exp2<true>(sv, [&](int) { return nm2; }, acc);
-          else
-            add_exp2<false>(sv, [&](int) { return nm2; }, acc);
+        const int key = (t0 + i) * kTileRows + row, ps = i & 1;
+        if (u > 0) {
+          if (i >= 2 && !mbar_wait(&bar_part_empty[ps], ((i >> 1) - 1) & 1, G.err)) break;
+          s_part[ps][u - 1][row] = sum;
+          mbar_arrive(&bar_part_full[ps]);
         } else {
-          const ulonglong2* nl =
-              reinterpret_cast<const ulonglong2*>(sLse + (kPass == kSums ? slot : w) * kTileRows + 64 * h);
-          ulonglong2 v = make_ulonglong2(0, 0);
-          auto column = [&](int e) {
-            if (e % 2 == 0) v = nl[e / 2];
-            return e % 2 == 0 ? v.x : v.y;
-          };
-          if (full)
-            add_exp2<true>(sv, column, acc);
-          else
-            add_exp2<false>(sv, column, acc);
-        }
-      }
-      if (kPass == kStream) {
-        // this buffer's k-th tile; the second tile of query rows hands its sums to the first's warpgroup
-        sum = total(acc);
-        const int k = i >> 1, key = key0 + row;
-        uint64_t *filled = &bar_part_full[buf][k & 1], *read = &bar_part_empty[buf][k & 1];
-        if (w == 1) {
-          if (k >= 2 && !mbar_wait(read, (k >> 1 & 1) ^ 1, G.err)) {
-            s_abort = 1;
-            break;
-          }
-          s_part[buf][k & 1][row] = sum;
-          mbar_arrive(filled);
-        } else {
-          if (na > 1) {
-            if (!mbar_wait(filled, k >> 1 & 1, G.err)) {
-              s_abort = 1;
-              break;
-            }
-            sum += s_part[buf][k & 1][row];
-            mbar_arrive(read);
-          }
+          if (!mbar_wait(&bar_part_full[ps], (i >> 1) & 1, G.err)) break;
+          for (int k = 0; k < 2 * na - 1; ++k) sum += s_part[ps][k][row];
+          mbar_arrive(&bar_part_empty[ps]);
           if (key < len) {
             float* o = a.out + r * a.out_stride + key;
             *o = a.accumulate ? *o + sum : sum;
@@ -624,16 +666,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     if (kPass != kStream) {
       sum = total(acc);
-      if (buf == 1) s_row[w][row] = make_float2(m, sum);
+      if (h == 1) s_row[w][row] = make_float2(m, sum);
     }
   }
 
   // ============================ teardown ============================
   tc_fence_before();
   __syncthreads();
-  if (kPass != kStream && warp >= 4 && warp < 12 && (warp - 4) / 4 < na) {
-    // the first buffer's warpgroups add what the second's found
-    const int w = (warp - 4) / 4, row = 32 * (warp & 3) + lane, tile = 2 * pair + w;
+  if (kPass != kStream && warp >= 4 && (warp - 4) / 8 < na && ((warp - 4) / 4 & 1) == 0) {
+    // the first half's warpgroups add what the second's found
+    const int w = (warp - 4) / 8, row = 32 * (warp & 3) + lane, tile = 2 * pair + w;
     const float2 other = s_row[w][row];
     if (kPass == kLse) {
       const float2 ml = merge_ml(make_float2(m, sum), other);
