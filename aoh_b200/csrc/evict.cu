@@ -62,9 +62,15 @@ __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+// No memory clobber: several are in flight at once, between two cluster barriers.
+__device__ __forceinline__ uint4 ld_dsmem_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
 
 struct SelectShared {
-  uint32_t hist[kBins];
+  alignas(16) uint32_t hist[kBins];
   uint32_t scan[kSelWarps];
   uint32_t gt[kSelWarps], eq[kSelWarps];  // keys above / equal to the threshold, by warp
   uint32_t total[2];                      // of this CTA
@@ -93,8 +99,10 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   }
   if (a.take == 0) return;  // the same for every CTA of the cluster
 
-  if (a.resident)
+  if (a.resident) {
+#pragma unroll 8
     for (int i = tid; i < cnt; i += kSelThreads) keys[i] = weight_key(wm[i]);
+  }
   auto key = [&](int i) { return a.resident ? keys[i] : weight_key(wm[i]); };
 
   uint32_t prefix = 0, left = (uint32_t)a.take;  // the threshold's leading bits, keys still to take
@@ -123,17 +131,29 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       cluster_sync_all();
     else
       __syncthreads();
-    // thread t sums bins [4t, 4t + 4) counted from the top over the cluster
+    // thread t sums the bins kBins - 1 - 4 t and the three below over the cluster
+    constexpr int per = kBins / kSelThreads;
+    static_assert(per == 4, "a thread's bins are one 16-byte load");
+    const uint32_t* top = &s.hist[kBins - per * (tid + 1)];
     uint32_t c[4] = {0, 0, 0, 0};
-    const int per = kBins / kSelThreads;
+    if (a.cluster > 1) {
+      uint4 v[kSelMaxCluster];
 #pragma unroll
-    for (int j = 0; j < per; ++j) {
-      const int b = kBins - 1 - (tid * per + j);
-      if (a.cluster > 1) {
-        for (int r = 0; r < a.cluster; ++r) c[j] += ld_dsmem_u32(mapa_shared(&s.hist[b], r));
-      } else {
-        c[j] = s.hist[b];
+      for (int r = 0; r < kSelMaxCluster; ++r)
+        v[r] = r < a.cluster ? ld_dsmem_v4(mapa_shared(top, r)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kSelMaxCluster; ++r) {
+        c[0] += v[r].w;
+        c[1] += v[r].z;
+        c[2] += v[r].y;
+        c[3] += v[r].x;
       }
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(top);
+      c[0] = v.w;
+      c[1] = v.z;
+      c[2] = v.y;
+      c[3] = v.x;
     }
     const uint32_t mine = c[0] + c[1] + c[2] + c[3];
     uint32_t incl = mine;

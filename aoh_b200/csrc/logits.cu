@@ -16,11 +16,16 @@
 // pass reads, 1 bit a token; the count words are read for the tokens it names.
 //
 // Bound: HBM, logits in and fp32 out (6 bytes a token for bf16 logits, 1/4
-// byte for the two bitmaps).  One cluster of 8 CTAs takes a row, each an
-// eighth of the vocabulary; the greedy token is reduced over the cluster in
-// shared memory, so one launch and no workspace.  Biased tokens are marked in
-// a shared-memory bitmap first, left out by the main pass and done one by one
-// behind it: the sum over a token listed more than once has a fixed order.
+// byte for the two bitmaps), and latency for a few rows.  One cluster of 8 CTAs
+// takes a row, each an eighth of the vocabulary; the greedy token is reduced
+// over the cluster in shared memory, so one launch and no workspace.  A thread
+// has the loads of four groups of 8 tokens (or 8 single ones) in flight before
+// it works on any.  A CTA's biased tokens are listed in shared memory first, in
+// the order given, and marked in a bitmap there; the main pass leaves them out
+// and a thread for each listed token does it alone, so that the sum over a
+// token listed more than once has a fixed order.
+#include <climits>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -28,7 +33,8 @@ namespace aoh {
 namespace {
 
 constexpr int kCluster = 8;
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kMaxBias = 4096;  // biases of a row (32 KB of shared memory if all fall into one slice)
 constexpr uint32_t kInPrompt = 0x80000000u;
 
 struct LogitsArgs {
@@ -85,8 +91,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* x) {
 struct RowPenalties {
   float rep, pres, freq;
   const uint32_t* counts;
-  __device__ __forceinline__ float apply(float x, int t) const {
-    const uint32_t w = counts[t];
+  __device__ __forceinline__ float apply(float x, uint32_t w) const {
     x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
     const uint32_t n = w & ~kInPrompt;
     x = __fsub_rn(x, __fmul_rn(freq, (float)n));
@@ -100,17 +105,35 @@ __device__ __forceinline__ unsigned long long greedy_key(float x, int t) {
   u = x != x ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
   return ((unsigned long long)u << 32) | (uint32_t)~t;
 }
-__device__ __forceinline__ unsigned long long shfl_xor_u64(unsigned long long v, int off) {
-  return __shfl_xor_sync(0xffffffffu, v, off);
-}
+
+// The best of a thread's tokens, seen in ascending order.  -inf gives no key:
+// a row of nothing else has token 0.
+struct Best {
+  float x = -INFINITY;
+  int t = INT_MAX, nan_t = INT_MAX;
+  __device__ __forceinline__ void one(float v, int at) {
+    if (v > x) {
+      x = v;
+      t = at;
+    }
+    if (v != v) nan_t = min(nan_t, at);
+  }
+  __device__ __forceinline__ unsigned long long key() const {
+    unsigned long long k = t == INT_MAX ? 0 : greedy_key(x, t);
+    return nan_t == INT_MAX ? k : greedy_key(NAN, nan_t);
+  }
+};
 
 template <typename T, typename O, bool kWide>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
     logits_kernel(const __grid_constant__ LogitsArgs a) {
-  extern __shared__ uint32_t biased[];  // slice / 32 words (with biases)
+  extern __shared__ uint32_t smem[];  // with biases: a bit per token of the slice, then the slice's (id, value) list
   __shared__ unsigned long long best_warp[kThreads / 32];
   __shared__ unsigned long long best_cta[kCluster];
-  const int rank = (int)cluster_ctarank();
+  __shared__ int s_count[kThreads / 32];
+  uint32_t* biased = smem;
+  int2* list = reinterpret_cast<int2*>(smem + a.slice / 32);
+  const int rank = (int)cluster_ctarank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / kCluster;
   const int lo = rank * a.slice, hi = min(lo + a.slice, a.vocab);  // may be empty
   const int words = (a.vocab + 31) >> 5;
@@ -126,96 +149,165 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads)
     const int r = a.allowed_rows ? a.allowed_rows[row] : row;
     if (r >= 0 && r < a.n_allowed) allowed = a.allowed + (long long)r * words;
   }
-  const int32_t* bias_ids = a.bias_ids + (long long)row * a.n_bias;
-  const float* bias = a.bias + (long long)row * a.n_bias;
-  unsigned long long best = 0;
+  const bool greedy = a.greedy != nullptr;
+  Best best;
 
+  int listed = 0;
   if (a.n_bias) {
-    for (int i = threadIdx.x; i < a.slice / 32; i += kThreads) biased[i] = 0;
+    const int32_t* ids = a.bias_ids + (long long)row * a.n_bias;
+    const float* values = a.bias + (long long)row * a.n_bias;
+    for (int i = tid; i < a.slice / 32; i += kThreads) biased[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.n_bias; i += kThreads) {
-      const int t = bias_ids[i];
-      if (t >= lo && t < hi) atomicOr(&biased[(t - lo) >> 5], 1u << (t & 31));
+    for (int i0 = 0; i0 < a.n_bias; i0 += kThreads) {
+      const int i = i0 + tid;
+      const int id = i < a.n_bias ? ids[i] : -1;
+      const float v = i < a.n_bias ? values[i] : 0.f;
+      const bool in = id >= lo && id < hi;
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      if (lane == 0) s_count[warp] = __popc(m);
+      if (in) atomicOr(&biased[(id - lo) >> 5], 1u << (id & 31));
+      __syncthreads();
+      int at = listed + __popc(m & ((1u << lane) - 1u));
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) at += s_count[w];
+        listed += s_count[w];
+      }
+      if (in) list[at] = make_int2(id, __float_as_int(v));
+      __syncthreads();
     }
-    __syncthreads();
   }
 
-  // the tokens [t, t + n) of one 32-token word, bit j of the masks is token t + j
   if (kWide) {
-    // a thread takes 8 tokens at a time (vocab is a multiple of 8 here)
-    for (int t = lo + threadIdx.x * 8; t < hi; t += kThreads * 8) {
-      float x[8];
-      load8(x_row + t, x);
-      const int sh = t & 31;
-      const uint32_t s = seen ? seen[t >> 5] >> sh & 0xffu : 0u;
-      const uint32_t al = allowed ? allowed[t >> 5] >> sh & 0xffu : 0xffu;
-      const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> sh & 0xffu : 0u;
-      if (s) {
+    // groups of 8 tokens (vocab is a multiple of 8 here), four in flight
+    constexpr int U = 4;
+    for (int t0 = lo + tid * 8; t0 < hi; t0 += U * kThreads * 8) {
+      float x[U][8];
+      uint32_t s[U], al[U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (s >> j & 1) x[j] = pen.apply(x[j], t + j);
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kThreads * 8;
+        s[u] = 0;
+        al[u] = 0xffu;
+        if (t < hi) {
+          load8(x_row + t, x[u]);
+          if (seen) s[u] = seen[t >> 5] >> (t & 31) & 0xffu;
+          if (allowed) al[u] = allowed[t >> 5] >> (t & 31) & 0xffu;
+        }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (!(al >> j & 1)) x[j] = -INFINITY;
-      if (a.greedy) {
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kThreads * 8;
+        if (t >= hi) break;
+        if (s[u]) {
+          const uint4 c0 = reinterpret_cast<const uint4*>(pen.counts + t)[0], c1 = reinterpret_cast<const uint4*>(pen.counts + t)[1];
+          const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!(bi >> j & 1)) best = max(best, greedy_key(x[j], t + j));
-      }
-      if (!bi) {
-        store8(out + t, x);
-      } else {
+          for (int j = 0; j < 8; ++j)
+            if (s[u] >> j & 1) x[u][j] = pen.apply(x[u][j], c[j]);
+        }
+        if (al[u] != 0xffu) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (!(bi >> j & 1)) store1(out + t + j, x[j]);
+          for (int j = 0; j < 8; ++j)
+            if (!(al[u] >> j & 1)) x[u][j] = -INFINITY;
+        }
+        const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> (t & 31) & 0xffu : 0u;
+        if (bi) {  // without the biased ones
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(bi >> j & 1)) {
+              store1(out + t + j, x[u][j]);
+              best.one(x[u][j], t + j);
+            }
+          continue;
+        }
+        store8(out + t, x[u]);
+        if (greedy) {
+          const float mx = fmaxf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])),
+                                 fmaxf(fmaxf(x[u][4], x[u][5]), fmaxf(x[u][6], x[u][7])));
+          bool nan = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) nan |= x[u][j] != x[u][j];
+          if (mx > best.x || nan) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) best.one(x[u][j], t + j);
+          }
+        }
       }
     }
   } else {
-    // rows that are not 16-byte aligned: a lane takes one token of the warp's word
-    const int lane = threadIdx.x & 31;
-    for (int t = lo + (int)threadIdx.x; t < hi; t += kThreads) {
-      float x = load1(x_row + t);
-      if (seen && (seen[t >> 5] >> lane & 1)) x = pen.apply(x, t);
-      if (allowed && !(allowed[t >> 5] >> lane & 1)) x = -INFINITY;
-      if (a.n_bias && (biased[(t - lo) >> 5] >> lane & 1)) continue;
-      if (a.greedy) best = max(best, greedy_key(x, t));
-      store1(out + t, x);
+    // rows that are not 16-byte aligned: a lane takes one token of the warp's word, eight words in flight
+    constexpr int U = 8;
+    for (int t0 = lo + tid; t0 < hi; t0 += U * kThreads) {
+      float x[U];
+      uint32_t s[U], al[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kThreads;
+        s[u] = 0;
+        al[u] = 1;
+        x[u] = 0.f;
+        if (t < hi) {
+          x[u] = load1(x_row + t);
+          if (seen) s[u] = seen[t >> 5] >> lane & 1;
+          if (allowed) al[u] = allowed[t >> 5] >> lane & 1;
+        }
+      }
+      uint32_t c[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) c[u] = s[u] ? pen.counts[t0 + u * kThreads] : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kThreads;
+        if (t >= hi) break;
+        if (s[u]) x[u] = pen.apply(x[u], c[u]);
+        if (!al[u]) x[u] = -INFINITY;
+        if (a.n_bias && (biased[(t - lo) >> 5] >> lane & 1)) continue;
+        store1(out + t, x[u]);
+        if (greedy) best.one(x[u], t);
+      }
     }
   }
+  unsigned long long key = best.key();
 
-  for (int i = threadIdx.x; i < a.n_bias; i += kThreads) {
-    const int t = bias_ids[i];
-    if (t < lo || t >= hi) continue;
+  for (int i = tid; i < listed; i += kThreads) {
+    const int t = list[i].x;
+    float sum = 0.f;
+    int n = 0;  // how often t is listed so far
     bool first = true;
-    for (int j = 0; j < i && first; ++j) first = bias_ids[j] != t;
+    for (int j = 0; j < listed; ++j) {
+      const int2 e = list[j];
+      if (e.x != t) continue;
+      if (j < i) first = false;
+      sum = n++ == 0 ? __int_as_float(e.y) : __fadd_rn(sum, __int_as_float(e.y));
+    }
     if (!first) continue;
-    float sum = bias[i];
-    for (int j = i + 1; j < a.n_bias; ++j)
-      if (bias_ids[j] == t) sum = __fadd_rn(sum, bias[j]);
     float x = load1(x_row + t);
-    if (seen && (seen[t >> 5] >> (t & 31) & 1)) x = pen.apply(x, t);
+    if (seen && (seen[t >> 5] >> (t & 31) & 1)) x = pen.apply(x, pen.counts[t]);
     x = __fadd_rn(x, sum);
     if (allowed && !(allowed[t >> 5] >> (t & 31) & 1)) x = -INFINITY;
-    if (a.greedy) best = max(best, greedy_key(x, t));
+    if (greedy && x != -INFINITY) key = max(key, greedy_key(x, t));
     store1(out + t, x);
   }
 
-  if (!a.greedy) return;
+  if (!greedy) return;
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) best = max(best, shfl_xor_u64(best, off));
-  if ((threadIdx.x & 31) == 0) best_warp[threadIdx.x >> 5] = best;
+  for (int off = 16; off > 0; off >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, off));
+  if (lane == 0) best_warp[warp] = key;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kThreads / 32; ++i) best = max(best, best_warp[i]);
+  if (tid == 0) {
+#pragma unroll
+    for (int i = 1; i < kThreads / 32; ++i) key = max(key, best_warp[i]);
     const uint32_t to = mapa_shared(&best_cta[rank], 0);
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(best) : "memory");
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
   }
   cluster_sync_all();
-  if (rank == 0 && threadIdx.x == 0) {
-    best = best_cta[0];
-    for (int i = 1; i < kCluster; ++i) best = max(best, best_cta[i]);
-    a.greedy[row] = (long long)(uint32_t) ~(uint32_t)best;
+  if (rank == 0 && tid == 0) {
+    key = best_cta[0];
+#pragma unroll
+    for (int i = 1; i < kCluster; ++i) key = max(key, best_cta[i]);
+    // no key: every logit is -inf, and token 0 the first of equal ones
+    a.greedy[row] = key == 0 ? 0 : (long long)(uint32_t) ~(uint32_t)key;
   }
 }
 
@@ -240,7 +332,7 @@ __global__ void history_add_kernel(uint32_t* counts, uint32_t* seen, int vocab, 
 
 template <typename T, typename O>
 int launch(const LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
-  const size_t smem = a.n_bias ? (size_t)a.slice / 8 : 0;
+  const size_t smem = a.n_bias ? (size_t)a.slice / 8 + (size_t)a.n_bias * sizeof(int2) : 0;
   auto kernel = wide ? logits_kernel<T, O, true> : logits_kernel<T, O, false>;
   if (smem > 40 * 1024) {
     // an attribute of the function and device: setting it again to the same or a smaller need is harmless
@@ -274,6 +366,7 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   if (p.logits == p.out && (p.dtype != p.out_dtype || (p.rows > 1 && p.row_stride != p.out_stride)))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: in place needs the same type and strides", who);
   if (p.vocab > (1 << 23)) return fail(AOH_ERR_UNSUPPORTED, "%s: vocabulary of %d", who, p.vocab);
+  if (p.n_bias > kMaxBias) return fail(AOH_ERR_UNSUPPORTED, "%s: %d biases of a row, at most %d", who, p.n_bias, kMaxBias);
   if (p.rows > (1 << 27)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
   if (p.rows == 0) return AOH_OK;
   LogitsArgs a{};

@@ -19,7 +19,9 @@
 // Bound: HBM, each of q and k read and written once.  A CTA computes the
 // half x tokens sine / cosine pairs of its tokens once into shared memory and
 // all its heads use them; a row is held by `lanes` (a power of two) threads
-// with 16-byte loads of both members of each rotated pair.
+// with 16-byte loads of both members of each rotated pair.  A thread loads its
+// share of up to four rows before the sines are computed, so that memory works
+// through the fp64 arithmetic.
 #include "common.cuh"
 #include "internal.h"
 
@@ -65,8 +67,7 @@ struct alignas(sizeof(T) * VEC) Pack {
 };
 
 template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float* x) {
-  const Pack<T, VEC> r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+__device__ __forceinline__ void unpack(const Pack<T, VEC>& r, float* x) {
 #pragma unroll
   for (int j = 0; j < VEC; ++j) x[j] = to_f(r.v[j]);
 }
@@ -79,8 +80,9 @@ __device__ __forceinline__ void store(T* p, const float* x) {
 }
 
 // An item is VEC rotated pairs (i.., i + half..) or, behind them, up to
-// 2 * VEC dimensions that pass through.
-template <typename T, int VEC, int ITEMS>
+// 2 * VEC dimensions that pass through.  A thread has ITEMS items of each of
+// ROWS rows.
+template <typename T, int VEC, int ITEMS, int ROWS>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
   __shared__ float2 cs[kMaxTokens * kMaxHalf];
   const int half = a.half, lanes = 1 << a.lanes_log2;
@@ -89,30 +91,11 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   const int head0 = blockIdx.y * a.heads;
   const int nh = min(a.heads, a.hq + a.g - head0);
   const int lane = threadIdx.x & (lanes - 1);
-  const int groups = kThreads >> a.lanes_log2;
+  const int groups = kThreads >> a.lanes_log2, group = threadIdx.x >> a.lanes_log2;
+  const int rows = ntok * nh;  // at most ROWS * groups
   const int pairs = half / VEC;
   const int rest = (a.d - 2 * half) / VEC;  // chunks of VEC behind the rotated dimensions
   const int items = pairs + (rest + 1) / 2;
-
-  float x[ITEMS][2][VEC];
-  const T* src = nullptr;
-  T* dst = nullptr;
-  const T* w = nullptr;
-  int tok = 0;
-  auto locate = [&](int row) {
-    tok = row / nh;
-    const int h = head0 + row % nh;
-    const long long t = tok0 + tok, b = t / a.q_len, c = t % a.q_len;
-    if (h < a.hq) {
-      src = static_cast<const T*>(a.q) + b * a.qs[0] + c * a.qs[1] + h * a.qs[2];
-      dst = static_cast<T*>(a.q_out) + (t * a.hq + h) * a.d;
-      w = static_cast<const T*>(a.qw);
-    } else {
-      src = static_cast<const T*>(a.k) + b * a.ks[0] + c * a.ks[1] + (h - a.hq) * a.ks[2];
-      dst = static_cast<T*>(a.k_out) + (t * a.g + (h - a.hq)) * a.d;
-      w = static_cast<const T*>(a.kw);
-    }
-  };
   // offsets of an item's two chunks (the second -1 where there is none)
   auto chunks = [&](int it, int& o0, int& o1) {
     if (it < pairs) {
@@ -124,27 +107,26 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
       o1 = c + 1 < rest ? o0 + VEC : -1;
     }
   };
-  auto fetch = [&]() {
+  Pack<T, VEC> raw[ROWS][ITEMS][2];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = group + r * groups;
+    if (row >= rows) break;
+    const int h = head0 + row % nh;
+    const long long t = tok0 + row / nh, b = t / a.q_len, c = t % a.q_len;
+    const T* src = h < a.hq ? static_cast<const T*>(a.q) + b * a.qs[0] + c * a.qs[1] + h * a.qs[2]
+                            : static_cast<const T*>(a.k) + b * a.ks[0] + c * a.ks[1] + (h - a.hq) * a.ks[2];
 #pragma unroll
     for (int n = 0; n < ITEMS; ++n) {
       const int it = lane + (n << a.lanes_log2);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) x[n][0][j] = x[n][1][j] = 0.f;
+      raw[r][n][0] = raw[r][n][1] = Pack<T, VEC>{};
       if (it < items) {
         int o0, o1;
         chunks(it, o0, o1);
-        load<T, VEC>(src + o0, x[n][0]);
-        if (o1 >= 0) load<T, VEC>(src + o1, x[n][1]);
+        raw[r][n][0] = *reinterpret_cast<const Pack<T, VEC>*>(src + o0);
+        if (o1 >= 0) raw[r][n][1] = *reinterpret_cast<const Pack<T, VEC>*>(src + o1);
       }
     }
-  };
-
-  int row = threadIdx.x >> a.lanes_log2;
-  const int rows = ntok * nh;
-  // the first row is on its way while the sines and cosines are computed
-  if (row < rows) {
-    locate(row);
-    fetch();
   }
   for (int e = threadIdx.x; e < ntok * half; e += kThreads) {
     const int t = e / half, i = e % half;
@@ -158,17 +140,28 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
     cs[e] = make_float2(c * a.scaling, s * a.scaling);
   }
   __syncthreads();
-
-  // the loop runs as often for every thread of a warp, which shuffles below
-  const int rounds = (rows + groups - 1) / groups;
-  for (int r = 0; r < rounds; ++r) {
-    const bool live = row < rows;
-    if (live && w) {
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int row = group + r * groups;
+    if (row >= rows) break;
+    const int tok = row / nh, h = head0 + row % nh;
+    const long long t = tok0 + tok;
+    const bool is_q = h < a.hq;
+    T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.hq + h) * a.d : static_cast<T*>(a.k_out) + (t * a.g + (h - a.hq)) * a.d;
+    const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
+    float x[ITEMS][2][VEC];
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {
+      unpack<T, VEC>(raw[r][n][0], x[n][0]);
+      unpack<T, VEC>(raw[r][n][1], x[n][1]);
+    }
+    if (w) {
       float ss = 0.f;
 #pragma unroll
       for (int n = 0; n < ITEMS; ++n)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) ss += x[n][0][j] * x[n][0][j] + x[n][1][j] * x[n][1][j];
+      // the row's lanes are consecutive, and take this branch together
       const unsigned mask = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
       for (int off = lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(mask, ss, off);
       const float inv = rsqrtf(ss / (float)a.d + a.eps);
@@ -178,44 +171,49 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
         if (it >= items) continue;
         int o0, o1;
         chunks(it, o0, o1);
-        float w0[VEC], w1[VEC];
-        load<T, VEC>(w + o0, w0);
+        float v[VEC];
+        unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o0), v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[n][0][j] *= inv * w0[j];
+        for (int j = 0; j < VEC; ++j) x[n][0][j] *= inv * v[j];
         if (o1 >= 0) {
-          load<T, VEC>(w + o1, w1);
+          unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o1), v);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) x[n][1][j] *= inv * w1[j];
+          for (int j = 0; j < VEC; ++j) x[n][1][j] *= inv * v[j];
         }
       }
     }
-    if (live) {
 #pragma unroll
-      for (int n = 0; n < ITEMS; ++n) {
-        const int it = lane + (n << a.lanes_log2);
-        if (it >= items) continue;
-        int o0, o1;
-        chunks(it, o0, o1);
-        if (it < pairs) {
-          const float2* row_cs = cs + tok * half + o0;
+    for (int n = 0; n < ITEMS; ++n) {
+      const int it = lane + (n << a.lanes_log2);
+      if (it >= items) continue;
+      int o0, o1;
+      chunks(it, o0, o1);
+      if (it < pairs) {
+        const float2* row_cs = cs + tok * half + o0;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float2 t = row_cs[j];
-            const float u = x[n][0][j], v = x[n][1][j];
-            x[n][0][j] = u * t.x - v * t.y;
-            x[n][1][j] = v * t.x + u * t.y;
-          }
+        for (int j = 0; j < VEC; ++j) {
+          const float2 c = row_cs[j];
+          const float u = x[n][0][j], v = x[n][1][j];
+          x[n][0][j] = u * c.x - v * c.y;
+          x[n][1][j] = v * c.x + u * c.y;
         }
-        store<T, VEC>(dst + o0, x[n][0]);
-        if (o1 >= 0) store<T, VEC>(dst + o1, x[n][1]);
       }
-    }
-    row += groups;
-    if (row < rows) {
-      locate(row);
-      fetch();
+      store<T, VEC>(dst + o0, x[n][0]);
+      if (o1 >= 0) store<T, VEC>(dst + o1, x[n][1]);
     }
   }
+}
+
+template <typename T, int VEC, int ITEMS, int ROWS>
+int launch_rows(RopeAxesArgs& a, cudaStream_t st) {
+  const int heads = a.hq + a.g, most = ROWS * (kThreads >> a.lanes_log2);
+  a.heads = std::min(heads, most);
+  a.tokens = std::max(1, std::min(kMaxTokens, most / heads));
+  const long long gx = (a.n_tokens + a.tokens - 1) / a.tokens;
+  const int gy = (heads + a.heads - 1) / a.heads;
+  if (gx > 0x7fffffffLL || gy > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many rows");
+  rope_axes_kernel<T, VEC, ITEMS, ROWS><<<dim3((unsigned)gx, (unsigned)gy), kThreads, 0, st>>>(a);
+  return cuda_check(cudaGetLastError(), "aoh_rope_axes_qk launch");
 }
 
 template <typename T, int VEC>
@@ -224,28 +222,17 @@ int launch(RopeAxesArgs& a, int num_sms, cudaStream_t st) {
   a.lanes_log2 = 0;
   while ((1 << a.lanes_log2) < items && a.lanes_log2 < 5) ++a.lanes_log2;
   const int per_lane = (items + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
-  const int groups = kThreads >> a.lanes_log2, heads = a.hq + a.g;
-  // Few rows: a CTA takes one round of rows of one token, so that the rows
-  // spread over the SMs (the sines are computed by each of them).  Many: four
-  // tokens and all their heads.
-  if (a.n_tokens * heads <= 4LL * num_sms * groups) {
-    a.tokens = 1;
-    a.heads = std::min(heads, groups);
+  // Few rows: one a thread, so that they spread over the SMs (the sines are
+  // computed by each of a token's CTAs).  Many: four.
+  const bool few = a.n_tokens * (a.hq + a.g) <= 4LL * num_sms * (kThreads >> a.lanes_log2);
+  if constexpr (VEC > 1) {
+    // 16-byte items of at most 256 dimensions: at most 32, one a lane
+    return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 4>(a, st);
   } else {
-    a.tokens = kMaxTokens;
-    a.heads = heads;
+    if (per_lane == 1) return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 4>(a, st);
+    if (per_lane == 2) return few ? launch_rows<T, VEC, 2, 1>(a, st) : launch_rows<T, VEC, 2, 4>(a, st);
+    return few ? launch_rows<T, VEC, 4, 1>(a, st) : launch_rows<T, VEC, 4, 2>(a, st);  // at most 128 items over 32 lanes
   }
-  const long long gx = (a.n_tokens + a.tokens - 1) / a.tokens;
-  if (gx > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many tokens");
-  const dim3 grid((unsigned)gx, (unsigned)((heads + a.heads - 1) / a.heads));
-  if (grid.y > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many heads");
-  if (per_lane == 1)
-    rope_axes_kernel<T, VEC, 1><<<grid, kThreads, 0, st>>>(a);
-  else if (per_lane == 2)
-    rope_axes_kernel<T, VEC, 2><<<grid, kThreads, 0, st>>>(a);
-  else  // scalar items of up to 256 dimensions: at most 128 over 32 lanes
-    rope_axes_kernel<T, VEC, 4><<<grid, kThreads, 0, st>>>(a);
-  return cuda_check(cudaGetLastError(), "aoh_rope_axes_qk launch");
 }
 
 }  // namespace

@@ -81,8 +81,8 @@ def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *
     In this order, in fp32: tokens of the prompt or output are divided by
     ``repetition`` (multiplied where not positive); ``frequency`` times its count
     and ``presence`` are taken from a token of the output; ``bias`` = (ids (N, K)
-    int32, values (N, K) float32) is added, ids outside [0, V) (padding) left out
-    and repeated ids added up; tokens whose bit of ``allowed`` is 0 become -inf.
+    int32, values (N, K) float32, K <= 4096) is added, ids outside [0, V)
+    (padding) left out and repeated ids added up; tokens whose bit of ``allowed`` is 0 become -inf.
     repetition (> 0), presence, frequency: numbers or float32 (N,); they need
     ``history``.  allowed (M, ceil(V / 32)) int32, bit t % 32 of word t // 32 for
     token t; row n has allowed[n], or allowed[allowed_rows[n]] (int32 (N,); an

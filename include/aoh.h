@@ -375,7 +375,7 @@ typedef struct {
   int32_t vocab;
   int32_t dtype;           /* aoh_dtype */
   int32_t out_dtype;
-  int32_t n_bias;
+  int32_t n_bias;          /* <= 4096 */
   int32_t n_allowed;
   float repetition_scalar;
   float presence_scalar;
