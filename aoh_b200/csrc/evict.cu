@@ -6,15 +6,15 @@
 // of their positions; of equal weights the lower position first.  NaN ranks
 // like -inf, -0 like +0.
 //   A cluster of 1 to 8 CTAs takes a row, each CTA a contiguous part of the
-//   middle, which it reads from memory once and holds in shared memory as
-//   32-bit keys in the order of the weights.  Three passes over 11, 11 and 10
-//   bits find the exact bits of the smallest kept weight: every CTA counts its
-//   part, and all of them add up the cluster's histograms.  A count of larger
-//   and of equal keys per warp, summed over warps and CTAs, then gives every
-//   kept key its place, so the output needs no sorting.
-//   Bound: HBM (4 bytes a key in, 8 bytes a kept key out) and the latency of
-//   the passes; a part that does not fit shared memory is read again by each
-//   pass.
+//   middle, which it reads from memory once and holds in registers (up to 32 a
+//   thread) as 32-bit keys in the order of the weights; a part larger than that
+//   is read again by each step.  Three passes over 11, 11 and 10 bits find the
+//   exact bits of the smallest kept weight: every CTA counts its part, and all
+//   of them add up the cluster's histograms.  A count of larger and of equal
+//   keys per warp, summed over warps and CTAs, then gives every kept key its
+//   place, so the output needs no sorting.
+//   Bound: the latency of the passes (HBM would take 4 bytes a key in, 8 bytes a
+//   kept key out).
 //
 // evict: retrieval units' kept rows go to positions 0..keep-1 of the other
 // cache; a streaming unit's sink rows keep their place and the rows of its
@@ -33,19 +33,18 @@ namespace {
 // ---------------------------------------------------------------------------
 // select
 // ---------------------------------------------------------------------------
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kSelMaxCluster = 8;
-constexpr int kSelResident = 48 * 1024;  // keys of a part held in shared memory (192 KB)
+constexpr int kSelMaxKeys = 32;  // of a thread, in registers
 
 struct SelectArgs {
   const float* w;
   long long w_stride;
   int n, sink, recent, take;  // take: keys chosen from the middle
   int keep;
-  int cluster, part;  // CTAs of a row, keys of a part (a multiple of 32)
-  int resident;       // the part is held in shared memory
+  int cluster, part;  // CTAs of a row, keys of a part (a multiple of kSelThreads)
   int32_t* kept;
   float* kept_w;
 };
@@ -63,23 +62,21 @@ __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
   return v;
 }
 // No memory clobber: several are in flight at once, between two cluster barriers.
-__device__ __forceinline__ uint4 ld_dsmem_v4(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+__device__ __forceinline__ uint2 ld_dsmem_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
 
-struct SelectShared {
-  alignas(16) uint32_t hist[kBins];
-  uint32_t scan[kSelWarps];
-  uint32_t gt[kSelWarps], eq[kSelWarps];  // keys above / equal to the threshold, by warp
-  uint32_t total[2];                      // of this CTA
-  uint32_t bin, above;
-};
-
+// Keys per thread: kKeys, in registers; kKeys = 0: any number, from memory.
+// Warp w has the part's keys [w * 32 * per, (w + 1) * 32 * per), 32 neighbours
+// at a time, so that a ballot keeps their order.
+template <int kKeys>
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_constant__ SelectArgs a) {
-  extern __shared__ uint32_t keys[];
-  __shared__ SelectShared s;
+  __shared__ alignas(16) uint32_t s_hist[3][kBins];  // one a pass: the cluster reads one while the next is filled
+  __shared__ uint32_t s_scan[kSelWarps], s_eq[kSelWarps];
+  __shared__ uint32_t s_total[2];  // this CTA's larger and equal keys
+  __shared__ uint32_t s_bin, s_above;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = a.cluster > 1 ? (int)cluster_ctarank() : 0;
   const long long row = blockIdx.x / a.cluster;
@@ -89,7 +86,120 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   const float* wm = w + a.sink + lo;
   int32_t* kept = a.kept + row * a.keep;
   float* kept_w = a.kept_w ? a.kept_w + row * a.keep : nullptr;
+  auto sync = [&] {
+    if (a.cluster > 1)
+      cluster_sync_all();
+    else
+      __syncthreads();
+  };
 
+  if (a.take > 0) {  // the same for every CTA of the cluster
+    const int per = a.part / kSelThreads;  // <= kKeys
+    const int i0 = warp * 32 * per + lane;
+    float x[kKeys ? kKeys : 1];
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j) x[j] = j < per && i0 + 32 * j < cnt ? wm[i0 + 32 * j] : 0.f;
+    // f(key, its index) for each of the thread's keys; every lane of a warp together
+    auto each = [&](auto&& f) {
+      if constexpr (kKeys > 0) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+          if (j < per) f(weight_key(x[j]), i0 + 32 * j);
+      } else {
+        for (int j = 0; j < per; ++j) f(i0 + 32 * j < cnt ? weight_key(wm[i0 + 32 * j]) : 0u, i0 + 32 * j);
+      }
+    };
+    for (int i = tid; i < 3 * kBins / 4; i += kSelThreads) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+
+    uint32_t prefix = 0, left = (uint32_t)a.take;  // the threshold's leading bits, keys still to take
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digit = pass == 2 ? 1023u : 2047u;
+      uint32_t* hist = s_hist[pass];
+      each([&](uint32_t k, int i) {  // digits above this one agree with the threshold
+        if (i < cnt && (pass == 0 || k >> (pass == 2 ? 10 : 21) == prefix)) atomicAdd(&hist[k >> shift & digit], 1u);
+      });
+      sync();
+      // thread t sums the bins kBins - 1 - 2 t and the one below over the cluster
+      static_assert(kBins == 2 * kSelThreads, "a thread's bins are one 8-byte load");
+      const uint32_t* top = hist + kBins - 2 * (tid + 1);
+      uint2 c = make_uint2(0, 0);  // y: the upper bin
+      if (a.cluster > 1) {
+        uint2 v[kSelMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kSelMaxCluster; ++r) v[r] = r < a.cluster ? ld_dsmem_v2(mapa_shared(top, r)) : make_uint2(0, 0);
+#pragma unroll
+        for (int r = 0; r < kSelMaxCluster; ++r) {
+          c.x += v[r].x;
+          c.y += v[r].y;
+        }
+      } else {
+        c = *reinterpret_cast<const uint2*>(top);
+      }
+      uint32_t incl = c.x + c.y;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+      }
+      if (lane == 31) s_scan[warp] = incl;
+      __syncthreads();
+      const uint32_t before = incl - c.x - c.y + __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0u);
+      if (before < left && before + c.x + c.y >= left) {  // one thread
+        const bool upper = before + c.y >= left;
+        s_bin = (uint32_t)(kBins - 1 - 2 * tid - (upper ? 0 : 1));
+        s_above = before + (upper ? 0 : c.y);
+      }
+      __syncthreads();
+      prefix = pass == 0 ? s_bin : pass == 1 ? prefix << 11 | s_bin : prefix << 10 | s_bin;
+      left -= s_above;
+    }
+    // prefix: the threshold's bits; `left` of the keys equal to it are taken
+    const uint32_t thr = prefix;
+
+    uint32_t gt = 0, eq = 0;
+    each([&](uint32_t k, int i) {
+      gt += i < cnt && k > thr;
+      eq += i < cnt && k == thr;
+    });
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    if (lane == 0) {
+      s_scan[warp] = gt;
+      s_eq[warp] = eq;
+    }
+    __syncthreads();
+    // larger / equal keys before this warp's
+    uint32_t bg = __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0u);
+    uint32_t be = __reduce_add_sync(0xffffffffu, lane < warp ? s_eq[lane] : 0u);
+    if (a.cluster > 1) {
+      if (tid == kSelThreads - 1) {
+        s_total[0] = bg + gt;
+        s_total[1] = be + eq;
+      }
+      cluster_sync_all();
+      uint2 v = make_uint2(0, 0);
+      if (lane < rank) v = make_uint2(ld_dsmem_u32(mapa_shared(&s_total[0], lane)), ld_dsmem_u32(mapa_shared(&s_total[1], lane)));
+      bg += __reduce_add_sync(0xffffffffu, v.x);
+      be += __reduce_add_sync(0xffffffffu, v.y);
+      cluster_arrive();  // no CTA leaves while another may still read its counts
+    }
+    const unsigned below = (1u << lane) - 1u;
+    each([&](uint32_t k, int i) {
+      const bool is_gt = i < cnt && k > thr, is_eq = i < cnt && k == thr;
+      const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
+      const uint32_t re = be + __popc(me & below);
+      if (is_gt || (is_eq && re < left)) {
+        const int at = a.sink + (int)(bg + __popc(mg & below) + min(re, left));
+        kept[at] = a.sink + lo + i;
+        if (kept_w) kept_w[at] = wm[i];
+      }
+      bg += __popc(mg);
+      be += __popc(me);
+    });
+  }
   // the first and the last keys are kept as they are
   for (int i = rank * kSelThreads + tid; i < a.sink + a.recent; i += a.cluster * kSelThreads) {
     const int at = i < a.sink ? i : a.keep - a.sink - a.recent + i;
@@ -97,150 +207,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     kept[at] = p;
     if (kept_w) kept_w[at] = w[p];
   }
-  if (a.take == 0) return;  // the same for every CTA of the cluster
-
-  if (a.resident) {
-#pragma unroll 8
-    for (int i = tid; i < cnt; i += kSelThreads) keys[i] = weight_key(wm[i]);
-  }
-  auto key = [&](int i) { return a.resident ? keys[i] : weight_key(wm[i]); };
-
-  uint32_t prefix = 0, left = (uint32_t)a.take;  // the threshold's leading bits, keys still to take
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-    const int bins = pass == 2 ? 1024 : kBins;
-    for (int i = tid; i < kBins; i += kSelThreads) s.hist[i] = 0;
-    __syncthreads();
-    for (int i0 = warp * 32; i0 < cnt; i0 += kSelThreads) {
-      const int i = i0 + lane;
-      const uint32_t k = i < cnt ? key(i) : 0;
-      // digits above this one agree with the threshold
-      const bool in = i < cnt && (pass == 0 || k >> (shift + (pass == 2 ? 10 : 11)) == prefix);
-      const uint32_t b = k >> shift & (uint32_t)(bins - 1);
-      const unsigned m = __ballot_sync(0xffffffffu, in);
-      if (m == 0) continue;
-      // many equal weights (zeros) would be added one by one to one address
-      const uint32_t b0 = __shfl_sync(0xffffffffu, b, __ffs(m) - 1);
-      const unsigned same = __ballot_sync(0xffffffffu, in && b == b0);
-      if (lane == __ffs(m) - 1)
-        atomicAdd(&s.hist[b0], (uint32_t)__popc(same));
-      else if (in && b != b0)
-        atomicAdd(&s.hist[b], 1u);
-    }
-    if (a.cluster > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    // thread t sums the bins kBins - 1 - 4 t and the three below over the cluster
-    constexpr int per = kBins / kSelThreads;
-    static_assert(per == 4, "a thread's bins are one 16-byte load");
-    const uint32_t* top = &s.hist[kBins - per * (tid + 1)];
-    uint32_t c[4] = {0, 0, 0, 0};
-    if (a.cluster > 1) {
-      uint4 v[kSelMaxCluster];
-#pragma unroll
-      for (int r = 0; r < kSelMaxCluster; ++r)
-        v[r] = r < a.cluster ? ld_dsmem_v4(mapa_shared(top, r)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < kSelMaxCluster; ++r) {
-        c[0] += v[r].w;
-        c[1] += v[r].z;
-        c[2] += v[r].y;
-        c[3] += v[r].x;
-      }
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(top);
-      c[0] = v.w;
-      c[1] = v.z;
-      c[2] = v.y;
-      c[3] = v.x;
-    }
-    const uint32_t mine = c[0] + c[1] + c[2] + c[3];
-    uint32_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
-      if (lane >= off) incl += v;
-    }
-    if (lane == 31) s.scan[warp] = incl;
-    __syncthreads();
-    uint32_t before = incl - mine;
-    for (int i = 0; i < warp; ++i) before += s.scan[i];
-    if (before < left && before + mine >= left) {
-#pragma unroll
-      for (int j = 0; j < per; ++j) {
-        if (before < left && before + c[j] >= left) {
-          s.bin = (uint32_t)(kBins - 1 - (tid * per + j));
-          s.above = before;
-        }
-        before += c[j];
-      }
-    }
-    // every CTA has read the histograms before any is cleared
-    if (a.cluster > 1)
-      cluster_sync_all();
-    else
-      __syncthreads();
-    prefix = pass == 0 ? s.bin : pass == 1 ? prefix << 11 | s.bin : prefix << 10 | s.bin;
-    left -= s.above;
-  }
-  // prefix: the threshold's bits; `left` of the keys equal to it are taken
-  const uint32_t thr = prefix;
-
-  // keys of warp w: a contiguous range of whole 32-key groups
-  const int groups = (cnt + 31) / 32, per_warp = (groups + kSelWarps - 1) / kSelWarps;
-  const int g0 = min(groups, warp * per_warp), g1 = min(groups, g0 + per_warp);
-  uint32_t gt = 0, eq = 0;
-  for (int g = g0; g < g1; ++g) {
-    const int i = g * 32 + lane;
-    const uint32_t k = i < cnt ? key(i) : 0;
-    gt += __popc(__ballot_sync(0xffffffffu, i < cnt && k > thr));
-    eq += __popc(__ballot_sync(0xffffffffu, i < cnt && k == thr));
-  }
-  if (lane == 0) {
-    s.gt[warp] = gt;
-    s.eq[warp] = eq;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    uint32_t tg = 0, te = 0;
-    for (int i = 0; i < kSelWarps; ++i) {
-      tg += s.gt[i];
-      te += s.eq[i];
-    }
-    s.total[0] = tg;
-    s.total[1] = te;
-  }
-  if (a.cluster > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
-  uint32_t bg = 0, be = 0;  // larger / equal keys before this warp's range
-  for (int r = 0; r < rank; ++r) {
-    bg += ld_dsmem_u32(mapa_shared(&s.total[0], r));
-    be += ld_dsmem_u32(mapa_shared(&s.total[1], r));
-  }
-  for (int i = 0; i < warp; ++i) {
-    bg += s.gt[i];
-    be += s.eq[i];
-  }
-  const unsigned below = (1u << lane) - 1u;
-  for (int g = g0; g < g1; ++g) {
-    const int i = g * 32 + lane;
-    const uint32_t k = i < cnt ? key(i) : 0;
-    const bool is_gt = i < cnt && k > thr, is_eq = i < cnt && k == thr;
-    const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
-    const uint32_t rank_eq = be + __popc(me & below);
-    if (is_gt || (is_eq && rank_eq < left)) {
-      const int at = a.sink + (int)(bg + __popc(mg & below) + min(rank_eq, left));
-      kept[at] = a.sink + lo + i;
-      if (kept_w) kept_w[at] = wm[i];
-    }
-    bg += __popc(mg);
-    be += __popc(me);
-  }
-  // no CTA leaves while another may still read its totals
-  if (a.cluster > 1) cluster_sync_all();
+  if (a.take > 0 && a.cluster > 1) cluster_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -349,11 +316,8 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   int dev = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
-  static PerDeviceOnce once;
-  rc = once.run(dev, [&] {
-    return cuda_check(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelResident * 4),
-                      "aoh_select_keys shared memory");
-  });
+  int sms = 0;
+  rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
   if (rc) return rc;
   SelectArgs a{};
   a.w = weights;
@@ -364,17 +328,21 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   a.keep = keep;
   a.take = keep - sink - recent;
   const int mid = n - sink - recent;
-  // a CTA for every 4096 keys of a row, 8 at most: below that the passes' barriers cost more than their loads
+  // A CTA for every 8192 keys of a row, 8 at most, as long as all of them are
+  // one wave of the GPU (an eighth of the SMs cannot be filled with clusters of
+  // 8: 18 rows of 64K take 38 us in them, 32 rows in clusters of 4 22 us); a
+  // thread then has 8 keys, or more.
   a.cluster = 1;
-  while (a.cluster < kSelMaxCluster && a.cluster * 4096 < mid) a.cluster *= 2;
-  a.part = ((mid + a.cluster - 1) / a.cluster + 31) / 32 * 32;
-  a.resident = a.part <= kSelResident;
+  while (a.cluster < kSelMaxCluster && a.cluster * 8 * kSelThreads < mid &&
+         ((long long)rows * a.cluster * 2 <= sms * 7 / 8 || a.cluster * kSelMaxKeys * kSelThreads < mid))
+    a.cluster *= 2;
+  a.part = ((mid + a.cluster - 1) / a.cluster + kSelThreads - 1) / kSelThreads * kSelThreads;
+  const int per = a.part / kSelThreads;
   a.kept = kept;
   a.kept_w = kept_weights;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * a.cluster));
   cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = a.resident ? (size_t)a.part * 4 : 0;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -382,7 +350,12 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, select_kernel, a), "aoh_select_keys launch");
+  auto kernel = per <= 2    ? select_kernel<2>
+                : per <= 8  ? select_kernel<8>
+                : per <= 16 ? select_kernel<16>
+                : per <= kSelMaxKeys ? select_kernel<kSelMaxKeys>
+                                     : select_kernel<0>;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "aoh_select_keys launch");
 }
 
 extern "C" int aoh_kv_evict(aoh_kv_cache* src, aoh_kv_cache* dst, int32_t past_len, const int32_t* kept,

@@ -16,15 +16,16 @@
 // pass reads, 1 bit a token; the count words are read for the tokens it names.
 //
 // Bound: HBM, logits in and fp32 out (6 bytes a token for bf16 logits, 1/4
-// byte for the two bitmaps), and latency for a few rows.  One cluster of 8 CTAs
-// takes a row, each an eighth of the vocabulary; the greedy token is reduced
-// over the cluster in shared memory, so one launch and no workspace.  A thread
-// has the loads of four groups of 8 tokens (or 8 single ones) in flight before
-// it works on any.  A CTA's biased tokens are listed in shared memory first, in
-// the order given, and marked in a bitmap there; the main pass leaves them out
-// and a thread for each listed token does it alone, so that the sum over a
-// token listed more than once has a fixed order.
+// byte for the two bitmaps), and latency for a few rows.  A cluster of up to 16
+// CTAs takes a row, each a slice of the vocabulary of 8192 tokens (or more,
+// where 16 slices do not reach): a thread then has all its loads, four groups
+// of 8 tokens, in flight at once.  The greedy token is reduced over the cluster
+// in shared memory, so one launch and no workspace.  A CTA's biased tokens are
+// listed in shared memory, in the order given, and marked in a bitmap there;
+// the main pass leaves them out and a thread for each listed token does it
+// alone, so that the sum over a token listed more than once has a fixed order.
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "internal.h"
@@ -32,15 +33,20 @@
 namespace aoh {
 namespace {
 
-constexpr int kCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kThreads = 256;
 constexpr int kMaxBias = 4096;  // biases of a row (32 KB of shared memory if all fall into one slice)
+constexpr int kSlice = kThreads * 32;  // tokens whose loads a CTA has in flight at once (a quarter where rows are not aligned)
+constexpr int kMaxVocab = 1 << 23;
 constexpr uint32_t kInPrompt = 0x80000000u;
+// two bits a token of the largest slice, and the list
+constexpr int kMaxSmem = kMaxVocab / kMaxCluster / 4 + kMaxBias * 8;
 
 struct LogitsArgs {
   const void* logits;
   long long row_stride;  // elements
-  int vocab, slice;      // tokens of one CTA, a multiple of 256
+  int vocab;
+  int cluster, slice;    // CTAs of a row, tokens of one CTA (a multiple of 256)
   const uint32_t *counts, *seen;
   const float *repetition, *presence, *frequency;  // per row, or null: the scalar
   float repetition_s, presence_s, frequency_s;
@@ -60,21 +66,40 @@ __device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float x) { *p = __float2bfloat16(x); }
 
-// 8 consecutive elements, 16-byte aligned
-__device__ __forceinline__ void load8(const float* p, float* x) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-  x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* x) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = bf16_lo(w[j]);
-    x[2 * j + 1] = bf16_hi(w[j]);
+// 8 consecutive elements, 16-byte aligned, as loaded and as floats
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = reinterpret_cast<const float4*>(p)[0];
+    b = reinterpret_cast<const float4*>(p)[1];
   }
-}
+  __device__ __forceinline__ void get(float* x) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float* x) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = bf16_lo(w[j]);
+      x[2 * j + 1] = bf16_hi(w[j]);
+    }
+  }
+};
+template <typename T>
+struct Raw1 {
+  T a;
+  __device__ __forceinline__ void load(const T* p) { a = *p; }
+  __device__ __forceinline__ void get(float* x) const { x[0] = load1(&a); }
+};
 __device__ __forceinline__ void store8(float* p, const float* x) {
   reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -91,11 +116,13 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float* x) {
 struct RowPenalties {
   float rep, pres, freq;
   const uint32_t* counts;
+  // w: the token's count word; 0 leaves x as it is
   __device__ __forceinline__ float apply(float x, uint32_t w) const {
-    x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
     const uint32_t n = w & ~kInPrompt;
-    x = __fsub_rn(x, __fmul_rn(freq, (float)n));
-    return n ? __fsub_rn(x, pres) : x;
+    float y = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+    y = __fsub_rn(y, __fmul_rn(freq, (float)n));
+    y = n ? __fsub_rn(y, pres) : y;
+    return w ? y : x;
   }
 };
 
@@ -104,6 +131,17 @@ __device__ __forceinline__ unsigned long long greedy_key(float x, int t) {
   uint32_t u = __float_as_uint(x + 0.f);
   u = x != x ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
   return ((unsigned long long)u << 32) | (uint32_t)~t;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // The best of a thread's tokens, seen in ascending order.  -inf gives no key:
@@ -118,6 +156,14 @@ struct Best {
     }
     if (v != v) nan_t = min(nan_t, at);
   }
+  // v, from the last of a group to the first, of which mx (NaN if any is) is the largest
+  __device__ __forceinline__ void note(float v, float mx, int at) {
+    if (v == mx) {
+      x = mx;
+      t = at;
+    }
+    if (v != v) nan_t = min(nan_t, at);
+  }
   __device__ __forceinline__ unsigned long long key() const {
     unsigned long long k = t == INT_MAX ? 0 : greedy_key(x, t);
     return nan_t == INT_MAX ? k : greedy_key(NAN, nan_t);
@@ -125,16 +171,17 @@ struct Best {
 };
 
 template <typename T, typename O, bool kWide>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
-    logits_kernel(const __grid_constant__ LogitsArgs a) {
-  extern __shared__ uint32_t smem[];  // with biases: a bit per token of the slice, then the slice's (id, value) list
+__global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ LogitsArgs a) {
+  // with biases: two bits per token of the slice, then the slice's (id, value) list
+  extern __shared__ __align__(16) uint32_t smem[];
   __shared__ unsigned long long best_warp[kThreads / 32];
-  __shared__ unsigned long long best_cta[kCluster];
+  __shared__ unsigned long long best_cta[kMaxCluster];
   __shared__ int s_count[kThreads / 32];
-  uint32_t* biased = smem;
-  int2* list = reinterpret_cast<int2*>(smem + a.slice / 32);
-  const int rank = (int)cluster_ctarank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / kCluster;
+  uint32_t *biased = smem, *repeated = smem + a.slice / 32;
+  int2* list = reinterpret_cast<int2*>(smem + a.slice / 16);
+  const int rank = a.cluster > 1 ? (int)cluster_ctarank() : 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / a.cluster;
   const int lo = rank * a.slice, hi = min(lo + a.slice, a.vocab);  // may be empty
   const int words = (a.vocab + 31) >> 5;
   const T* x_row = static_cast<const T*>(a.logits) + row * a.row_stride;
@@ -152,11 +199,34 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
   const bool greedy = a.greedy != nullptr;
   Best best;
 
+  // A thread's tokens of one round: U units of N neighbours, a stride apart.
+  // Rows that are not 16-byte aligned take single tokens, a lane each of a word.
+  constexpr int N = kWide ? 8 : 1, U = kWide ? 4 : 8;
+  constexpr uint32_t kOnes = (1u << N) - 1u;
+  using Raw = typename std::conditional<kWide, Raw8<T>, Raw1<T>>::type;
+  Raw raw[U];
+  uint32_t s[U], al[U];
+  auto fetch = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kThreads * N;
+      s[u] = 0;
+      al[u] = kOnes;
+      if (t < hi) {
+        raw[u].load(x_row + t);
+        if (seen) s[u] = seen[t >> 5] >> (t & 31) & kOnes;
+        if (allowed) al[u] = allowed[t >> 5] >> (t & 31) & kOnes;
+      }
+    }
+  };
+  const int first = lo + tid * N;
+  fetch(first);
+
   int listed = 0;
   if (a.n_bias) {
     const int32_t* ids = a.bias_ids + (long long)row * a.n_bias;
     const float* values = a.bias + (long long)row * a.n_bias;
-    for (int i = tid; i < a.slice / 32; i += kThreads) biased[i] = 0;
+    for (int i = tid; i < a.slice / 16; i += kThreads) smem[i] = 0;
     __syncthreads();
     for (int i0 = 0; i0 < a.n_bias; i0 += kThreads) {
       const int i = i0 + tid;
@@ -165,7 +235,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
       const bool in = id >= lo && id < hi;
       const unsigned m = __ballot_sync(0xffffffffu, in);
       if (lane == 0) s_count[warp] = __popc(m);
-      if (in) atomicOr(&biased[(id - lo) >> 5], 1u << (id & 31));
+      if (in) {
+        const uint32_t bit = 1u << (id & 31);
+        if (atomicOr(&biased[(id - lo) >> 5], bit) & bit) atomicOr(&repeated[(id - lo) >> 5], bit);
+      }
       __syncthreads();
       int at = listed + __popc(m & ((1u << lane) - 1u));
 #pragma unroll
@@ -178,116 +251,80 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
     }
   }
 
-  if (kWide) {
-    // groups of 8 tokens (vocab is a multiple of 8 here), four in flight
-    constexpr int U = 4;
-    for (int t0 = lo + tid * 8; t0 < hi; t0 += U * kThreads * 8) {
-      float x[U][8];
-      uint32_t s[U], al[U];
+  for (int t0 = first; t0 < hi; t0 += U * kThreads * N) {
+    if (t0 != first) fetch(t0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kThreads * 8;
-        s[u] = 0;
-        al[u] = 0xffu;
-        if (t < hi) {
-          load8(x_row + t, x[u]);
-          if (seen) s[u] = seen[t >> 5] >> (t & 31) & 0xffu;
-          if (allowed) al[u] = allowed[t >> 5] >> (t & 31) & 0xffu;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kThreads * 8;
-        if (t >= hi) break;
-        if (s[u]) {
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * kThreads * N;
+      if (t >= hi) break;
+      float x[N];
+      raw[u].get(x);
+      if (s[u]) {
+        uint32_t c[N];
+        if constexpr (kWide) {
           const uint4 c0 = reinterpret_cast<const uint4*>(pen.counts + t)[0], c1 = reinterpret_cast<const uint4*>(pen.counts + t)[1];
-          const uint32_t c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (s[u] >> j & 1) x[u][j] = pen.apply(x[u][j], c[j]);
+          c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w;
+          c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+        } else {
+          c[0] = pen.counts[t];
         }
-        if (al[u] != 0xffu) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(al[u] >> j & 1)) x[u][j] = -INFINITY;
-        }
-        const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> (t & 31) & 0xffu : 0u;
-        if (bi) {  // without the biased ones
+        for (int j = 0; j < N; ++j) x[j] = pen.apply(x[j], c[j]);
+      }
+      if (al[u] != kOnes) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(bi >> j & 1)) {
-              store1(out + t + j, x[u][j]);
-              best.one(x[u][j], t + j);
-            }
-          continue;
-        }
-        store8(out + t, x[u]);
+        for (int j = 0; j < N; ++j) x[j] = al[u] >> j & 1 ? x[j] : -INFINITY;
+      }
+      const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> (t & 31) & kOnes : 0u;
+      if (bi || !kWide) {  // one by one, without the biased ones
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (!(bi >> j & 1)) {
+            store1(out + t + j, x[j]);
+            if (greedy) best.one(x[j], t + j);
+          }
+        continue;
+      }
+      if constexpr (kWide) {
+        store8(out + t, x);
         if (greedy) {
-          const float mx = fmaxf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])),
-                                 fmaxf(fmaxf(x[u][4], x[u][5]), fmaxf(x[u][6], x[u][7])));
-          bool nan = false;
+          const float mx = max_nan(max_nan(max_nan(x[0], x[1], x[2]), x[3], x[4]), max_nan(x[5], x[6], x[7]));
+          if (!(mx <= best.x)) {  // larger, or NaN
 #pragma unroll
-          for (int j = 0; j < 8; ++j) nan |= x[u][j] != x[u][j];
-          if (mx > best.x || nan) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) best.one(x[u][j], t + j);
+            for (int j = N - 1; j >= 0; --j) best.note(x[j], mx, t + j);
           }
         }
-      }
-    }
-  } else {
-    // rows that are not 16-byte aligned: a lane takes one token of the warp's word, eight words in flight
-    constexpr int U = 8;
-    for (int t0 = lo + tid; t0 < hi; t0 += U * kThreads) {
-      float x[U];
-      uint32_t s[U], al[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kThreads;
-        s[u] = 0;
-        al[u] = 1;
-        x[u] = 0.f;
-        if (t < hi) {
-          x[u] = load1(x_row + t);
-          if (seen) s[u] = seen[t >> 5] >> lane & 1;
-          if (allowed) al[u] = allowed[t >> 5] >> lane & 1;
-        }
-      }
-      uint32_t c[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) c[u] = s[u] ? pen.counts[t0 + u * kThreads] : 0;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int t = t0 + u * kThreads;
-        if (t >= hi) break;
-        if (s[u]) x[u] = pen.apply(x[u], c[u]);
-        if (!al[u]) x[u] = -INFINITY;
-        if (a.n_bias && (biased[(t - lo) >> 5] >> lane & 1)) continue;
-        store1(out + t, x[u]);
-        if (greedy) best.one(x[u], t);
       }
     }
   }
   unsigned long long key = best.key();
 
+  // a biased token, with the sum of its biases
+  auto finish = [&](int t, float sum) {
+    const uint32_t count = seen ? pen.counts[t] : 0u;
+    const bool ok = !allowed || allowed[t >> 5] >> (t & 31) & 1;
+    float y = pen.apply(load1(x_row + t), count);
+    y = ok ? __fadd_rn(y, sum) : -INFINITY;
+    if (greedy && y != -INFINITY) key = max(key, greedy_key(y, t));
+    store1(out + t, y);
+  };
   for (int i = tid; i < listed; i += kThreads) {
-    const int t = list[i].x;
-    float sum = 0.f;
-    int n = 0;  // how often t is listed so far
-    bool first = true;
-    for (int j = 0; j < listed; ++j) {
-      const int2 e = list[j];
-      if (e.x != t) continue;
-      if (j < i) first = false;
-      sum = n++ == 0 ? __int_as_float(e.y) : __fadd_rn(sum, __int_as_float(e.y));
+    const int2 e = list[i];
+    float sum = __int_as_float(e.y);
+    if (repeated[(e.x - lo) >> 5] >> (e.x & 31) & 1) {
+      // listed more than once: the first entry adds them up in their order, from -0, which leaves the first as it is
+      int first = -1;
+      sum = -0.f;
+#pragma unroll 4
+      for (int j = 0; j < listed; ++j) {
+        const int2 o = list[j];
+        const float next = __fadd_rn(sum, __int_as_float(o.y));
+        sum = o.x == e.x ? next : sum;
+        first = o.x == e.x && first < 0 ? j : first;
+      }
+      if (first != i) continue;
     }
-    if (!first) continue;
-    float x = load1(x_row + t);
-    if (seen && (seen[t >> 5] >> (t & 31) & 1)) x = pen.apply(x, pen.counts[t]);
-    x = __fadd_rn(x, sum);
-    if (allowed && !(allowed[t >> 5] >> (t & 31) & 1)) x = -INFINITY;
-    if (greedy && x != -INFINITY) key = max(key, greedy_key(x, t));
-    store1(out + t, x);
+    finish(e.x, sum);
   }
 
   if (!greedy) return;
@@ -298,17 +335,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads, 4)
   if (tid == 0) {
 #pragma unroll
     for (int i = 1; i < kThreads / 32; ++i) key = max(key, best_warp[i]);
-    const uint32_t to = mapa_shared(&best_cta[rank], 0);
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
+    if (a.cluster > 1) {
+      const uint32_t to = mapa_shared(&best_cta[rank], 0);
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(key) : "memory");
+    }
   }
-  cluster_sync_all();
-  if (rank == 0 && tid == 0) {
-    key = best_cta[0];
-#pragma unroll
-    for (int i = 1; i < kCluster; ++i) key = max(key, best_cta[i]);
-    // no key: every logit is -inf, and token 0 the first of equal ones
-    a.greedy[row] = key == 0 ? 0 : (long long)(uint32_t) ~(uint32_t)key;
+  if (a.cluster > 1) {
+    cluster_sync_all();
+    if (rank == 0 && tid == 0) {
+      key = best_cta[0];
+      for (int i = 1; i < a.cluster; ++i) key = max(key, best_cta[i]);
+    }
   }
+  // no key: every logit is -inf, and token 0 the first of equal ones
+  if (rank == 0 && tid == 0) a.greedy[row] = key == 0 ? 0 : (long long)(uint32_t) ~(uint32_t)key;
 }
 
 // history[n, ids[n, i]]: +1 in the output, or the mark of the prompt
@@ -330,18 +370,37 @@ __global__ void history_add_kernel(uint32_t* counts, uint32_t* seen, int vocab, 
   }
 }
 
+template <typename T, typename O, bool kWide>
+int launch(const LogitsArgs& a, int rows, cudaStream_t st) {
+  auto kernel = logits_kernel<T, O, kWide>;
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  static PerDeviceOnce once;
+  rc = once.run(dev, [&] {
+    const int e = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                             "aoh_logits_penalize cluster size");
+    return e ? e
+             : cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem),
+                          "aoh_logits_penalize shared memory");
+  });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * a.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = a.n_bias ? (size_t)a.slice / 4 + (size_t)a.n_bias * sizeof(int2) : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "aoh_logits_penalize launch");
+}
 template <typename T, typename O>
 int launch(const LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
-  const size_t smem = a.n_bias ? (size_t)a.slice / 8 + (size_t)a.n_bias * sizeof(int2) : 0;
-  auto kernel = wide ? logits_kernel<T, O, true> : logits_kernel<T, O, false>;
-  if (smem > 40 * 1024) {
-    // an attribute of the function and device: setting it again to the same or a smaller need is harmless
-    const int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                              "aoh_logits_penalize shared memory");
-    if (rc) return rc;
-  }
-  kernel<<<rows * kCluster, kThreads, smem, st>>>(a);
-  return cuda_check(cudaGetLastError(), "aoh_logits_penalize launch");
+  return wide ? launch<T, O, true>(a, rows, st) : launch<T, O, false>(a, rows, st);
 }
 
 }  // namespace
@@ -365,15 +424,20 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: %d mask rows for %d rows", who, p.n_allowed, p.rows);
   if (p.logits == p.out && (p.dtype != p.out_dtype || (p.rows > 1 && p.row_stride != p.out_stride)))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: in place needs the same type and strides", who);
-  if (p.vocab > (1 << 23)) return fail(AOH_ERR_UNSUPPORTED, "%s: vocabulary of %d", who, p.vocab);
+  if (p.vocab > kMaxVocab) return fail(AOH_ERR_UNSUPPORTED, "%s: vocabulary of %d", who, p.vocab);
   if (p.n_bias > kMaxBias) return fail(AOH_ERR_UNSUPPORTED, "%s: %d biases of a row, at most %d", who, p.n_bias, kMaxBias);
-  if (p.rows > (1 << 27)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
+  if (p.rows > (1 << 26)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
   if (p.rows == 0) return AOH_OK;
+  const int vin = p.dtype == AOH_BF16 ? 8 : 4, vout = p.out_dtype == AOH_BF16 ? 8 : 4;
+  const bool wide = p.vocab % 8 == 0 && (p.rows == 1 || (p.row_stride % vin == 0 && p.out_stride % vout == 0)) &&
+                    reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   LogitsArgs a{};
   a.logits = p.logits;
   a.row_stride = p.row_stride;
   a.vocab = p.vocab;
-  a.slice = ((p.vocab + kCluster - 1) / kCluster + 255) / 256 * 256;
+  a.cluster = 1;
+  while (a.cluster < kMaxCluster && a.cluster * (wide ? kSlice : kSlice / 4) < p.vocab) a.cluster *= 2;
+  a.slice = ((p.vocab + a.cluster - 1) / a.cluster + 255) / 256 * 256;
   a.counts = reinterpret_cast<const uint32_t*>(p.counts);
   a.seen = reinterpret_cast<const uint32_t*>(p.seen);
   a.repetition = p.repetition;
@@ -391,9 +455,6 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   a.out = p.out;
   a.out_stride = p.out_stride;
   a.greedy = reinterpret_cast<long long*>(p.greedy);
-  const int vin = p.dtype == AOH_BF16 ? 8 : 4, vout = p.out_dtype == AOH_BF16 ? 8 : 4;
-  const bool wide = p.vocab % 8 == 0 && (p.rows == 1 || (p.row_stride % vin == 0 && p.out_stride % vout == 0)) &&
-                    reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p.dtype == AOH_BF16)
     return p.out_dtype == AOH_BF16 ? launch<__nv_bfloat16, __nv_bfloat16>(a, p.rows, wide, st)

@@ -16,12 +16,13 @@
 // the reduction to one turn are done in fp64, the sine and cosine of the
 // remainder in fp32 (their error is a few 2^-24).
 //
-// Bound: HBM, each of q and k read and written once.  A CTA computes the
-// half x tokens sine / cosine pairs of its tokens once into shared memory and
-// all its heads use them; a row is held by `lanes` (a power of two) threads
-// with 16-byte loads of both members of each rotated pair.  A thread loads its
-// share of up to four rows before the sines are computed, so that memory works
-// through the fp64 arithmetic.
+// Bound: HBM, each of q and k read and written once.  A CTA computes the sines
+// and cosines of its tokens once into shared memory and all its rows use them
+// (eight of them in every thread's registers took 128 registers a thread and
+// was slower); a row is held by `lanes` (a power of two) threads with 16-byte
+// loads of both members of each rotated pair, which are under way while the
+// sines are computed.  Two rows a thread and five CTAs an SM keep enough loads
+// in flight.
 #include "common.cuh"
 #include "internal.h"
 
@@ -40,7 +41,8 @@ struct RopeAxesArgs {
   long long qs[3], ks[3], ps[3];  // strides in elements: batch, token, head / axis, batch, token
   long long n_tokens;
   int q_len, hq, g, d, half;
-  int tokens, heads;  // of one CTA
+  int tokens, heads;     // of one CTA
+  uint32_t heads_magic;  // floor(2^32 / heads) + 1: row / heads is the high word of row * magic (rows of a CTA are few)
   int lanes_log2;
   float eps, scaling;
   bool pos64;
@@ -62,7 +64,7 @@ __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat
 
 // VEC consecutive elements (16 bytes, or one).
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
+struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
@@ -83,19 +85,30 @@ __device__ __forceinline__ void store(T* p, const float* x) {
 // 2 * VEC dimensions that pass through.  A thread has ITEMS items of each of
 // ROWS rows.
 template <typename T, int VEC, int ITEMS, int ROWS>
-__global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
-  __shared__ float2 cs[kMaxTokens * kMaxHalf];
+__global__ void __launch_bounds__(kThreads, ITEMS > 1 || ROWS > 2 ? 3 : 5)
+    rope_axes_kernel(const __grid_constant__ RopeAxesArgs a) {
+  __shared__ alignas(16) float s_cos[kMaxTokens * kMaxHalf], s_sin[kMaxTokens * kMaxHalf];
   const int half = a.half, lanes = 1 << a.lanes_log2;
-  const long long tok0 = (long long)blockIdx.x * a.tokens;
-  const int ntok = (int)min((long long)a.tokens, a.n_tokens - tok0);
+  const unsigned tok0 = blockIdx.x * (unsigned)a.tokens;
+  const int ntok = (int)min((unsigned)a.tokens, (unsigned)a.n_tokens - tok0);
   const int head0 = blockIdx.y * a.heads;
   const int nh = min(a.heads, a.hq + a.g - head0);
   const int lane = threadIdx.x & (lanes - 1);
   const int groups = kThreads >> a.lanes_log2, group = threadIdx.x >> a.lanes_log2;
-  const int rows = ntok * nh;  // at most ROWS * groups
+  const int rows = ntok * a.heads;  // at most ROWS * groups; the last of a token's CTAs may leave some out
   const int pairs = half / VEC;
   const int rest = (a.d - 2 * half) / VEC;  // chunks of VEC behind the rotated dimensions
   const int items = pairs + (rest + 1) / 2;
+  // (batch, token) of the CTA's first token; the few behind it are counted on
+  const unsigned b0 = tok0 / (unsigned)a.q_len, c0 = tok0 - b0 * (unsigned)a.q_len;
+  auto locate = [&](int tok, int& b, int& c) {
+    b = (int)b0;
+    c = (int)c0 + tok;
+    while (c >= a.q_len) {
+      c -= a.q_len;
+      ++b;
+    }
+  };
   // offsets of an item's two chunks (the second -1 where there is none)
   auto chunks = [&](int it, int& o0, int& o1) {
     if (it < pairs) {
@@ -107,13 +120,21 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
       o1 = c + 1 < rest ? o0 + VEC : -1;
     }
   };
-  Pack<T, VEC> raw[ROWS][ITEMS][2];
+  int toks[ROWS], hs[ROWS];  // -1: no such row
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int row = group + r * groups;
-    if (row >= rows) break;
-    const int h = head0 + row % nh;
-    const long long t = tok0 + row / nh, b = t / a.q_len, c = t % a.q_len;
+    toks[r] = (int)__umulhi((unsigned)row, a.heads_magic);
+    const int h = row - toks[r] * a.heads;
+    hs[r] = row < rows && h < nh ? head0 + h : -1;
+  }
+  Pack<T, VEC> raw[ROWS][ITEMS][2];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int h = hs[r];
+    if (h < 0) continue;
+    int b, c;
+    locate(toks[r], b, c);
     const T* src = h < a.hq ? static_cast<const T*>(a.q) + b * a.qs[0] + c * a.qs[1] + h * a.qs[2]
                             : static_cast<const T*>(a.k) + b * a.ks[0] + c * a.ks[1] + (h - a.hq) * a.ks[2];
 #pragma unroll
@@ -129,58 +150,43 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
     }
   }
   for (int e = threadIdx.x; e < ntok * half; e += kThreads) {
-    const int t = e / half, i = e % half;
-    const long long n = tok0 + t;
-    const long long at = a.axis[i] * a.ps[0] + (n / a.q_len) * a.ps[1] + (n % a.q_len) * a.ps[2];
+    const int t = (unsigned)e / (unsigned)half, i = e - t * half;
+    int b, c;
+    locate(t, b, c);
+    const long long at = a.axis[i] * a.ps[0] + b * a.ps[1] + c * a.ps[2];
     const double p = a.pos64 ? (double)static_cast<const long long*>(a.pos)[at]
                              : (double)static_cast<const int*>(a.pos)[at];
     const double turns = p * (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    cs[e] = make_float2(c * a.scaling, s * a.scaling);
+    float s, co;
+    sincospif((float)(2.0 * (turns - rint(turns))), &s, &co);
+    s_cos[e] = co * a.scaling;
+    s_sin[e] = s * a.scaling;
   }
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int row = group + r * groups;
-    if (row >= rows) break;
-    const int tok = row / nh, h = head0 + row % nh;
-    const long long t = tok0 + tok;
+    const int tok = toks[r], h = hs[r];
+    if (h < 0) continue;  // a row's lanes together
+    const long long t = (long long)tok0 + tok;
     const bool is_q = h < a.hq;
     T* dst = is_q ? static_cast<T*>(a.q_out) + (t * a.hq + h) * a.d : static_cast<T*>(a.k_out) + (t * a.g + (h - a.hq)) * a.d;
     const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
-    float x[ITEMS][2][VEC];
-#pragma unroll
-    for (int n = 0; n < ITEMS; ++n) {
-      unpack<T, VEC>(raw[r][n][0], x[n][0]);
-      unpack<T, VEC>(raw[r][n][1], x[n][1]);
-    }
+    float inv = 1.f;
     if (w) {
       float ss = 0.f;
 #pragma unroll
       for (int n = 0; n < ITEMS; ++n)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) ss += x[n][0][j] * x[n][0][j] + x[n][1][j] * x[n][1][j];
+        for (int e = 0; e < 2; ++e) {
+          float x[VEC];
+          unpack<T, VEC>(raw[r][n][e], x);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) ss += x[j] * x[j];
+        }
       // the row's lanes are consecutive, and take this branch together
       const unsigned mask = lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u) << (threadIdx.x & 31 & ~(lanes - 1));
       for (int off = lanes >> 1; off > 0; off >>= 1) ss += __shfl_xor_sync(mask, ss, off);
-      const float inv = rsqrtf(ss / (float)a.d + a.eps);
-#pragma unroll
-      for (int n = 0; n < ITEMS; ++n) {
-        const int it = lane + (n << a.lanes_log2);
-        if (it >= items) continue;
-        int o0, o1;
-        chunks(it, o0, o1);
-        float v[VEC];
-        unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o0), v);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) x[n][0][j] *= inv * v[j];
-        if (o1 >= 0) {
-          unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o1), v);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) x[n][1][j] *= inv * v[j];
-        }
-      }
+      inv = rsqrtf(ss / (float)a.d + a.eps);
     }
 #pragma unroll
     for (int n = 0; n < ITEMS; ++n) {
@@ -188,18 +194,33 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
       if (it >= items) continue;
       int o0, o1;
       chunks(it, o0, o1);
-      if (it < pairs) {
-        const float2* row_cs = cs + tok * half + o0;
+      float x[2][VEC];
+      unpack<T, VEC>(raw[r][n][0], x[0]);
+      unpack<T, VEC>(raw[r][n][1], x[1]);
+      if (w) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float2 c = row_cs[j];
-          const float u = x[n][0][j], v = x[n][1][j];
-          x[n][0][j] = u * c.x - v * c.y;
-          x[n][1][j] = v * c.x + u * c.y;
+        for (int e = 0; e < 2; ++e) {
+          const int o = e ? o1 : o0;
+          if (o < 0) continue;
+          float v[VEC];
+          unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o), v);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) x[e][j] *= inv * v[j];
         }
       }
-      store<T, VEC>(dst + o0, x[n][0]);
-      if (o1 >= 0) store<T, VEC>(dst + o1, x[n][1]);
+      if (it < pairs) {
+        // 16-byte items: half and o0 are multiples of VEC, so these are 16-byte loads too
+        const Pack<float, VEC> c = *reinterpret_cast<const Pack<float, VEC>*>(s_cos + tok * half + o0);
+        const Pack<float, VEC> d = *reinterpret_cast<const Pack<float, VEC>*>(s_sin + tok * half + o0);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float u = x[0][j], v = x[1][j];
+          x[0][j] = u * c.v[j] - v * d.v[j];
+          x[1][j] = v * c.v[j] + u * d.v[j];
+        }
+      }
+      store<T, VEC>(dst + o0, x[0]);
+      if (o1 >= 0) store<T, VEC>(dst + o1, x[1]);
     }
   }
 }
@@ -209,9 +230,10 @@ int launch_rows(RopeAxesArgs& a, cudaStream_t st) {
   const int heads = a.hq + a.g, most = ROWS * (kThreads >> a.lanes_log2);
   a.heads = std::min(heads, most);
   a.tokens = std::max(1, std::min(kMaxTokens, most / heads));
+  a.heads_magic = (uint32_t)((1ULL << 32) / a.heads + 1);  // a q and a k head at least
   const long long gx = (a.n_tokens + a.tokens - 1) / a.tokens;
   const int gy = (heads + a.heads - 1) / a.heads;
-  if (gx > 0x7fffffffLL || gy > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many rows");
+  if (a.n_tokens > 0x7fffffffLL || gy > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many rows");
   rope_axes_kernel<T, VEC, ITEMS, ROWS><<<dim3((unsigned)gx, (unsigned)gy), kThreads, 0, st>>>(a);
   return cuda_check(cudaGetLastError(), "aoh_rope_axes_qk launch");
 }
@@ -223,15 +245,15 @@ int launch(RopeAxesArgs& a, int num_sms, cudaStream_t st) {
   while ((1 << a.lanes_log2) < items && a.lanes_log2 < 5) ++a.lanes_log2;
   const int per_lane = (items + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
   // Few rows: one a thread, so that they spread over the SMs (the sines are
-  // computed by each of a token's CTAs).  Many: four.
+  // computed by each of a token's CTAs).  Many: two.
   const bool few = a.n_tokens * (a.hq + a.g) <= 4LL * num_sms * (kThreads >> a.lanes_log2);
   if constexpr (VEC > 1) {
     // 16-byte items of at most 256 dimensions: at most 32, one a lane
-    return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 4>(a, st);
+    return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 2>(a, st);
   } else {
-    if (per_lane == 1) return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 4>(a, st);
-    if (per_lane == 2) return few ? launch_rows<T, VEC, 2, 1>(a, st) : launch_rows<T, VEC, 2, 4>(a, st);
-    return few ? launch_rows<T, VEC, 4, 1>(a, st) : launch_rows<T, VEC, 4, 2>(a, st);  // at most 128 items over 32 lanes
+    if (per_lane == 1) return few ? launch_rows<T, VEC, 1, 1>(a, st) : launch_rows<T, VEC, 1, 2>(a, st);
+    if (per_lane == 2) return launch_rows<T, VEC, 2, 1>(a, st);
+    return launch_rows<T, VEC, 4, 1>(a, st);  // at most 128 items over 32 lanes
   }
 }
 
