@@ -146,19 +146,22 @@ def stream_handle(stream=None) -> int:
     return s.cuda_stream
 
 
+_get_device = _raw_stream = None  # torch's, bound on first use: this module loads without torch
+
+
 def launch(device, fn, what: str, *args) -> None:
     """fn(*args, stream) with ``device`` (a tensor's) current, on its current stream."""
-    import torch
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(device.index))
+    global _get_device, _raw_stream
+    if _raw_stream is None:
+        import torch
+        # the device and the stream's handle alone: the objects torch.cuda makes of them take 3 us
+        _get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    index = device.index
+    if index == _get_device():
+        rc = fn(*args, _raw_stream(index))
     else:
+        import torch
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
+            rc = fn(*args, _raw_stream(index))
     if rc:
         check(rc, what)
-
-
-def _raw_stream(index: int) -> int:
-    # the handle alone: building a torch.cuda.Stream object for it takes 3 us
-    import torch
-    return torch._C._cuda_getCurrentRawStream(index)

@@ -132,6 +132,7 @@ class AoHKVCache:
                                        C.c_void_p(_lib.stream_handle())), "AoHKVCache.bind")
         self._reserved = 0
         self._ws = None
+        self._pool_view = None
         if reserve_all:
             self.reserve(self.max_context)
 
@@ -199,7 +200,9 @@ class AoHKVCache:
 
     def pool_view(self) -> torch.Tensor:
         """The pool as (num_pages, 2, 16, head_dim) of the cache dtype."""
-        return self.pool.view(self.dtype).view(self.num_pages, 2, PAGE_SIZE, self.head_dim)
+        if self._pool_view is None:
+            self._pool_view = self.pool.view(self.dtype).view(self.num_pages, 2, PAGE_SIZE, self.head_dim)
+        return self._pool_view
 
     def device_status(self) -> int:
         """Read and clear the device check word (0: no bounds check or bounded

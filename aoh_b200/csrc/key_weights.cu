@@ -10,7 +10,7 @@
 // key is summed by one CTA in a fixed order, so results do not depend on timing.
 //
 // This file holds the entry point and the kernels for any type: 64 rows x 64
-// keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.  bf16
+// (or 32) keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.  bf16
 // caches run those of key_weights_sm100.cu: one pass over K for few query rows
 // (single tokens), tensor cores for more.
 #include "common.cuh"
@@ -21,9 +21,10 @@
 namespace aoh {
 namespace {
 
-constexpr int kTile = 64;                 // query rows and keys of a tile
+constexpr int kTile = 64;                 // query rows of a tile, and keys of the first pass's
+constexpr int kSumKeys = 32;              // keys of the second pass's tiles: twice the CTAs, which 64 leave uneven
 constexpr int kStride = kHeadDim + 4;     // floats of a row in shared memory: 16-byte rows on distinct banks
-constexpr int kSmem = 2 * kTile * kStride * 4;
+constexpr int kSmem = 2 * kTile * kStride * 4, kSumSmem = (kTile + kSumKeys) * kStride * 4;
 
 // Four dimensions of a stored row, as loaded and as floats.
 template <typename T>
@@ -61,22 +62,22 @@ __device__ __forceinline__ void load_queries(const KeyWeightsArgs& a, int b, int
   for (int i = 0; i < kLoads; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
-// Keys [j0, j0 + 64) of a unit; rows that are not stored are zero.
-template <typename T>
+// Keys [j0, j0 + KT) of a unit; rows that are not stored are zero.
+template <typename T, int KT>
 __device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int j0, int len, float* sm) {
   const int base = a.g.unit_offset[unit], n_pages = a.g.unit_offset[unit + 1] - base;
   const int r0 = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
-  int pages[kTile / kPage];
+  int pages[KT / kPage];
 #pragma unroll
-  for (int i = 0; i < kTile / kPage; ++i) {
+  for (int i = 0; i < KT / kPage; ++i) {
     const int p = j0 / kPage + i;
     pages[i] = p * kPage < len && p < n_pages ? a.g.block_table[base + p] : -1;
     if (pages[i] >= a.g.num_pages) pages[i] = -1;
     if (pages[i] < 0 && p * kPage < len && threadIdx.x == 0) atomicOr(a.g.err, kErrBadPage);
   }
-  Raw4<T> v[kLoads];
+  Raw4<T> v[KT / 8];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
+  for (int i = 0; i < KT / 8; ++i) {
     const int r = r0 + 8 * i, slot = r % kPage;
     const int page = pages[8 * i / kPage];  // r0 < 8: row r is in page 8 i / 16
     v[i] = Raw4<T>{};
@@ -88,26 +89,27 @@ __device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int
     }
   }
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
+  for (int i = 0; i < KT / 8; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
 // s[i][j]: row 4 ty + i, key tx + 16 j, in the log2 domain
-__device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][4]) {
+template <int J>
+__device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][J]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < J; ++j) s[i][j] = 0.f;
 #pragma unroll 4
   for (int d = 0; d < kHeadDim; d += 4) {
-    float4 q[4], k[4];
+    float4 q[4], k[J];
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(qs + (4 * ty + i) * kStride + d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStride + d);
+    for (int j = 0; j < J; ++j) k[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStride + d);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < J; ++j) {
         s[i][j] = fmaf(q[i].x, k[j].x, s[i][j]);
         s[i][j] = fmaf(q[i].y, k[j].y, s[i][j]);
         s[i][j] = fmaf(q[i].z, k[j].z, s[i][j]);
@@ -117,7 +119,7 @@ __device__ __forceinline__ void tile_scores(const float* qs, const float* ks, in
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] *= kScoreScale;
+    for (int j = 0; j < J; ++j) s[i][j] *= kScoreScale;
 }
 
 // Keys a row may see: j <= past + token.
@@ -130,7 +132,7 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
   const int r = blockIdx.y, unit = a.row_unit[r];
   if (a.g.unit_offset[unit] == a.g.unit_offset[unit + 1]) return;
   const int past = key_weights_past(a);
-  const int rows = a.q_len * a.g.grp, row0 = blockIdx.x * kTile;
+  const int rows = a.q_len * a.g.grp, row0 = blockIdx.z * kTile;
   const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
   const long long rows_total = (long long)a.units * rows;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
@@ -139,14 +141,16 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
   // key tiles up to the last one that any row of the tile sees, split evenly
   const int len = last_key(a, past, min(row0 + kTile, rows) - 1) + 1;
   const int tiles = (len + kTile - 1) / kTile;
-  const int t0 = (int)((long long)tiles * blockIdx.z / splits), t1 = (int)((long long)tiles * (blockIdx.z + 1) / splits);
+  const int t0 = (int)((long long)tiles * blockIdx.x / splits), t1 = (int)((long long)tiles * (blockIdx.x + 1) / splits);
+  const bool idle = row0 + 8 * (int)(threadIdx.x >> 5) >= rows;  // a warp has 8 rows: none of them is one
   float m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
   for (int t = t0; t < t1; ++t) {
     __syncthreads();
-    load_keys<T>(a, unit, t * kTile, len, ks);
+    load_keys<T, kTile>(a, unit, t * kTile, len, ks);
     __syncthreads();
+    if (idle) continue;
     float s[4][4];
     tile_scores(qs, ks, ty, tx, s);
 #pragma unroll
@@ -178,11 +182,11 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
     for (int off = 8; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
     const int row = row0 + 4 * ty + i;
     if (tx == 0 && row < rows)
-      part[blockIdx.z * rows_total + (long long)r * rows + row] = make_float2(mm, ll);
+      part[blockIdx.x * rows_total + (long long)r * rows + row] = make_float2(mm, ll);
   }
 }
 
-// The weights of 64 keys, summed over every query row of the unit.
+// The weights of kSumKeys keys, summed over every query row of the unit.
 template <typename T>
 __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
@@ -190,33 +194,47 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
   const int r = blockIdx.y, unit = a.row_unit[r];
   const int past = key_weights_past(a);
   const int len = past + a.q_len, rows = a.q_len * a.g.grp;
-  const int j0 = blockIdx.x * kTile;
+  const int j0 = blockIdx.x * kSumKeys;
   if (j0 >= len) return;
   const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
   const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
   const long long rows_total = (long long)a.units * rows;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   float *qs = sm, *ks = sm + kTile * kStride;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int J = kSumKeys / 16;
+  float w[J] = {};
   if (stored) {
-    load_keys<T>(a, unit, j0, len, ks);
+    load_keys<T, kSumKeys>(a, unit, j0, len, ks);
     // the first token that sees key j0
     const int tok0 = max(0, j0 - past);
     for (int row0 = tok0 * a.g.grp; row0 < rows; row0 += kTile) {
       __syncthreads();
       load_queries<T>(a, b, g, row0, rows, qs);
-      if (threadIdx.x < kTile && row0 + threadIdx.x < rows) {
-        const float2* p = part + (long long)r * rows + row0 + threadIdx.x;
+      {  // -lse of the tile's rows from their key ranges, four threads a row
+        const int row = threadIdx.x >> 2;
         float mm = -INFINITY, ll = 0.f;
-        for (int i = 0; i < splits; ++i) mm = fmaxf(mm, p[i * rows_total].x);
-        for (int i = 0; i < splits; ++i) {
-          const float2 v = p[i * rows_total];
-          if (v.y > 0.f) ll += v.y * fast_exp2(v.x - mm);
+        if (row0 + row < rows) {
+          const float2* p = part + (long long)r * rows + row0 + row;
+#pragma unroll 8
+          for (int i = threadIdx.x & 3; i < splits; i += 4) {
+            const float2 v = p[i * rows_total];
+            const float top = fmaxf(mm, v.x);
+            if (v.y > 0.f) ll = ll * fast_exp2(mm - top) + v.y * fast_exp2(v.x - top);
+            mm = top;
+          }
         }
-        lse[threadIdx.x] = mm + log2f(ll);
+#pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+          const float om = __shfl_xor_sync(0xffffffffu, mm, off), ol = __shfl_xor_sync(0xffffffffu, ll, off);
+          const float top = fmaxf(mm, om);
+          ll = (ll > 0.f ? ll * fast_exp2(mm - top) : 0.f) + (ol > 0.f ? ol * fast_exp2(om - top) : 0.f);
+          mm = top;
+        }
+        if ((threadIdx.x & 3) == 0) lse[row] = mm + log2f(ll);
       }
       __syncthreads();
-      float s[4][4];
+      if (row0 + 8 * (int)(threadIdx.x >> 5) >= rows) continue;  // none of this warp's 8 rows is one
+      float s[4][J];
       tile_scores(qs, ks, ty, tx, s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -225,7 +243,7 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
         const int last = last_key(a, past, row);
         const float e = lse[4 * ty + i];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < J; ++j)
           if (j0 + tx + 16 * j <= last) w[j] += fast_exp2(s[i][j] - e);
       }
     }
@@ -233,11 +251,11 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
   // over the 16 groups of rows, in their order
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) qs[ty * kTile + tx + 16 * j] = w[j];
+  for (int j = 0; j < J; ++j) qs[ty * kSumKeys + tx + 16 * j] = w[j];
   __syncthreads();
-  if (threadIdx.x < kTile && j0 + threadIdx.x < len) {
+  if (threadIdx.x < kSumKeys && j0 + threadIdx.x < len) {
     float x = 0.f;
-    for (int i = 0; i < 16; ++i) x += qs[i * kTile + threadIdx.x];
+    for (int i = 0; i < 16; ++i) x += qs[i * kSumKeys + threadIdx.x];
     float* o = a.out + r * a.out_stride + j0 + threadIdx.x;
     *o = a.accumulate ? *o + x : x;
   }
@@ -252,14 +270,15 @@ int launch_any(const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws, cudaS
   rc = once.run(dev, [] {
     int e = cuda_check(cudaFuncSetAttribute(key_lse_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
                        "key_lse shared memory");
-    return e ? e : cuda_check(cudaFuncSetAttribute(key_sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
+    return e ? e : cuda_check(cudaFuncSetAttribute(key_sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem),
                               "key_sum shared memory");
   });
   if (rc) return rc;
-  const int key_tiles = (a.max_len + kTile - 1) / kTile;
+  const int key_tiles = (a.max_len + kSumKeys - 1) / kSumKeys;
   float2* part = reinterpret_cast<float2*>(ws + p.part);
-  key_lse_kernel<T><<<dim3(p.row_tiles, a.units, p.splits), 256, kSmem, st>>>(a, part, p.splits);
-  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSmem, st>>>(a, part, p.splits);
+  if (p.row_tiles > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_key_weights: too many queries");
+  key_lse_kernel<T><<<dim3(p.splits, a.units, p.row_tiles), 256, kSmem, st>>>(a, part, p.splits);
+  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSumSmem, st>>>(a, part, p.splits);
   return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
 }
 

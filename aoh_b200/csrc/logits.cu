@@ -20,10 +20,12 @@
 // CTAs takes a row, each a slice of the vocabulary of 8192 tokens (or more,
 // where 16 slices do not reach): a thread then has all its loads, four groups
 // of 8 tokens, in flight at once.  The greedy token is reduced over the cluster
-// in shared memory, so one launch and no workspace.  A CTA's biased tokens are
-// listed in shared memory, in the order given, and marked in a bitmap there;
-// the main pass leaves them out and a thread for each listed token does it
-// alone, so that the sum over a token listed more than once has a fixed order.
+// in shared memory, so one launch and no workspace.  The main pass copies and
+// masks; the few tokens with a count or a bias are listed in shared memory and
+// done behind it, a thread each: the division of the penalties, in every group
+// that holds one such token, cost more than the copy.  A CTA's biases are
+// listed in the order given, so that the sum over a token listed more than once
+// has a fixed order.
 #include <climits>
 #include <type_traits>
 
@@ -37,10 +39,10 @@ constexpr int kMaxCluster = 16;
 constexpr int kThreads = 256;
 constexpr int kMaxBias = 4096;  // biases of a row (32 KB of shared memory if all fall into one slice)
 constexpr int kSlice = kThreads * 32;  // tokens whose loads a CTA has in flight at once (a quarter where rows are not aligned)
-constexpr int kMaxVocab = 1 << 23;
+constexpr int kMaxVocab = 1 << 21;
 constexpr uint32_t kInPrompt = 0x80000000u;
 // two bits a token of the largest slice, and the list
-constexpr int kMaxSmem = kMaxVocab / kMaxCluster / 4 + kMaxBias * 8;
+constexpr int kMaxSmem = 160 * 1024;
 
 struct LogitsArgs {
   const void* logits;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   __shared__ unsigned long long best_cta[kMaxCluster];
   __shared__ int s_count[kThreads / 32];
   uint32_t *biased = smem, *repeated = smem + a.slice / 32;
-  int2* list = reinterpret_cast<int2*>(smem + a.slice / 16);
+  int2* list = reinterpret_cast<int2*>(smem + a.slice / 16);  // biases
   const int rank = a.cluster > 1 ? (int)cluster_ctarank() : 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / a.cluster;
@@ -201,15 +203,17 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
 
   // A thread's tokens of one round: U units of N neighbours, a stride apart.
   // Rows that are not 16-byte aligned take single tokens, a lane each of a word.
-  constexpr int N = kWide ? 8 : 1, U = kWide ? 4 : 8;
+  constexpr int N = kWide ? 8 : 1, U = kWide ? 4 : 8, kRound = U * N * kThreads;
   constexpr uint32_t kOnes = (1u << N) - 1u;
+  __shared__ uint16_t s_list[kRound];  // tokens with a count, from the round's first on
+  __shared__ int s_listed;
   using Raw = typename std::conditional<kWide, Raw8<T>, Raw1<T>>::type;
   Raw raw[U];
   uint32_t s[U], al[U];
-  auto fetch = [&](int t0) {
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int t = t0 + u * kThreads * N;
+      const int t = base + (u * kThreads + tid) * N;
       s[u] = 0;
       al[u] = kOnes;
       if (t < hi) {
@@ -219,10 +223,10 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
       }
     }
   };
-  const int first = lo + tid * N;
-  fetch(first);
+  fetch(lo);
+  if (tid == 0) s_listed = 0;
 
-  int listed = 0;
+  int n_biased = 0;
   if (a.n_bias) {
     const int32_t* ids = a.bias_ids + (long long)row * a.n_bias;
     const float* values = a.bias + (long long)row * a.n_bias;
@@ -240,91 +244,132 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         if (atomicOr(&biased[(id - lo) >> 5], bit) & bit) atomicOr(&repeated[(id - lo) >> 5], bit);
       }
       __syncthreads();
-      int at = listed + __popc(m & ((1u << lane) - 1u));
+      int at = n_biased + __popc(m & ((1u << lane) - 1u));
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) at += s_count[w];
-        listed += s_count[w];
+        n_biased += s_count[w];
       }
       if (in) list[at] = make_int2(id, __float_as_int(v));
       __syncthreads();
     }
+  } else if (seen) {
+    __syncthreads();
   }
 
-  for (int t0 = first; t0 < hi; t0 += U * kThreads * N) {
-    if (t0 != first) fetch(t0);
+  unsigned long long key = 0;
+  auto put = [&](int t, float y) {
+    if (greedy && y != -INFINITY) key = max(key, greedy_key(y, t));
+    store1(out + t, y);
+  };
+  for (int base = lo; base < hi; base += kRound) {
+    if (base != lo) fetch(base);
+    int n_special = 0;
+    uint32_t sp[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int t = t0 + u * kThreads * N;
-      if (t >= hi) break;
+      const int t = base + (u * kThreads + tid) * N;
+      sp[u] = 0;
+      if (t >= hi) continue;
       float x[N];
       raw[u].get(x);
-      if (s[u]) {
-        uint32_t c[N];
-        if constexpr (kWide) {
-          const uint4 c0 = reinterpret_cast<const uint4*>(pen.counts + t)[0], c1 = reinterpret_cast<const uint4*>(pen.counts + t)[1];
-          c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w;
-          c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
-        } else {
-          c[0] = pen.counts[t];
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = pen.apply(x[j], c[j]);
-      }
       if (al[u] != kOnes) {
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = al[u] >> j & 1 ? x[j] : -INFINITY;
       }
       const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> (t & 31) & kOnes : 0u;
-      if (bi || !kWide) {  // one by one, without the biased ones
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (!(bi >> j & 1)) {
-            store1(out + t + j, x[j]);
-            if (greedy) best.one(x[j], t + j);
-          }
-        continue;
-      }
-      if constexpr (kWide) {
+      sp[u] = s[u] & al[u] & ~bi;
+      n_special += __popc(sp[u]);
+      // tokens that are done again below are stored as they came: in place they must stay, and they are overwritten
+      if constexpr (kWide)
         store8(out + t, x);
-        if (greedy) {
+      else
+        store1(out + t, x[0]);
+      if (greedy) {
+        const uint32_t later = sp[u] | bi;
+        if (later) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] = later >> j & 1 ? -INFINITY : x[j];
+        }
+        if constexpr (kWide) {
           const float mx = max_nan(max_nan(max_nan(x[0], x[1], x[2]), x[3], x[4]), max_nan(x[5], x[6], x[7]));
           if (!(mx <= best.x)) {  // larger, or NaN
 #pragma unroll
             for (int j = N - 1; j >= 0; --j) best.note(x[j], mx, t + j);
           }
+        } else {
+          best.one(x[0], t);
         }
       }
     }
-  }
-  unsigned long long key = best.key();
-
-  // a biased token, with the sum of its biases
-  auto finish = [&](int t, float sum) {
-    const uint32_t count = seen ? pen.counts[t] : 0u;
-    const bool ok = !allowed || allowed[t >> 5] >> (t & 31) & 1;
-    float y = pen.apply(load1(x_row + t), count);
-    y = ok ? __fadd_rn(y, sum) : -INFINITY;
-    if (greedy && y != -INFINITY) key = max(key, greedy_key(y, t));
-    store1(out + t, y);
-  };
-  for (int i = tid; i < listed; i += kThreads) {
-    const int2 e = list[i];
-    float sum = __int_as_float(e.y);
-    if (repeated[(e.x - lo) >> 5] >> (e.x & 31) & 1) {
-      // listed more than once: the first entry adds them up in their order, from -0, which leaves the first as it is
-      int first = -1;
-      sum = -0.f;
-#pragma unroll 4
-      for (int j = 0; j < listed; ++j) {
-        const int2 o = list[j];
-        const float next = __fadd_rn(sum, __int_as_float(o.y));
-        sum = o.x == e.x ? next : sum;
-        first = o.x == e.x && first < 0 ? j : first;
+    if (!seen) continue;
+    // the list, in any order: its tokens do not depend on one another
+    if (__any_sync(0xffffffffu, n_special > 0)) {
+      int incl = n_special;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
       }
-      if (first != i) continue;
+      int at = 0;
+      if (lane == 31) at = atomicAdd(&s_listed, incl);
+      at = __shfl_sync(0xffffffffu, at, 31) + incl - n_special;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        for (uint32_t m = sp[u]; m; m &= m - 1) s_list[at++] = (uint16_t)((u * kThreads + tid) * N + __ffs(m) - 1);
     }
-    finish(e.x, sum);
+    __syncthreads();
+    const int n_listed = s_listed;
+    // four a thread in flight: a slice of frequent tokens lists thousands
+    for (int i0 = tid; i0 < n_listed; i0 += 4 * kThreads) {
+      int t[4];
+      uint32_t count[4];
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kThreads;
+        t[u] = i < n_listed ? base + s_list[i] : -1;
+        if (t[u] >= 0) {
+          count[u] = pen.counts[t[u]];
+          x[u] = load1(x_row + t[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (t[u] >= 0) put(t[u], pen.apply(x[u], count[u]));
+    }
+    if (base + kRound < hi) {
+      __syncthreads();
+      if (tid == 0) s_listed = 0;
+      __syncthreads();
+    }
+  }
+  key = max(key, best.key());
+
+  if (n_biased) {
+    if (!seen) __syncthreads();  // the main pass has stored its tokens
+    for (int i = tid; i < n_biased; i += kThreads) {
+      const int2 e = list[i];
+      const int t = e.x;
+      const uint32_t count = seen ? pen.counts[t] : 0u;
+      const bool ok = !allowed || allowed[t >> 5] >> (t & 31) & 1;
+      const float x = load1(x_row + t);
+      float sum = __int_as_float(e.y);
+      if (repeated[(t - lo) >> 5] >> (t & 31) & 1) {
+        // listed more than once: the first entry adds them up in their order, from -0, which leaves the first as it is
+        int first = -1;
+        sum = -0.f;
+#pragma unroll 4
+        for (int j = 0; j < n_biased; ++j) {
+          const int2 o = list[j];
+          const float next = __fadd_rn(sum, __int_as_float(o.y));
+          sum = o.x == t ? next : sum;
+          first = o.x == t && first < 0 ? j : first;
+        }
+        if (first != i) continue;
+      }
+      put(t, ok ? __fadd_rn(pen.apply(x, count), sum) : -INFINITY);
+    }
   }
 
   if (!greedy) return;
@@ -435,8 +480,16 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   a.logits = p.logits;
   a.row_stride = p.row_stride;
   a.vocab = p.vocab;
+  // 16 CTAs a row take the least time for a few rows, but then 8, which fill the
+  // SMs in one wave, and 4 (64 rows of 128K, all features: 28 / 21 / 24 us).
+  int dev = 0, sms = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+  if (rc) return rc;
+  const int most = p.rows * 16LL <= 2 * sms ? 16 : p.rows * 8LL <= 4 * sms ? 8 : 4;
   a.cluster = 1;
-  while (a.cluster < kMaxCluster && a.cluster * (wide ? kSlice : kSlice / 4) < p.vocab) a.cluster *= 2;
+  while (a.cluster < most && a.cluster * (wide ? kSlice : kSlice / 4) < p.vocab) a.cluster *= 2;
   a.slice = ((p.vocab + a.cluster - 1) / a.cluster + 255) / 256 * 256;
   a.counts = reinterpret_cast<const uint32_t*>(p.counts);
   a.seen = reinterpret_cast<const uint32_t*>(p.seen);

@@ -97,15 +97,16 @@ def select_keys(weights: torch.Tensor, keep: int, *, sink: int = 0, recent: int 
     if sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError(f"sink {sink} and recent {recent} must be non-negative and fit keep {keep}")
     lead = weights.shape[:-1]
-    rows = lead.numel()
     kept = weights.new_empty((*lead, keep), dtype=torch.int32)
     kept_w = weights.new_empty((*lead, keep))
-    if rows == 0 or keep == 0:
+    if kept.numel() == 0:
         return kept, kept_w
-    w = weights.reshape(rows, n)  # a view, or a copy where the rows are not evenly spaced
-    if n > 1 and w.stride(1) != 1:
+    # rows evenly spaced: a view, or a copy where they are not
+    w = weights if weights.dim() == 2 else weights.reshape(-1, n)
+    stride, one = w.stride()
+    if n > 1 and one != 1:
         raise ValueError("the last dimension of weights must be contiguous")
-    _lib.launch(weights.device, _lib.lib().aoh_select_keys, "aoh_select_keys", w.data_ptr(), w.stride(0), rows, n, keep,
+    _lib.launch(weights.device, _lib.lib().aoh_select_keys, "aoh_select_keys", w.data_ptr(), stride, w.shape[0], n, keep,
                 sink, recent, kept.data_ptr(), kept_w.data_ptr())
     return kept, kept_w
 

@@ -372,7 +372,7 @@ typedef struct {
   int64_t row_stride;
   int64_t out_stride;
   int32_t rows;
-  int32_t vocab;
+  int32_t vocab;           /* <= 2^21 */
   int32_t dtype;           /* aoh_dtype */
   int32_t out_dtype;
   int32_t n_bias;          /* <= 4096 */
