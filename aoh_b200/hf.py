@@ -20,6 +20,11 @@ the prompt in one forward with every head causal over it, then decode steps.
     make_cache, n_ret, n_str = patch_aoh_model(model, labels, 128, 256)
     cache = make_cache(max_context=65536)
     logits = model(input_ids=chunk, past_key_values=cache, use_cache=True).logits
+
+The retrieval heads' keys can be bounded (no counterpart in the reference):
+``cache.track_weights()`` before the prompt lets every forward add up the
+attention that each key receives, ``cache = cache.evict(keep)`` cuts the
+retrieval heads to the ``keep`` keys that matter, and the model goes on with it.
 """
 from __future__ import annotations
 
@@ -31,6 +36,8 @@ import torch
 
 from .attention import aoh_attention, rope_qk
 from .cache import AoHKVCache
+from .eviction import KeyWeights
+from .logits import TokenHistory, penalize_logits
 
 try:  # the Cache base class the model's forward expects (the reference subclasses it too)
     from transformers.cache_utils import Cache
@@ -46,7 +53,8 @@ except ImportError:  # transformers absent: the adapter is unavailable, the runt
 class AoHModelCache(Cache):
     """The paged cache as a transformers ``Cache``, with the reference's hooks
     (benchmark_llama31.py:155-166): ``update`` is a no-op (the patched forward
-    appends), sequence length and mask sizes come from ``kv_seq_len``."""
+    appends), sequence length and mask sizes come from ``kv_seq_len`` -- and,
+    once keys were evicted, from the tokens seen, whose positions go on."""
 
     def __init__(self, paged: AoHKVCache):
         if Cache is object:
@@ -56,6 +64,28 @@ class AoHModelCache(Cache):
         else:
             super().__init__(layers=[DynamicLayer() for _ in range(paged.num_layers)])
         self.paged = paged
+        self.key_weights: KeyWeights | None = None  # the retrieval keys' attention so far (track_weights)
+
+    def track_weights(self) -> KeyWeights:
+        """From now on, add up the attention that each retrieval key receives."""
+        if self.key_weights is None:
+            self.key_weights = KeyWeights(self.paged)
+        return self.key_weights
+
+    def evict(self, keep: int, max_context: int | None = None) -> "AoHModelCache":
+        """A cache of ``max_context`` tokens (default: keep + 1024) with the
+        ``keep`` keys of every retrieval head that received the most attention --
+        the sink's and the window's among them --, the streaming heads' rows, and
+        the kept keys' weights.  This one stays as it is."""
+        if self.key_weights is None:
+            raise RuntimeError("evict needs the keys' weights: call track_weights() before the prompt")
+        p = self.paged
+        small = AoHKVCache(p.labels, p.num_q_heads, batch=p.batch, sink_size=p.sink_size, recent_size=p.recent_size,
+                           max_context=int(max_context or keep + 1024), dtype=p.dtype, device=p.device, owned=p.owned,
+                           head_dim=p.head_dim, backend=p.backend)
+        new = AoHModelCache(small)
+        new.key_weights = self.key_weights.evict(keep, small)
+        return new
 
     @property
     def kv_seq_len(self) -> int:
@@ -69,7 +99,7 @@ class AoHModelCache(Cache):
         return key_states, value_states
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
-        return self.paged.kv_seq_len
+        return self.paged.kv_seq_len + getattr(self.paged, "evicted", 0)
 
     def get_max_cache_shape(self):
         return None
@@ -82,7 +112,7 @@ class AoHModelCache(Cache):
             q_len = cache_position
         else:
             q_len = int(cache_position.numel())
-        return self.paged.kv_seq_len + q_len, 0
+        return self.get_seq_length() + q_len, 0
 
 
 def make_aoh_forward(layer_idx: int, num_q: int, num_kv: int, head_dim: int):
@@ -107,8 +137,9 @@ def make_aoh_forward(layer_idx: int, num_q: int, num_kv: int, head_dim: int):
                 and head_dim == 128):
             # QK-norm (Qwen3) and RoPE in one kernel, straight into the layout the attention takes
             cos, sin = position_embeddings
-            q, k = rope_qk(q.contiguous(), k.contiguous(), cos.to(torch.bfloat16).contiguous(),
-                           sin.to(torch.bfloat16).contiguous(), None if qn is None else qn.weight,
+            # one row of positions for the whole batch comes as (1, C, D)
+            cos, sin = (t.to(torch.bfloat16).expand(bsz, q_len, head_dim).contiguous() for t in (cos, sin))
+            q, k = rope_qk(q.contiguous(), k.contiguous(), cos, sin, None if qn is None else qn.weight,
                            None if kn is None else kn.weight, getattr(qn, "variance_epsilon", 1e-6))
         else:
             q, k = q.transpose(1, 2), k.transpose(1, 2)
@@ -123,7 +154,10 @@ def make_aoh_forward(layer_idx: int, num_q: int, num_kv: int, head_dim: int):
             q = q.transpose(1, 2).to(dt).contiguous()
             k = k.transpose(1, 2).to(dt).contiguous()
         v = v.to(dt).contiguous()
+        past = None if cache.device_length else cache.kv_seq_len
         out = aoh_attention(cache, layer_idx, q, k, v)  # attend, append, advance after the last layer
+        if past_key_values.key_weights is not None:
+            past_key_values.key_weights.add(layer_idx, q, past_len=past)
         out = out.reshape(bsz, q_len, num_q * head_dim).to(hidden_states.dtype)
         return self.o_proj(out), None
 
@@ -181,9 +215,17 @@ class ModelDecodeGraph:
     and its position are fixed tensors written before each replay.  Pages for
     ``max_steps`` tokens are reserved up front.  ``step(token_ids)`` returns the
     step's logits (B, 1, vocab) -- a tensor the next step overwrites.
+
+    ``controls``: keyword arguments of :func:`penalize_logits` (repetition,
+    presence, frequency, bias, allowed, allowed_rows) whose tensors the caller
+    may rewrite between steps, e.g. a grammar's mask.  The step then appends its
+    input token to ``history`` (a TokenHistory of B rows), if given, and returns
+    the processed float32 logits; ``next_ids`` (B,) holds the greedy tokens, which
+    ``step(g.next_ids)`` takes without a trip to the host.
     """
 
-    def __init__(self, model, cache: AoHModelCache, max_steps: int):
+    def __init__(self, model, cache: AoHModelCache, max_steps: int, history: TokenHistory | None = None,
+                 controls: dict | None = None):
         import ctypes as C
 
         from . import _lib
@@ -194,6 +236,8 @@ class ModelDecodeGraph:
         if paged.backend != "eager" and paged.kv_seq_len == 0:
             raise ValueError("prefill the prompt before capturing decode steps")
         self.model, self.cache, self.paged = model, cache, paged
+        self.history = history
+        self.controls = None if controls is None and history is None else dict(controls or {})
         dev = paged.device
         B = paged.batch
         self.ids = torch.zeros((B, 1), dtype=torch.long, device=dev)
@@ -210,15 +254,26 @@ class ModelDecodeGraph:
             # append (an append at this position would already overwrite a
             # streaming head's ring slot whose row the first replay still attends)
             _lib.check(self._L.aoh_kv_set_decode_append(paged._h, 0), "aoh_kv_set_decode_append")
+            weights = cache.key_weights
+            before = None if weights is None else weights.rows.clone()
             try:
                 with torch.no_grad():
-                    self._forward()
+                    logits = self._forward()
+                    if self.controls is not None:  # without the history's update
+                        penalize_logits(logits[:, -1], history, greedy=True, **self.controls)
             finally:
                 _lib.check(self._L.aoh_kv_set_decode_append(paged._h, 1), "aoh_kv_set_decode_append")
+                if weights is not None:  # the dry run's token counts for nothing
+                    weights.rows.copy_(before)
             torch.cuda.synchronize(dev)
             self.graph = torch.cuda.CUDAGraph()
             with torch.no_grad(), torch.cuda.graph(self.graph):
                 self.logits = self._forward()
+                if self.controls is not None:
+                    if history is not None:
+                        history.append(self.ids)
+                    out, self.next_ids = penalize_logits(self.logits[:, -1], history, greedy=True, **self.controls)
+                    self.logits = out[:, None]
                 _lib.check(self._L.aoh_kv_advance(paged._h, 1, C.c_void_p(_lib.stream_handle())), "aoh_kv_advance")
         finally:
             paged.device_length = False
@@ -231,7 +286,7 @@ class ModelDecodeGraph:
                    "aoh_kv_set_length")
 
     def _inputs(self, token_ids: torch.Tensor) -> None:
-        t = self.paged.kv_seq_len
+        t = self.paged.tokens_seen
         self.ids.copy_(token_ids.view(self.ids.shape), non_blocking=True)
         self.pos.fill_(t)
         self.cpos.fill_(t)
@@ -241,7 +296,8 @@ class ModelDecodeGraph:
                           past_key_values=self.cache, use_cache=True).logits
 
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
-        """Decode one token per sequence (token_ids: (B,) or (B, 1)) and advance."""
+        """Decode one token per sequence (token_ids: (B,) or (B, 1)) and advance.
+        With controls, token_ids counts as output before its logits are processed."""
         self._inputs(token_ids)
         self.graph.replay()
         self.paged.kv_seq_len += 1
