@@ -6,7 +6,6 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .cache import _dtype_code
 
 
 class TokenHistory:
@@ -57,19 +56,13 @@ class TokenHistory:
                     ids.shape[1], None if lengths is None else lengths.data_ptr(), prompt)
 
 
-def _ptr(t: torch.Tensor | None) -> int:
-    return 0 if t is None else t.data_ptr()
+_DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 
 
-def _per_row(x, name: str, rows: int, device, neutral: float):
-    """(pointer or 0, scalar) of a penalty given as a number, a (rows,) tensor or None."""
-    if x is None:
-        return 0, neutral
-    if isinstance(x, torch.Tensor):
-        if x.dtype != torch.float32 or x.shape != (rows,) or x.device != device or not x.is_contiguous():
-            raise ValueError(f"{name} must be a number or a contiguous float32 tensor ({rows},) on {device}")
-        return x.data_ptr(), neutral
-    return 0, float(x)
+def _row_tensor(x, name: str, rows: int, device) -> int:
+    if x.dtype != torch.float32 or x.shape != (rows,) or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous float32 tensor ({rows},) on {device}")
+    return x.data_ptr()
 
 
 def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *, repetition=None, presence=None,
@@ -91,55 +84,78 @@ def penalize_logits(logits: torch.Tensor, history: TokenHistory | None = None, *
     it must not overlap them otherwise.  With ``greedy`` returns (out, ids (N,)
     int64): the largest fp32 result, the lowest id of equal ones, NaN above every
     number, 0 where nothing is allowed."""
-    if logits.dim() != 2 or not logits.is_cuda:
+    # a call's Python is most of the time that a single row takes: each property is read once
+    shape, strides, dev = logits.shape, logits.stride(), logits.device
+    if len(shape) != 2 or not logits.is_cuda:
         raise ValueError("logits must be a CUDA tensor (N, V)")
-    N, V = logits.shape
-    dev = logits.device
-    code = _dtype_code(logits.dtype)
-    if V < 1 or (V > 1 and logits.stride(1) != 1):
+    N, V = shape
+    code = _DTYPES.get(logits.dtype)
+    if code is None:
+        raise ValueError(f"logits must be torch.bfloat16 or torch.float32, got {logits.dtype}")
+    if V < 1 or (V > 1 and strides[1] != 1):
         raise ValueError("the vocabulary of logits must be contiguous and not empty")
+    # pointers, 0 where there is none, and the numbers that stand for a missing one
+    counts = seen = rep = pres = freq = 0
+    rep_s, pres_s, freq_s = 1.0, 0.0, 0.0
     if history is None:
         if repetition is not None or presence is not None or frequency is not None:
             raise ValueError("penalties need a history")
-    elif history.rows != N or history.vocab != V or history.device != dev:
-        raise ValueError(f"history of ({history.rows}, {history.vocab}) on {history.device} for logits {(N, V)} on {dev}")
-    if repetition is not None and not isinstance(repetition, torch.Tensor) and not repetition > 0:
-        raise ValueError("repetition must be positive")
-    rep, rep_s = _per_row(repetition, "repetition", N, dev, 1.0)
-    pres, pres_s = _per_row(presence, "presence", N, dev, 0.0)
-    freq, freq_s = _per_row(frequency, "frequency", N, dev, 0.0)
-    ids = values = None
-    K = 0
+    else:
+        if history.rows != N or history.vocab != V or history.device != dev:
+            raise ValueError(f"history of ({history.rows}, {history.vocab}) on {history.device} for logits {(N, V)} "
+                             f"on {dev}")
+        counts, seen = history.counts.data_ptr(), history.seen.data_ptr()
+        if repetition is not None:
+            if isinstance(repetition, torch.Tensor):
+                rep = _row_tensor(repetition, "repetition", N, dev)
+            elif repetition > 0:
+                rep_s = float(repetition)
+            else:
+                raise ValueError("repetition must be positive")
+        if presence is not None:
+            if isinstance(presence, torch.Tensor):
+                pres = _row_tensor(presence, "presence", N, dev)
+            else:
+                pres_s = float(presence)
+        if frequency is not None:
+            if isinstance(frequency, torch.Tensor):
+                freq = _row_tensor(frequency, "frequency", N, dev)
+            else:
+                freq_s = float(frequency)
+    ids = values = K = 0
     if bias is not None:
-        ids, values = bias
-        K = ids.shape[1] if ids.dim() == 2 else -1
-        if ids.dtype != torch.int32 or values.dtype != torch.float32 or ids.shape != (N, K) \
-                or values.shape != (N, K) or ids.device != dev or values.device != dev \
-                or not ids.is_contiguous() or not values.is_contiguous():
+        i, v = bias
+        K = i.shape[1] if i.dim() == 2 else -1
+        if i.dtype != torch.int32 or v.dtype != torch.float32 or i.shape != (N, K) or v.shape != (N, K) \
+                or i.device != dev or v.device != dev or not i.is_contiguous() or not v.is_contiguous():
             raise ValueError(f"bias must be contiguous int32 ids and float32 values of one shape ({N}, K) on {dev}")
-    M = 0
+        ids, values = i.data_ptr(), v.data_ptr()
+    mask = rows = M = 0
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] != -(-V // 32) \
-                or allowed.device != dev or not allowed.is_contiguous():
-            raise ValueError(f"allowed must be contiguous int32 (rows, {-(-V // 32)}) on {dev}")
-        M = allowed.shape[0]
+        words = -(-V // 32)
+        if allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[1] != words or allowed.device != dev \
+                or not allowed.is_contiguous():
+            raise ValueError(f"allowed must be contiguous int32 (rows, {words}) on {dev}")
+        mask, M = allowed.data_ptr(), allowed.shape[0]
         if allowed_rows is None and M != N:
             raise ValueError(f"{M} mask rows for {N} rows of logits need allowed_rows")
-    if allowed_rows is not None and (allowed is None or allowed_rows.dtype != torch.int32
-                                     or allowed_rows.shape != (N,) or allowed_rows.device != dev
-                                     or not allowed_rows.is_contiguous()):
-        raise ValueError(f"allowed_rows must be contiguous int32 ({N},) on {dev}, with allowed")
+    if allowed_rows is not None:
+        if allowed is None or allowed_rows.dtype != torch.int32 or allowed_rows.shape != (N,) \
+                or allowed_rows.device != dev or not allowed_rows.is_contiguous():
+            raise ValueError(f"allowed_rows must be contiguous int32 ({N},) on {dev}, with allowed")
+        rows = allowed_rows.data_ptr()
     if out is None:
-        out = logits.new_empty((N, V), dtype=torch.float32)
-    elif out.shape != (N, V) or out.device != dev or (V > 1 and out.stride(1) != 1) \
-            or (N > 1 and out.stride(0) < V):
-        raise ValueError(f"out must be ({N}, {V}) on {dev}, its vocabulary contiguous and its rows apart")
-    out_code = _dtype_code(out.dtype)
-    best = logits.new_empty((N,), dtype=torch.int64) if greedy else None
+        out = logits.new_empty(shape, dtype=torch.float32)
+        out_stride, out_code = V, _lib.F32
+    else:
+        out_stride, out_code = out.stride(0) if out.dim() == 2 else 0, _DTYPES.get(out.dtype)
+        if out.shape != shape or out.device != dev or (V > 1 and out.stride(1) != 1) or (N > 1 and out_stride < V):
+            raise ValueError(f"out must be ({N}, {V}) on {dev}, its vocabulary contiguous and its rows apart")
+        if out_code is None:
+            raise ValueError(f"out must be torch.bfloat16 or torch.float32, got {out.dtype}")
+    best = logits.new_empty(N, dtype=torch.int64) if greedy else None
     if N:
-        args = _lib.pack_logits(
-            logits.data_ptr(), out.data_ptr(), _ptr(best), _ptr(history and history.counts),
-            _ptr(history and history.seen), rep, pres, freq, _ptr(ids), _ptr(values), _ptr(allowed), _ptr(allowed_rows),
-            logits.stride(0), out.stride(0), N, V, code, out_code, K, M, rep_s, pres_s, freq_s, 0)
-        _lib.launch(dev, _lib.lib().aoh_logits_penalize, "aoh_logits_penalize", args)
+        _lib.launch(dev, _lib.lib().aoh_logits_penalize, "aoh_logits_penalize", _lib.pack_logits(
+            logits.data_ptr(), out.data_ptr(), best.data_ptr() if greedy else 0, counts, seen, rep, pres, freq, ids,
+            values, mask, rows, strides[0], out_stride, N, V, code, out_code, K, M, rep_s, pres_s, freq_s, 0))
     return (out, best) if greedy else out
