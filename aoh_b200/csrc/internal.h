@@ -53,6 +53,12 @@ struct PerDeviceOnce {
 // The calling thread's current device.
 int current_device(int* device);
 
+// A retrieval unit: its index, where its block table starts, and how many
+// entries that has (0: stored on another device).
+struct alignas(16) RetrievalRow {
+  int32_t unit, table, held, pad;
+};
+
 // Kernel-side view of the cache geometry (passed by value).
 struct CacheGeom {
   int B, Hq, G, grp, L;
@@ -86,7 +92,7 @@ struct aoh_kv_cache {
   int32_t* dev_table = nullptr;
   int32_t* dev_err = nullptr;   // [0] check word, [1] device-resident sequence length
   int32_t* dev_unit_row = nullptr;  // per unit: its index among the retrieval units (stored here or not), -1: streaming
-  int32_t* dev_row_unit = nullptr;  // per retrieval unit in that order: its unit
+  aoh::RetrievalRow* dev_rows = nullptr;  // the retrieval units in that order
   int32_t len_hint = 0;          // host copy of the device length (plans kernels in device mode)
   bool bound = false;
   int device = -1;

@@ -129,8 +129,8 @@ __device__ __forceinline__ int last_key(const KeyWeightsArgs& a, int past, int r
 template <typename T>
 __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
-  const int r = blockIdx.y, unit = a.row_unit[r];
-  if (a.g.unit_offset[unit] == a.g.unit_offset[unit + 1]) return;
+  const int r = blockIdx.y, unit = a.rows[r].unit;
+  if (a.rows[r].held == 0) return;
   const int past = key_weights_past(a);
   const int rows = a.q_len * a.g.grp, row0 = blockIdx.z * kTile;
   const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
@@ -191,12 +191,12 @@ template <typename T>
 __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
   __shared__ float lse[kTile];
-  const int r = blockIdx.y, unit = a.row_unit[r];
+  const int r = blockIdx.y, unit = a.rows[r].unit;
   const int past = key_weights_past(a);
   const int len = past + a.q_len, rows = a.q_len * a.g.grp;
   const int j0 = blockIdx.x * kSumKeys;
   if (j0 >= len) return;
-  const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
+  const bool stored = a.rows[r].held > 0;
   const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
   const long long rows_total = (long long)a.units * rows;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
@@ -350,7 +350,7 @@ extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len,
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);
   int row0 = 0;
   for (int l = 0; l < layer; ++l) row0 += c->cfg.batch * retrieval_heads(c, l);
-  a.row_unit = c->dev_row_unit + row0;
+  a.rows = c->dev_rows + row0;
   a.unit0 = c->unit(layer, 0, 0);
   a.past_len = past_len;
   a.past_len_dev = device_len ? c->dev_err + 1 : nullptr;

@@ -10,7 +10,7 @@ namespace aoh {
 // row = token * grp + head.
 struct KeyWeightsArgs {
   CacheGeom g;
-  const int32_t* row_unit;  // per retrieval row of this layer: its unit
+  const RetrievalRow* rows;  // the layer's retrieval rows
   int unit0;                // first unit of the layer
   int units;                // retrieval rows of the layer: B * n_ret
   int past_len;             // keys cached before these queries

@@ -53,8 +53,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
   __shared__ float2 red[kFewWarps][NT * 8];
   const KeyWeightsArgs& a = f.a;
   griddep_launch_dependents();  // the sums wait for this grid to finish
-  const int r = blockIdx.y, unit = a.row_unit[r];
-  const int base = a.g.unit_offset[unit], held = a.g.unit_offset[unit + 1] - base;
+  const int r = blockIdx.y;
+  const RetrievalRow info = a.rows[r];
+  const int unit = info.unit, base = info.table, held = info.held;
   if (held == 0) return;
   const int past = key_weights_past(a), len = past + a.q_len;
   const int n_pages = (len + kPage - 1) / kPage;
@@ -186,8 +187,8 @@ constexpr int kFewKeys = 4;
 __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
   __shared__ float lse[kFewRows];
   const KeyWeightsArgs& a = f.a;
-  const int r = blockIdx.y, unit = a.row_unit[r];
-  const bool stored = a.g.unit_offset[unit] != a.g.unit_offset[unit + 1];
+  const int r = blockIdx.y;
+  const bool stored = a.rows[r].held > 0;
   const int len = key_weights_past(a) + a.q_len;
   const int j0 = blockIdx.x * 256 * kFewKeys + threadIdx.x;
   griddep_wait();
@@ -368,8 +369,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int r = item % a.units;
   // causal: late query rows see more keys, early keys are seen by more rows -- the long items first
   const int pair = kPass == kLse ? t.pairs - 1 - item / a.units : item / a.units;
-  const int unit = a.row_unit[r];
-  const int base = G.unit_offset[unit], held = G.unit_offset[unit + 1] - base;
+  const RetrievalRow info = a.rows[r];
+  const int unit = info.unit, base = info.table, held = info.held;
   const int past = key_weights_past(a), len = past + a.q_len;
   const int b = (unit - a.unit0) / G.G, kvh = (unit - a.unit0) % G.G;
   const int tt = t.tile_tokens;
@@ -398,6 +399,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     return;
   }
 
+  // K rows of 128 keys: lane = (page, 64-dim half), 2 KB each; the page id is not looked at until the tile's turn
+  auto wanted = [&](int tile) { return lane < 16 && (tile * 8 + (lane >> 1)) * kPage < len; };
+  auto fetch_id = [&](int tile) {
+    const int p = tile * 8 + (lane >> 1);
+    return wanted(tile) && p < held ? G.block_table[base + p] : -1;
+  };
+  int id_next = -1, id_second = -1;
+  if (warp == 0) {
+    if (kKeysStreamed) {
+      if (n > 0) id_next = fetch_id(t0);
+    } else {
+      id_next = fetch_id(2 * pair);
+      if (na > 1) id_second = fetch_id(2 * pair + 1);
+    }
+  }
   if (warp == 1) {
     tmem_alloc(&s_tmem, kTmemCols);
     tmem_relinquish();
@@ -431,18 +447,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       reinterpret_cast<uint4*>(tiles + h * kHalfTile + row * 128)[i % 8] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  if (kPass == kStream) {
-    // -lse of the resident query rows from their key ranges
-    griddep_wait();
-    const long long rows = (long long)a.units * t.row_tiles * kTileRows;
-    if (tid < na * kTileRows) {
-      const float2* p = t.part + ((long long)r * t.row_tiles + 2 * pair) * kTileRows + tid;
-      float2 ml = make_float2(-INFINITY, 0.f);
-#pragma unroll 8
-      for (int s = 0; s < t.lse_splits; ++s) ml = merge_ml(ml, p[s * rows]);
-      sLse[tid] = ml.y > 0.f ? -(ml.x + log2f(ml.y)) : -INFINITY;
-    }
-  }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
@@ -452,15 +456,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp == 0) {
     // ============================ loads ============================
-    const int32_t* bt = G.block_table + base;
     const uint8_t* pool = static_cast<const uint8_t*>(G.pool);
     const uint32_t q_bytes = (uint32_t)q_rows * 256;
-    // K rows of 128 keys: lane = (page, 64-dim half), 2 KB each
-    auto key_id = [&](int tile) {
-      const int p = tile * 8 + (lane >> 1);
-      if (lane >= 16 || p * kPage >= len) return -1;
-      const int id = p < held ? bt[p] : -1;
-      if (id >= 0 && id < G.num_pages) return id;
+    auto check_id = [&](int tile, int id) {
+      if (!wanted(tile) || (id >= 0 && id < G.num_pages)) return id;
       atomicOr(G.err, kErrBadPage);
       return -1;
     };
@@ -489,18 +488,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; w < na; ++w) load_queries(2 * pair + w, sA + w * kTileBytes, &bar_a);
       }
     } else {
-      const int id0 = key_id(2 * pair), id1 = na > 1 ? key_id(2 * pair + 1) : -1;
+      const int id0 = check_id(2 * pair, id_next), id1 = na > 1 ? check_id(2 * pair + 1, id_second) : -1;
       expect_blocks(&bar_a, __popc(__ballot_sync(0xffffffffu, id0 >= 0)) + __popc(__ballot_sync(0xffffffffu, id1 >= 0)));
       copy_keys(id0, sA, &bar_a);
       copy_keys(id1, sA + kTileBytes, &bar_a);
       griddep_wait();  // the lse that the first pass found
     }
     int issued = 0;
-    int id_next = kKeysStreamed && n > 0 ? key_id(t0) : -1;
     for (int i = 0; i < n; ++i) {
       const int s = i % kStages;
-      const int id = id_next;
-      if (kKeysStreamed && i + 1 < n) id_next = key_id(t0 + i + 1);
+      const int id = kKeysStreamed ? check_id(t0 + i, id_next) : -1;
+      if (kKeysStreamed && i + 1 < n) id_next = fetch_id(t0 + i + 1);
       if (lane == 0 && i >= kStages && !s_abort) {
         if (!mbar_wait(&bar_empty[s], (i / kStages - 1) & 1, G.err)) s_abort = 1;
       }
@@ -543,6 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!(ok = mbar_wait_warp(&bar_full[s], round & 1, G.err))) break;
       const int buf = i & 1;
       for (int w = 0; w < na && ok; ++w) {
+        if (kPass == kStream && i == 2 && w == 0) griddep_wait();  // as the warpgroups that give the buffers back
         if (i >= 2 && !(ok = mbar_wait_warp(&bar_s_empty[w][buf], ((i >> 1) - 1) & 1, G.err))) break;
         tc_fence_after();
         const uint64_t tile = res + w * (kTileBytes / 16);
@@ -567,7 +566,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t s_col = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + w * 2 * kTileRows + 64 * h;
     const int tile = 2 * pair + w;
     const int last = past + tile * tt + row / G.grp;  // kLse: last key the row's query sees
-    if (kPass == kSums) griddep_wait();
+    if (kPass != kLse) griddep_wait();
+    if (kPass == kStream) {
+      // -lse of the resident query rows from their key ranges, while the first products are made
+      const long long rows = (long long)a.units * t.row_tiles * kTileRows;
+      const int i = tid - 128;
+      if (i < na * kTileRows) {
+        const float2* p = t.part + ((long long)r * t.row_tiles + 2 * pair) * kTileRows + i;
+        float2 ml = make_float2(-INFINITY, 0.f);
+#pragma unroll 8
+        for (int k = 0; k < t.lse_splits; ++k) ml = merge_ml(ml, p[k * rows]);
+        sLse[i] = ml.y > 0.f ? -(ml.x + log2f(ml.y)) : -INFINITY;
+      }
+      named_bar_sync(1, na * 256);  // all threads of this role
+    }
     uint64_t acc[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[k] = 0;

@@ -182,10 +182,10 @@ int aoh_kv_create(const aoh_kv_config* cfg, aoh_kv_cache** out) {
 void aoh_kv_destroy(aoh_kv_cache* cache) { delete cache; }
 
 static int64_t tables_entries(const aoh_kv_cache* c) {
-  // [unit_offset: n_units+1][pad to 4][table][pad to 4][err: 4][unit_row: n_units][row_unit: n_units]
+  // [unit_offset: n_units+1][pad to 4][table][pad to 4][err: 4][rows: 4 * n_units][unit_row: n_units]
   int64_t head = ((int64_t)c->n_units + 1 + 3) / 4 * 4;
   int64_t tab = ((int64_t)c->table.size() + 3) / 4 * 4;
-  return head + tab + 4 + 2LL * c->n_units;
+  return head + tab + 4 + 5LL * c->n_units;
 }
 
 int aoh_kv_buffer_sizes(const aoh_kv_cache* c, int64_t* pool_bytes, int64_t* table_bytes) {
@@ -215,23 +215,31 @@ int aoh_kv_bind(aoh_kv_cache* c, void* pool, void* tables, aoh_stream stream) {
   c->dev_table = c->dev_base + head;
   int64_t tab = ((int64_t)c->table.size() + 3) / 4 * 4;
   c->dev_err = c->dev_table + tab;
-  c->dev_unit_row = c->dev_err + 4;
-  c->dev_row_unit = c->dev_unit_row + c->n_units;
+  c->dev_rows = reinterpret_cast<RetrievalRow*>(c->dev_err + 4);
+  c->dev_unit_row = c->dev_err + 4 + 4LL * c->n_units;
   rc = cuda_check(cudaMemcpyAsync(c->dev_unit_offset, c->unit_offset.data(),
                                   sizeof(int32_t) * c->unit_offset.size(), cudaMemcpyHostToDevice, st),
                   "upload unit offsets");
   if (rc) return rc;
   rc = cuda_check(cudaMemsetAsync(c->dev_err, 0, 16, st), "clear check word");
   if (rc) return rc;
-  std::vector<int32_t> rows(2 * (size_t)c->n_units, -1);  // unit_row, row_unit
+  std::vector<RetrievalRow> rows(c->n_units);
+  std::vector<int32_t> unit_row(c->n_units, -1);
   for (int32_t u = 0, n = 0; u < c->n_units; ++u) {
     if (!c->retrieval(u / (c->cfg.batch * c->cfg.num_kv_heads), u % c->cfg.num_kv_heads)) continue;
-    rows[c->n_units + n] = u;
-    rows[u] = n++;
+    rows[n] = {u, c->unit_offset[u], c->unit_offset[u + 1] - c->unit_offset[u], 0};
+    unit_row[u] = n++;
   }
-  rc = cuda_check(cudaMemcpyAsync(c->dev_unit_row, rows.data(), sizeof(int32_t) * rows.size(), cudaMemcpyHostToDevice, st),
-                  "upload unit rows");
-  if (rc) return rc;
+  rc = cuda_check(cudaMemcpyAsync(c->dev_rows, rows.data(), sizeof(RetrievalRow) * rows.size(), cudaMemcpyHostToDevice, st),
+                  "upload retrieval rows");
+  if (!rc)
+    rc = cuda_check(cudaMemcpyAsync(c->dev_unit_row, unit_row.data(), sizeof(int32_t) * unit_row.size(),
+                                    cudaMemcpyHostToDevice, st),
+                    "upload unit rows");
+  if (rc) {
+    cudaStreamSynchronize(st);  // the host copies must stay alive until the async copies ran
+    return rc;
+  }
   c->bound = true;
   c->dirty_lo = 0;
   c->dirty_hi = (int64_t)c->table.size();
