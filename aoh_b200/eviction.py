@@ -161,7 +161,7 @@ class KeyWeights:
     def layer(self, layer_idx: int) -> torch.Tensor:
         """(batch, n_ret, max_context) of one layer, a view."""
         lo, hi = self._first[layer_idx], self._first[layer_idx + 1]
-        return self.rows[lo:hi].view(self.cache.batch, self.cache.n_ret[layer_idx], -1)
+        return self.rows[lo:hi].view(self.cache.batch, self.cache.n_ret[layer_idx], self.rows.shape[1])
 
     def add(self, layer_idx: int, q: torch.Tensor, past_len: int | None = None) -> None:
         """Add what the queries q gave (see :func:`key_weights`)."""
@@ -172,8 +172,10 @@ class KeyWeights:
         last ``recent`` (default: the cache's window) among them -- and copy them
         into ``into``.  Returns its KeyWeights, with the kept keys' sums."""
         c = self.cache
-        kept, weights = select_keys(self.rows[:, :c.kv_seq_len], keep, sink=c.sink_size if sink is None else sink,
-                                    recent=c.recent_size if recent is None else recent)
+        sink, recent = c.sink_size if sink is None else sink, c.recent_size if recent is None else recent
+        if keep == c.kv_seq_len:  # all of them, however short the sequence is
+            sink, recent = keep, 0
+        kept, weights = select_keys(self.rows[:, :c.kv_seq_len], keep, sink=sink, recent=recent)
         evict(c, kept, into)
         new = KeyWeights(into)
         new.rows[:, :keep] = weights

@@ -422,7 +422,9 @@ def same_bits(a, b):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("N,V,K", [(1, 1, 0), (1, 31, 1), (2, 64, 5), (3, 4096, 0), (5, 4097, 300), (2, 32_003, 7),
-                                   (1, 128_256, 16), (3, 50_000, 2000)])
+                                   (1, 128_256, 16), (3, 50_000, 2000),
+                                   # more rows, fewer CTAs each: slices of several rounds, aligned rows and not
+                                   (40, 70_000, 9), (80, 40_001, 0), (2, 400_000, 4096)])
 def test_penalize_logits(dtype, N, V, K):
     g = gen(N * V + K)
     x = randn(g, N, V, dtype=dtype) * 3
@@ -579,6 +581,31 @@ def test_prefill_evict_decode():
     was = torch.gather(sums.rows, 1, kept.long()).double().sum(1)
     assert ((total - was - 12).abs() <= 1e-3).all()
     assert small.device_status() == 0 and cache.device_status() == 0
+
+
+def test_key_weights_object():
+    """Rows by layer and sequence, sums moved by an eviction, sequences shorter than the window."""
+    labels = [[1, 0, 1], [0, 0, 0], [0, 1, 0]]
+    cache, k, _ = filled(labels, 6, 2, 60, BF16, 14, 16, 48, max_context=70)
+    sums = KeyWeights(cache)
+    assert sums.rows.shape == (6, 70)
+    q = [randn(gen(i), 2, 2, 6, 128, dtype=BF16) for i in range(3)]
+    for _ in range(2):
+        for layer in range(3):
+            sums.add(layer, q[layer], past_len=58)
+    for layer, heads in ((0, [0, 2]), (2, [1])):
+        want, tol = weights_exact(q[layer], k[layer], heads, 58)
+        got = sums.layer(layer)[:, :, :60].double().cpu()
+        assert got.shape == want.shape and ((got - 2 * want).abs() <= 2 * tol * want + 2.0 ** -100).all()
+    assert (sums.rows[:, 60:] == 0).all()
+    # 60 tokens are fewer than the sink and the window: all of them stay
+    into = AoHKVCache(labels, 6, batch=2, sink_size=16, recent_size=48, max_context=80)
+    moved = sums.evict(60, into)
+    assert torch.equal(moved.rows[:, :60], sums.rows[:, :60]) and moved.cache is into and into.tokens_seen == 60
+    with pytest.raises(ValueError):
+        sums.evict(50, into)  # some would have to go, and the window does not fit
+    with pytest.raises(ValueError):
+        sums.evict(61, into)
 
 
 def test_operators_on_a_side_stream_and_in_a_graph():
