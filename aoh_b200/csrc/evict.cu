@@ -96,15 +96,22 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
   if (a.take > 0) {  // the same for every CTA of the cluster
     const int per = a.part / kSelThreads;  // <= kKeys
     const int i0 = warp * 32 * per + lane;
-    float x[kKeys ? kKeys : 1];
+    // Behind the last key: 0, below every weight's key.  It is counted, but the
+    // `take` largest keys, among which the threshold is sought, are weights.
+    uint32_t key[kKeys ? kKeys : 1];
+    if constexpr (kKeys > 0) {
+      float x[kKeys];
 #pragma unroll
-    for (int j = 0; j < kKeys; ++j) x[j] = j < per && i0 + 32 * j < cnt ? wm[i0 + 32 * j] : 0.f;
+      for (int j = 0; j < kKeys; ++j) x[j] = i0 + 32 * j < cnt ? wm[i0 + 32 * j] : 0.f;
+#pragma unroll
+      for (int j = 0; j < kKeys; ++j) key[j] = i0 + 32 * j < cnt ? weight_key(x[j]) : 0u;
+    }
     // f(key, its index) for each of the thread's keys; every lane of a warp together
     auto each = [&](auto&& f) {
       if constexpr (kKeys > 0) {
 #pragma unroll
         for (int j = 0; j < kKeys; ++j)
-          if (j < per) f(weight_key(x[j]), i0 + 32 * j);
+          if (j < per) f(key[j], i0 + 32 * j);
       } else {
         for (int j = 0; j < per; ++j) f(i0 + 32 * j < cnt ? weight_key(wm[i0 + 32 * j]) : 0u, i0 + 32 * j);
       }
@@ -118,8 +125,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digit = pass == 2 ? 1023u : 2047u;
       uint32_t* hist = s_hist[pass];
-      each([&](uint32_t k, int i) {  // digits above this one agree with the threshold
-        if (i < cnt && (pass == 0 || k >> (pass == 2 ? 10 : 21) == prefix)) atomicAdd(&hist[k >> shift & digit], 1u);
+      each([&](uint32_t k, int) {  // digits above this one agree with the threshold
+        if (pass == 0 || k >> (pass == 2 ? 10 : 21) == prefix) atomicAdd(&hist[k >> shift & digit], 1u);
       });
       sync();
       // thread t sums the bins kBins - 1 - 2 t and the one below over the cluster
@@ -160,9 +167,9 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     const uint32_t thr = prefix;
 
     uint32_t gt = 0, eq = 0;
-    each([&](uint32_t k, int i) {
-      gt += i < cnt && k > thr;
-      eq += i < cnt && k == thr;
+    each([&](uint32_t k, int) {
+      gt += k > thr;
+      eq += k == thr;
     });
     gt = __reduce_add_sync(0xffffffffu, gt);
     eq = __reduce_add_sync(0xffffffffu, eq);
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     }
     const unsigned below = (1u << lane) - 1u;
     each([&](uint32_t k, int i) {
-      const bool is_gt = i < cnt && k > thr, is_eq = i < cnt && k == thr;
+      const bool is_gt = k > thr, is_eq = k == thr;
       const unsigned mg = __ballot_sync(0xffffffffu, is_gt), me = __ballot_sync(0xffffffffu, is_eq);
       const uint32_t re = be + __popc(me & below);
       if (is_gt || (is_eq && re < left)) {

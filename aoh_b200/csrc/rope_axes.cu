@@ -39,10 +39,13 @@ struct RopeAxesArgs {
   const void* pos;
   const float* inv_freq;
   long long qs[3], ks[3], ps[3];  // strides in elements: batch, token, head / axis, batch, token
+  int qn[3], kn[3], pn[3];        // the same, where no offset leaves 31 bits
+  bool narrow;
   long long n_tokens;
   int q_len, hq, g, d, half;
   int tokens, heads;     // of one CTA
-  uint32_t heads_magic;  // floor(2^32 / heads) + 1: row / heads is the high word of row * magic (rows of a CTA are few)
+  // floor(2^32 / x) + 1: n / x is the high word of n * magic for the few n of a CTA
+  uint32_t heads_magic, half_magic;
   int lanes_log2;
   float eps, scaling;
   bool pos64;
@@ -70,15 +73,30 @@ struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) Pack {
 
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const Pack<T, VEC>& r, float* x) {
+  if constexpr (sizeof(T) == 2 && VEC == 8) {  // two at a time
+    const uint4 u = *reinterpret_cast<const uint4*>(&r);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) x[j] = to_f(r.v[j]);
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = bf16_lo(w[j]);
+      x[2 * j + 1] = bf16_hi(w[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = to_f(r.v[j]);
+  }
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store(T* p, const float* x) {
-  Pack<T, VEC> r;
+  if constexpr (sizeof(T) == 2 && VEC == 8) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+  } else {
+    Pack<T, VEC> r;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) r.v[j] = from_f<T>(x[j]);
-  *reinterpret_cast<Pack<T, VEC>*>(p) = r;
+    for (int j = 0; j < VEC; ++j) r.v[j] = from_f<T>(x[j]);
+    *reinterpret_cast<Pack<T, VEC>*>(p) = r;
+  }
 }
 
 // An item is VEC rotated pairs (i.., i + half..) or, behind them, up to
@@ -135,8 +153,12 @@ __global__ void __launch_bounds__(kThreads, ITEMS > 1 || ROWS > 2 ? 3 : 5)
     if (h < 0) continue;
     int b, c;
     locate(toks[r], b, c);
-    const T* src = h < a.hq ? static_cast<const T*>(a.q) + b * a.qs[0] + c * a.qs[1] + h * a.qs[2]
-                            : static_cast<const T*>(a.k) + b * a.ks[0] + c * a.ks[1] + (h - a.hq) * a.ks[2];
+    long long off;
+    if (a.narrow)
+      off = h < a.hq ? b * a.qn[0] + c * a.qn[1] + h * a.qn[2] : b * a.kn[0] + c * a.kn[1] + (h - a.hq) * a.kn[2];
+    else
+      off = h < a.hq ? b * a.qs[0] + c * a.qs[1] + h * a.qs[2] : b * a.ks[0] + c * a.ks[1] + (h - a.hq) * a.ks[2];
+    const T* src = static_cast<const T*>(h < a.hq ? a.q : a.k) + off;
 #pragma unroll
     for (int n = 0; n < ITEMS; ++n) {
       const int it = lane + (n << a.lanes_log2);
@@ -150,10 +172,11 @@ __global__ void __launch_bounds__(kThreads, ITEMS > 1 || ROWS > 2 ? 3 : 5)
     }
   }
   for (int e = threadIdx.x; e < ntok * half; e += kThreads) {
-    const int t = (unsigned)e / (unsigned)half, i = e - t * half;
+    const int t = half > 1 ? (int)__umulhi((unsigned)e, a.half_magic) : e, i = e - t * half;
     int b, c;
     locate(t, b, c);
-    const long long at = a.axis[i] * a.ps[0] + b * a.ps[1] + c * a.ps[2];
+    const long long at = a.narrow ? a.axis[i] * a.pn[0] + b * a.pn[1] + c * a.pn[2]
+                                  : a.axis[i] * a.ps[0] + b * a.ps[1] + c * a.ps[2];
     const double p = a.pos64 ? (double)static_cast<const long long*>(a.pos)[at]
                              : (double)static_cast<const int*>(a.pos)[at];
     const double turns = p * (double)a.inv_freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
@@ -231,6 +254,7 @@ int launch_rows(RopeAxesArgs& a, cudaStream_t st) {
   a.heads = std::min(heads, most);
   a.tokens = std::max(1, std::min(kMaxTokens, most / heads));
   a.heads_magic = (uint32_t)((1ULL << 32) / a.heads + 1);  // a q and a k head at least
+  a.half_magic = (uint32_t)((1ULL << 32) / a.half + 1);    // not used with half 1
   const long long gx = (a.n_tokens + a.tokens - 1) / a.tokens;
   const int gy = (heads + a.heads - 1) / a.heads;
   if (a.n_tokens > 0x7fffffffLL || gy > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many rows");
@@ -322,6 +346,22 @@ extern "C" int aoh_rope_axes_qk(const aoh_rope_axes_args* args, aoh_stream strea
     a.ks[i] = p.k_strides[i];
     a.ps[i] = p.position_strides[i];
   }
+  // 32-bit offsets, a third of the integer work of 64-bit ones, where the farthest element allows them
+  auto farthest = [](const int64_t* s, int64_t n0, int64_t n1, int64_t n2) {
+    return (n0 - 1) * std::abs(s[0]) + (n1 - 1) * std::abs(s[1]) + (n2 - 1) * std::abs(s[2]);
+  };
+  const int64_t limit = 1LL << 30;
+  a.narrow = true;
+  for (int i = 0; i < 3; ++i) {
+    a.narrow = a.narrow && std::abs(p.q_strides[i]) < limit && std::abs(p.k_strides[i]) < limit &&
+               std::abs(p.position_strides[i]) < limit;
+    a.qn[i] = (int)p.q_strides[i];
+    a.kn[i] = (int)p.k_strides[i];
+    a.pn[i] = (int)p.position_strides[i];
+  }
+  a.narrow = a.narrow && farthest(p.q_strides, p.batch, p.q_len, p.num_q_heads) < limit &&
+             farthest(p.k_strides, p.batch, p.q_len, p.num_kv_heads) < limit &&
+             farthest(p.position_strides, n_axes, p.batch, p.q_len) < limit;
   a.q_len = p.q_len;
   a.hq = p.num_q_heads;
   a.g = p.num_kv_heads;
