@@ -92,7 +92,8 @@ __device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int
   for (int i = 0; i < KT / 8; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
-// s[i][j]: row 4 ty + i, key tx + 16 j, in the log2 domain
+// s[i][j] = q . k of row 4 ty + i and key tx + 16 j.  The scaling to the log2
+// domain is left to the subtraction of a row's maximum, one rounding for both.
 template <int J>
 __device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][J]) {
 #pragma unroll
@@ -116,10 +117,6 @@ __device__ __forceinline__ void tile_scores(const float* qs, const float* ks, in
         s[i][j] = fmaf(q[i].w, k[j].w, s[i][j]);
       }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[i][j] *= kScoreScale;
 }
 
 // Keys a row may see: j <= past + token.
@@ -162,13 +159,14 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
         if (t * kTile + tx + 16 * j > last) s[i][j] = -INFINITY;
         mt = fmaxf(mt, s[i][j]);
       }
+      mt *= kScoreScale;
       if (mt > m[i]) {
         l[i] *= fast_exp2(m[i] - mt);
         m[i] = mt;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (s[i][j] > -INFINITY) l[i] += fast_exp2(s[i][j] - m[i]);
+        if (s[i][j] > -INFINITY) l[i] += fast_exp2(fmaf(s[i][j], kScoreScale, -m[i]));
     }
   }
   // the 16 threads of a row
@@ -190,7 +188,7 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
 template <typename T>
 __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
   extern __shared__ float sm[];
-  __shared__ float lse[kTile];
+  __shared__ float2 ml[kTile];  // of a row: its maximum and 1 / sum
   const int r = blockIdx.y, unit = a.rows[r].unit;
   const int past = key_weights_past(a);
   const int len = past + a.q_len, rows = a.q_len * a.g.grp;
@@ -210,7 +208,7 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
     for (int row0 = tok0 * a.g.grp; row0 < rows; row0 += kTile) {
       __syncthreads();
       load_queries<T>(a, b, g, row0, rows, qs);
-      {  // -lse of the tile's rows from their key ranges, four threads a row
+      {  // the tile's rows' maxima and sums from their key ranges, four threads a row
         const int row = threadIdx.x >> 2;
         float mm = -INFINITY, ll = 0.f;
         if (row0 + row < rows) {
@@ -230,7 +228,7 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
           ll = (ll > 0.f ? ll * fast_exp2(mm - top) : 0.f) + (ol > 0.f ? ol * fast_exp2(om - top) : 0.f);
           mm = top;
         }
-        if ((threadIdx.x & 3) == 0) lse[row] = mm + log2f(ll);
+        if ((threadIdx.x & 3) == 0) ml[row] = make_float2(mm, 1.f / ll);
       }
       __syncthreads();
       if (row0 + 8 * (int)(threadIdx.x >> 5) >= rows) continue;  // none of this warp's 8 rows is one
@@ -241,10 +239,10 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ Ke
         const int row = row0 + 4 * ty + i;
         if (row >= rows) continue;
         const int last = last_key(a, past, row);
-        const float e = lse[4 * ty + i];
+        const float2 e = ml[4 * ty + i];
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          if (j0 + tx + 16 * j <= last) w[j] += fast_exp2(s[i][j] - e);
+          if (j0 + tx + 16 * j <= last) w[j] = fmaf(fast_exp2(fmaf(s[i][j], kScoreScale, -e.x)), e.y, w[j]);
       }
     }
   }

@@ -43,7 +43,7 @@ constexpr int kFewWarps = 8;
 struct FewArgs {
   KeyWeightsArgs a;
   float2* part;   // [split][unit row][row]
-  float* score;   // [unit row][key][rows_even], log2 domain, -inf where a row does not see the key
+  float* score;   // [unit row][key][rows_even]: q . k, -inf where a row does not see the key
   int rows, rows_even, splits;
   long long score_unit;  // floats of a unit's scores
 };
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s[h][e] = j0 + 8 * h <= last[n][e] ? c[n][2 * h + e] * kScoreScale : -INFINITY;
+        for (int e = 0; e < 2; ++e) s[h][e] = j0 + 8 * h <= last[n][e] ? c[n][2 * h + e] : -INFINITY;
       const int col = n * 8 + 2 * tq;
       if (col < f.rows_even) {
         float* o = f.score + r * f.score_unit + (long long)j0 * f.rows_even + col;
@@ -146,12 +146,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float mt = fmaxf(s[0][e], s[1][e]);
+        // the scaling is part of the subtraction's one rounding: scaled by itself, a score of 16 is 1e-6 off
+        const float mt = fmaxf(s[0][e], s[1][e]) * kScoreScale;
         if (mt > m[n][e]) {
           l[n][e] *= fast_exp2(m[n][e] - mt);
           m[n][e] = mt;
         }
-        if (m[n][e] > -INFINITY) l[n][e] += fast_exp2(s[0][e] - m[n][e]) + fast_exp2(s[1][e] - m[n][e]);
+        if (m[n][e] > -INFINITY)
+          l[n][e] += fast_exp2(fmaf(s[0][e], kScoreScale, -m[n][e])) + fast_exp2(fmaf(s[1][e], kScoreScale, -m[n][e]));
       }
     }
 #pragma unroll
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
 // Weights of 1024 keys from their scores, four keys a thread.
 constexpr int kFewKeys = 4;
 __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
-  __shared__ float lse[kFewRows];
+  __shared__ float2 ml[kFewRows];  // of a row: its maximum and 1 / sum (their rounded logarithm would be 1e-6 off)
   const KeyWeightsArgs& a = f.a;
   const int r = blockIdx.y;
   const bool stored = a.rows[r].held > 0;
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
       l = m > -INFINITY ? l * fast_exp2(m - mm) : 0.f;
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-      if (lane == 0) lse[row] = mm + log2f(l);
+      if (lane == 0) ml[row] = make_float2(mm, 1.f / l);
     }
   }
   __syncthreads();
@@ -228,8 +230,8 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
       for (int k = 0; k < kFewKeys; ++k) {
         if (j0 + 256 * k >= len) continue;
         if (row > 0) v[k] = *reinterpret_cast<const float2*>(s + (long long)(j0 + 256 * k) * f.rows_even + row);
-        w[k] += fast_exp2(v[k].x - lse[row]);
-        if (row + 1 < f.rows) w[k] += fast_exp2(v[k].y - lse[row + 1]);
+        w[k] = fmaf(fast_exp2(fmaf(v[k].x, kScoreScale, -ml[row].x)), ml[row].y, w[k]);
+        if (row + 1 < f.rows) w[k] = fmaf(fast_exp2(fmaf(v[k].y, kScoreScale, -ml[row + 1].x)), ml[row + 1].y, w[k]);
       }
     }
   }
