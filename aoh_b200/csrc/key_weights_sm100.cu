@@ -789,18 +789,22 @@ int launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t
   return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 
-// Ranges that `items` CTAs' lists of `tiles` tiles are cut into, one CTA per
-// SM: the fewest tile periods, a range costing its tiles and about four for a
-// CTA's start and end.  Candidates: a few ranges, and what fills 1 to 4 waves.
-int plan_ranges(long long items, int tiles, int sms) {
+// Ranges that `items` CTAs' lists of at most `tiles` tiles are cut into, one CTA
+// per SM: the fewest tile periods, a range costing its tiles and about four for
+// a CTA's start and end.  Candidates: a few ranges, and what fills 1 to 4 waves.
+// 4096 tokens over 16384 keys, 4 units: `even` lists in 1, 2, 3, 4, 7 ranges
+// 311, 319, 327, 304, 335 us; uneven ones 343, 288, 296, 298, 321 us.
+int plan_ranges(long long items, int tiles, int sms, bool even) {
   int best = 1;
   double least = 1e300;
   for (int k = 1; k <= 12; ++k) {
     const long long s = k <= 8 ? k : (k - 8) * (long long)sms / items;
     if (s < 1 || s > std::min(tiles, 256)) continue;
     const double ctas = (double)items * s / sms;
-    // several waves overlap at their ends: half a range is lost, not a whole one
-    const double cost = (ctas > 1 ? ctas + 0.5 : 1.0) * ((tiles + s - 1) / s + 4);
+    // lists of one length end in whole waves; of uneven ones, the long ones
+    // first, the waves overlap at their ends and half a range is lost
+    const double waves = ctas <= 1 ? 1.0 : even ? (double)(((long long)items * s + sms - 1) / sms) : ctas + 0.5;
+    const double cost = waves * ((tiles + s - 1) / s + 4);
     if (cost < least * 0.98) {
       best = (int)s;
       least = cost;
@@ -851,10 +855,11 @@ void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int 
   p.tile_tokens = std::min(kTileRows / grp, q_len);
   p.row_tiles = (q_len + p.tile_tokens - 1) / p.tile_tokens;
   const long long lse_items = (long long)units * ((p.row_tiles + 1) / 2), sum_items = (long long)units * key_pairs(max_len);
-  p.splits = plan_ranges(lse_items, (max_len + kTileRows - 1) / kTileRows, sms);
+  // causal: the first tokens' rows have max_len - q_len keys, the last ones' max_len
+  p.splits = plan_ranges(lse_items, (max_len + kTileRows - 1) / kTileRows, sms, max_len - q_len >= max_len / 4 * 3);
   // up to two tiles of query rows stay resident in the second pass too, which then needs the ranges alone
   p.stream = p.row_tiles <= 2;
-  p.row_splits = p.stream ? p.splits : plan_ranges(sum_items, p.row_tiles, sms);
+  p.row_splits = p.stream ? p.splits : plan_ranges(sum_items, p.row_tiles, sms, false);
   const size_t rows = (size_t)units * p.row_tiles * kTileRows;
   p.part = 0;
   p.lse = p.stream || p.splits > 1 ? align256(rows * p.splits * sizeof(float2)) : 0;
