@@ -5,160 +5,182 @@
 //
 // i.e. the column sums of the softmax matrix whose product with V the
 // attention entry points compute.  A weight needs its row's maximum and sum
-// over all keys first, so two passes over K: one for every query row's (m, l),
-// by key ranges that fill the GPU, one that adds up exp(s - lse) per key.  Each
-// key is summed by one CTA in a fixed order, so results do not depend on timing.
+// over all keys first, so a call has two passes: one for every query row's
+// (m, l), by key ranges that fill the GPU, one that adds up exp(s - lse) per
+// key.  Each key is summed by one CTA in a fixed order, so results do not depend
+// on timing.
 //
-// This file holds the entry point and the kernels for any type: 64 rows x 64
-// (or 32) keys per tile in fp32 on the CUDA cores, 4 x 4 products a thread.  bf16
-// caches run those of key_weights_sm100.cu: one pass over K for few query rows
-// (single tokens), tensor cores for more.
+// This file holds the entry point and the kernels for any type.  Their first
+// pass also writes the scores, 4 bytes each, and the second reads them: 128
+// products on the CUDA cores cost 3.6 ps, a write and a read of 4 bytes 1.2 ps.
+// The query rows are taken in blocks whose scores fit L2, two launches a block.
+// 2 x 33 tokens of 6 heads over 2023 keys, fp32: 18 us a call,
+// of which the scores take 12; with the scores computed again 35.
+// bf16 caches run the kernels of key_weights_sm100.cu: one pass over K for few
+// query rows (single tokens), tensor cores for more.
 #include "common.cuh"
 #include "internal.h"
+#include "fast_math.cuh"
 #include "key_weights.h"
 #include "page_layout.cuh"
 
 namespace aoh {
 namespace {
 
-constexpr int kTile = 64;                 // query rows of a tile, and keys of the first pass's
-constexpr int kSumKeys = 32;              // keys of the second pass's tiles: twice the CTAs, which 64 leave uneven
+constexpr int kTile = 64;                 // query rows, and keys, of a tile
+constexpr int kSumKeys = 32;              // keys of a CTA of the second pass
+constexpr int kSumRows = 128;             // query rows whose maximum and sum it holds at a time
 constexpr int kStride = kHeadDim + 4;     // floats of a row in shared memory: 16-byte rows on distinct banks
-constexpr int kSmem = 2 * kTile * kStride * 4, kSumSmem = (kTile + kSumKeys) * kStride * 4;
+constexpr int any_smem(int tile_rows) { return (kTile + tile_rows) * kStride * 4; }
+constexpr long long kScoreBytes = 96 << 20;  // of a block of query rows, if 16 rows need no more: three quarters of L2
 
-// Four dimensions of a stored row, as loaded and as floats.
-template <typename T>
-struct Raw4;
-template <>
-struct Raw4<float> {
-  float4 v;
-  __device__ float4 get() const { return v; }
-};
-template <>
-struct Raw4<__nv_bfloat16> {
-  uint2 v;
-  __device__ float4 get() const { return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)); }
+// A block of query rows: rows row_base .. row_base + rows - 1 of every unit.
+struct AnyArgs {
+  KeyWeightsArgs a;
+  float2* part;        // (key range, retrieval row, query row): maximum, sum
+  float* score;        // (retrieval row, query row, key): q . k
+  long long score_row; // floats of a query row's scores
+  int splits, row_base, rows, tile_rows;
 };
 
-constexpr int kLoads = kTile * (kHeadDim / 4) / 256;  // of a thread for a tile: row 8 i + warp, dimensions 4 lane ..
+// Four dimensions of a stored row into shared memory; fp32 without a register in between.
+__device__ __forceinline__ void copy4(float* dst, const float* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(float* dst, const __nv_bfloat16* src) {
+  const uint2 v = *reinterpret_cast<const uint2*>(src);
+  *reinterpret_cast<float4*>(dst) = make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The loads of a tile are all issued before any is stored: a thread's eight
-// would otherwise each wait for memory in turn.
+// A warp's 8 query rows from `row` on; rows from row_end on are zero.
 template <typename T>
-__device__ __forceinline__ void load_queries(const KeyWeightsArgs& a, int b, int g, int row0, int rows, float* sm) {
-  const int r0 = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
-  Raw4<T> v[kLoads];
+__device__ __forceinline__ void load_queries(const KeyWeightsArgs& a, int b, int g, int row, int row_end, float* sm) {
+  const int c = (threadIdx.x & 31) * 4;
+  int tok = row / a.g.grp, h = row % a.g.grp;
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int row = row0 + r0 + 8 * i;
-    v[i] = Raw4<T>{};
-    if (row < rows) {
-      const int tok = row / a.g.grp, h = g * a.g.grp + row % a.g.grp;
-      v[i] = *reinterpret_cast<const Raw4<T>*>(static_cast<const T*>(a.q) +
-                                               (((long long)b * a.q_len + tok) * a.g.Hq + h) * kHeadDim + c);
-    }
+  for (int i = 0; i < 8; ++i) {
+    float* dst = sm + i * kStride + c;
+    if (row + i < row_end)
+      copy4(dst, static_cast<const T*>(a.q) + (((long long)b * a.q_len + tok) * a.g.Hq + g * a.g.grp + h) * kHeadDim + c);
+    else
+      *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (++h == a.g.grp) h = 0, ++tok;
   }
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
-// Keys [j0, j0 + KT) of a unit; rows that are not stored are zero.
-template <typename T, int KT>
-__device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int unit, int j0, int len, float* sm) {
-  const int base = a.g.unit_offset[unit], n_pages = a.g.unit_offset[unit + 1] - base;
-  const int r0 = threadIdx.x >> 5, c = (threadIdx.x & 31) * 4;
-  int pages[KT / kPage];
-#pragma unroll
-  for (int i = 0; i < KT / kPage; ++i) {
-    const int p = j0 / kPage + i;
-    pages[i] = p * kPage < len && p < n_pages ? a.g.block_table[base + p] : -1;
-    if (pages[i] >= a.g.num_pages) pages[i] = -1;
-    if (pages[i] < 0 && p * kPage < len && threadIdx.x == 0) atomicOr(a.g.err, kErrBadPage);
-  }
-  Raw4<T> v[KT / 8];
-#pragma unroll
-  for (int i = 0; i < KT / 8; ++i) {
-    const int r = r0 + 8 * i, slot = r % kPage;
-    const int page = pages[8 * i / kPage];  // r0 < 8: row r is in page 8 i / 16
-    v[i] = Raw4<T>{};
-    if (page >= 0 && j0 + r < len) {
+// The page of keys j0 + 16 lane .. of a unit (lanes 0 to 3), -1 where there is none.
+__device__ __forceinline__ int fetch_page(const KeyWeightsArgs& a, const RetrievalRow& info, int j0, int len) {
+  const int lane = threadIdx.x & 31, p = j0 / kPage + lane;
+  return lane < kTile / kPage && p * kPage < len && p < info.held ? a.g.block_table[info.table + p] : -1;
+}
+
+// 64 keys from j0 on, the warps' rows in turn; rows that are not stored are zero.
+template <typename T>
+__device__ __forceinline__ void load_keys(const KeyWeightsArgs& a, int my_page, int j0, int len, float* sm) {
+  const int lane = threadIdx.x & 31, c = lane * 4, warps = blockDim.x >> 5;
+  if (threadIdx.x < kTile / kPage && j0 + (int)threadIdx.x * kPage < len && (my_page < 0 || my_page >= a.g.num_pages))
+    atomicOr(a.g.err, kErrBadPage);
+#pragma unroll 8
+  for (int r = threadIdx.x >> 5; r < kTile; r += warps) {
+    const int page = __shfl_sync(0xffffffffu, my_page, r / kPage), slot = r % kPage;
+    float* dst = sm + r * kStride + c;
+    if (page >= 0 && page < a.g.num_pages && j0 + r < len) {
       const char* p = static_cast<const char*>(a.g.pool);
       p += sizeof(T) == 4 ? (long long)page * kPageF32Bytes + 4 * f32_elem_offset(0, slot, c)
                           : (long long)page * kPageBf16Bytes + 2 * bf16_elem_offset(0, slot, c);
-      v[i] = *reinterpret_cast<const Raw4<T>*>(p);
+      copy4(dst, reinterpret_cast<const T*>(p));
+    } else {
+      *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
-#pragma unroll
-  for (int i = 0; i < KT / 8; ++i) *reinterpret_cast<float4*>(sm + (r0 + 8 * i) * kStride + c) = v[i].get();
 }
 
-// s[i][j] = q . k of row 4 ty + i and key tx + 16 j.  The scaling to the log2
-// domain is left to the subtraction of a row's maximum, one rounding for both.
-template <int J>
-__device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][J]) {
+// s[i][j] = q . k of row 4 ty + i and key tx + 16 j, even and odd dimensions
+// added apart: one packed product for two.  The scaling to the log2 domain is
+// left to the subtraction of a row's maximum, one rounding for both.
+__device__ __forceinline__ void tile_scores(const float* qs, const float* ks, int ty, int tx, float (&s)[4][4]) {
+  uint64_t acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < J; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0;
 #pragma unroll 4
   for (int d = 0; d < kHeadDim; d += 4) {
-    float4 q[4], k[J];
+    ulonglong2 q[4], k[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(qs + (4 * ty + i) * kStride + d);
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const ulonglong2*>(qs + (4 * ty + i) * kStride + d);
 #pragma unroll
-    for (int j = 0; j < J; ++j) k[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * kStride + d);
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const ulonglong2*>(ks + (tx + 16 * j) * kStride + d);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        s[i][j] = fmaf(q[i].x, k[j].x, s[i][j]);
-        s[i][j] = fmaf(q[i].y, k[j].y, s[i][j]);
-        s[i][j] = fmaf(q[i].z, k[j].z, s[i][j]);
-        s[i][j] = fmaf(q[i].w, k[j].w, s[i][j]);
-      }
+      for (int j = 0; j < 4; ++j) acc[i][j] = f2_fma(q[i].y, k[j].y, f2_fma(q[i].x, k[j].x, acc[i][j]));
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float x, y;
+      f2_unpack(acc[i][j], x, y);
+      s[i][j] = x + y;
+    }
 }
 
 // Keys a row may see: j <= past + token.
 __device__ __forceinline__ int last_key(const KeyWeightsArgs& a, int past, int row) { return past + row / a.g.grp; }
 
-// (m, l) of 64 query rows over one range of keys.
+// Scores and (m, l) of up to 64 query rows over one range of keys: a warp for 8
+// rows, a thread for 4 rows and 4 keys of each tile.
 template <typename T>
-__global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
+__global__ void __launch_bounds__(256, 3) key_lse_kernel(const __grid_constant__ AnyArgs k) {
   extern __shared__ float sm[];
-  const int r = blockIdx.y, unit = a.rows[r].unit;
-  if (a.rows[r].held == 0) return;
+  const KeyWeightsArgs& a = k.a;
+  griddep_launch_dependents();  // the sums wait for this grid to finish
+  const int r = blockIdx.y;
+  const RetrievalRow info = a.rows[r];
+  if (info.held == 0) return;
   const int past = key_weights_past(a);
-  const int rows = a.q_len * a.g.grp, row0 = blockIdx.z * kTile;
-  const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
-  const long long rows_total = (long long)a.units * rows;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  float *qs = sm, *ks = sm + kTile * kStride;
-  load_queries<T>(a, b, g, row0, rows, qs);
+  const int row0 = k.row_base + blockIdx.z * k.tile_rows, row_end = min(row0 + k.tile_rows, k.row_base + k.rows);
+  const int b = (info.unit - a.unit0) / a.g.G, g = (info.unit - a.unit0) % a.g.G;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15, warp_row = row0 + 8 * (int)(threadIdx.x >> 5);
+  float *ks = sm, *qs = sm + kTile * kStride;
   // key tiles up to the last one that any row of the tile sees, split evenly
-  const int len = last_key(a, past, min(row0 + kTile, rows) - 1) + 1;
+  const int len = last_key(a, past, row_end - 1) + 1;
   const int tiles = (len + kTile - 1) / kTile;
-  const int t0 = (int)((long long)tiles * blockIdx.x / splits), t1 = (int)((long long)tiles * (blockIdx.x + 1) / splits);
-  const bool idle = row0 + 8 * (int)(threadIdx.x >> 5) >= rows;  // a warp has 8 rows: none of them is one
+  const int t0 = (int)((long long)tiles * blockIdx.x / k.splits), t1 = (int)((long long)tiles * (blockIdx.x + 1) / k.splits);
+  int page = fetch_page(a, info, t0 * kTile, len);
+  if (t0 < t1) load_queries<T>(a, b, g, warp_row, row_end, qs + (threadIdx.x >> 5) * 8 * kStride);
   float m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.f;
   for (int t = t0; t < t1; ++t) {
+    if (t > t0) __syncthreads();
+    load_keys<T>(a, page, t * kTile, len, ks);
+    if (t + 1 < t1) page = fetch_page(a, info, (t + 1) * kTile, len);
+    copies_wait();
     __syncthreads();
-    load_keys<T, kTile>(a, unit, t * kTile, len, ks);
-    __syncthreads();
-    if (idle) continue;
+    if (warp_row >= row_end) continue;
     float s[4][4];
     tile_scores(qs, ks, ty, tx, s);
+    const int key = t * kTile + tx;
+    int row = row0 + 4 * ty, tok = row / a.g.grp, h = row % a.g.grp;
+    float* out = k.score + ((long long)r * k.rows + (row - k.row_base)) * k.score_row + key;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int last = last_key(a, past, row0 + 4 * ty + i);
+    for (int i = 0; i < 4; ++i, ++row) {
+      const int last = past + tok;
       float mt = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (t * kTile + tx + 16 * j > last) s[i][j] = -INFINITY;
+        if (key + 16 * j <= last) {
+          if (row < row_end) out[16 * j] = s[i][j];
+        } else {
+          s[i][j] = -INFINITY;
+        }
         mt = fmaxf(mt, s[i][j]);
       }
+      out += k.score_row;
+      if (++h == a.g.grp) h = 0, ++tok;
       mt *= kScoreScale;
       if (mt > m[i]) {
         l[i] *= fast_exp2(m[i] - mt);
@@ -179,82 +201,72 @@ __global__ void __launch_bounds__(256) key_lse_kernel(const __grid_constant__ Ke
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
     const int row = row0 + 4 * ty + i;
-    if (tx == 0 && row < rows)
-      part[blockIdx.x * rows_total + (long long)r * rows + row] = make_float2(mm, ll);
+    if (tx == 0 && row < row_end)
+      k.part[((long long)blockIdx.x * a.units + r) * k.rows + (row - k.row_base)] = make_float2(mm, ll);
   }
 }
 
-// The weights of kSumKeys keys, summed over every query row of the unit.
-template <typename T>
-__global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ KeyWeightsArgs a, float2* part, int splits) {
-  extern __shared__ float sm[];
-  __shared__ float2 ml[kTile];  // of a row: its maximum and 1 / sum
-  const int r = blockIdx.y, unit = a.rows[r].unit;
-  const int past = key_weights_past(a);
-  const int len = past + a.q_len, rows = a.q_len * a.g.grp;
-  const int j0 = blockIdx.x * kSumKeys;
+// The weights of kSumKeys keys, a lane each, summed over the block's query
+// rows: row 8 i + warp of every 128.
+__global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ AnyArgs k) {
+  constexpr int kMine = kSumRows / 8;
+  __shared__ float2 ml[kSumRows];  // of a row: its maximum and 1 / sum
+  __shared__ float sums[8][kSumKeys];
+  const KeyWeightsArgs& a = k.a;
+  const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int past = key_weights_past(a), len = past + a.q_len, j0 = (int)blockIdx.x * kSumKeys, key = j0 + lane;
   if (j0 >= len) return;
   const bool stored = a.rows[r].held > 0;
-  const int b = (unit - a.unit0) / a.g.G, g = (unit - a.unit0) % a.g.G;
-  const long long rows_total = (long long)a.units * rows;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  float *qs = sm, *ks = sm + kTile * kStride;
-  constexpr int J = kSumKeys / 16;
-  float w[J] = {};
-  if (stored) {
-    load_keys<T, kSumKeys>(a, unit, j0, len, ks);
-    // the first token that sees key j0
-    const int tok0 = max(0, j0 - past);
-    for (int row0 = tok0 * a.g.grp; row0 < rows; row0 += kTile) {
-      __syncthreads();
-      load_queries<T>(a, b, g, row0, rows, qs);
-      {  // the tile's rows' maxima and sums from their key ranges, four threads a row
-        const int row = threadIdx.x >> 2;
-        float mm = -INFINITY, ll = 0.f;
-        if (row0 + row < rows) {
-          const float2* p = part + (long long)r * rows + row0 + row;
-#pragma unroll 8
-          for (int i = threadIdx.x & 3; i < splits; i += 4) {
-            const float2 v = p[i * rows_total];
-            const float top = fmaxf(mm, v.x);
-            if (v.y > 0.f) ll = ll * fast_exp2(mm - top) + v.y * fast_exp2(v.x - top);
-            mm = top;
-          }
+  griddep_wait();
+  float w = 0.f;
+  // rows of the block from the first token on that sees this key (and this CTA's first key)
+  const int first = max(0, key - past) * a.g.grp - k.row_base;
+  for (int i0 = max(0, max(0, j0 - past) * a.g.grp - k.row_base); stored && i0 < k.rows; i0 += kSumRows) {
+    float s[kMine];
+    const float* score = k.score + ((long long)r * k.rows + i0 + warp) * k.score_row + key;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int row = i0 + warp + 8 * i;
+      s[i] = row < k.rows && row >= first && key < len ? score[8 * i * k.score_row] : -INFINITY;
+    }
+    // the rows' maxima and sums from their key ranges, two threads a row
+    const int mine = i0 + (threadIdx.x >> 1);
+    float mm = -INFINITY, ll = 0.f;
+    if (mine < k.rows) {
+      const float2* p = k.part + (long long)r * k.rows + mine;
+      for (int s0 = threadIdx.x & 1; s0 < k.splits; s0 += 2 * kMine) {
+        float2 v[kMine];
+        float top = mm;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          v[i] = s0 + 2 * i < k.splits ? p[(long long)(s0 + 2 * i) * a.units * k.rows] : make_float2(-INFINITY, 0.f);
+          top = fmaxf(top, v[i].x);
         }
+        if (ll > 0.f) ll *= fast_exp2(mm - top);
 #pragma unroll
-        for (int off = 1; off < 4; off <<= 1) {
-          const float om = __shfl_xor_sync(0xffffffffu, mm, off), ol = __shfl_xor_sync(0xffffffffu, ll, off);
-          const float top = fmaxf(mm, om);
-          ll = (ll > 0.f ? ll * fast_exp2(mm - top) : 0.f) + (ol > 0.f ? ol * fast_exp2(om - top) : 0.f);
-          mm = top;
-        }
-        if ((threadIdx.x & 3) == 0) ml[row] = make_float2(mm, 1.f / ll);
-      }
-      __syncthreads();
-      if (row0 + 8 * (int)(threadIdx.x >> 5) >= rows) continue;  // none of this warp's 8 rows is one
-      float s[4][J];
-      tile_scores(qs, ks, ty, tx, s);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 4 * ty + i;
-        if (row >= rows) continue;
-        const int last = last_key(a, past, row);
-        const float2 e = ml[4 * ty + i];
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-          if (j0 + tx + 16 * j <= last) w[j] = fmaf(fast_exp2(fmaf(s[i][j], kScoreScale, -e.x)), e.y, w[j]);
+        for (int i = 0; i < kMine; ++i)
+          if (v[i].y > 0.f) ll = fmaf(v[i].y, fast_exp2(v[i].x - top), ll);
+        mm = top;
       }
     }
-  }
-  // over the 16 groups of rows, in their order
-  __syncthreads();
+    const float om = __shfl_xor_sync(0xffffffffu, mm, 1), ol = __shfl_xor_sync(0xffffffffu, ll, 1), top = fmaxf(mm, om);
+    ll = (ll > 0.f ? ll * fast_exp2(mm - top) : 0.f) + (ol > 0.f ? ol * fast_exp2(om - top) : 0.f);
+    if (i0 > 0) __syncthreads();
+    if ((threadIdx.x & 1) == 0) ml[threadIdx.x >> 1] = make_float2(top, 1.f / ll);
+    __syncthreads();
 #pragma unroll
-  for (int j = 0; j < J; ++j) qs[ty * kSumKeys + tx + 16 * j] = w[j];
+    for (int i = 0; i < kMine; ++i) {
+      const float2 e = ml[warp + 8 * i];
+      if (s[i] != -INFINITY) w = fmaf(fast_exp2(fmaf(s[i], kScoreScale, -e.x)), e.y, w);
+    }
+  }
+  sums[warp][lane] = w;
   __syncthreads();
-  if (threadIdx.x < kSumKeys && j0 + threadIdx.x < len) {
+  if (warp == 0 && key < len) {
     float x = 0.f;
-    for (int i = 0; i < 16; ++i) x += qs[i * kSumKeys + threadIdx.x];
-    float* o = a.out + r * a.out_stride + j0 + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x += sums[i][lane];
+    float* o = a.out + r * a.out_stride + key;
     *o = a.accumulate ? *o + x : x;
   }
 }
@@ -266,18 +278,31 @@ int launch_any(const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws, cudaS
   if (rc) return rc;
   static PerDeviceOnce once;
   rc = once.run(dev, [] {
-    int e = cuda_check(cudaFuncSetAttribute(key_lse_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem),
-                       "key_lse shared memory");
-    return e ? e : cuda_check(cudaFuncSetAttribute(key_sum_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSumSmem),
-                              "key_sum shared memory");
+    return cuda_check(cudaFuncSetAttribute(key_lse_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, any_smem(kTile)),
+                      "key_lse shared memory");
   });
   if (rc) return rc;
-  const int key_tiles = (a.max_len + kSumKeys - 1) / kSumKeys;
-  float2* part = reinterpret_cast<float2*>(ws + p.part);
   if (p.row_tiles > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_key_weights: too many queries");
-  key_lse_kernel<T><<<dim3(p.splits, a.units, p.row_tiles), 256, kSmem, st>>>(a, part, p.splits);
-  key_sum_kernel<T><<<dim3(key_tiles, a.units), 256, kSumSmem, st>>>(a, part, p.splits);
-  return cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+  AnyArgs k;
+  k.a = a;
+  k.part = reinterpret_cast<float2*>(ws + p.part);
+  k.score = reinterpret_cast<float*>(ws + p.score);
+  k.score_row = a.max_len;
+  k.splits = p.splits;
+  k.tile_rows = p.tile_rows;
+  const int rows = a.q_len * a.g.grp;
+  for (k.row_base = 0; k.row_base < rows; k.row_base += p.rows) {
+    k.rows = std::min(p.rows, rows - k.row_base);
+    const int row_tiles = (k.rows + p.tile_rows - 1) / p.tile_rows;
+    key_lse_kernel<T><<<dim3(p.splits, a.units, row_tiles), 4 * p.tile_rows, any_smem(p.tile_rows), st>>>(k);
+    rc = cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+    if (rc) return rc;
+    rc = launch_dependent(key_sum_kernel, dim3((a.max_len + kSumKeys - 1) / kSumKeys, a.units), 256, 0, st,
+                          "aoh_key_weights sums launch", k);
+    if (rc) return rc;
+    k.a.accumulate = 1;
+  }
+  return AOH_OK;
 }
 
 int retrieval_heads(const aoh_kv_cache* c, int layer) {
@@ -295,12 +320,18 @@ KeyWeightsPlan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
   } else if (c->cfg.dtype == AOH_BF16 && grp <= 128) {
     plan_key_weights_tensor(c, units, max_len, q_len, p);
   } else {
+    // as many rows a block as have room for their scores, in whole tiles (of 16 rows at least)
+    const long long row_bytes = (long long)units * max_len * sizeof(float), room = kScoreBytes / std::max(1LL, row_bytes);
+    if (p.rows > room) p.rows = (int)(room >= kTile ? room / kTile * kTile : std::max(16LL, room / 16 * 16));
     p.row_tiles = (p.rows + kTile - 1) / kTile;
+    p.tile_rows = ((p.rows + p.row_tiles - 1) / p.row_tiles + 7) / 8 * 8;  // tiles of like height: 66 rows = 40 + 26
     const int key_tiles = (max_len + kTile - 1) / kTile;
-    // enough CTAs for three per SM
-    const long long ctas = std::max(1LL, (long long)units * p.row_tiles);
-    p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles), (3LL * std::max(1, c->num_sms) + ctas - 1) / ctas));
-    p.bytes = (size_t)p.splits * units * p.rows * sizeof(float2);
+    // as many CTAs as the SMs hold at a time: three of 64 rows, five of 8
+    const long long ctas = std::max(1LL, (long long)units * p.row_tiles), resident = 224 * 1024 / any_smem(p.tile_rows);
+    p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles),
+                                                      (resident * std::max(1, c->num_sms) + ctas - 1) / ctas));
+    p.score = align256((size_t)p.splits * units * p.rows * sizeof(float2));
+    p.bytes = p.score + (size_t)p.rows * row_bytes;
   }
   return p;
 }

@@ -24,14 +24,14 @@ struct KeyWeightsArgs {
 };
 
 // How a call is run and where its workspace's parts begin (bytes).
-//   any:     (m, l) of every query row by key range, then the sums
+//   any:     for some query rows after others: their scores and (m, l) by key range, then the sums
 //   few:     scores of every (key, query row) and (m, l) by key range, then the sums
 //   tensor:  (m, l) by key range, the rows' -lse, the sums by row range
 enum class KeyWeightsKind { any, few, tensor };
 struct KeyWeightsPlan {
   KeyWeightsKind kind = KeyWeightsKind::any;
-  int rows = 0;            // query rows of a unit
-  int row_tiles = 0;
+  int rows = 0;            // query rows of a unit; any: that a pair of launches takes
+  int row_tiles = 0, tile_rows = 0;
   int tile_tokens = 0;     // tensor: tokens of a row tile
   int splits = 1;          // key ranges
   int row_splits = 1;      // tensor: row ranges of the sums
@@ -56,6 +56,23 @@ inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // planned for is cut to it, so that no weight lands behind a row of `out`.
 __device__ __forceinline__ int key_weights_past(const KeyWeightsArgs& a) {
   return a.past_len_dev ? max(0, min(*a.past_len_dev, a.max_len - a.q_len)) : a.past_len;
+}
+
+
+// Launch that may start while the kernel before it finishes (it waits for that kernel itself).
+template <class F, class... A>
+int launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
 }
 #endif
 

@@ -772,23 +772,6 @@ int encode_queries(CUtensorMap* map, const KeyWeightsArgs& a, int tile_tokens) {
 }
 
 int key_pairs(int max_len) { return ((max_len + kTileRows - 1) / kTileRows + 1) / 2; }
-
-// Launch that may start while the kernel before it finishes (it waits for that kernel itself).
-template <class F, class... A>
-int launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
-}
-
 // Ranges that `items` CTAs' lists of at most `tiles` tiles are cut into, one CTA
 // per SM: the fewest tile periods, a range costing its tiles and about four for
 // a CTA's start and end.  Candidates: a few ranges, and what fills 1 to 4 waves.

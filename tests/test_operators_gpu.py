@@ -221,6 +221,22 @@ def test_key_weights_long(C):
     assert torch.equal(key_weights(cache, 1, q, past_len=past), got)  # a fixed order of sums
 
 
+@pytest.mark.parametrize("G,grp,C,past", [
+    (1, 8, 600, 6_000),    # 4800 rows over 6600 keys: a second block of 1024 rows
+    (8, 1, 20, 100_003),   # 8 units of 20 rows over many keys: blocks of 16 rows
+])
+def test_key_weights_f32_in_blocks_of_rows(G, grp, C, past):
+    """More scores than one block of query rows has room for; added to what is there."""
+    cache, k, _ = filled([[1] * G], G * grp, 1, past + C, F32, C)
+    q = randn(gen(C), 1, C, G * grp, 128, dtype=F32)
+    got = key_weights(cache, 0, q, past_len=past)
+    check_weights(got, q, k[0], range(G), past)
+    twice = got.clone()
+    key_weights(cache, 0, q, past_len=past, out=twice, accumulate=True)
+    # an addition to another start rounds once a block in another place
+    assert ((twice - 2 * got).abs() <= 4 * 2.0 ** -24 * twice).all()
+
+
 def test_key_weights_large_scores():
     """Scores far apart: one key takes nearly everything; no overflow."""
     cache, k, _ = filled([[1]], 4, 1, 900, BF16, 1)
