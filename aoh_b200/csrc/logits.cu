@@ -17,15 +17,18 @@
 //
 // Bound: HBM, logits in and fp32 out (6 bytes a token for bf16 logits, 1/4
 // byte for the two bitmaps), and latency for a few rows.  A cluster of up to 16
-// CTAs takes a row, each a slice of the vocabulary of 8192 tokens (or more,
-// where 16 slices do not reach): a thread then has all its loads, four groups
-// of 8 tokens, in flight at once.  The greedy token is reduced over the cluster
+// CTAs takes a row, 8192 tokens each (or more, where 16 CTAs do not reach): a
+// thread then has all its loads, four groups of 8 tokens, in flight at once.
+// The CTAs take 64 tokens in turn: vocabularies are sorted by frequency, and the
+// CTA of a row's first tokens would list nearly all of the row's history
+// (64 x 128K: its listed tokens took 9 us of 13).  The greedy token is reduced over the cluster
 // in shared memory, so one launch and no workspace.  The main pass copies and
 // masks; the few tokens with a count or a bias are listed in shared memory and
 // done behind it, a thread each: the division of the penalties, in every group
 // that holds one such token, cost more than the copy.  A CTA's biases are
-// listed in the order given, so that the sum over a token listed more than once
-// has a fixed order.
+// listed in the order given, and the entries of one token linked in that order:
+// their sum has a fixed order (37 rows x 32003 with 300 biases, 240 of them in
+// one slice: DUP us; with the whole list read for each sum 19).
 #include <climits>
 #include <type_traits>
 
@@ -37,18 +40,22 @@ namespace {
 
 constexpr int kMaxCluster = 16;
 constexpr int kThreads = 256;
-constexpr int kMaxBias = 4096;  // biases of a row (32 KB of shared memory if all fall into one slice)
-constexpr int kSlice = kThreads * 32;  // tokens whose loads a CTA has in flight at once (a quarter where rows are not aligned)
+constexpr int kMaxBias = 4096;  // biases of a row (64 KB of shared memory if all fall into one slice)
+constexpr int kSlice = kThreads * 32;  // tokens whose loads a CTA has in flight at once (half of them where rows are not aligned)
+constexpr int kTurn = 64;              // tokens that a row's CTAs take in turn
 constexpr int kMaxVocab = 1 << 21;
 constexpr uint32_t kInPrompt = 0x80000000u;
-// two bits a token of the largest slice, and the list
-constexpr int kMaxSmem = 160 * 1024;
+// two bits a token of the largest slice, and the list of 4096 biases: 192.3 KB
+constexpr int kMaxSmem = 196 * 1024;
+
+// Entries that a list of n biases is given: whole groups of 16, with those behind the last.
+__host__ __device__ constexpr int bias_room(int n) { return (n + 31) / 16 * 16; }
 
 struct LogitsArgs {
   const void* logits;
   long long row_stride;  // elements
   int vocab;
-  int cluster, slice;    // CTAs of a row, tokens of one CTA (a multiple of 256)
+  int cluster, cluster_log, slice;  // CTAs of a row, tokens of one CTA (a multiple of 256)
   const uint32_t *counts, *seen;
   const float *repetition, *presence, *frequency;  // per row, or null: the scalar
   float repetition_s, presence_s, frequency_s;
@@ -174,17 +181,22 @@ struct Best {
 
 template <typename T, typename O, bool kWide>
 __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_constant__ LogitsArgs a) {
-  // with biases: two bits per token of the slice, then the slice's (id, value) list
+  // with biases: two bits per token of the slice, then the slice's list: ids, values, next entry of the same token
   extern __shared__ __align__(16) uint32_t smem[];
   __shared__ unsigned long long best_warp[kThreads / 32];
   __shared__ unsigned long long best_cta[kMaxCluster];
   __shared__ int s_count[kThreads / 32];
   uint32_t *biased = smem, *repeated = smem + a.slice / 32;
-  int2* list = reinterpret_cast<int2*>(smem + a.slice / 16);  // biases
+  int* b_id = reinterpret_cast<int*>(smem + a.slice / 16);  // behind the last 16 times -1
+  float* b_value = reinterpret_cast<float*>(b_id + bias_room(a.n_bias));
+  int* b_next = b_id + 2 * bias_room(a.n_bias);         // INT_MAX: none
+  int* b_later = b_id + 3 * bias_room(a.n_bias);        // not 0: an entry before is of the same token
   const int rank = a.cluster > 1 ? (int)cluster_ctarank() : 0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / a.cluster;
-  const int lo = rank * a.slice, hi = min(lo + a.slice, a.vocab);  // may be empty
+  // token of the CTA's p-th place, and a token's place
+  auto token = [&](int p) { return ((((p / kTurn) << a.cluster_log) + rank) * kTurn) | (p % kTurn); };
+  auto place = [&](int t) { return (((t / kTurn) >> a.cluster_log) * kTurn) | (t % kTurn); };
   const int words = (a.vocab + 31) >> 5;
   const T* x_row = static_cast<const T*>(a.logits) + row * a.row_stride;
   O* out = static_cast<O*>(a.out) + row * a.out_stride;
@@ -203,45 +215,64 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
 
   // A thread's tokens of one round: U units of N neighbours, a stride apart.
   // Rows that are not 16-byte aligned take single tokens, a lane each of a word.
-  constexpr int N = kWide ? 8 : 1, U = kWide ? 4 : 8, kRound = U * N * kThreads;
+  constexpr int N = kWide ? 8 : 1, U = kWide ? 4 : 16, kRound = U * N * kThreads;
   constexpr uint32_t kOnes = (1u << N) - 1u;
-  __shared__ uint16_t s_list[kRound];  // tokens with a count, from the round's first on
+  __shared__ uint16_t s_list[kRound];  // places of tokens with a count, from the round's first on
   __shared__ int s_listed;
   using Raw = typename std::conditional<kWide, Raw8<T>, Raw1<T>>::type;
   Raw raw[U];
-  uint32_t s[U], al[U];
+  // bits of a unit's tokens: a byte each (wide), or in word `lane` those of the warp's unit `lane`
+  constexpr int W = kWide ? U : 1;
+  uint32_t s[W], al[W];
   auto fetch = [&](int base) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int t = base + (u * kThreads + tid) * N;
+      const int t = token(base + (u * kThreads + tid) * N);
+      if (t < a.vocab) raw[u].load(x_row + t);
+    }
+#pragma unroll
+    for (int u = 0; u < W; ++u) {
+      const int t = token(kWide ? base + (u * kThreads + tid) * N : base + lane * kThreads + warp * 32);
+      const bool in = t < a.vocab && (kWide || lane < U);
       s[u] = 0;
-      al[u] = kOnes;
-      if (t < hi) {
-        raw[u].load(x_row + t);
-        if (seen) s[u] = seen[t >> 5] >> (t & 31) & kOnes;
-        if (allowed) al[u] = allowed[t >> 5] >> (t & 31) & kOnes;
+      al[u] = 0xffffffffu;
+      if (kWide) {
+        if (in && seen) s[u] = reinterpret_cast<const uint8_t*>(seen)[t / 8];
+        if (in && allowed) al[u] = reinterpret_cast<const uint8_t*>(allowed)[t / 8];
+      } else {
+        if (in && seen) s[u] = seen[t / 32];
+        if (in && allowed) al[u] = allowed[t / 32];
       }
     }
   };
-  fetch(lo);
+  // the first biases are asked for before the logits: their list is made while those are on their way
+  const int32_t* ids = a.bias_ids + (long long)row * a.n_bias;
+  const float* values = a.bias + (long long)row * a.n_bias;
+  int id_next = tid < a.n_bias ? ids[tid] : -1;
+  float v_next = tid < a.n_bias ? values[tid] : 0.f;
+  fetch(0);
   if (tid == 0) s_listed = 0;
 
   int n_biased = 0;
   if (a.n_bias) {
-    const int32_t* ids = a.bias_ids + (long long)row * a.n_bias;
-    const float* values = a.bias + (long long)row * a.n_bias;
     for (int i = tid; i < a.slice / 16; i += kThreads) smem[i] = 0;
     __syncthreads();
     for (int i0 = 0; i0 < a.n_bias; i0 += kThreads) {
-      const int i = i0 + tid;
-      const int id = i < a.n_bias ? ids[i] : -1;
-      const float v = i < a.n_bias ? values[i] : 0.f;
-      const bool in = id >= lo && id < hi;
+      const int id = id_next, i = i0 + kThreads + tid;
+      const float v = v_next;
+      if (i < a.n_bias) {
+        id_next = ids[i];
+        v_next = values[i];
+      } else {
+        id_next = -1;
+      }
+      const bool in = id >= 0 && id < a.vocab && ((id / kTurn) & (a.cluster - 1)) == rank;
       const unsigned m = __ballot_sync(0xffffffffu, in);
       if (lane == 0) s_count[warp] = __popc(m);
       if (in) {
         const uint32_t bit = 1u << (id & 31);
-        if (atomicOr(&biased[(id - lo) >> 5], bit) & bit) atomicOr(&repeated[(id - lo) >> 5], bit);
+        const int word = place(id) / 32;
+        if (atomicOr(&biased[word], bit) & bit) atomicOr(&repeated[word], bit);
       }
       __syncthreads();
       int at = n_biased + __popc(m & ((1u << lane) - 1u));
@@ -250,8 +281,42 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
         if (w < warp) at += s_count[w];
         n_biased += s_count[w];
       }
-      if (in) list[at] = make_int2(id, __float_as_int(v));
+      if (in) {
+        b_id[at] = id;
+        b_value[at] = v;
+        b_later[at] = 0;
+      }
       __syncthreads();
+    }
+    if (tid < 16) b_id[n_biased + tid] = -1;
+    __syncthreads();
+    // entries of one token are linked in their order, while the logits are on their way
+    for (int i0 = warp * 32; i0 < n_biased; i0 += kThreads) {
+      const int i = i0 + lane, id = i < n_biased ? b_id[i] : -1;
+      const bool more = id >= 0 && repeated[place(id) / 32] >> (id & 31) & 1;
+      if (!__any_sync(0xffffffffu, more)) continue;
+      // the first entry behind i of its token, by its place in a group of four
+      int next[4] = {INT_MAX, INT_MAX, INT_MAX, INT_MAX};
+      auto look = [&](int j, bool check) {  // 16 entries
+        int4 o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = reinterpret_cast<const int4*>(b_id + j)[k];
+#pragma unroll
+        for (int k = 3; k >= 0; --k) {
+          if (o[k].x == id && (!check || j + 4 * k > i)) next[0] = j + 4 * k;
+          if (o[k].y == id && (!check || j + 4 * k + 1 > i)) next[1] = j + 4 * k + 1;
+          if (o[k].z == id && (!check || j + 4 * k + 2 > i)) next[2] = j + 4 * k + 2;
+          if (o[k].w == id && (!check || j + 4 * k + 3 > i)) next[3] = j + 4 * k + 3;
+        }
+      };
+      int j = (n_biased - 1) / 16 * 16;
+      for (; j >= i0 + 32; j -= 16) look(j, false);
+      for (; j >= i0; j -= 16) look(j, true);
+      const int found = min(min(next[0], next[1]), min(next[2], next[3]));
+      if (more) {
+        b_next[i] = found;
+        if (found != INT_MAX) b_later[found] = 1;
+      }
     }
   } else if (seen) {
     __syncthreads();
@@ -262,23 +327,25 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
     if (greedy && y != -INFINITY) key = max(key, greedy_key(y, t));
     store1(out + t, y);
   };
-  for (int base = lo; base < hi; base += kRound) {
-    if (base != lo) fetch(base);
+  for (int base = 0; base < a.slice; base += kRound) {
+    if (base) fetch(base);
     int n_special = 0;
     uint32_t sp[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int t = base + (u * kThreads + tid) * N;
+      const int p = base + (u * kThreads + tid) * N, t = token(p);
+      const uint32_t se = kWide ? s[u % W] : __shfl_sync(0xffffffffu, s[0], u) >> lane & 1u;
+      const uint32_t alw = kWide ? al[u % W] & kOnes : __shfl_sync(0xffffffffu, al[0], u) >> lane & 1u;
       sp[u] = 0;
-      if (t >= hi) continue;
+      if (t >= a.vocab) continue;
       float x[N];
       raw[u].get(x);
-      if (al[u] != kOnes) {
+      if (alw != kOnes) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = al[u] >> j & 1 ? x[j] : -INFINITY;
+        for (int j = 0; j < N; ++j) x[j] = alw >> j & 1 ? x[j] : -INFINITY;
       }
-      const uint32_t bi = a.n_bias ? biased[(t - lo) >> 5] >> (t & 31) & kOnes : 0u;
-      sp[u] = s[u] & al[u] & ~bi;
+      const uint32_t bi = a.n_bias ? biased[p / 32] >> (p & 31) & kOnes : 0u;
+      sp[u] = se & alw & ~bi;
       n_special += __popc(sp[u]);
       // tokens that are done again below are stored as they came: in place they must stay, and they are overwritten
       if constexpr (kWide)
@@ -328,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * kThreads;
-        t[u] = i < n_listed ? base + s_list[i] : -1;
+        t[u] = i < n_listed ? token(base + s_list[i]) : -1;
         if (t[u] >= 0) {
           count[u] = pen.counts[t[u]];
           x[u] = load1(x_row + t[u]);
@@ -338,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
       for (int u = 0; u < 4; ++u)
         if (t[u] >= 0) put(t[u], pen.apply(x[u], count[u]));
     }
-    if (base + kRound < hi) {
+    if (base + kRound < a.slice) {
       __syncthreads();
       if (tid == 0) s_listed = 0;
       __syncthreads();
@@ -347,27 +414,17 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   key = max(key, best.key());
 
   if (n_biased) {
-    if (!seen) __syncthreads();  // the main pass has stored its tokens
+    if (!seen) __syncthreads();  // the main pass has stored its tokens, and the entries are linked
     for (int i = tid; i < n_biased; i += kThreads) {
-      const int2 e = list[i];
-      const int t = e.x;
+      if (b_later[i]) continue;
+      const int t = b_id[i];
       const uint32_t count = seen ? pen.counts[t] : 0u;
       const bool ok = !allowed || allowed[t >> 5] >> (t & 31) & 1;
       const float x = load1(x_row + t);
-      float sum = __int_as_float(e.y);
-      if (repeated[(t - lo) >> 5] >> (t & 31) & 1) {
-        // listed more than once: the first entry adds them up in their order, from -0, which leaves the first as it is
-        int first = -1;
-        sum = -0.f;
-#pragma unroll 4
-        for (int j = 0; j < n_biased; ++j) {
-          const int2 o = list[j];
-          const float next = __fadd_rn(sum, __int_as_float(o.y));
-          sum = o.x == t ? next : sum;
-          first = o.x == t && first < 0 ? j : first;
-        }
-        if (first != i) continue;
-      }
+      float sum = b_value[i];
+      // listed more than once: added up in their order
+      if (repeated[place(t) / 32] >> (t & 31) & 1)
+        for (int j = b_next[i]; j != INT_MAX; j = b_next[j]) sum = __fadd_rn(sum, b_value[j]);
       put(t, ok ? __fadd_rn(pen.apply(x, count), sum) : -INFINITY);
     }
   }
@@ -433,7 +490,7 @@ int launch(const LogitsArgs& a, int rows, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * a.cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = a.n_bias ? (size_t)a.slice / 4 + (size_t)a.n_bias * sizeof(int2) : 0;
+  cfg.dynamicSmemBytes = a.n_bias ? (size_t)a.slice / 4 + 4 * (size_t)bias_room(a.n_bias) * sizeof(int) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -489,8 +546,12 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   if (rc) return rc;
   const int most = p.rows * 16LL <= 2 * sms ? 16 : p.rows * 8LL <= 4 * sms ? 8 : 4;
   a.cluster = 1;
-  while (a.cluster < most && a.cluster * (wide ? kSlice : kSlice / 4) < p.vocab) a.cluster *= 2;
-  a.slice = ((p.vocab + a.cluster - 1) / a.cluster + 255) / 256 * 256;
+  while (a.cluster < most && a.cluster * (wide ? kSlice : kSlice / 2) < p.vocab) {
+    a.cluster *= 2;
+    ++a.cluster_log;
+  }
+  const int turns = (p.vocab + kTurn - 1) / kTurn;
+  a.slice = ((turns + a.cluster - 1) / a.cluster * kTurn + 255) / 256 * 256;
   a.counts = reinterpret_cast<const uint32_t*>(p.counts);
   a.seen = reinterpret_cast<const uint32_t*>(p.seen);
   a.repetition = p.repetition;

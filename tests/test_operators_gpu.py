@@ -517,6 +517,25 @@ def test_penalize_logits_rows_and_strides():
     assert penalize_logits(x[:0]).shape == (0, V)
 
 
+@pytest.mark.parametrize("N,V,V_of_ids", [(75, 1 << 21, 1 << 21), (75, 1 << 21, 64), (2, 700, 3), (20, 5_001, 5_001)])
+def test_biases_as_many_as_a_row_may_have(N, V, V_of_ids):
+    """4096 biases of a row -- of few tokens, or of the largest vocabulary -- added up in their order."""
+    g = gen(V_of_ids + N)
+    x = torch.zeros((N, V), device="cuda", dtype=BF16)
+    ids = torch.randint(0, V_of_ids, (N, 4096), generator=g, device="cuda").int()
+    ids[:, 1000:1003] = -1
+    values = randn(g, N, 4096)
+    got, best = penalize_logits(x, bias=(ids, values), greedy=True)
+    for n in {0, N // 2, N - 1}:
+        want = np.zeros(V, np.float32)
+        for i, v in zip(ids[n].tolist(), values[n].cpu().numpy()):
+            if i >= 0:
+                want[i] += v  # from 0 instead of from the first: the same sum
+        assert same_bits(got[n].cpu().numpy() + np.float32(0), want)
+        assert best[n] == int(np.argmax(want))
+    assert int((got != 0).sum()) <= N * 4096
+
+
 def test_greedy_ties_nan_and_empty_rows():
     V = 40_000
     x = torch.zeros((5, V), device="cuda")
