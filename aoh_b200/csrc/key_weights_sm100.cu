@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sB = sA + 2 * kTileBytes;                                     // ring of streamed tiles
   float* sLse = reinterpret_cast<float*>(sB + kStages * kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  if (kPass != kSums || t.splits > 1) griddep_launch_dependents();
+  if (kPass == kLse || (kPass == kSums && t.splits > 1)) griddep_launch_dependents();  // not the call's last kernel
 
   // this CTA's resident pair and range of streamed tiles
   const int split = blockIdx.x % t.splits;

@@ -114,6 +114,21 @@ def test_rope_axes_far_and_negative_positions():
     assert ((qo.double().cpu() - want).abs() <= err + far + want.abs() * 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rope_axes_rows_more_than_32_bits_apart(dtype):
+    """Sequences whose rows lie more than 2^31 elements apart, as views of one buffer."""
+    apart, Hq, G, D = 2 ** 31 + 64, 3, 1, 64
+    buf = torch.empty(apart + 4096, device="cuda", dtype=dtype)
+    q, k = buf.as_strided((2, 2, Hq, D), (apart, 512, D, 1)), buf.as_strided((2, 2, G, D), (apart, 512, D, 1), 256)
+    q.copy_(randn(gen(1), 2, 2, Hq, D, dtype=dtype))
+    k.copy_(randn(gen(2), 2, 2, G, D, dtype=dtype))
+    pos = torch.tensor([[[3, 4], [70_000, 70_001]]], device="cuda")
+    inv = 1e4 ** (-torch.arange(32, device="cuda", dtype=F32) / 32)
+    got = rope_axes_qk(q, k, pos, inv, (32,))
+    want = rope_axes_qk(q.contiguous(), k.contiguous(), pos, inv, (32,))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rope_axes_agrees_with_rope_qk():
     """One axis of ordinary positions is the framework's other rotation, up to the roundings that one makes."""
     g = gen(7)
@@ -257,6 +272,19 @@ def test_key_weights_ignores_what_the_cache_does_not_hold_yet():
     cache.append_layer(0, bad, bad)
     got = key_weights(cache, 0, randn(gen(1), 1, 7, 8, 128, dtype=BF16), past_len=196)
     assert torch.equal(got, want) and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype,C", [(BF16, 60), (BF16, 140), (F32, 7), (F32, 60)])
+def test_key_weights_of_chunks_ignore_what_is_not_held_yet(dtype, C):
+    """The same for the kernels that take more query rows, and for fp32."""
+    T = 331  # 11 slots of the last page in use
+    cache, k, _ = filled([[1, 0]], 8, 1, T, dtype, C, max_context=384)
+    q = randn(gen(1), 1, C, 8, 128, dtype=dtype)
+    want = key_weights(cache, 0, q, past_len=T - C)
+    check_weights(want, q, k[0], [0], T - C)
+    bad = torch.full((1, 5, 2, 128), float("nan"), device="cuda", dtype=dtype)
+    cache.append_layer(0, bad, bad)
+    assert torch.equal(key_weights(cache, 0, q, past_len=T - C), want)
 
 
 def test_key_weights_of_units_stored_elsewhere_are_zero():
@@ -722,6 +750,21 @@ def test_key_weights_with_the_devices_length():
         want[..., :past + 1] += key_weights(cache, 0, q, past_len=past)
     # the split into key ranges may differ from the plan for the full length: fp32 sums in another order
     assert torch.allclose(out, want, rtol=1e-4, atol=0) and (out[..., 284:] == 0).all()
+
+
+def test_key_weights_f32_with_the_devices_length():
+    from aoh_b200 import _lib
+
+    cache, k, _ = filled([[1, 0]], 8, 2, 150, F32, 13, max_context=160)
+    cache.reserve(160)
+    q = randn(gen(2), 2, 1, 8, 128, dtype=F32)
+    out = torch.full((2, 1, 170), 3.0, device="cuda")
+    _lib.check(_lib.lib().aoh_kv_set_length(cache._h, 140, _lib.stream_handle()))
+    cache.device_length = True
+    key_weights(cache, 0, q, out=out)
+    cache.device_length = False
+    check_weights(out[..., :141], q, k[0][:, :141], [0], 140)
+    assert (out[..., 141:] == 3).all()
 
 
 # -- refusals -------------------------------------------------------------------------
