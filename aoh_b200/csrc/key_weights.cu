@@ -315,9 +315,9 @@ KeyWeightsPlan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
   KeyWeightsPlan p;
   const int units = c->cfg.batch * retrieval_heads(c, layer), grp = c->cfg.num_q_heads / c->cfg.num_kv_heads;
   p.rows = q_len * grp;
-  if (c->cfg.dtype == AOH_BF16 && p.rows <= kFewRows) {
-    plan_key_weights_few(c, units, max_len, p);
-  } else if (c->cfg.dtype == AOH_BF16 && grp <= 128) {
+  if (c->cfg.dtype == AOH_BF16 && p.rows <= kOneRows && plan_key_weights_few(c, units, max_len, p)) return p;
+  p.kind = KeyWeightsKind::any;
+  if (c->cfg.dtype == AOH_BF16 && grp <= 128) {
     plan_key_weights_tensor(c, units, max_len, q_len, p);
   } else {
     // as many rows a block as have room for their scores, in whole tiles (of 16 rows at least)
@@ -373,7 +373,7 @@ extern "C" int aoh_key_weights(aoh_kv_cache* c, int32_t layer, int32_t past_len,
   if (a.units > 65535) return fail(AOH_ERR_UNSUPPORTED, "%s: too many units", who);
   if ((long long)q_len * a.g.grp > (1 << 30)) return fail(AOH_ERR_UNSUPPORTED, "%s: too many queries", who);
   const KeyWeightsPlan p = plan(c, layer, max_len, q_len);
-  if (!workspace || workspace_bytes < p.bytes)
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, p.bytes);
   if (reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(AOH_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned", who);

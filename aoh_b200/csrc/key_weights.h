@@ -25,7 +25,7 @@ struct KeyWeightsArgs {
 
 // How a call is run and where its workspace's parts begin (bytes).
 //   any:     for some query rows after others: their scores and (m, l) by key range, then the sums
-//   few:     scores of every (key, query row) and (m, l) by key range, then the sums
+//   few:     scores of every (key, query row) and (m, l) by key range, then the sums; or both by a cluster
 //   tensor:  (m, l) by key range, the rows' -lse, the sums by row range
 enum class KeyWeightsKind { any, few, tensor };
 struct KeyWeightsPlan {
@@ -35,19 +35,24 @@ struct KeyWeightsPlan {
   int tile_tokens = 0;     // tensor: tokens of a row tile
   int splits = 1;          // key ranges
   int row_splits = 1;      // tensor: row ranges of the sums
+  bool one = false;        // few: one launch, no workspace
   bool stream = false;     // tensor: the query rows stay resident in the second pass too
   size_t part = 0, score = 0, lse = 0, sums = 0, bytes = 0;
 };
 
 // Launchers of the bf16 kernels (key_weights_sm100.cu).
-void plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p);
+// false: too many rows and keys
+bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p);
 void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int q_len, KeyWeightsPlan& p);
 int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
                            cudaStream_t st);
 int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
                               cudaStream_t st);
 
-constexpr int kFewRows = 32;  // query rows of a unit that the few-rows kernel takes
+// Query rows of a unit that the few-rows kernels take: up to 32 where one launch
+// does, else 16.  24 rows x 32768 keys, 2 units: 27 us, on the tensor cores 21;
+// 16 rows: 18.
+constexpr int kFewRows = 16, kOneRows = 32;
 
 inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 

@@ -5,9 +5,11 @@
 // bytes a key.  few_scores_kernel keeps the rows of Q as mma fragments and
 // streams the pages of a key range from global memory straight into A
 // fragments: the product does not depend on the order of the 128 dimensions,
-// so a lane takes whole 16-byte chunks and Q is laid out to match.  It writes
-// the scores (4 bytes a key and row, which stay in L2) and the range's (m, l);
-// few_sum_kernel turns them into weights.
+// so a lane takes whole 16-byte chunks and Q is laid out to match.  For a few
+// thousand keys a cluster takes a unit, keeps its scores in shared memory and
+// writes the weights: one launch.  For more, every SM takes key ranges; their
+// scores (4 bytes a key and row, which stay in L2) and (m, l) go to a workspace
+// and few_sum_kernel turns them into weights.
 //
 // More rows: tensor_pass_kernel, the same product three ways.  A CTA keeps up
 // to two 128-row tiles of one operand in shared memory and streams 128-row
@@ -39,6 +41,8 @@ namespace {
 // few query rows
 // ---------------------------------------------------------------------------
 constexpr int kFewWarps = 8;
+constexpr int kMaxOne = 16;             // CTAs of a unit's cluster
+constexpr int kOneSmem = 160 * 1024;    // scores of one of them
 
 struct FewArgs {
   KeyWeightsArgs a;
@@ -48,16 +52,25 @@ struct FewArgs {
   long long score_unit;  // floats of a unit's scores
 };
 
-template <int NT>  // tiles of 8 query rows
+// NT tiles of 8 query rows.  kOne: the ranges of a unit are the CTAs of a
+// cluster, which keep their scores in shared memory, combine their (m, l)
+// across it and write the weights: one launch and no workspace.
+template <int NT, bool kOne>
 __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_kernel(const __grid_constant__ FewArgs f) {
   __shared__ float2 red[kFewWarps][NT * 8];
+  extern __shared__ __align__(16) float own_scores[];  // kOne: [key of the range][rows_even]
   const KeyWeightsArgs& a = f.a;
-  griddep_launch_dependents();  // the sums wait for this grid to finish
+  if (!kOne) griddep_launch_dependents();  // the sums wait for this grid to finish
   const int r = blockIdx.y;
   const RetrievalRow info = a.rows[r];
   const int unit = info.unit, base = info.table, held = info.held;
-  if (held == 0) return;
   const int past = key_weights_past(a), len = past + a.q_len;
+  if (held == 0) {  // not stored here: no weight
+    if (kOne && !a.accumulate)
+      for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < len; j += gridDim.x * blockDim.x)
+        a.out[r * a.out_stride + j] = 0.f;
+    return;
+  }
   const int n_pages = (len + kPage - 1) / kPage;
   const int b = (unit - a.unit0) / a.g.G, kvh = (unit - a.unit0) % a.g.G;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, tq = lane & 3;
@@ -140,7 +153,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
         for (int e = 0; e < 2; ++e) s[h][e] = j0 + 8 * h <= last[n][e] ? c[n][2 * h + e] : -INFINITY;
       const int col = n * 8 + 2 * tq;
       if (col < f.rows_even) {
-        float* o = f.score + r * f.score_unit + (long long)j0 * f.rows_even + col;
+        float* o = kOne ? own_scores + (j0 - p0 * kPage) * f.rows_even + col
+                        : f.score + r * f.score_unit + (long long)j0 * f.rows_even + col;
         *reinterpret_cast<float2*>(o) = make_float2(s[0][0], s[0][1]);
         *reinterpret_cast<float2*>(o + 8 * f.rows_even) = make_float2(s[1][0], s[1][1]);
       }
@@ -180,7 +194,47 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
       const float2 v = red[w][threadIdx.x];
       if (v.y > 0.f) ll += v.y * fast_exp2(v.x - mm);
     }
-    f.part[((long long)blockIdx.x * a.units + r) * f.rows + threadIdx.x] = make_float2(mm, ll);
+    if (kOne)
+      red[0][threadIdx.x] = make_float2(mm, ll);  // a thread reads its own column of red alone
+    else
+      f.part[((long long)blockIdx.x * a.units + r) * f.rows + threadIdx.x] = make_float2(mm, ll);
+  }
+  if constexpr (kOne) {
+    __shared__ float2 ml[NT * 8];  // of a row: its maximum and 1 / sum
+    __syncwarp();
+    cluster_sync_all();
+    if (threadIdx.x < f.rows) {
+      float mm = -INFINITY, ll = 0.f;
+      float2 v[kMaxOne];
+#pragma unroll
+      for (int i = 0; i < kMaxOne; ++i) {
+        v[i] = make_float2(-INFINITY, 0.f);
+        if (i < f.splits)
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+                       : "=f"(v[i].x), "=f"(v[i].y)
+                       : "r"(mapa_shared(&red[0][threadIdx.x], i)));
+        mm = fmaxf(mm, v[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < kMaxOne; ++i)
+        if (v[i].y > 0.f) ll = fmaf(v[i].y, fast_exp2(v[i].x - mm), ll);
+      ml[threadIdx.x] = make_float2(mm, 1.f / ll);
+    }
+    __syncwarp();
+    cluster_arrive();  // no CTA's red is read from here on
+    __syncthreads();
+    const int n = min(p1 * kPage, len) - p0 * kPage;
+    for (int j = threadIdx.x; j < n; j += kFewWarps * 32) {
+      float w = 0.f;
+      for (int row = 0; row < f.rows; row += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(own_scores + j * f.rows_even + row);
+        w = fmaf(fast_exp2(fmaf(x.x, kScoreScale, -ml[row].x)), ml[row].y, w);
+        if (row + 1 < f.rows) w = fmaf(fast_exp2(fmaf(x.y, kScoreScale, -ml[row + 1].x)), ml[row + 1].y, w);
+      }
+      float* o = a.out + r * a.out_stride + p0 * kPage + j;
+      *o = a.accumulate ? *o + w : w;
+    }
+    cluster_wait();
   }
 }
 
@@ -774,14 +828,15 @@ int encode_queries(CUtensorMap* map, const KeyWeightsArgs& a, int tile_tokens) {
 int key_pairs(int max_len) { return ((max_len + kTileRows - 1) / kTileRows + 1) / 2; }
 // Ranges that `items` CTAs' lists of at most `tiles` tiles are cut into, one CTA
 // per SM: the fewest tile periods, a range costing its tiles and about four for
-// a CTA's start and end.  Candidates: a few ranges, and what fills 1 to 4 waves.
+// a CTA's start and end.  Candidates: a few ranges, what fills 1 to 4 waves, and
+// ranges of 1 to 8 tiles (2 items of 64 tiles: 8 ranges 21 us, 64 ranges 14 us).
 // 4096 tokens over 16384 keys, 4 units: `even` lists in 1, 2, 3, 4, 7 ranges
 // 311, 319, 327, 304, 335 us; uneven ones 343, 288, 296, 298, 321 us.
 int plan_ranges(long long items, int tiles, int sms, bool even) {
   int best = 1;
   double least = 1e300;
-  for (int k = 1; k <= 12; ++k) {
-    const long long s = k <= 8 ? k : (k - 8) * (long long)sms / items;
+  for (int k = 1; k <= 20; ++k) {
+    const long long s = k <= 8 ? k : k <= 12 ? (k - 8) * (long long)sms / items : (tiles + 20 - k) / (21 - k);
     if (s < 1 || s > std::min(tiles, 256)) continue;
     const double ctas = (double)items * s / sms;
     // lists of one length end in whole waves; of uneven ones, the long ones
@@ -796,17 +851,64 @@ int plan_ranges(long long items, int tiles, int sms, bool even) {
   return best;
 }
 
+// Most pages of a unit that a cluster takes (half of them for more than 16
+// rows).  On the device and from Python, one launch against two: 8 rows x 4096
+// keys 5.6 / 10.0 us against 6.2 / 14.3, x 8192 6.9 / 10.0 against 6.3 / 14.4, x
+// 16384 9.0 / 10.4 against 6.9 / 14.5.
+constexpr int kOnePages = 512;
+// bytes of the scores of one of n CTAs
+size_t one_smem(int pages, int n, int rows_even) { return (size_t)((pages + n - 1) / n) * kPage * rows_even * sizeof(float); }
+
+template <int NT>
+int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
+  auto kernel = few_scores_kernel<NT, true>;
+  static PerDeviceOnce once;
+  const int rc = once.run(c->device, [&] {
+    const int e = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                             "aoh_key_weights cluster size");
+    return e ? e
+             : cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem),
+                          "aoh_key_weights shared memory");
+  });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)f.splits, (unsigned)f.a.units);
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.dynamicSmemBytes = one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows_even);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)f.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, f), "aoh_key_weights launch");
+}
+
 }  // namespace
 
-void plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p) {
+bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p) {
   p.kind = KeyWeightsKind::few;
   const int pages = (max_len + kPage - 1) / kPage;
+  const size_t rows_even = (p.rows + 1) / 2 * 2;
+  // A cluster a unit where its 16 CTAs read K fast enough.  More than 16 rows
+  // leave an SM one CTA, and clusters of 16 of those do not fit every GPC (8
+  // units of 32 rows x 4096 keys: 20 us, with 8 CTAs 15).
+  const int most = p.rows > kFewRows && units * kMaxOne > c->num_sms / 2 ? kMaxOne / 2 : kMaxOne;
+  const int one = std::max(1, std::min(most, pages / (2 * kFewWarps)));  // at least two pages for each of a CTA's warps
+  if (pages <= (p.rows <= kFewRows ? kOnePages : kOnePages / 2) && units * one <= c->num_sms &&
+      one_smem(pages, one, (int)rows_even) <= kOneSmem) {
+    p.splits = one;
+    p.one = true;
+    return true;
+  }
+  if (p.rows > kFewRows) return false;
   // two CTAs per SM in one wave, at least two pages for each of a CTA's warps
   p.splits = std::max(1, std::min(2 * std::max(1, c->num_sms) / std::max(1, units), pages / (2 * kFewWarps)));
-  const size_t rows_even = (p.rows + 1) / 2 * 2;
   p.part = 0;
   p.score = align256((size_t)p.splits * units * p.rows * sizeof(float2));
   p.bytes = p.score + (size_t)units * pages * kPage * rows_even * sizeof(float);
+  return true;
 }
 
 int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws,
@@ -820,12 +922,17 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
   f.splits = p.splits;
   f.score_unit = (long long)((a.max_len + kPage - 1) / kPage) * kPage * f.rows_even;
   const dim3 grid(p.splits, a.units);
+  if (p.one) {
+    f.part = nullptr;
+    f.score = nullptr;
+    return p.rows <= 8    ? launch_few_one<1>(c, f, st)
+           : p.rows <= 16 ? launch_few_one<2>(c, f, st)
+                          : launch_few_one<4>(c, f, st);
+  }
   if (p.rows <= 8)
-    few_scores_kernel<1><<<grid, kFewWarps * 32, 0, st>>>(f);
-  else if (p.rows <= 16)
-    few_scores_kernel<2><<<grid, kFewWarps * 32, 0, st>>>(f);
+    few_scores_kernel<1, false><<<grid, kFewWarps * 32, 0, st>>>(f);
   else
-    few_scores_kernel<4><<<grid, kFewWarps * 32, 0, st>>>(f);
+    few_scores_kernel<2, false><<<grid, kFewWarps * 32, 0, st>>>(f);
   const int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
   return rc ? rc
             : launch_dependent(few_sum_kernel, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 256, 0, st,

@@ -74,9 +74,10 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
     if out.stride(2) != 1 or stride < total or (B > 1 and out.stride(0) != R * stride):
         raise ValueError("out's rows must be contiguous and evenly spaced over (batch, n_ret)")
     L = cache._L
-    ws = q.new_empty(L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n), dtype=torch.uint8)
+    nbytes = L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _lib.launch(q.device, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
-                out.data_ptr(), stride, bool(accumulate), ws.data_ptr(), ws.numel())
+                out.data_ptr(), stride, bool(accumulate), ws.data_ptr() if nbytes else None, nbytes)
     return out
 
 

@@ -252,6 +252,23 @@ def test_key_weights_f32_in_blocks_of_rows(G, grp, C, past):
     assert ((twice - 2 * got).abs() <= 4 * 2.0 ** -24 * twice).all()
 
 
+@pytest.mark.parametrize("C,T", [(1, 8192), (1, 8193), (2, 8191), (2, 255), (5, 4096), (5, 4097), (6, 4096), (7, 511)])
+@pytest.mark.parametrize("labels", [[1, 1], [1, 0]])
+def test_key_weights_where_the_kernels_change(labels, C, T):
+    """Groups of 6: 6 to 42 query rows, around the lengths that one launch takes; the other sequence is not
+    stored here."""
+    owned = np.array([[[1, 1], [0, 0]]])
+    cache, k, _ = filled([labels], 12, 2, T, BF16, T + C, owned=owned)
+    q = randn(gen(C), 2, C, 12, 128, dtype=BF16) * 1.5
+    heads = [g for g, x in enumerate(labels) if x]
+    out = torch.full((2, len(heads), T + 3), 1.0, device="cuda")
+    key_weights(cache, 0, q, past_len=T - C, out=out)
+    check_weights(out[:1, :, :T], q[:1], k[0][:1], heads, T - C)
+    assert (out[1, :, :T] == 0).all() and (out[..., T:] == 1).all()
+    again = key_weights(cache, 0, q, past_len=T - C)
+    assert torch.equal(again, out[..., :T])
+
+
 def test_key_weights_large_scores():
     """Scores far apart: one key takes nearly everything; no overflow."""
     cache, k, _ = filled([[1]], 4, 1, 900, BF16, 1)
