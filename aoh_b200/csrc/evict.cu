@@ -56,6 +56,12 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// The weight of a key, unless that may be NaN (like -inf) or -0 (like +0): then as it is in memory.
+__device__ __forceinline__ float key_weight(uint32_t k, const float* p) {
+  constexpr uint32_t kNegInf = ~0xff800000u, kZero = 0x80000000u;
+  return k == kNegInf || k == kZero ? *p : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
 __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       if (is_gt || (is_eq && re < left)) {
         const int at = a.sink + (int)(bg + __popc(mg & below) + min(re, left));
         kept[at] = a.sink + lo + i;
-        if (kept_w) kept_w[at] = wm[i];
+        if (kept_w) kept_w[at] = key_weight(k, wm + i);
       }
       bg += __popc(mg);
       be += __popc(me);

@@ -28,7 +28,7 @@
 // that holds one such token, cost more than the copy.  A CTA's biases are
 // listed in the order given, and the entries of one token linked in that order:
 // their sum has a fixed order (37 rows x 32003 with 300 biases, 240 of them in
-// one slice: DUP us; with the whole list read for each sum 19).
+// one slice: 17 us; with the whole list read for each sum 19).
 #include <climits>
 #include <type_traits>
 
@@ -537,14 +537,16 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   a.logits = p.logits;
   a.row_stride = p.row_stride;
   a.vocab = p.vocab;
-  // 16 CTAs a row take the least time for a few rows, but then 8, which fill the
-  // SMs in one wave, and 4 (64 rows of 128K, all features: 28 / 21 / 24 us).
+  // 16 CTAs a row take the least time while all of them have an SM's third part
+  // (24 rows of 128K, all features, with 16 / 8: 10.6 / 11.4 us, 32 rows 14.2 /
+  // 11.7), then 8, and 4 once those are more than one wave (64 rows: 21.4 with
+  // 16, 16.0 with 8, 18.1 with 4).
   int dev = 0, sms = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
   rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
   if (rc) return rc;
-  const int most = p.rows * 16LL <= 2 * sms ? 16 : p.rows * 8LL <= 4 * sms ? 8 : 4;
+  const int most = p.rows * 16LL <= 3 * sms ? 16 : p.rows * 8LL <= 4 * sms ? 8 : 4;
   a.cluster = 1;
   while (a.cluster < most && a.cluster * (wide ? kSlice : kSlice / 2) < p.vocab) {
     a.cluster *= 2;
