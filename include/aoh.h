@@ -306,8 +306,9 @@ AOH_API int aoh_kv_append(aoh_kv_cache* cache, int32_t layer, int32_t past_len, 
  * to out instead of writing it.  Units not stored here get (add) zeros.
  * q (batch, q_len, num_q_heads, 128) as for aoh_attn_prefill.  workspace:
  * 16-byte aligned device memory of aoh_key_weights_workspace_bytes() for the
- * same lengths, of any contents, not shared by calls that overlap.  Scores are
- * fp32 and sums are made in a fixed order. */
+ * same lengths, of any contents, not shared by calls that overlap; NULL will do
+ * where that is 0 (a few query rows and keys, or arguments that cannot run).
+ * Scores are fp32 and sums are made in a fixed order. */
 AOH_API size_t aoh_key_weights_workspace_bytes(const aoh_kv_cache* cache, int32_t layer, int32_t past_len,
                                                int32_t q_len);
 AOH_API int aoh_key_weights(aoh_kv_cache* cache, int32_t layer, int32_t past_len, int32_t q_len, const void* q,
