@@ -742,6 +742,37 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager, outs))
 
 
+@pytest.mark.parametrize("dtype,C,T", [
+    (BF16, 1, 20_000), (BF16, 2, 700),      # few query rows: two launches, one
+    (BF16, 40, 3_000), (BF16, 300, 3_000),  # the tensor cores: query rows resident, keys resident
+    (F32, 9, 1_000),
+])
+def test_key_weights_in_two_graphs_and_eager_at_once(dtype, C, T):
+    """Each call has its own workspace: graphs replayed beside one another and beside an eager call."""
+    cache, k, _ = filled([[1, 1]], 8, 1, T, dtype, C)
+    qs = [randn(gen(i), 1, C, 8, 128, dtype=dtype) for i in range(3)]
+    want = [key_weights(cache, 0, q, past_len=T - C) for q in qs]
+    graphs = []
+    for q in qs[:2]:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            w = key_weights(cache, 0, q, past_len=T - C)
+            key_weights(cache, 0, q, past_len=T - C, out=w, accumulate=True)
+        graphs.append((gr, w))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for (gr, _), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        eager = key_weights(cache, 0, qs[2], past_len=T - C)
+    torch.cuda.synchronize()
+    assert torch.equal(eager, want[2])
+    for (_, w), x in zip(graphs, want):
+        # added to what one call gave: blocks of rows or ranges may be added one by one
+        assert ((w - 2 * x).abs() <= 4 * 2.0 ** -24 * w).all()
+
+
 def test_key_weights_with_the_devices_length():
     """A captured single-token call reads the length that the graph advances."""
     from aoh_b200 import _lib
