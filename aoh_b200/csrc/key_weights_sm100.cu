@@ -28,6 +28,8 @@
 // MUFU alone would take 1024 cycles an SM for a product that the tensor cores
 // do in 512.  Four warpgroups keep it fed, and one pair in eight goes to a
 // polynomial of the same accuracy on the FMA pipe.
+#include <type_traits>
+
 #include "common.cuh"
 #include "fast_math.cuh"
 #include "internal.h"
@@ -47,8 +49,9 @@ constexpr int kOneSmem = 160 * 1024;    // scores of one of them
 struct FewArgs {
   KeyWeightsArgs a;
   float2* part;   // [split][unit row][row]
-  float* score;   // [unit row][key][rows_even]: q . k, -inf where a row does not see the key
-  int rows, rows_even, splits;
+  float* score;   // [unit row][key][stride]: q . k, -inf where a row does not see the key
+  int rows, splits;
+  int cols, stride;      // of a key: scores that are written (no rows behind `rows`: -inf), floats
   long long score_unit;  // floats of a unit's scores
 };
 
@@ -58,7 +61,7 @@ struct FewArgs {
 template <int NT, bool kOne>
 __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_kernel(const __grid_constant__ FewArgs f) {
   __shared__ float2 red[kFewWarps][NT * 8];
-  extern __shared__ __align__(16) float own_scores[];  // kOne: [key of the range][rows_even]
+  extern __shared__ __align__(16) float own_scores[];  // kOne: [key of the range][stride]
   const KeyWeightsArgs& a = f.a;
   if (!kOne) griddep_launch_dependents();  // the sums wait for this grid to finish
   const int r = blockIdx.y;
@@ -152,11 +155,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
 #pragma unroll
         for (int e = 0; e < 2; ++e) s[h][e] = j0 + 8 * h <= last[n][e] ? c[n][2 * h + e] : -INFINITY;
       const int col = n * 8 + 2 * tq;
-      if (col < f.rows_even) {
-        float* o = kOne ? own_scores + (j0 - p0 * kPage) * f.rows_even + col
-                        : f.score + r * f.score_unit + (long long)j0 * f.rows_even + col;
+      if (col < f.cols) {
+        float* o = kOne ? own_scores + (j0 - p0 * kPage) * f.stride + col
+                        : f.score + r * f.score_unit + (long long)j0 * f.stride + col;
         *reinterpret_cast<float2*>(o) = make_float2(s[0][0], s[0][1]);
-        *reinterpret_cast<float2*>(o + 8 * f.rows_even) = make_float2(s[1][0], s[1][1]);
+        *reinterpret_cast<float2*>(o + 8 * f.stride) = make_float2(s[1][0], s[1][1]);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -227,7 +230,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
     for (int j = threadIdx.x; j < n; j += kFewWarps * 32) {
       float w = 0.f;
       for (int row = 0; row < f.rows; row += 2) {
-        const float2 x = *reinterpret_cast<const float2*>(own_scores + j * f.rows_even + row);
+        const float2 x = *reinterpret_cast<const float2*>(own_scores + j * f.stride + row);
         w = fmaf(fast_exp2(fmaf(x.x, kScoreScale, -ml[row].x)), ml[row].y, w);
         if (row + 1 < f.rows) w = fmaf(fast_exp2(fmaf(x.y, kScoreScale, -ml[row + 1].x)), ml[row + 1].y, w);
       }
@@ -238,10 +241,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
   }
 }
 
-// Weights of 1024 keys from their scores, four keys a thread.
+// Weights of 1024 keys from their scores, four keys a thread, S scores a key
+// (f.stride), all of whose loads are in flight at once.
 constexpr int kFewKeys = 4;
+template <int S>
 __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
-  __shared__ float2 ml[kFewRows];  // of a row: its maximum and 1 / sum (their rounded logarithm would be 1e-6 off)
+  using Vec = typename std::conditional<S == 2, float2, float4>::type;
+  constexpr int V = sizeof(Vec) / 4;
+  __shared__ float2 ml[S];  // of a row: its maximum and 1 / sum (their rounded logarithm would be 1e-6 off)
   const KeyWeightsArgs& a = f.a;
   const int r = blockIdx.y;
   const bool stored = a.rows[r].held > 0;
@@ -250,13 +257,16 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
   griddep_wait();
   if (blockIdx.x * 256 * kFewKeys >= len) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the first two rows' scores are on their way while the ranges are combined
+  // the scores are on their way while the ranges are combined
   const float* s = f.score + r * f.score_unit;
-  float2 v[kFewKeys];
+  Vec v[kFewKeys][S / V];
 #pragma unroll
   for (int k = 0; k < kFewKeys; ++k)
-    v[k] = stored && j0 + 256 * k < len ? *reinterpret_cast<const float2*>(s + (long long)(j0 + 256 * k) * f.rows_even)
-                                        : make_float2(-INFINITY, -INFINITY);
+    if (stored && j0 + 256 * k < len) {
+#pragma unroll
+      for (int c = 0; c < S / V; ++c) v[k][c] = reinterpret_cast<const Vec*>(s + (long long)(j0 + 256 * k) * S)[c];
+    }
+  if (threadIdx.x >= f.rows && threadIdx.x < S) ml[threadIdx.x] = make_float2(0.f, 0.f);
   if (stored) {
     for (int row = warp; row < f.rows; row += 8) {
       float m = -INFINITY, l = 0.f;
@@ -277,15 +287,17 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
     }
   }
   __syncthreads();
-  float w[kFewKeys] = {0.f, 0.f, 0.f, 0.f};
-  if (stored) {
-    for (int row = 0; row < f.rows; row += 2) {
+  float w[kFewKeys] = {};
 #pragma unroll
-      for (int k = 0; k < kFewKeys; ++k) {
-        if (j0 + 256 * k >= len) continue;
-        if (row > 0) v[k] = *reinterpret_cast<const float2*>(s + (long long)(j0 + 256 * k) * f.rows_even + row);
-        w[k] = fmaf(fast_exp2(fmaf(v[k].x, kScoreScale, -ml[row].x)), ml[row].y, w[k]);
-        if (row + 1 < f.rows) w[k] = fmaf(fast_exp2(fmaf(v[k].y, kScoreScale, -ml[row + 1].x)), ml[row + 1].y, w[k]);
+  for (int k = 0; k < kFewKeys; ++k) {
+    if (!stored || j0 + 256 * k >= len) continue;
+#pragma unroll
+    for (int c = 0; c < S / V; ++c) {
+      const float* x = reinterpret_cast<const float*>(&v[k][c]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float2 m = ml[c * V + e];
+        w[k] = fmaf(fast_exp2(fmaf(x[e], kScoreScale, -m.x)), m.y, w[k]);
       }
     }
   }
@@ -856,8 +868,15 @@ int plan_ranges(long long items, int tiles, int sms, bool even) {
 // keys 5.6 / 10.0 us against 6.2 / 14.3, x 8192 6.9 / 10.0 against 6.3 / 14.4, x
 // 16384 9.0 / 10.4 against 6.9 / 14.5.
 constexpr int kOnePages = 512;
+// Floats of a key's scores: in a cluster two more than are written, which keeps
+// the keys of a warp on distinct banks; else 2, 4, 8 or 16, for wide loads.
+int one_cols(int rows) { return (rows + 1) / 2 * 2; }
+int one_stride(int rows) { return one_cols(rows) + 2; }
+int few_stride(int rows) { return rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
 // bytes of the scores of one of n CTAs
-size_t one_smem(int pages, int n, int rows_even) { return (size_t)((pages + n - 1) / n) * kPage * rows_even * sizeof(float); }
+size_t one_smem(int pages, int n, int rows) {
+  return (size_t)((pages + n - 1) / n) * kPage * one_stride(rows) * sizeof(float);
+}
 
 template <int NT>
 int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
@@ -874,7 +893,7 @@ int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)f.splits, (unsigned)f.a.units);
   cfg.blockDim = dim3(kFewWarps * 32);
-  cfg.dynamicSmemBytes = one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows_even);
+  cfg.dynamicSmemBytes = one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -890,14 +909,13 @@ int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
 bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeightsPlan& p) {
   p.kind = KeyWeightsKind::few;
   const int pages = (max_len + kPage - 1) / kPage;
-  const size_t rows_even = (p.rows + 1) / 2 * 2;
   // A cluster a unit where its 16 CTAs read K fast enough.  More than 16 rows
   // leave an SM one CTA, and clusters of 16 of those do not fit every GPC (8
   // units of 32 rows x 4096 keys: 20 us, with 8 CTAs 15).
   const int most = p.rows > kFewRows && units * kMaxOne > c->num_sms / 2 ? kMaxOne / 2 : kMaxOne;
   const int one = std::max(1, std::min(most, pages / (2 * kFewWarps)));  // at least two pages for each of a CTA's warps
   if (pages <= (p.rows <= kFewRows ? kOnePages : kOnePages / 2) && units * one <= c->num_sms &&
-      one_smem(pages, one, (int)rows_even) <= kOneSmem) {
+      one_smem(pages, one, p.rows) <= kOneSmem) {
     p.splits = one;
     p.one = true;
     return true;
@@ -907,7 +925,7 @@ bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeig
   p.splits = std::max(1, std::min(2 * std::max(1, c->num_sms) / std::max(1, units), pages / (2 * kFewWarps)));
   p.part = 0;
   p.score = align256((size_t)p.splits * units * p.rows * sizeof(float2));
-  p.bytes = p.score + (size_t)units * pages * kPage * rows_even * sizeof(float);
+  p.bytes = p.score + (size_t)units * pages * kPage * few_stride(p.rows) * sizeof(float);
   return true;
 }
 
@@ -918,9 +936,10 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
   f.part = reinterpret_cast<float2*>(ws + p.part);
   f.score = reinterpret_cast<float*>(ws + p.score);
   f.rows = p.rows;
-  f.rows_even = (p.rows + 1) / 2 * 2;
   f.splits = p.splits;
-  f.score_unit = (long long)((a.max_len + kPage - 1) / kPage) * kPage * f.rows_even;
+  f.cols = p.one ? one_cols(p.rows) : few_stride(p.rows);
+  f.stride = p.one ? one_stride(p.rows) : f.cols;
+  f.score_unit = (long long)((a.max_len + kPage - 1) / kPage) * kPage * f.stride;
   const dim3 grid(p.splits, a.units);
   if (p.one) {
     f.part = nullptr;
@@ -934,9 +953,13 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
   else
     few_scores_kernel<2, false><<<grid, kFewWarps * 32, 0, st>>>(f);
   const int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
-  return rc ? rc
-            : launch_dependent(few_sum_kernel, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 256, 0, st,
-                               "aoh_key_weights sums launch", f);
+  if (rc) return rc;
+  auto sums = f.stride == 2   ? few_sum_kernel<2>
+              : f.stride == 4 ? few_sum_kernel<4>
+              : f.stride == 8 ? few_sum_kernel<8>
+                              : few_sum_kernel<16>;
+  return launch_dependent(sums, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 256, 0, st,
+                          "aoh_key_weights sums launch", f);
 }
 
 void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int q_len, KeyWeightsPlan& p) {
