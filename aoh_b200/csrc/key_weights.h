@@ -50,8 +50,7 @@ int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, co
                               cudaStream_t st);
 
 // Query rows of a unit that the few-rows kernels take: up to 32 where one launch
-// does, else 16.  24 rows x 32768 keys, 2 units: 27 us, on the tensor cores 21;
-// 16 rows: 18.
+// does, else 16 (16 rows x 32768 keys, 2 units: 16 us, on the tensor cores 21).
 constexpr int kFewRows = 16, kOneRows = 32;
 
 inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }

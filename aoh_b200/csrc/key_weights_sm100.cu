@@ -863,10 +863,10 @@ int plan_ranges(long long items, int tiles, int sms, bool even) {
   return best;
 }
 
-// Most pages of a unit that a cluster takes (half of them for more than 16
-// rows).  On the device and from Python, one launch against two: 8 rows x 4096
-// keys 5.6 / 10.0 us against 6.2 / 14.3, x 8192 6.9 / 10.0 against 6.3 / 14.4, x
-// 16384 9.0 / 10.4 against 6.9 / 14.5.
+// Most pages of a unit that a cluster takes.  On the device and from Python, one
+// launch against two: 4 rows x 4096 keys 5.6 / 10.0 us against 6.2 / 14.3, x 8192
+// 6.9 / 10.0 against 6.3 / 14.4, x 16384 9.0 / 10.4 against 6.9 / 14.5; 32 rows x
+// 8192 keys 11.0 / 12.5 against 14.0 / 16.5 on the tensor cores.
 constexpr int kOnePages = 512;
 // Floats of a key's scores: in a cluster two more than are written, which keeps
 // the keys of a warp on distinct banks; else 2, 4, 8 or 16, for wide loads.
@@ -911,10 +911,10 @@ bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeig
   const int pages = (max_len + kPage - 1) / kPage;
   // A cluster a unit where its 16 CTAs read K fast enough.  More than 16 rows
   // leave an SM one CTA, and clusters of 16 of those do not fit every GPC (8
-  // units of 32 rows x 4096 keys: 20 us, with 8 CTAs 15).
+  // units of 32 rows x 4096 keys: 20 us, with 8 CTAs 11).
   const int most = p.rows > kFewRows && units * kMaxOne > c->num_sms / 2 ? kMaxOne / 2 : kMaxOne;
   const int one = std::max(1, std::min(most, pages / (2 * kFewWarps)));  // at least two pages for each of a CTA's warps
-  if (pages <= (p.rows <= kFewRows ? kOnePages : kOnePages / 2) && units * one <= c->num_sms &&
+  if (pages <= kOnePages && units * one <= c->num_sms &&
       one_smem(pages, one, p.rows) <= kOneSmem) {
     p.splits = one;
     p.one = true;

@@ -252,7 +252,7 @@ def test_key_weights_f32_in_blocks_of_rows(G, grp, C, past):
     assert ((twice - 2 * got).abs() <= 4 * 2.0 ** -24 * twice).all()
 
 
-@pytest.mark.parametrize("C,T", [(1, 8192), (1, 8193), (2, 8191), (2, 255), (5, 4096), (5, 4097), (6, 4096), (7, 511)])
+@pytest.mark.parametrize("C,T", [(1, 8192), (1, 8193), (2, 8191), (2, 255), (5, 4096), (5, 4097), (5, 8192), (5, 8193), (6, 4096), (7, 511)])
 @pytest.mark.parametrize("labels", [[1, 1], [1, 0]])
 def test_key_weights_where_the_kernels_change(labels, C, T):
     """Groups of 6: 6 to 42 query rows, around the lengths that one launch takes; the other sequence is not
