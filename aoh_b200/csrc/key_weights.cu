@@ -14,8 +14,8 @@
 // pass also writes the scores, 4 bytes each, and the second reads them: 128
 // products on the CUDA cores cost 3.6 ps, a write and a read of 4 bytes 1.2 ps.
 // The query rows are taken in blocks whose scores fit L2, two launches a block.
-// 2 x 33 tokens, 3 groups of 2 heads, over 2023 keys, fp32: 18 us a call,
-// of which the scores take 12; with the scores computed again 35.
+// 2 x 33 tokens, 3 groups of 2 heads, over 2023 keys, fp32: 16 us a call,
+// of which the scores take 10; with the scores computed again 35.
 // bf16 caches run the kernels of key_weights_sm100.cu: one pass over K for few
 // query rows (single tokens), tensor cores for more.
 #include "common.cuh"
@@ -323,10 +323,14 @@ KeyWeightsPlan plan(const aoh_kv_cache* c, int layer, int max_len, int q_len) {
     // as many rows a block as have room for their scores, in whole tiles (of 16 rows at least)
     const long long row_bytes = (long long)units * max_len * sizeof(float), room = kScoreBytes / std::max(1LL, row_bytes);
     if (p.rows > room) p.rows = (int)(room >= kTile ? room / kTile * kTile : std::max(16LL, room / 16 * 16));
-    p.row_tiles = (p.rows + kTile - 1) / kTile;
-    p.tile_rows = ((p.rows + p.row_tiles - 1) / p.row_tiles + 7) / 8 * 8;  // tiles of like height: 66 rows = 40 + 26
     const int key_tiles = (max_len + kTile - 1) / kTile;
-    // as many CTAs as the SMs hold at a time: three of 64 rows, five of 8
+    // Up to 64 rows a tile, or 32 where one key tile for every CTA is no more than
+    // one wave: 2 x 3 units of 66 rows x 2023 keys 14.7 us, with 64 rows 15.9; 4
+    // units of 400 rows x 4000 keys 87, with 64 rows 70.
+    p.row_tiles = (p.rows + kTile - 1) / kTile;
+    if ((long long)units * p.row_tiles * key_tiles <= 3LL * c->num_sms) p.row_tiles = (p.rows + kTile / 2 - 1) / (kTile / 2);
+    p.tile_rows = ((p.rows + p.row_tiles - 1) / p.row_tiles + 7) / 8 * 8;  // tiles of like height: 66 rows = 24 + 24 + 18
+    // as many CTAs as the SMs hold at a time: three of 64 rows, four of 32, five of 8
     const long long ctas = std::max(1LL, (long long)units * p.row_tiles), resident = 224 * 1024 / any_smem(p.tile_rows);
     p.splits = (int)std::max(1LL, std::min<long long>(std::min(64, key_tiles),
                                                       (resident * std::max(1, c->num_sms) + ctas - 1) / ctas));
