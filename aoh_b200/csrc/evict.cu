@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
       __syncthreads();
   };
 
+  griddep_wait();
   if (a.take > 0) {  // the same for every CTA of the cluster
     const int per = a.part / kSelThreads;  // <= kKeys
     const int i0 = warp * 32 * per + lane;
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kEvictWarps * 32)
     evict_kernel(CacheGeom src, CacheGeom dst, const int32_t* unit_row, const int32_t* kept, long long kept_stride,
                  int keep, int len, int chunks) {
   const int unit = blockIdx.x / chunks;
+  griddep_wait();
   if (dst.unit_offset[unit + 1] == dst.unit_offset[unit]) return;  // not stored here
   const int row = unit_row[unit];
   const bool retrieval = row >= 0;
@@ -353,22 +355,13 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   const int per = a.part / kSelThreads;
   a.kept = kept;
   a.kept_w = kept_weights;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(rows * a.cluster));
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   auto kernel = per <= 2    ? select_kernel<2>
                 : per <= 8  ? select_kernel<8>
                 : per <= 16 ? select_kernel<16>
                 : per <= kSelMaxKeys ? select_kernel<kSelMaxKeys>
                                      : select_kernel<0>;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "aoh_select_keys launch");
+  return launch_dependent(kernel, dim3((unsigned)(rows * a.cluster)), a.cluster, kSelThreads, 0,
+                          static_cast<cudaStream_t>(stream), "aoh_select_keys launch", a);
 }
 
 extern "C" int aoh_kv_evict(aoh_kv_cache* src, aoh_kv_cache* dst, int32_t past_len, const int32_t* kept,
@@ -410,12 +403,8 @@ extern "C" int aoh_kv_evict(aoh_kv_cache* src, aoh_kv_cache* dst, int32_t past_l
   if (blocks > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "%s: too many rows", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const CacheGeom gs = src->geom(), gd = dst->geom();
-  if (a.dtype == AOH_BF16)
-    evict_kernel<true><<<(unsigned)blocks, kEvictWarps * 32, 0, st>>>(gs, gd, src->dev_unit_row, kept, kept_stride, keep,
-                                                                      past_len, chunks);
-  else
-    evict_kernel<false><<<(unsigned)blocks, kEvictWarps * 32, 0, st>>>(gs, gd, src->dev_unit_row, kept, kept_stride, keep,
-                                                                       past_len, chunks);
   dst->last_write_layer = kEveryLayer;
-  return cuda_check(cudaGetLastError(), "aoh_kv_evict launch");
+  return launch_dependent(a.dtype == AOH_BF16 ? evict_kernel<true> : evict_kernel<false>, dim3((unsigned)blocks), 1,
+                          kEvictWarps * 32, 0, st, "aoh_kv_evict launch", gs, gd, (const int32_t*)src->dev_unit_row, kept,
+                          (long long)kept_stride, keep, past_len, chunks);
 }

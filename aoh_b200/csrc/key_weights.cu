@@ -136,6 +136,7 @@ template <typename T>
 __global__ void __launch_bounds__(256, 3) key_lse_kernel(const __grid_constant__ AnyArgs k) {
   extern __shared__ float sm[];
   const KeyWeightsArgs& a = k.a;
+  griddep_wait();
   griddep_launch_dependents();  // the sums wait for this grid to finish
   const int r = blockIdx.y;
   const RetrievalRow info = a.rows[r];
@@ -214,10 +215,10 @@ __global__ void __launch_bounds__(256) key_sum_kernel(const __grid_constant__ An
   __shared__ float sums[8][kSumKeys];
   const KeyWeightsArgs& a = k.a;
   const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
   const int past = key_weights_past(a), len = past + a.q_len, j0 = (int)blockIdx.x * kSumKeys, key = j0 + lane;
   if (j0 >= len) return;
   const bool stored = a.rows[r].held > 0;
-  griddep_wait();
   float w = 0.f;
   // rows of the block from the first token on that sees this key (and this CTA's first key)
   const int first = max(0, key - past) * a.g.grp - k.row_base;
@@ -294,10 +295,10 @@ int launch_any(const KeyWeightsArgs& a, const KeyWeightsPlan& p, char* ws, cudaS
   for (k.row_base = 0; k.row_base < rows; k.row_base += p.rows) {
     k.rows = std::min(p.rows, rows - k.row_base);
     const int row_tiles = (k.rows + p.tile_rows - 1) / p.tile_rows;
-    key_lse_kernel<T><<<dim3(p.splits, a.units, row_tiles), 4 * p.tile_rows, any_smem(p.tile_rows), st>>>(k);
-    rc = cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+    rc = launch_dependent(key_lse_kernel<T>, dim3(p.splits, a.units, row_tiles), 1, 4 * p.tile_rows, any_smem(p.tile_rows),
+                          st, "aoh_key_weights launch", k);
     if (rc) return rc;
-    rc = launch_dependent(key_sum_kernel, dim3((a.max_len + kSumKeys - 1) / kSumKeys, a.units), 256, 0, st,
+    rc = launch_dependent(key_sum_kernel, dim3((a.max_len + kSumKeys - 1) / kSumKeys, a.units), 1, 256, 0, st,
                           "aoh_key_weights sums launch", k);
     if (rc) return rc;
     k.a.accumulate = 1;

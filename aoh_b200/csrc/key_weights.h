@@ -61,23 +61,6 @@ inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 __device__ __forceinline__ int key_weights_past(const KeyWeightsArgs& a) {
   return a.past_len_dev ? max(0, min(*a.past_len_dev, a.max_len - a.q_len)) : a.past_len;
 }
-
-
-// Launch that may start while the kernel before it finishes (it waits for that kernel itself).
-template <class F, class... A>
-int launch_dependent(F kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...), what);
-}
 #endif
 
 // 1 / sqrt(128) * log2(e): scores in the log2 domain

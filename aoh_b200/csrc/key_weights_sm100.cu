@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
   __shared__ float2 red[kFewWarps][NT * 8];
   extern __shared__ __align__(16) float own_scores[];  // kOne: [key of the range][stride]
   const KeyWeightsArgs& a = f.a;
+  griddep_wait();
   if (!kOne) griddep_launch_dependents();  // the sums wait for this grid to finish
   const int r = blockIdx.y;
   const RetrievalRow info = a.rows[r];
@@ -429,6 +430,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sB = sA + 2 * kTileBytes;                                     // ring of streamed tiles
   float* sLse = reinterpret_cast<float*>(sB + kStages * kTileBytes);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  if (kPass == kLse) griddep_wait();  // before the next pass may start: it reads the lengths without waiting itself
   if (kPass == kLse || (kPass == kSums && t.splits > 1)) griddep_launch_dependents();  // not the call's last kernel
 
   // this CTA's resident pair and range of streamed tiles
@@ -444,7 +446,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int tt = t.tile_tokens;
   const int key_tiles = (len + kTileRows - 1) / kTileRows;
   const int na = min(2, (kQueriesResident ? t.row_tiles : key_tiles) - 2 * pair);  // a device length may leave none
-  if (na <= 0) return;
+  if (na <= 0) {
+    if (kPass != kLse) griddep_wait();  // no grid ends before those in front of it
+    return;
+  }
   int first = 0, end;  // streamed tiles that any resident row needs
   if (kPass == kSums) {
     first = max(0, 2 * pair * kTileRows - past) / tt;
@@ -456,6 +461,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int n = first + (int)((long long)(end - first) * (split + 1) / t.splits) - t0;
   if (held == 0) {  // not stored here: no weight
     if (kPass == kLse) return;
+    griddep_wait();
     const int lo = kPass == kSums ? 2 * pair * kTileRows : t0 * kTileRows;
     const int hi = min(len, kPass == kSums ? lo + 2 * kTileRows : (t0 + n) * kTileRows);
     for (int j = lo + tid; j < hi; j += kTcThreads) {
@@ -890,18 +896,8 @@ int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
                           "aoh_key_weights shared memory");
   });
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)f.splits, (unsigned)f.a.units);
-  cfg.blockDim = dim3(kFewWarps * 32);
-  cfg.dynamicSmemBytes = one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)f.splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, f), "aoh_key_weights launch");
+  return launch_dependent(kernel, dim3((unsigned)f.splits, (unsigned)f.a.units), f.splits, kFewWarps * 32,
+                          one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows), st, "aoh_key_weights launch", f);
 }
 
 }  // namespace
@@ -941,6 +937,7 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
   f.stride = p.one ? one_stride(p.rows) : f.cols;
   f.score_unit = (long long)((a.max_len + kPage - 1) / kPage) * kPage * f.stride;
   const dim3 grid(p.splits, a.units);
+  int rc = AOH_OK;
   if (p.one) {
     f.part = nullptr;
     f.score = nullptr;
@@ -949,16 +946,15 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
                           : launch_few_one<4>(c, f, st);
   }
   if (p.rows <= 8)
-    few_scores_kernel<1, false><<<grid, kFewWarps * 32, 0, st>>>(f);
+    rc = launch_dependent(few_scores_kernel<1, false>, grid, 1, kFewWarps * 32, 0, st, "aoh_key_weights scores launch", f);
   else
-    few_scores_kernel<2, false><<<grid, kFewWarps * 32, 0, st>>>(f);
-  const int rc = cuda_check(cudaGetLastError(), "aoh_key_weights scores launch");
+    rc = launch_dependent(few_scores_kernel<2, false>, grid, 1, kFewWarps * 32, 0, st, "aoh_key_weights scores launch", f);
   if (rc) return rc;
   auto sums = f.stride == 2   ? few_sum_kernel<2>
               : f.stride == 4 ? few_sum_kernel<4>
               : f.stride == 8 ? few_sum_kernel<8>
                               : few_sum_kernel<16>;
-  return launch_dependent(sums, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 256, 0, st,
+  return launch_dependent(sums, dim3((a.max_len + 256 * kFewKeys - 1) / (256 * kFewKeys), a.units), 1, 256, 0, st,
                           "aoh_key_weights sums launch", f);
 }
 
@@ -1011,24 +1007,24 @@ int launch_key_weights_tensor(const aoh_kv_cache* c, const KeyWeightsArgs& a, co
   const long long g1 = (long long)a.units * t.pairs * p.splits;
   const long long g2 = p.stream ? g1 : (long long)a.units * key_pairs(a.max_len) * p.row_splits;
   if (g1 > 0x7fffffffLL || g2 > 0x7fffffffLL) return fail(AOH_ERR_UNSUPPORTED, "aoh_key_weights: too many tiles");
-  tensor_pass_kernel<kLse><<<(unsigned)g1, kTcThreads, kTcSmem, st>>>(tm, t);
-  rc = cuda_check(cudaGetLastError(), "aoh_key_weights launch");
+  rc = launch_dependent(tensor_pass_kernel<kLse>, dim3((unsigned)g1), 1, kTcThreads, kTcSmem, st, "aoh_key_weights launch",
+                        tm, t);
   if (rc) return rc;
   if (p.stream)
-    return launch_dependent(tensor_pass_kernel<kStream>, dim3((unsigned)g2), kTcThreads, kTcSmem, st,
+    return launch_dependent(tensor_pass_kernel<kStream>, dim3((unsigned)g2), 1, kTcThreads, kTcSmem, st,
                             "aoh_key_weights sums launch", tm, t);
   if (p.splits > 1) {
     const long long rows = (long long)a.units * p.row_tiles * kTileRows;
-    rc = launch_dependent(combine_lse_kernel, dim3((unsigned)(rows / 32)), 256, 0, st, "aoh_key_weights combine launch",
+    rc = launch_dependent(combine_lse_kernel, dim3((unsigned)(rows / 32)), 1, 256, 0, st, "aoh_key_weights combine launch",
                           (const float2*)t.part, t.neg_lse, rows, p.splits);
     if (rc) return rc;
   }
   t.pairs = key_pairs(a.max_len);
   t.splits = p.row_splits;
-  rc = launch_dependent(tensor_pass_kernel<kSums>, dim3((unsigned)g2), kTcThreads, kTcSmem, st,
+  rc = launch_dependent(tensor_pass_kernel<kSums>, dim3((unsigned)g2), 1, kTcThreads, kTcSmem, st,
                         "aoh_key_weights sums launch", tm, t);
   if (rc || p.row_splits == 1) return rc;
-  return launch_dependent(combine_sums_kernel, dim3((a.max_len + 255) / 256, a.units), 256, 0, st,
+  return launch_dependent(combine_sums_kernel, dim3((a.max_len + 255) / 256, a.units), 1, 256, 0, st,
                           "aoh_key_weights combine launch", t);
 }
 

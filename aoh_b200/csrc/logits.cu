@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   auto token = [&](int p) { return ((((p / kTurn) << a.cluster_log) + rank) * kTurn) | (p % kTurn); };
   auto place = [&](int t) { return (((t / kTurn) >> a.cluster_log) * kTurn) | (t % kTurn); };
   const int words = (a.vocab + 31) >> 5;
+  griddep_wait();
   const T* x_row = static_cast<const T*>(a.logits) + row * a.row_stride;
   O* out = static_cast<O*>(a.out) + row * a.out_stride;
   const uint32_t* seen = a.seen ? a.seen + (long long)row * words : nullptr;
@@ -458,6 +459,7 @@ template <typename I>
 __global__ void history_add_kernel(uint32_t* counts, uint32_t* seen, int vocab, const I* ids, long long id_stride,
                                    int per_row, const int32_t* lengths, bool prompt) {
   const int row = blockIdx.y;
+  griddep_wait();
   const int n = lengths ? min(lengths[row], per_row) : per_row;
   const int words = (vocab + 31) >> 5;
   for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
@@ -487,18 +489,9 @@ int launch(const LogitsArgs& a, int rows, cudaStream_t st) {
                           "aoh_logits_penalize shared memory");
   });
   if (rc) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * a.cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = a.n_bias ? (size_t)a.slice / 4 + 4 * (size_t)bias_room(a.n_bias) * sizeof(int) : 0;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "aoh_logits_penalize launch");
+  const size_t smem = a.n_bias ? (size_t)a.slice / 4 + 4 * (size_t)bias_room(a.n_bias) * sizeof(int) : 0;
+  return launch_dependent(kernel, dim3((unsigned)(rows * a.cluster)), a.cluster, kThreads, smem, st,
+                          "aoh_logits_penalize launch", a);
 }
 template <typename T, typename O>
 int launch(const LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
@@ -591,10 +584,8 @@ extern "C" int aoh_history_add(int32_t* counts, int32_t* seen, int32_t rows, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t *c = reinterpret_cast<uint32_t*>(counts), *s = reinterpret_cast<uint32_t*>(seen);
   if (ids_64)
-    history_add_kernel<long long><<<grid, 256, 0, st>>>(c, s, vocab, static_cast<const long long*>(ids), id_stride,
-                                                        per_row, lengths, prompt != 0);
-  else
-    history_add_kernel<int><<<grid, 256, 0, st>>>(c, s, vocab, static_cast<const int*>(ids), id_stride, per_row,
-                                                  lengths, prompt != 0);
-  return cuda_check(cudaGetLastError(), "aoh_history_add launch");
+    return launch_dependent(history_add_kernel<long long>, grid, 1, 256, 0, st, "aoh_history_add launch", c, s, vocab,
+                            static_cast<const long long*>(ids), (long long)id_stride, per_row, lengths, prompt != 0);
+  return launch_dependent(history_add_kernel<int>, grid, 1, 256, 0, st, "aoh_history_add launch", c, s, vocab,
+                          static_cast<const int*>(ids), (long long)id_stride, per_row, lengths, prompt != 0);
 }

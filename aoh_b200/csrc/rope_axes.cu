@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, ITEMS > 1 || ROWS > 2 ? 3 : 5)
     const int h = row - toks[r] * a.heads;
     hs[r] = row < rows && h < nh ? head0 + h : -1;
   }
+  griddep_wait();
   Pack<T, VEC> raw[ROWS][ITEMS][2];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -258,8 +259,8 @@ int launch_rows(RopeAxesArgs& a, cudaStream_t st) {
   const long long gx = (a.n_tokens + a.tokens - 1) / a.tokens;
   const int gy = (heads + a.heads - 1) / a.heads;
   if (a.n_tokens > 0x7fffffffLL || gy > 65535) return fail(AOH_ERR_UNSUPPORTED, "aoh_rope_axes_qk: too many rows");
-  rope_axes_kernel<T, VEC, ITEMS, ROWS><<<dim3((unsigned)gx, (unsigned)gy), kThreads, 0, st>>>(a);
-  return cuda_check(cudaGetLastError(), "aoh_rope_axes_qk launch");
+  return launch_dependent(rope_axes_kernel<T, VEC, ITEMS, ROWS>, dim3((unsigned)gx, (unsigned)gy), 1, kThreads, 0, st,
+                          "aoh_rope_axes_qk launch", a);
 }
 
 template <typename T, int VEC>
