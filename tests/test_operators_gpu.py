@@ -742,6 +742,52 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager, outs))
 
 
+@pytest.mark.parametrize("dtype,C,T", [(BF16, 1, 30_000), (BF16, 4, 2_000), (BF16, 64, 9_000), (BF16, 700, 5_000),
+                                       (F32, 30, 3_000)])
+def test_each_operator_waits_for_the_one_before(dtype, C, T):
+    """The operators one behind the other, each fed by the last one, give what they give one at a time."""
+    g = gen(T)
+    labels, Hq, keep = [[1, 0, 1, 1]], 16, 400
+    cache, k, _ = filled(labels, Hq, 1, T, dtype, C, 16, 32)
+    into = AoHKVCache(labels, Hq, sink_size=16, recent_size=32, max_context=512, dtype=dtype, reserve_all=True)
+    q0, k0 = randn(g, 1, C, Hq, 128, dtype=dtype), randn(g, 1, C, 4, 128, dtype=dtype)
+    pos = torch.arange(T - C, T, device="cuda").expand(1, 1, C)
+    inv = 1e4 ** (-torch.arange(64, device="cuda", dtype=F32) / 64)
+    x = randn(g, 40, 60_000, dtype=dtype)
+
+    def steps(after):
+        out = []
+        h = TokenHistory(40, 60_000)
+        q = rope_axes_qk(q0, k0, pos, inv, (64,))[0]
+        after()
+        q = rope_axes_qk(q, k0, pos, inv, (64,))[0]
+        after()
+        w = key_weights(cache, 0, q, past_len=T - C)
+        after()
+        key_weights(cache, 0, q, past_len=T - C, out=w, accumulate=True)
+        after()
+        kept, kw = select_keys(w.view(3, T), keep, sink=16, recent=32)
+        after()
+        evict(cache, kept, into)
+        after()
+        w2 = key_weights(into, 0, q[:, :1].contiguous(), past_len=keep - 1)
+        after()
+        y, ids = penalize_logits(x, greedy=True)
+        for _ in range(3):
+            after()
+            h.append(ids)
+            after()
+            y, ids = penalize_logits(y, h, frequency=3.0, presence=2.0, out=y, greedy=True)
+            out.append(ids)
+        return [q, w, kept, kw, w2, y, *out]
+
+    want = steps(torch.cuda.synchronize)
+    for _ in range(5):
+        into.pool.zero_()
+        got = steps(lambda: None)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("dtype,C,T", [
     (BF16, 1, 20_000), (BF16, 2, 700),      # few query rows: two launches, one
     (BF16, 40, 3_000), (BF16, 300, 3_000),  # the tensor cores: query rows resident, keys resident
