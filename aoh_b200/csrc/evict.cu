@@ -345,7 +345,7 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   const int mid = n - sink - recent;
   // A CTA for every 8192 keys of a row, 8 at most, as long as all of them are
   // one wave of the GPU (an eighth of the SMs cannot be filled with clusters of
-  // 8: 18 rows of 64K take 38 us in them, 32 rows in clusters of 4 22 us); a
+  // 8: 18 rows of 64K took 38 us in them, 32 rows in clusters of 4 22 us); a
   // thread then has 8 keys, or more.
   a.cluster = 1;
   while (a.cluster < kSelMaxCluster && a.cluster * 8 * kSelThreads < mid &&

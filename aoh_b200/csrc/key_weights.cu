@@ -14,7 +14,7 @@
 // pass also writes the scores, 4 bytes each, and the second reads them: 128
 // products on the CUDA cores cost 3.6 ps, a write and a read of 4 bytes 1.2 ps.
 // The query rows are taken in blocks whose scores fit L2, two launches a block.
-// 2 x 33 tokens, 3 groups of 2 heads, over 2023 keys, fp32: 16 us a call,
+// 2 x 33 tokens, 3 groups of 2 heads, over 2023 keys, fp32: 15 us a call,
 // of which the scores take 10; with the scores computed again 35.
 // bf16 caches run the kernels of key_weights_sm100.cu: one pass over K for few
 // query rows (single tokens), tensor cores for more.

@@ -870,9 +870,9 @@ int plan_ranges(long long items, int tiles, int sms, bool even) {
 }
 
 // Most pages of a unit that a cluster takes.  On the device and from Python, one
-// launch against two: 4 rows x 4096 keys 5.6 / 10.0 us against 6.2 / 14.3, x 8192
-// 6.9 / 10.0 against 6.3 / 14.4, x 16384 9.0 / 10.4 against 6.9 / 14.5; 32 rows x
-// 8192 keys 11.0 / 12.5 against 14.0 / 16.5 on the tensor cores.
+// launch against two, 2 units: 4 rows x 4096 keys 5.4 / 9.5 us against 5.8 / 13.6,
+// x 8192 7.4 / 9.5 against 6.2 / 13.7, x 16384 11.4 / 11.6 against 7.2 / 13.7; 32
+// rows x 8192 keys 10.7 / 10.9 against 13.5 / 13.9 on the tensor cores.
 constexpr int kOnePages = 512;
 // Floats of a key's scores: in a cluster two more than are written, which keeps
 // the keys of a warp on distinct banks; else 2, 4, 8 or 16, for wide loads.
