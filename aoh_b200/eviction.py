@@ -44,9 +44,11 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
     """
     if not 0 <= layer_idx < cache.num_layers:
         raise ValueError(f"layer_idx {layer_idx} out of range")
-    if q.dim() != 4:
+    # a call's Python is most of the time that a single token takes: each property is read once
+    shape, dev, B, R = q.shape, q.device, cache.batch, cache.n_ret[layer_idx]
+    if len(shape) != 4:
         raise ValueError("q must be (B, C, Hq, D)")
-    n = q.shape[1]
+    n = shape[1]
     _check_q(cache, q, n)
     if cache.device_length:
         if n != 1 or past_len is not None or out is None:
@@ -57,26 +59,26 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
         if past < 0:
             raise ValueError("past_len must be non-negative")
         total = past + n
-    B, R = cache.batch, cache.n_ret[layer_idx]
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs an out to add to")
-        out = q.new_empty((B, R, total), dtype=torch.float32)
+        out, stride = q.new_empty((B, R, total), dtype=torch.float32), total
     elif (out.dim() != 3 or out.shape[0] != B or out.shape[1] != R or out.shape[2] < total
-          or out.dtype != torch.float32 or out.device != cache.device):
+          or out.dtype != torch.float32 or out.device != dev):
         raise ValueError(f"out must be float32 (batch, n_ret, >= keys) = {(B, R, total)} on {cache.device}, "
                          f"got {out.dtype} {tuple(out.shape)}")
+    elif R > 0:
+        stride = out.stride(1) if R > 1 else out.stride(0) if B > 1 else out.shape[2]
+        if out.stride(2) != 1 or stride < total or (B > 1 and out.stride(0) != R * stride):
+            raise ValueError("out's rows must be contiguous and evenly spaced over (batch, n_ret)")
     if R == 0 or n == 0:
         if not accumulate:
             out[:, :, :total].zero_()
         return out
-    stride = out.stride(1) if R > 1 else out.stride(0) if B > 1 else max(out.shape[2], total)
-    if out.stride(2) != 1 or stride < total or (B > 1 and out.stride(0) != R * stride):
-        raise ValueError("out's rows must be contiguous and evenly spaced over (batch, n_ret)")
     L = cache._L
     nbytes = L.aoh_key_weights_workspace_bytes(cache._h, layer_idx, past, n)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _lib.launch(q.device, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
+    _lib.launch(dev, L.aoh_key_weights, "aoh_key_weights", cache._h, layer_idx, past, n, q.data_ptr(),
                 out.data_ptr(), stride, bool(accumulate), ws.data_ptr() if nbytes else None, nbytes)
     return out
 
