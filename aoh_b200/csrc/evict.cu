@@ -25,6 +25,7 @@
 //   rows is in flight at once.
 #include "common.cuh"
 #include "internal.h"
+#include "launch.cuh"
 #include "page_layout.cuh"
 
 namespace aoh {

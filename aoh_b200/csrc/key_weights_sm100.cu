@@ -34,6 +34,7 @@
 #include "fast_math.cuh"
 #include "internal.h"
 #include "key_weights.h"
+#include "launch.cuh"
 #include "page_layout.cuh"
 
 namespace aoh {

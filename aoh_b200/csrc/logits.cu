@@ -34,6 +34,7 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "launch.cuh"
 
 namespace aoh {
 namespace {

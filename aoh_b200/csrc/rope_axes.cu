@@ -25,6 +25,7 @@
 // in flight.
 #include "common.cuh"
 #include "internal.h"
+#include "launch.cuh"
 
 namespace aoh {
 namespace {
