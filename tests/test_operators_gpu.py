@@ -742,6 +742,43 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager, outs))
 
 
+def test_captured_behind_copies_and_joined_streams():
+    """In a captured graph: the first node, behind a copy, behind a fill, and where two streams meet."""
+    g = gen(5)
+    cache, k, _ = filled([[1, 1]], 8, 1, 600, BF16, 5)
+    q0, k0 = randn(g, 1, 1, 8, 128, dtype=BF16), randn(g, 1, 1, 2, 128, dtype=BF16)
+    pos, inv = torch.full((1, 1, 1), 599, device="cuda"), 1e4 ** (-torch.arange(64, device="cuda", dtype=F32) / 64)
+    x, buf = randn(g, 2, 9_000), torch.empty(2, 9_000, device="cuda")
+
+    def steps(side):
+        main = torch.cuda.current_stream()
+        q, kk = rope_axes_qk(q0, k0, pos, inv, (64,))
+        buf.copy_(x)
+        y, ids = penalize_logits(buf, greedy=True)
+        w = key_weights(cache, 0, q, past_len=599)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            w2 = key_weights(cache, 0, q, past_len=599)
+            kept2, _ = select_keys(w2.view(2, 600), 50)
+        w.zero_()
+        key_weights(cache, 0, q, past_len=599, out=w, accumulate=True)
+        main.wait_stream(side)
+        kept, kw = select_keys(w.view(2, 600), 50)
+        return q, kk, y, ids, w, w2, kept2, kept, kw
+
+    want = [t.clone() for t in steps(torch.cuda.Stream())]
+    torch.cuda.synchronize()
+    gr, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(gr):
+        got = steps(side)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 @pytest.mark.parametrize("dtype,C,T", [(BF16, 1, 30_000), (BF16, 4, 2_000), (BF16, 64, 9_000), (BF16, 700, 5_000),
                                        (F32, 30, 3_000)])
 def test_each_operator_waits_for_the_one_before(dtype, C, T):
