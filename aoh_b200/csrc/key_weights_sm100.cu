@@ -249,7 +249,7 @@ constexpr int kFewKeys = 4;
 template <int S>
 __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ FewArgs f) {
   using Vec = typename std::conditional<S == 2, float2, float4>::type;
-  constexpr int V = sizeof(Vec) / 4;
+  constexpr int V = sizeof(Vec) / 4, kRanges = 5;  // ranges of a lane whose (m, l) are loaded together
   __shared__ float2 ml[S];  // of a row: its maximum and 1 / sum (their rounded logarithm would be 1e-6 off)
   const KeyWeightsArgs& a = f.a;
   const int r = blockIdx.y;
@@ -272,11 +272,19 @@ __global__ void __launch_bounds__(256) few_sum_kernel(const __grid_constant__ Fe
   if (stored) {
     for (int row = warp; row < f.rows; row += 8) {
       float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-      for (int i = lane; i < f.splits; i += 32) {
-        const float2 p = f.part[((long long)i * a.units + r) * f.rows + row];
-        const float mm = fmaxf(m, p.x);
-        if (mm > -INFINITY) l = l * fast_exp2(m - mm) + p.y * fast_exp2(p.x - mm);
+      for (int i0 = lane; i0 < f.splits; i0 += 32 * kRanges) {
+        float2 p[kRanges];
+        float mm = m;
+#pragma unroll
+        for (int k = 0; k < kRanges; ++k) {
+          const int i = i0 + 32 * k;
+          p[k] = i < f.splits ? f.part[((long long)i * a.units + r) * f.rows + row] : make_float2(-INFINITY, 0.f);
+          mm = fmaxf(mm, p[k].x);
+        }
+        if (l > 0.f) l *= fast_exp2(m - mm);
+#pragma unroll
+        for (int k = 0; k < kRanges; ++k)
+          if (p[k].y > 0.f) l = fmaf(p[k].y, fast_exp2(p[k].x - mm), l);
         m = mm;
       }
       float mm = m;

@@ -308,7 +308,8 @@ AOH_API int aoh_kv_append(aoh_kv_cache* cache, int32_t layer, int32_t past_len, 
  * 16-byte aligned device memory of aoh_key_weights_workspace_bytes() for the
  * same lengths, of any contents, not shared by calls that overlap; NULL will do
  * where that is 0 (a few query rows and keys, or arguments that cannot run).
- * Scores are fp32 and sums are made in a fixed order. */
+ * Scores are fp32 and sums are made in a fixed order.  q and the keys are finite:
+ * a NaN may make weights NaN or be left out of the sums. */
 AOH_API size_t aoh_key_weights_workspace_bytes(const aoh_kv_cache* cache, int32_t layer, int32_t past_len,
                                                int32_t q_len);
 AOH_API int aoh_key_weights(aoh_kv_cache* cache, int32_t layer, int32_t past_len, int32_t q_len, const void* q,
