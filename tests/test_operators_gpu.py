@@ -742,6 +742,24 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(eager, outs))
 
 
+def test_operators_wait_for_copies_from_the_host():
+    """A kernel, a long copy from pinned memory, an operator on what arrives, a copy back."""
+    g = gen(9)
+    host = [torch.randn((64, 128_256), generator=torch.Generator().manual_seed(i)).pin_memory() for i in range(3)]
+    x, out = torch.empty((64, 128_256), device="cuda"), torch.empty((64, 128_256), device="cuda")
+    back = torch.empty((64, 128_256)).pin_memory()
+    q0, k0 = randn(g, 1, 64, 8, 128), randn(g, 1, 64, 8, 128)
+    pos, inv = torch.arange(64, device="cuda").expand(1, 1, 64), torch.ones(64, device="cuda")
+    for i in range(9):
+        rope_axes_qk(q0, k0, pos, inv, (64,))
+        x.copy_(host[i % 3], non_blocking=True)
+        _, ids = penalize_logits(x, out=out, greedy=True)
+        back.copy_(out, non_blocking=True)
+        x.fill_(9.0)
+        torch.cuda.synchronize()
+        assert torch.equal(back, host[i % 3]) and torch.equal(ids.cpu(), host[i % 3].argmax(1))
+
+
 def test_captured_behind_copies_and_joined_streams():
     """In a captured graph: the first node, behind a copy, behind a fill, and where two streams meet."""
     g = gen(5)
