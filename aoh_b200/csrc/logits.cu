@@ -199,6 +199,10 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   auto token = [&](int p) { return ((((p / kTurn) << a.cluster_log) + rank) * kTurn) | (p % kTurn); };
   auto place = [&](int t) { return (((t / kTurn) >> a.cluster_log) * kTurn) | (t % kTurn); };
   const int words = (a.vocab + 31) >> 5;
+  const bool greedy = a.greedy != nullptr;
+  // A CTA's shared memory may be reached once the CTA is known to run: all of the cluster
+  // arrive here, and wait before the best keys are handed to the first one (long done by then).
+  if (greedy && a.cluster > 1) cluster_arrive();
   griddep_wait();
   const T* x_row = static_cast<const T*>(a.logits) + row * a.row_stride;
   O* out = static_cast<O*>(a.out) + row * a.out_stride;
@@ -212,7 +216,6 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
     const int r = a.allowed_rows ? a.allowed_rows[row] : row;
     if (r >= 0 && r < a.n_allowed) allowed = a.allowed + (long long)r * words;
   }
-  const bool greedy = a.greedy != nullptr;
   Best best;
 
   // A thread's tokens of one round: U units of N neighbours, a stride apart.
@@ -436,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
   for (int off = 16; off > 0; off >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, off));
   if (lane == 0) best_warp[warp] = key;
   __syncthreads();
+  if (a.cluster > 1) cluster_wait();
   if (tid == 0) {
 #pragma unroll
     for (int i = 1; i < kThreads / 32; ++i) key = max(key, best_warp[i]);

@@ -1,0 +1,25 @@
+"""Edges of the operators around a decode step."""
+import pytest
+import torch
+
+from aoh_b200 import penalize_logits
+from tests.test_operators_gpu import gen, randn
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+# -- clusters ---------------------------------------------------------------------
+@pytest.mark.parametrize("N,V", [(5, 8_192), (9, 16_384), (16, 30_008), (16, 65_536), (27, 131_072), (70, 131_072),
+                                 (90, 131_072), (24, 32_771)])
+def test_greedy_token_of_every_cta_of_a_cluster(N, V):
+    """The largest logit in each CTA's part of the vocabulary in turn (64 tokens a turn, up to 16 CTAs)."""
+    x = randn(gen(V), N, V, dtype=BF16).clamp(max=3)
+    at = [(64 * r + 7 * r % 64) % V for r in range(N)]
+    at[-1] = V - 1
+    for r, t in enumerate(at):
+        x[r, t] = 4
+    outs = [penalize_logits(x, greedy=True) for _ in range(20)]  # one behind the other
+    for out, ids in outs:
+        assert ids.tolist() == at and torch.equal(out, x.float())
