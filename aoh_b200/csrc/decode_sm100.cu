@@ -566,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, kCluster == kClusterBig ? 1 : 3)
     // ============ cluster merge: 8 consecutive splits -> one partial (DSMEM) ============
     // nsplit is a multiple of kCluster and the unit's first CTA is cluster-aligned,
     // so this cluster holds splits [split - rank, split - rank + 8) of this unit only.
+    __syncwarp();  // the cluster's barriers are those for converged warps
     cluster_sync_all();
     const int rank = (int)cluster_ctarank();
     const int E = grp * kHeadDim;
@@ -601,6 +602,7 @@ __global__ void __launch_bounds__(kThreads, kCluster == kClusterBig ? 1 : 3)
     // This CTA's reads of the cluster's shared memory are done: it arrives now
     // and waits only before leaving (no CTA exits while another may still read
     // its partial), so the ticket and the combine overlap the slower members.
+    __syncwarp();
     cluster_arrive();
     // __syncthreads orders every thread's slice stores before the ticket, an
     // acq_rel atomic at GPU scope: cumulative over them (release) and, for the
@@ -692,6 +694,7 @@ __global__ void __launch_bounds__(kThreads, kCluster == kClusterBig ? 1 : 3)
       store_out8(a, out_u + e_lo + 8 * c, reinterpret_cast<const uint4*>(s_out)[c]);
     // ready for the next launch (which touches the workspace only after this grid completes)
     if (tid == 0) a.counters[u * kCluster + rank] = 0;
+    __syncwarp();
     cluster_wait();
     // the last cluster to store slice 0 follows every cluster of the unit past
     // its main loop: a split streaming unit's new token goes in now (its ring

@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
         s_total[0] = bg + gt;
         s_total[1] = be + eq;
       }
+      __syncwarp();  // the barrier is one for converged warps
       cluster_sync_all();
       uint2 v = make_uint2(0, 0);
       if (lane < rank) v = make_uint2(ld_dsmem_u32(mapa_shared(&s_total[0], lane)), ld_dsmem_u32(mapa_shared(&s_total[1], lane)));
@@ -222,6 +223,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const __grid_consta
     kept[at] = p;
     if (kept_w) kept_w[at] = w[p];
   }
+  __syncwarp();
   if (a.take > 0 && a.cluster > 1) cluster_wait();
 }
 

@@ -239,6 +239,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 4 ? 1 : 2) few_scores_ke
       float* o = a.out + r * a.out_stride + p0 * kPage + j;
       *o = a.accumulate ? *o + w : w;
     }
+    __syncwarp();
     cluster_wait();
   }
 }

@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 4) logits_kernel(const __grid_consta
     }
   }
   if (a.cluster > 1) {
+    __syncwarp();  // the barrier is one for converged warps
     cluster_sync_all();
     if (rank == 0 && tid == 0) {
       key = best_cta[0];

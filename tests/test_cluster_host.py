@@ -25,6 +25,7 @@ def _kernels():
             yield path.name, m[1], text[start:at]
 
 
+BARRIER_OR_ARRIVE = re.compile(r"\bcluster_(sync_all|wait|arrive)\(\)")
 REACHING = [k for k in _kernels() if REMOTE.search(k[2])]
 
 
@@ -36,3 +37,23 @@ def test_the_reading_finds_the_cluster_kernels():
 def test_a_cluster_barrier_stands_before_the_first_remote_access(file, kernel, body):
     barrier = BARRIER.search(body)
     assert barrier and barrier.start() < REMOTE.search(body).start(), (file, kernel)
+
+
+@pytest.mark.parametrize("file,kernel,body", REACHING, ids=[k[1] for k in REACHING])
+def test_warps_converge_before_a_cluster_barrier(file, kernel, body):
+    """The barriers are the .aligned ones: a branch on the thread just before one is closed by a warp or CTA
+    barrier."""
+    for m in BARRIER_OR_ARRIVE.finditer(body):
+        before = body[:m.start()].rstrip()
+        # the barrier's own condition, alike in every thread
+        before = re.sub(r"if (constexpr )?\([^()]*\)\s*\{?$", "", before).rstrip()
+        while before.endswith("}"):  # the blocks that end here, from the outermost to the innermost
+            depth, at = 0, len(before)
+            while True:
+                at -= 1
+                depth += {"}": 1, "{": -1}.get(before[at], 0)
+                if depth == 0:
+                    break
+            head = before[:at].rstrip().rsplit("\n", 1)[-1]
+            assert not re.search(r"\btid\b|threadIdx\.x|\blane\b|\bwarp\b", head), (file, kernel, head.strip())
+            before = before[at + 1:-1].rstrip()

@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from aoh_b200 import penalize_logits
-from tests.test_operators_gpu import gen, randn
+from aoh_b200 import penalize_logits, select_keys
+from tests.test_operators_gpu import check_select, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -23,3 +23,12 @@ def test_greedy_token_of_every_cta_of_a_cluster(N, V):
     outs = [penalize_logits(x, greedy=True) for _ in range(20)]  # one behind the other
     for out, ids in outs:
         assert ids.tolist() == at and torch.equal(out, x.float())
+
+
+@pytest.mark.parametrize("rows,n", [(1, 9_000), (3, 16_384), (2, 20_000), (1, 40_000), (2, 70_001), (2, 300_000)])
+def test_select_keys_in_clusters_one_behind_the_other(rows, n):
+    """Clusters of 2 to 8, parts in registers and in memory."""
+    w = (torch.rand((rows, n), generator=gen(n), device="cuda") * 50).floor()
+    check_select(w, n // 3, 4, 9)
+    outs = [select_keys(w, n // 3, sink=4, recent=9) for _ in range(20)]
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, outs[0]))
