@@ -14,10 +14,12 @@ namespace aoh {
 
 // Every wait in this library is bounded in wall-clock time (%globaltimer,
 // nanoseconds), counted from the wait's first unsuccessful poll.  A thread
-// enters an mbarrier wait only after its own griddepcontrol.wait, so the bound
-// covers work of its own grid, never the remaining run time of a predecessor
-// kernel; the gather wait starts early, but its predecessor (a decode kernel)
-// released it only after passing its own griddepcontrol.wait.
+// enters an mbarrier wait only after its own griddepcontrol.wait, or for a phase
+// that no predecessor holds up (copies of what was complete before it, products
+// of those), so the bound covers work of its own grid, never the remaining run
+// time of a predecessor kernel; the gather wait starts early, but its
+// predecessor (a decode kernel) released it only after passing its own
+// griddepcontrol.wait.
 //   kWaitNs: mbarrier phases of this CTA (pages, tiles, MMAs in flight): in
 //     normal operation microseconds.
 //   kPeerWaitNs: flags stored by kernels of other processes (output gather);

@@ -583,6 +583,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int s = i % kStages;
       const int id = kKeysStreamed ? check_id(t0 + i, id_next) : -1;
       if (kKeysStreamed && i + 1 < n) id_next = fetch_id(t0 + i + 1);
+      // the stages of the first two tiles come free without the pass before (products 0 and 1 are all that is made
+      // ahead of it); the later ones' bounded waits time this grid alone
+      if (kPass == kStream && i == kStages + 2) griddep_wait();
       if (lane == 0 && i >= kStages && !s_abort) {
         if (!mbar_wait(&bar_empty[s], (i / kStages - 1) & 1, G.err)) s_abort = 1;
       }

@@ -1,5 +1,6 @@
-"""Thread-block clusters, by reading the kernels: a CTA's shared memory is reached
-by the others only behind a cluster barrier, which is what tells that the CTA runs."""
+"""Orders that no run shows to be broken, by reading the kernels: a CTA's shared
+memory is reached by the others of its cluster only behind a cluster barrier, which
+is what tells that the CTA runs; a bounded wait does not time the kernel before."""
 import re
 from pathlib import Path
 
@@ -57,3 +58,14 @@ def test_warps_converge_before_a_cluster_barrier(file, kernel, body):
             head = before[:at].rstrip().rsplit("\n", 1)[-1]
             assert not re.search(r"\btid\b|threadIdx\.x|\blane\b|\bwarp\b", head), (file, kernel, head.strip())
             before = before[at + 1:-1].rstrip()
+
+
+def test_the_streamed_passs_loads_wait_for_the_pass_before():
+    """Stages from the third tile on come free only behind the pass before: the loading warp waits for that grid
+    itself before it enters a bounded wait for one."""
+    body = next(k[2] for k in _kernels() if k[1] == "tensor_pass_kernel")
+    loads = body[body.index("if (warp == 0) {\n    \n"):body.index("} else if (warp == 1)")]
+    free = loads.index("mbar_wait(&bar_empty")
+    assert re.search(r"kPass == kStream && i == kStages \+ 2\) griddep_wait\(\)", loads[:free])
+    # what is issued ahead: products 0 and 1
+    assert "kPass == kStream && i == 2 && w == 0) griddep_wait()" in body

@@ -2,8 +2,8 @@
 import pytest
 import torch
 
-from aoh_b200 import penalize_logits, select_keys
-from tests.test_operators_gpu import check_select, gen, randn
+from aoh_b200 import key_weights, penalize_logits, select_keys
+from tests.test_operators_gpu import check_select, check_weights, filled, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,14 @@ def test_select_keys_in_clusters_one_behind_the_other(rows, n):
     check_select(w, n // 3, 4, 9)
     outs = [select_keys(w, n // 3, sink=4, recent=9) for _ in range(20)]
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, outs[0]))
+
+
+# -- key weights ------------------------------------------------------------------
+@pytest.mark.parametrize("C,grp,T", [(32, 7, 90_000), (40, 3, 70_001), (5, 8, 120_003)])
+def test_key_weights_of_resident_rows_over_many_tiles(C, grp, T):
+    """One and two tiles of query rows, ranges of many key tiles: every stage of the ring is used several times."""
+    cache, k, _ = filled([[1, 1, 0]], 3 * grp, 1, T, BF16, C)
+    q = randn(gen(C), 1, C, 3 * grp, 128, dtype=BF16)
+    outs = [key_weights(cache, 0, q, past_len=T - C) for _ in range(4)]
+    check_weights(outs[0], q, k[0], [0, 1], T - C)
+    assert all(torch.equal(x, outs[0]) for x in outs) and cache.device_status() == 0
