@@ -912,18 +912,32 @@ size_t one_smem(int pages, int n, int rows) {
   return (size_t)((pages + n - 1) / n) * kPage * one_stride(rows) * sizeof(float);
 }
 
-template <int NT>
-int launch_few_one(const aoh_kv_cache* c, const FewArgs& f, cudaStream_t st) {
-  auto kernel = few_scores_kernel<NT, true>;
+// CTAs of a unit's cluster at most on `device`, 0 if that cannot be told; prepares the kernels, once.
+int one_largest(int device) {
   static PerDeviceOnce once;
-  const int rc = once.run(c->device, [&] {
-    const int e = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                             "aoh_key_weights cluster size");
-    return e ? e
-             : cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem),
-                          "aoh_key_weights shared memory");
+  static int largest[kMaxDevices];
+  const int rc = once.run(device, [device] {
+    int current = 0, n[3] = {};
+    int e = current_device(&current);  // a plan may be asked for while another device is the current one
+    if (e) return e;
+    if (current != device) e = cuda_check(cudaSetDevice(device), "cudaSetDevice");
+    auto ask = [&](auto kernel, int i) {
+      if (!e)
+        e = larger_cluster(kernel, kMaxOne, kMaxOne / 2, kFewWarps * 32, kOneSmem, "aoh_key_weights clusters", &n[i]);
+    };
+    ask(few_scores_kernel<1, true>, 0);
+    ask(few_scores_kernel<2, true>, 1);
+    ask(few_scores_kernel<4, true>, 2);
+    if (current != device) cudaSetDevice(current);
+    largest[device] = std::min(n[0], std::min(n[1], n[2]));
+    return e;
   });
-  if (rc) return rc;
+  return rc ? 0 : largest[device];
+}
+
+template <int NT>
+int launch_few_one(const FewArgs& f, cudaStream_t st) {
+  auto kernel = few_scores_kernel<NT, true>;
   return launch_dependent(kernel, dim3((unsigned)f.splits, (unsigned)f.a.units), f.splits, kFewWarps * 32,
                           one_smem((f.a.max_len + kPage - 1) / kPage, f.splits, f.rows), st, "aoh_key_weights launch", f);
 }
@@ -936,10 +950,10 @@ bool plan_key_weights_few(const aoh_kv_cache* c, int units, int max_len, KeyWeig
   // A cluster a unit where its 16 CTAs read K fast enough.  More than 16 rows
   // leave an SM one CTA, and clusters of 16 of those do not fit every GPC (8
   // units of 32 rows x 4096 keys: 20 us, with 8 CTAs 11).
-  const int most = p.rows > kFewRows && units * kMaxOne > c->num_sms / 2 ? kMaxOne / 2 : kMaxOne;
+  const int fits = pages <= kOnePages && c->bound ? one_largest(c->device) : 0;
+  const int most = std::min(fits, p.rows > kFewRows && units * kMaxOne > c->num_sms / 2 ? kMaxOne / 2 : kMaxOne);
   const int one = std::max(1, std::min(most, pages / (2 * kFewWarps)));  // at least two pages for each of a CTA's warps
-  if (pages <= kOnePages && units * one <= c->num_sms &&
-      one_smem(pages, one, p.rows) <= kOneSmem) {
+  if (fits && units * one <= c->num_sms && one_smem(pages, one, p.rows) <= kOneSmem) {
     p.splits = one;
     p.one = true;
     return true;
@@ -969,9 +983,9 @@ int launch_key_weights_few(const aoh_kv_cache* c, const KeyWeightsArgs& a, const
   if (p.one) {
     f.part = nullptr;
     f.score = nullptr;
-    return p.rows <= 8    ? launch_few_one<1>(c, f, st)
-           : p.rows <= 16 ? launch_few_one<2>(c, f, st)
-                          : launch_few_one<4>(c, f, st);
+    return p.rows <= 8    ? launch_few_one<1>(f, st)
+           : p.rows <= 16 ? launch_few_one<2>(f, st)
+                          : launch_few_one<4>(f, st);
   }
   if (p.rows <= 8)
     rc = launch_dependent(few_scores_kernel<1, false>, grid, 1, kFewWarps * 32, 0, st, "aoh_key_weights scores launch", f);

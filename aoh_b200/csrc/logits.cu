@@ -481,26 +481,39 @@ __global__ void history_add_kernel(uint32_t* counts, uint32_t* seen, int vocab, 
 }
 
 template <typename T, typename O, bool kWide>
-int launch(const LogitsArgs& a, int rows, cudaStream_t st) {
+int launch(LogitsArgs& a, int rows, cudaStream_t st) {
   auto kernel = logits_kernel<T, O, kWide>;
-  int dev = 0;
+  int dev = 0, sms = 0;
   int rc = current_device(&dev);
   if (rc) return rc;
   static PerDeviceOnce once;
+  static int largest[kMaxDevices];
   rc = once.run(dev, [&] {
-    const int e = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
-                             "aoh_logits_penalize cluster size");
-    return e ? e
-             : cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem),
-                          "aoh_logits_penalize shared memory");
+    return larger_cluster(kernel, kMaxCluster, kMaxCluster / 2, kThreads, kMaxSmem, "aoh_logits_penalize clusters",
+                          &largest[dev]);
   });
   if (rc) return rc;
+  rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+  if (rc) return rc;
+  // 16 CTAs a row take the least time while all of them have an SM's third part
+  // (24 rows of 128K, all features, with 16 / 8: 10.6 / 11.4 us, 32 rows 14.2 /
+  // 11.7), then 8, and 4 once those are more than one wave (64 rows: 21.4 with
+  // 16, 16.0 with 8, 18.1 with 4).
+  const int most = std::min(largest[dev], rows * 16LL <= 3 * sms ? 16 : rows * 8LL <= 4 * sms ? 8 : 4);
+  a.cluster = 1;
+  a.cluster_log = 0;
+  while (a.cluster < most && a.cluster * (kWide ? kSlice : kSlice / 2) < a.vocab) {
+    a.cluster *= 2;
+    ++a.cluster_log;
+  }
+  const int turns = (a.vocab + kTurn - 1) / kTurn;
+  a.slice = ((turns + a.cluster - 1) / a.cluster * kTurn + 255) / 256 * 256;
   const size_t smem = a.n_bias ? (size_t)a.slice / 4 + 4 * (size_t)bias_room(a.n_bias) * sizeof(int) : 0;
   return launch_dependent(kernel, dim3((unsigned)(rows * a.cluster)), a.cluster, kThreads, smem, st,
                           "aoh_logits_penalize launch", a);
 }
 template <typename T, typename O>
-int launch(const LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
+int launch(LogitsArgs& a, int rows, bool wide, cudaStream_t st) {
   return wide ? launch<T, O, true>(a, rows, st) : launch<T, O, false>(a, rows, st);
 }
 
@@ -536,23 +549,6 @@ extern "C" int aoh_logits_penalize(const aoh_logits_args* args, aoh_stream strea
   a.logits = p.logits;
   a.row_stride = p.row_stride;
   a.vocab = p.vocab;
-  // 16 CTAs a row take the least time while all of them have an SM's third part
-  // (24 rows of 128K, all features, with 16 / 8: 10.6 / 11.4 us, 32 rows 14.2 /
-  // 11.7), then 8, and 4 once those are more than one wave (64 rows: 21.4 with
-  // 16, 16.0 with 8, 18.1 with 4).
-  int dev = 0, sms = 0;
-  int rc = current_device(&dev);
-  if (rc) return rc;
-  rc = cuda_check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
-  if (rc) return rc;
-  const int most = p.rows * 16LL <= 3 * sms ? 16 : p.rows * 8LL <= 4 * sms ? 8 : 4;
-  a.cluster = 1;
-  while (a.cluster < most && a.cluster * (wide ? kSlice : kSlice / 2) < p.vocab) {
-    a.cluster *= 2;
-    ++a.cluster_log;
-  }
-  const int turns = (p.vocab + kTurn - 1) / kTurn;
-  a.slice = ((turns + a.cluster - 1) / a.cluster * kTurn + 255) / 256 * 256;
   a.counts = reinterpret_cast<const uint32_t*>(p.counts);
   a.seen = reinterpret_cast<const uint32_t*>(p.seen);
   a.repetition = p.repetition;

@@ -69,3 +69,15 @@ def test_the_streamed_passs_loads_wait_for_the_pass_before():
     assert re.search(r"kPass == kStream && i == kStages \+ 2\) griddep_wait\(\)", loads[:free])
     # what is issued ahead: products 0 and 1
     assert "kPass == kStream && i == 2 && w == 0) griddep_wait()" in body
+
+
+def test_clusters_that_are_not_portable_are_asked_for():
+    """A size that the kernel may be launched with, or half of it: where one attribute is set, so is the question."""
+    users = [p for p in sorted(CSRC.glob("*.cu")) if re.search(r"(kMaxCluster|kMaxOne) = 16", p.read_text())]
+    assert {p.name for p in users} >= {"key_weights_sm100.cu", "logits.cu"}
+    for path in users:
+        text = path.read_text()
+        assert "NonPortable" not in text and text.count("larger_cluster(") >= 1, path.name
+    text = (CSRC / "launch.cuh").read_text()
+    asked = text[text.index("int larger_cluster("):]
+    assert asked.index("NonPortableClusterSizeAllowed") < asked.index("cudaOccupancyMaxActiveClusters")
