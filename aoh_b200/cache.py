@@ -15,6 +15,7 @@ after the last layer of a forward (benchmark_llama31.py:249-250).
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 
 import numpy as np
 import torch
@@ -95,7 +96,8 @@ class AoHKVCache:
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.n_ret = [int((labels[i] >= 0.5).sum()) for i in range(self.num_layers)]
         self.n_str = [self.num_kv_heads - n for n in self.n_ret]
-        self.kv_seq_len = 0
+        self._kv_seq_len = 0
+        self._sums = weakref.WeakSet()  # the eviction.KeyWeights of this cache
         self.evicted = 0  # tokens seen that the retrieval heads hold no more (eviction.evict)
         # While True, decode calls read the device-resident length (set with
         # aoh_kv_set_length, advanced by aoh_kv_advance) instead of kv_seq_len and
@@ -142,6 +144,27 @@ class AoHKVCache:
 
     def get_max_cache_shape(self):
         return None
+
+    @property
+    def kv_seq_len(self) -> int:
+        """Tokens cached.  Set to 0 it starts a new sequence; set to less than it
+        was, it drops the last tokens.  Sums of key weights forget the dropped keys
+        (what the dropped queries gave to the keys that stay remains)."""
+        return self._kv_seq_len
+
+    @kv_seq_len.setter
+    def kv_seq_len(self, n: int) -> None:
+        dropped, self._kv_seq_len = n < self._kv_seq_len, n
+        if n == 0:
+            self.evicted = 0
+        if dropped or n == 0:
+            for sums in self._sums:
+                sums.rows[:, n:].zero_()
+
+    def reset(self) -> None:
+        """Start a new sequence in this cache: ``kv_seq_len = 0``.  Pages stay
+        reserved.  A captured decode step goes on where it was: capture it anew."""
+        self.kv_seq_len = 0
 
     @property
     def tokens_seen(self) -> int:

@@ -143,6 +143,7 @@ def evict(cache: AoHKVCache, kept: torch.Tensor, into: AoHKVCache) -> AoHKVCache
     into.reserve(keep)
     _lib.launch(kept.device, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, cache.kv_seq_len,
                 kept.data_ptr(), kept.stride(0), keep)
+    into.reset()  # and whatever was summed for its keys
     into.kv_seq_len = keep
     into.evicted = cache.tokens_seen - keep
     return into
@@ -153,12 +154,15 @@ class KeyWeights:
 
     ``rows`` (R, max_context) float32, zero at the start, R = batch *
     sum(n_ret) rows in (layer, sequence, KV head) order; column j belongs to the
-    key at cache position j."""
+    key at cache position j.  The sums follow the cache: they start at zero again from
+    the position that its ``kv_seq_len`` is set back to (0: a new sequence), and
+    everywhere when another cache is evicted into it."""
 
     def __init__(self, cache: AoHKVCache):
         self.cache = cache
         self.rows = torch.zeros((cache.batch * sum(cache.n_ret), cache.max_context), dtype=torch.float32,
                                 device=cache.device)
+        cache._sums.add(self)
         self._first = [cache.batch * sum(cache.n_ret[:i]) for i in range(cache.num_layers + 1)]
 
     def layer(self, layer_idx: int) -> torch.Tensor:

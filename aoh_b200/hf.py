@@ -95,6 +95,10 @@ class AoHModelCache(Cache):
     def kv_seq_len(self, n: int) -> None:
         self.paged.kv_seq_len = n
 
+    def reset(self) -> None:
+        """Start a new sequence: no tokens, positions from 0, no weights summed."""
+        self.paged.reset()
+
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None, **kwargs):
         return key_states, value_states
 

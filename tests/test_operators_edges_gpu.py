@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from aoh_b200 import key_weights, penalize_logits, select_keys
+from aoh_b200 import AoHKVCache, KeyWeights, evict, key_weights, penalize_logits, select_keys
 from tests.test_operators_gpu import check_select, check_weights, filled, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +43,60 @@ def test_key_weights_of_resident_rows_over_many_tiles(C, grp, T):
     outs = [key_weights(cache, 0, q, past_len=T - C) for _ in range(4)]
     check_weights(outs[0], q, k[0], [0, 1], T - C)
     assert all(torch.equal(x, outs[0]) for x in outs) and cache.device_status() == 0
+
+
+# -- caches used again --------------------------------------------------------------
+def test_a_cache_used_again_starts_from_nothing(cuda_device):
+    """After an eviction and for the next prompt: positions and sums are those of a fresh cache."""
+    from aoh_b200.hf import patch_aoh_model
+    from tests.test_hf_gpu import _tiny
+    from tests.test_operators_hf_gpu import LABELS, _prompt, _run
+
+    model = _tiny("llama")
+    make_cache, _, _ = patch_aoh_model(model, LABELS, 16, 48)
+    first, second = _prompt(250, seed=1), _prompt(180, seed=2)
+    fresh = make_cache(max_context=300)
+    fresh.track_weights()
+    want = _run(model, fresh, second, [0, 100, 179, 180])
+    used = make_cache(max_context=300)
+    used.track_weights()
+    _run(model, used, first, [0, 250])
+    moved = used.evict(120, max_context=300)
+    assert moved.get_seq_length() == 250
+    for cache, restart in ((used, lambda c: setattr(c, "kv_seq_len", 0)), (moved, lambda c: c.reset())):
+        restart(cache)
+        assert cache.get_seq_length() == cache.paged.tokens_seen == cache.paged.evicted == 0
+        got = _run(model, cache, second, [0, 100, 179, 180])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(cache.key_weights.rows, fresh.key_weights.rows)
+        assert cache.get_seq_length() == 180 and cache.paged.device_status() == 0
+
+
+def test_sums_forget_dropped_tokens():
+    """Tokens taken back and decoded otherwise: their keys' sums are those of the new tokens alone."""
+    cache, k, _ = filled([[1, 0, 1]], 6, 1, 200, BF16, 1, max_context=256)
+    sums, other = KeyWeights(cache), KeyWeights(cache)
+    q = randn(gen(1), 1, 200, 6, 128, dtype=BF16)
+    sums.add(0, q, past_len=0)
+    kept = sums.rows[:, :150].clone()
+    cache.kv_seq_len = 150
+    assert torch.equal(sums.rows[:, :150], kept) and (sums.rows[:, 150:] == 0).all() and (other.rows == 0).all()
+    again = randn(gen(2), 1, 50, 3, 128, dtype=BF16)
+    cache.append_layer(0, again, again)
+    sums.add(0, q[:, 150:])
+    new = key_weights(cache, 0, q[:, 150:])
+    cache.kv_seq_len = 200
+    assert torch.equal(sums.rows[:, 150:200], new[0, :, 150:])
+    cache.reset()
+    assert (sums.rows == 0).all()
+
+
+def test_evicting_into_a_cache_that_is_tracked():
+    """What the destination held is given up, its sums too."""
+    cache, k, _ = filled([[1, 0]], 4, 1, 120, BF16, 1, 16, 32)
+    into, _, _ = filled([[1, 0]], 4, 1, 200, BF16, 2, 16, 32)
+    old = KeyWeights(into)
+    old.add(0, randn(gen(1), 1, 200, 4, 128, dtype=BF16), past_len=0)
+    assert (old.rows > 0).all()
+    evict(cache, torch.arange(60, device="cuda", dtype=torch.int32)[None], into)
+    assert (old.rows == 0).all() and (into.kv_seq_len, into.evicted) == (60, 60)
