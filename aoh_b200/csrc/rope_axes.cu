@@ -49,7 +49,7 @@ struct RopeAxesArgs {
   uint32_t heads_magic, half_magic;
   int lanes_log2;
   float eps, scaling;
-  bool pos64;
+  bool pos64, norm_f32;
   uint8_t axis[kMaxHalf];
 };
 
@@ -228,7 +228,10 @@ __global__ void __launch_bounds__(kThreads, ITEMS > 1 || ROWS > 2 ? 3 : 5)
           const int o = e ? o1 : o0;
           if (o < 0) continue;
           float v[VEC];
-          unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o), v);
+          if (sizeof(T) == 2 && a.norm_f32)
+            unpack<float, VEC>(*reinterpret_cast<const Pack<float, VEC>*>(reinterpret_cast<const float*>(w) + o), v);
+          else
+            unpack<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(w + o), v);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) x[e][j] *= inv * v[j];
         }
@@ -342,6 +345,7 @@ extern "C" int aoh_rope_axes_qk(const aoh_rope_axes_args* args, aoh_stream strea
   a.k_out = p.k_out;
   a.pos = p.positions;
   a.pos64 = p.positions_64 != 0;
+  a.norm_f32 = p.norm_f32 != 0;
   a.inv_freq = p.inv_freq;
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = p.q_strides[i];

@@ -43,6 +43,7 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     ``sections``: A counts that sum to half.  The frequencies take their axes
     section by section, or, with ``interleaved``, in turn: frequency i takes axis
     a = i mod A while i < A * sections[a], else axis 0.
+    Norm weights (D,): both of q's type, or of another, then taken in fp32.
     ``scaling`` multiplies cos and sin.  Returns contiguous (q, k).
     """
     # a call's Python is most of the time that a single token takes: each property is read once
@@ -70,15 +71,18 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     if inv_freq.dtype != torch.float32 or inv_freq.device != dev or inv_freq.shape != (half,) \
             or not inv_freq.is_contiguous():
         raise ValueError(f"inv_freq must be a contiguous float32 tensor of sum(sections) = {half} on q's device")
-    qw = kw = 0
+    qw, kw, norm_f32 = 0, 0, False
     if q_norm_weight is not None or k_norm_weight is not None:
         if q_norm_weight is None or k_norm_weight is None:
             raise ValueError("give both norm weights or neither")
         for w in (q_norm_weight, k_norm_weight):
             if w.shape != (D,) or w.device != dev:
                 raise ValueError(f"norm weights must be ({D},) on q's device")
-        # held here until the launch
-        q_norm_weight, k_norm_weight = q_norm_weight.to(dt).contiguous(), k_norm_weight.to(dt).contiguous()
+        # of q's type as they are, of any other in fp32: none is rounded to bf16; held here until the launch
+        norm_f32 = q_norm_weight.dtype != dt or k_norm_weight.dtype != dt
+        if norm_f32:
+            q_norm_weight, k_norm_weight = q_norm_weight.float(), k_norm_weight.float()
+        q_norm_weight, k_norm_weight = q_norm_weight.contiguous(), k_norm_weight.contiguous()
         qw, kw = q_norm_weight.data_ptr(), k_norm_weight.data_ptr()
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
@@ -89,5 +93,5 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
     _lib.launch(dev, _lib.lib().aoh_rope_axes_qk, "aoh_rope_axes_qk", _lib.pack_rope_axes(
         q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), qw, kw, q_out.data_ptr(), k_out.data_ptr(),
         qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], *positions.stride(), *secs, A, bool(interleaved), code, wide, B, n, Hq,
-        G, D, eps, scaling, 0))
+        G, D, eps, scaling, norm_f32))
     return q_out, k_out

@@ -258,7 +258,7 @@ typedef struct {
   const void* k;             /* (batch, q_len, num_kv_heads, head_dim) */
   const void* positions;     /* (n_axes, batch, q_len) int64 if positions_64, else int32 */
   const float* inv_freq;     /* (half) */
-  const void* q_norm_weight; /* (head_dim) of dtype, or both NULL: no norm */
+  const void* q_norm_weight; /* (head_dim) of dtype (or fp32: norm_f32), or both NULL: no norm */
   const void* k_norm_weight;
   void* q_out;               /* contiguous, not aliasing the inputs */
   void* k_out;
@@ -278,7 +278,7 @@ typedef struct {
   int32_t head_dim;          /* even, <= 256 */
   float eps;
   float scaling;
-  int32_t reserved;          /* 0 */
+  int32_t norm_f32;          /* not 0: the norm weights are fp32, whatever dtype is */
 } aoh_rope_axes_args;
 AOH_API int aoh_rope_axes_qk(const aoh_rope_axes_args* args, aoh_stream stream);
 

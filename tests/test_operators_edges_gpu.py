@@ -2,12 +2,12 @@
 import pytest
 import torch
 
-from aoh_b200 import AoHKVCache, KeyWeights, evict, key_weights, penalize_logits, select_keys
-from tests.test_operators_gpu import check_select, check_weights, filled, gen, randn
+from aoh_b200 import AoHKVCache, KeyWeights, evict, key_weights, penalize_logits, rope_axes_qk, select_keys
+from tests.test_operators_gpu import check_rope, check_select, check_weights, filled, gen, randn
 
 pytestmark = pytest.mark.gpu
 
-BF16 = torch.bfloat16
+BF16, F32 = torch.bfloat16, torch.float32
 
 
 # -- clusters ---------------------------------------------------------------------
@@ -100,3 +100,21 @@ def test_evicting_into_a_cache_that_is_tracked():
     assert (old.rows > 0).all()
     evict(cache, torch.arange(60, device="cuda", dtype=torch.int32)[None], into)
     assert (old.rows == 0).all() and (into.kv_seq_len, into.evicted) == (60, 60)
+
+
+# -- rotary positions ----------------------------------------------------------------
+@pytest.mark.parametrize("D,sections", [(128, (64,)), (80, (12, 10, 10)), (256, (100, 28)), (70, (17, 3))])
+@pytest.mark.parametrize("dtype,wq,wk", [(BF16, F32, F32), (BF16, F32, BF16), (F32, BF16, F32), (BF16, torch.float16, F32),
+                                         (BF16, torch.float16, torch.float16)])
+def test_norm_weights_of_another_type_are_not_rounded(dtype, wq, wk, D, sections):
+    """fp32 weights beside bf16 rows: rounded once, in the result."""
+    g = gen(D)
+    q, k = randn(g, 2, 37, 6, D, dtype=dtype), randn(g, 2, 37, 2, D, dtype=dtype)
+    pos = torch.randint(0, 100_000, (len(sections), 2, 37), generator=g, device="cuda")
+    inv = 1e4 ** (-torch.arange(sum(sections), device="cuda", dtype=F32) / sum(sections))
+    w = [(1 + 0.1 * randn(g, D + 1)).to(t) for t in (wq, wk)]
+    for shift in (0, 1):  # weights aligned and not
+        a, b = (x[shift:shift + D] for x in w)
+        qo, ko = rope_axes_qk(q, k, pos, inv, sections, q_norm_weight=a, k_norm_weight=b)
+        check_rope(q, qo, pos, inv, sections, False, a, 1e-6, 1.0)
+        check_rope(k, ko, pos, inv, sections, False, b, 1e-6, 1.0)
