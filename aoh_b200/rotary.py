@@ -8,8 +8,6 @@ indices: after an eviction they go on counting (``AoHKVCache.tokens_seen``).
 """
 from __future__ import annotations
 
-import functools
-
 import torch
 
 from . import _lib
@@ -18,15 +16,21 @@ _DTYPES = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 _POSITIONS_64 = {torch.int64: 1, torch.int32: 0}
 
 
-@functools.lru_cache(maxsize=64)
+_known_sections: dict[tuple, tuple] = {}
+
+
 def _sections(sections: tuple):
     """(the sections padded to the 8 of the call's arguments, how many, their sum)."""
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= 8:
-        raise ValueError(f"1 to 8 sections, got {len(sections)}")
-    if max(map(abs, sections)) > 1 << 20:
-        raise ValueError(f"bad sections {sections}")
-    return sections + (0,) * (8 - len(sections)), len(sections), sum(sections)
+    values = tuple(int(s) for s in sections)
+    if not 1 <= len(values) <= 8:
+        raise ValueError(f"1 to 8 sections, got {len(values)}")
+    if max(map(abs, values)) > 1 << 20:
+        raise ValueError(f"bad sections {values}")
+    found = values + (0,) * (8 - len(values)), len(values), sum(values)
+    # only plain numbers are kept: a tensor is looked up by its identity, and its value may change
+    if len(_known_sections) < 64 and all(type(s) is int for s in sections):
+        _known_sections[sections] = found
+    return found
 
 
 def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections, *,
@@ -62,7 +66,9 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_
         raise ValueError("q and k must be CUDA tensors of one dtype on one device")
     if qs[3] != 1 or ks[3] != 1:
         raise ValueError("the head dimension of q and k must be contiguous")
-    secs, A, half = _sections(sections if type(sections) is tuple else tuple(sections))
+    if type(sections) is not tuple:
+        sections = tuple(sections)
+    secs, A, half = _known_sections.get(sections) or _sections(sections)
     if positions.shape != (A, B, n):
         raise ValueError(f"positions must have shape (axes, B, C) = {(A, B, n)}, got {tuple(positions.shape)}")
     wide = _POSITIONS_64.get(positions.dtype)

@@ -118,3 +118,16 @@ def test_norm_weights_of_another_type_are_not_rounded(dtype, wq, wk, D, sections
         qo, ko = rope_axes_qk(q, k, pos, inv, sections, q_norm_weight=a, k_norm_weight=b)
         check_rope(q, qo, pos, inv, sections, False, a, 1e-6, 1.0)
         check_rope(k, ko, pos, inv, sections, False, b, 1e-6, 1.0)
+
+
+def test_sections_given_as_tensors_that_change():
+    """A call takes the sections' values of its own time."""
+    q, k = randn(gen(1), 1, 9, 2, 64), randn(gen(2), 1, 9, 1, 64)
+    pos = torch.randint(0, 1000, (2, 1, 9), generator=gen(3), device="cuda")
+    inv = 1e4 ** (-torch.arange(32, device="cuda", dtype=F32) / 32)
+    sections = (torch.tensor(20), torch.tensor(12))
+    for a in (20, 5, 20):
+        sections[0].fill_(a)
+        sections[1].fill_(32 - a)
+        got, _ = rope_axes_qk(q, k, pos, inv, sections)
+        check_rope(q, got, pos, inv, (a, 32 - a), False, None, 0, 1.0)
