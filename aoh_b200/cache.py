@@ -97,7 +97,7 @@ class AoHKVCache:
         self.n_ret = [int((labels[i] >= 0.5).sum()) for i in range(self.num_layers)]
         self.n_str = [self.num_kv_heads - n for n in self.n_ret]
         self._kv_seq_len = 0
-        self._sums = weakref.WeakSet()  # the eviction.KeyWeights of this cache
+        self._sums: list[weakref.ref] = []  # the eviction.KeyWeights of this cache
         self.evicted = 0  # tokens seen that the retrieval heads hold no more (eviction.evict)
         # While True, decode calls read the device-resident length (set with
         # aoh_kv_set_length, advanced by aoh_kv_advance) instead of kv_seq_len and
@@ -157,9 +157,18 @@ class AoHKVCache:
         dropped, self._kv_seq_len = n < self._kv_seq_len, n
         if n == 0:
             self.evicted = 0
-        if dropped or n == 0:
-            for sums in self._sums:
+        if self._sums and (dropped or n == 0):
+            self._forget(n)
+
+    def _forget(self, n: int) -> None:
+        """Nothing is summed any more for the keys from position n on."""
+        for ref in self._sums:
+            sums = ref()
+            if sums is not None:
                 sums.rows[:, n:].zero_()
+
+    def _track(self, sums) -> None:
+        self._sums = [ref for ref in self._sums if ref() is not None] + [weakref.ref(sums)]
 
     def reset(self) -> None:
         """Start a new sequence in this cache: ``kv_seq_len = 0``.  Pages stay

@@ -106,10 +106,11 @@ def select_keys(weights: torch.Tensor, keep: int, *, sink: int = 0, recent: int 
         return kept, kept_w
     # rows evenly spaced: a view, or a copy where they are not
     w = weights if weights.dim() == 2 else weights.reshape(-1, n)
+    rows = w.shape[0]
     stride, one = w.stride()
     if n > 1 and one != 1:
         raise ValueError("the last dimension of weights must be contiguous")
-    _lib.launch(weights.device, _lib.lib().aoh_select_keys, "aoh_select_keys", w.data_ptr(), stride, w.shape[0], n, keep,
+    _lib.launch(weights.device, _lib.lib().aoh_select_keys, "aoh_select_keys", w.data_ptr(), stride, rows, n, keep,
                 sink, recent, kept.data_ptr(), kept_w.data_ptr())
     return kept, kept_w
 
@@ -128,24 +129,25 @@ def evict(cache: AoHKVCache, kept: torch.Tensor, into: AoHKVCache) -> AoHKVCache
         raise ValueError("into must be another cache")
     if cache.device_length or into.device_length:
         raise ValueError("a cache in device-length mode cannot be evicted")
-    R = cache.batch * sum(cache.n_ret)
-    if kept.dim() != 2 or kept.shape[0] != R or kept.dtype != torch.int32 or kept.device != cache.device:
-        raise ValueError(f"kept must be int32 ({R}, keep) on {cache.device}, got {kept.dtype} {tuple(kept.shape)}")
-    keep = kept.shape[1]
-    if keep > 1 and kept.stride(1) != 1:
+    R, shape, dev = cache.batch * sum(cache.n_ret), kept.shape, cache.device
+    if len(shape) != 2 or shape[0] != R or kept.dtype != torch.int32 or kept.device != dev:
+        raise ValueError(f"kept must be int32 ({R}, keep) on {dev}, got {kept.dtype} {tuple(shape)}")
+    keep, (stride, one) = shape[1], kept.stride()
+    if keep > 1 and one != 1:
         raise ValueError("the rows of kept must be contiguous")
-    if into.device != cache.device:
-        raise ValueError(f"the caches are on {cache.device} and {into.device}")
-    if keep > cache.kv_seq_len:
-        raise ValueError(f"keep {keep} of {cache.kv_seq_len} tokens")
+    if into.device != dev:
+        raise ValueError(f"the caches are on {dev} and {into.device}")
+    total = cache._kv_seq_len
+    if keep > total:
+        raise ValueError(f"keep {keep} of {total} tokens")
     if keep > into.max_context:
         raise ValueError(f"keep {keep} exceeds the destination's max_context {into.max_context}")
     into.reserve(keep)
-    _lib.launch(kept.device, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, cache.kv_seq_len,
-                kept.data_ptr(), kept.stride(0), keep)
-    into.reset()  # and whatever was summed for its keys
-    into.kv_seq_len = keep
-    into.evicted = cache.tokens_seen - keep
+    _lib.launch(dev, cache._L.aoh_kv_evict, "aoh_kv_evict", cache._h, into._h, total, kept.data_ptr(), stride, keep)
+    if into._sums:
+        into._forget(0)
+    into._kv_seq_len = keep
+    into.evicted = total + cache.evicted - keep
     return into
 
 
@@ -162,7 +164,7 @@ class KeyWeights:
         self.cache = cache
         self.rows = torch.zeros((cache.batch * sum(cache.n_ret), cache.max_context), dtype=torch.float32,
                                 device=cache.device)
-        cache._sums.add(self)
+        cache._track(self)
         self._first = [cache.batch * sum(cache.n_ret[:i]) for i in range(cache.num_layers + 1)]
 
     def layer(self, layer_idx: int) -> torch.Tensor:
