@@ -354,7 +354,8 @@ extern "C" int aoh_select_keys(const float* weights, int64_t row_stride, int32_t
   while (a.cluster < kSelMaxCluster && a.cluster * 8 * kSelThreads < mid &&
          ((long long)rows * a.cluster * 2 <= sms * 7 / 8 || a.cluster * kSelMaxKeys * kSelThreads < mid))
     a.cluster *= 2;
-  a.part = ((mid + a.cluster - 1) / a.cluster + kSelThreads - 1) / kSelThreads * kSelThreads;
+  const int64_t keys = ((int64_t)mid + a.cluster - 1) / a.cluster;  // of a CTA; mid may be the largest int
+  a.part = (int)((keys + kSelThreads - 1) / kSelThreads * kSelThreads);
   const int per = a.part / kSelThreads;
   a.kept = kept;
   a.kept_w = kept_weights;

@@ -59,6 +59,8 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
         if past < 0:
             raise ValueError("past_len must be non-negative")
         total = past + n
+        if total >= 1 << 31:
+            raise ValueError(f"{total} keys are more than 32 bits count")
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs an out to add to")
@@ -107,6 +109,8 @@ def select_keys(weights: torch.Tensor, keep: int, *, sink: int = 0, recent: int 
     # rows evenly spaced: a view, or a copy where they are not
     w = weights if weights.dim() == 2 else weights.reshape(-1, n)
     rows = w.shape[0]
+    if rows >> 31 or n >> 31:
+        raise ValueError(f"weights {tuple(weights.shape)}: rows and keys must fit 32 bits")
     stride, one = w.stride()
     if n > 1 and one != 1:
         raise ValueError("the last dimension of weights must be contiguous")

@@ -16,8 +16,8 @@ class TokenHistory:
     Updates are stream-ordered, need no host read and can be captured."""
 
     def __init__(self, rows: int, vocab: int, device=None):
-        if rows < 0 or vocab < 1:
-            raise ValueError("rows must be non-negative and vocab positive")
+        if not 0 <= rows < 1 << 31 or not 1 <= vocab < 1 << 31:
+            raise ValueError("rows must be non-negative and vocab positive, both of 32 bits")
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         self.rows, self.vocab = int(rows), int(vocab)
         self.counts = torch.zeros((self.rows, self.vocab), dtype=torch.int32, device=self.device)
@@ -47,6 +47,8 @@ class TokenHistory:
         if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (self.rows,)
                                     or lengths.device != self.device or not lengths.is_contiguous()):
             raise ValueError(f"lengths must be contiguous int32 ({self.rows},) on {self.device}")
+        if ids.shape[1] >= 1 << 31:
+            raise ValueError(f"{ids.shape[1]} ids of a row are more than 32 bits count")
         if ids.numel() == 0:
             return
         if ids.shape[1] > 1 and ids.stride(1) != 1:

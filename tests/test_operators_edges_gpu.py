@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from aoh_b200 import AoHKVCache, KeyWeights, evict, key_weights, penalize_logits, rope_axes_qk, select_keys
+from aoh_b200 import KeyWeights, TokenHistory, evict, key_weights, penalize_logits, rope_axes_qk, select_keys
 from tests.test_operators_gpu import check_rope, check_select, check_weights, filled, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -32,6 +32,32 @@ def test_select_keys_in_clusters_one_behind_the_other(rows, n):
     check_select(w, n // 3, 4, 9)
     outs = [select_keys(w, n // 3, sink=4, recent=9) for _ in range(20)]
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, outs[0]))
+
+
+def test_select_keys_of_the_longest_row():
+    """2^31 - 1 keys, as many as 32 bits count: parts of 2^28 keys."""
+    n = 2 ** 31 - 1
+    at = [3, 2 ** 28 - 1, 2 ** 28, 2 ** 30 + 17, 2 ** 31 - 9]
+    w = torch.zeros(1, n, device="cuda")
+    w[0, at] = torch.tensor([1.0, 5.0, 2.0, 3.0, 4.0], device="cuda")
+    kept, kw = select_keys(w, 9, sink=1, recent=1)
+    want = sorted([0, 1, 2, *at, n - 1])
+    assert kept[0].tolist() == want and torch.equal(kw, w[:, want])
+
+
+def test_sizes_that_32_bits_do_not_count_are_refused():
+    """Cut to 32 bits they would be other sizes."""
+    w = torch.empty(2 ** 32 + 40, device="cuda", dtype=torch.float32)  # 17 GB, never read
+    with pytest.raises(ValueError):
+        select_keys(w, 10)
+    with pytest.raises(ValueError):
+        select_keys(w[:, None], 1)
+    history = TokenHistory(1, 8)
+    with pytest.raises(ValueError):
+        history.append(w.view(torch.int32)[None])
+    cache, _, _ = filled([[1]], 1, 1, 20, BF16, 1, 0, 0)
+    with pytest.raises(ValueError):
+        key_weights(cache, 0, torch.zeros(1, 1, 1, 128, device="cuda", dtype=BF16), past_len=2 ** 32 + 19, out=w[None, None])
 
 
 # -- key weights ------------------------------------------------------------------
@@ -93,7 +119,7 @@ def test_sums_forget_dropped_tokens():
 
 def test_evicting_into_a_cache_that_is_tracked():
     """What the destination held is given up, its sums too."""
-    cache, k, _ = filled([[1, 0]], 4, 1, 120, BF16, 1, 16, 32)
+    cache, _, _ = filled([[1, 0]], 4, 1, 120, BF16, 1, 16, 32)
     into, _, _ = filled([[1, 0]], 4, 1, 200, BF16, 2, 16, 32)
     old = KeyWeights(into)
     old.add(0, randn(gen(1), 1, 200, 4, 128, dtype=BF16), past_len=0)
