@@ -78,6 +78,7 @@ _SIGNATURES = {
     "aoh_kv_set_peers": (C.c_int, [_vp, _i32, _i32, C.POINTER(_vp), C.c_size_t, C.POINTER(_vp)]),
     "aoh_gather_wait": (C.c_int, [_vp, _i32, _i32, _vp]),
     "aoh_diag_exp2_poly": (C.c_int, [_vp, _vp, _i32, _vp]),
+    "aoh_diag_exp2_poly_f32": (C.c_int, [_vp, _vp, _i32, _vp]),
     "aoh_rope_qk": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
                               _vp]),
     "aoh_rope_axes_qk": (C.c_int, [C.c_char_p, _vp]),  # the packed aoh_rope_axes_args

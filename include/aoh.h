@@ -471,6 +471,9 @@ AOH_API int aoh_gather_wait(aoh_kv_cache* cache, int32_t layer, int32_t past_len
  * on the fraction, the integer part added to the exponent; x in [-126, 8]);
  * x and out: device float32 arrays of n elements. */
 AOH_API int aoh_diag_exp2_poly(const float* x, float* out, int32_t n, aoh_stream stream);
+/* The same as the sums of key weights compute it there (a polynomial of degree 5, to
+ * fp32 accuracy). */
+AOH_API int aoh_diag_exp2_poly_f32(const float* x, float* out, int32_t n, aoh_stream stream);
 
 #ifdef __cplusplus
 }

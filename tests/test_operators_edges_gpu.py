@@ -1,8 +1,12 @@
 """Edges of the operators around a decode step."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
-from aoh_b200 import KeyWeights, TokenHistory, evict, key_weights, penalize_logits, rope_axes_qk, select_keys
+from aoh_b200 import (AoHKVCache, KeyWeights, TokenHistory, _lib, evict, key_weights, penalize_logits, rope_axes_qk,
+                      select_keys)
 from tests.test_operators_gpu import check_rope, check_select, check_weights, filled, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -57,7 +61,8 @@ def test_sizes_that_32_bits_do_not_count_are_refused():
         history.append(w.view(torch.int32)[None])
     cache, _, _ = filled([[1]], 1, 1, 20, BF16, 1, 0, 0)
     with pytest.raises(ValueError):
-        key_weights(cache, 0, torch.zeros(1, 1, 1, 128, device="cuda", dtype=BF16), past_len=2 ** 32 + 19, out=w[None, None])
+        key_weights(cache, 0, torch.zeros(1, 1, 1, 128, device="cuda", dtype=BF16), past_len=2 ** 32 + 19,
+                    out=w[None, None])
 
 
 # -- key weights ------------------------------------------------------------------
@@ -69,6 +74,51 @@ def test_key_weights_of_resident_rows_over_many_tiles(C, grp, T):
     outs = [key_weights(cache, 0, q, past_len=T - C) for _ in range(4)]
     check_weights(outs[0], q, k[0], [0, 1], T - C)
     assert all(torch.equal(x, outs[0]) for x in outs) and cache.device_status() == 0
+
+
+def test_the_sums_exp2_polynomial():
+    """Against 2^x in 64 bits: 1.55e-7 of the fit and five roundings of at most 2^-24 each, of which the fit's factors
+    f <= 1/2 leave one and a half: below 2.5e-7; at the clamped end next to nothing."""
+    xs = np.concatenate([np.linspace(-126, 8, 2_000_001), np.arange(-126, 9), np.arange(-126, 8) + 0.5,
+                         [-126.5, -1000, -np.inf]]).astype(np.float32)
+    x = torch.from_numpy(xs).cuda()
+    out = torch.empty_like(x)
+    _lib.check(_lib.lib().aoh_diag_exp2_poly_f32(x.data_ptr(), out.data_ptr(), x.numel(), _lib.stream_handle()))
+    got, want = out.cpu().numpy().astype(np.float64), np.exp2(xs.astype(np.float64))
+    m = xs >= -125
+    assert (np.abs(got[m] - want[m]) <= 2.5e-7 * want[m]).all()
+    assert (got[~m] >= 0).all() and (np.abs(got[~m] - want[~m]) <= 2.0 ** -125).all()
+
+
+@pytest.mark.parametrize("C,row", [(c, r) for c in (3, 40, 200, 300, 700)
+                                   for r in (0, 1, 14, 15, 31, 39, 46, 47, 143, 270, 655) if r < c])
+def test_key_weights_of_exact_scores(C, row):
+    """Scores without an error of their own: what is left is the softmax's.  One query row spreads its weight over
+    1024 keys, the others give theirs to one key; every product has one term that is not zero.
+
+    Bound, in steps of 2^-24 of an exponent's error times ln 2: the scale's constant, 3 x 12; the exponent's own
+    rounding, 32 (|x| < 64), in the weight and in the sum's terms; -lse's rounding 16 (below 32) and its logarithm's
+    8; the sum's additions, 8 a key tile of a thread, at most 9 tiles, and 16 of the merges, 88 / ln 2, and an
+    exponential's 2.5e-7 (4.2 steps) in both, 12: (2 * (36 + 32) + 24 + 127 + 12) = 299 steps = 1.24e-5.  The one
+    key's weight: its maximum of 98 and -lse rounded, 64 steps each, and the additions: fewer."""
+    T, keys = 1024 + C, 1024
+    cache = AoHKVCache([[1]], 1, sink_size=0, recent_size=0, max_context=T)
+    k = torch.zeros(1, T, 1, 128, device="cuda", dtype=BF16)
+    k[0, :keys, 0, 5] = (12 * torch.rand(keys, generator=gen(row), device="cuda") - 6).to(BF16)
+    k[0, 7, 0] = 0
+    k[0, 7, 0, 9] = 24  # takes the other rows' weight
+    k[0, keys:, 0, 5] = -100  # out of reach of the row
+    cache.append_layer(0, k, k)
+    q = torch.zeros(1, C, 1, 128, device="cuda", dtype=BF16)
+    q[0, :, 0, 9] = 32
+    q[0, row, 0] = 0
+    q[0, row, 0, 5] = 8
+    got = key_weights(cache, 0, q, past_len=keys)[0, 0].double().cpu()
+    x = 8 * k[0, :keys + row + 1, 0, 5].double().cpu() / math.sqrt(128)
+    want = torch.zeros(T, dtype=torch.float64)
+    want[:keys + row + 1] = torch.softmax(x, 0)
+    want[7] += C - 1
+    assert ((got - want).abs() <= 1.24e-5 * want + 2.0 ** -80).all()
 
 
 # -- caches used again --------------------------------------------------------------
@@ -130,8 +180,8 @@ def test_evicting_into_a_cache_that_is_tracked():
 
 # -- rotary positions ----------------------------------------------------------------
 @pytest.mark.parametrize("D,sections", [(128, (64,)), (80, (12, 10, 10)), (256, (100, 28)), (70, (17, 3))])
-@pytest.mark.parametrize("dtype,wq,wk", [(BF16, F32, F32), (BF16, F32, BF16), (F32, BF16, F32), (BF16, torch.float16, F32),
-                                         (BF16, torch.float16, torch.float16)])
+@pytest.mark.parametrize("dtype,wq,wk", [(BF16, F32, F32), (BF16, F32, BF16), (F32, BF16, F32),
+                                         (BF16, torch.float16, F32), (BF16, torch.float16, torch.float16)])
 def test_norm_weights_of_another_type_are_not_rounded(dtype, wq, wk, D, sections):
     """fp32 weights beside bf16 rows: rounded once, in the result."""
     g = gen(D)
