@@ -1006,8 +1006,11 @@ void plan_key_weights_tensor(const aoh_kv_cache* c, int units, int max_len, int 
   p.tile_tokens = std::min(kTileRows / grp, q_len);
   p.row_tiles = (q_len + p.tile_tokens - 1) / p.tile_tokens;
   const long long lse_items = (long long)units * ((p.row_tiles + 1) / 2), sum_items = (long long)units * key_pairs(max_len);
-  // causal: the first tokens' rows have max_len - q_len keys, the last ones' max_len
-  p.splits = plan_ranges(lse_items, (max_len + kTileRows - 1) / kTileRows, sms, max_len - q_len >= max_len / 4 * 3);
+  // Causal: the first tokens' rows have max_len - q_len keys, the last ones' max_len.  Taken as even from a quarter
+  // on.  30 sizes each (1 to 12 units, 2K to 46K keys) for which the two ways give different ranges, the call's time
+  // taken as even to that as uneven: cached part 0 to 0.25 of the keys 0.99, 1.00, 1.01, 1.01, 1.02, 1.00; 0.3 0.99,
+  // 0.4 0.98, 0.5 to 0.7 0.97; above (10 sizes each) 0.95 to 0.98.
+  p.splits = plan_ranges(lse_items, (max_len + kTileRows - 1) / kTileRows, sms, 4LL * (max_len - q_len) >= max_len);
   // up to two tiles of query rows stay resident in the second pass too, which then needs the ranges alone
   p.stream = p.row_tiles <= 2;
   p.row_splits = p.stream ? p.splits : plan_ranges(sum_items, p.row_tiles, sms, false);
