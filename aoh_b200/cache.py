@@ -172,7 +172,7 @@ class AoHKVCache:
 
     def reset(self) -> None:
         """Start a new sequence in this cache: ``kv_seq_len = 0``.  Pages stay
-        reserved.  A captured decode step goes on where it was: capture it anew."""
+        reserved.  (A captured DecodeStepGraph holds its own length: make it anew.)"""
         self.kv_seq_len = 0
 
     @property

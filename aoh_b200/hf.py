@@ -218,7 +218,9 @@ class ModelDecodeGraph:
     advances it (the reference's ``kv_seq_len += 1``, :249-250), and the token
     and its position are fixed tensors written before each replay.  Pages for
     ``max_steps`` tokens are reserved up front.  ``step(token_ids)`` returns the
-    step's logits (B, 1, vocab) -- a tensor the next step overwrites.
+    step's logits (B, 1, vocab) -- a tensor the next step overwrites.  The graph
+    follows the cache's ``kv_seq_len``: after other forwards, or after ``reset()``
+    and the next prompt, it goes on from there.
 
     ``controls``: keyword arguments of :func:`penalize_logits` (repetition,
     presence, frequency, bias, allowed, allowed_rows) whose tensors the caller
@@ -247,9 +249,8 @@ class ModelDecodeGraph:
         self.ids = torch.zeros((B, 1), dtype=torch.long, device=dev)
         self.pos = torch.zeros((B, 1), dtype=torch.long, device=dev)
         self.cpos = torch.zeros((1,), dtype=torch.long, device=dev)
-        paged.reserve(paged.kv_seq_len + max_steps + 1)
-        self._L, self._C = paged._L, C
-        self._set_length(paged.kv_seq_len)
+        self._L, self._C, self._max_steps = paged._L, C, max_steps
+        self._follow()
         self._inputs(torch.zeros((B, 1), dtype=torch.long, device=dev))
         paged.device_length = True
         try:
@@ -281,11 +282,14 @@ class ModelDecodeGraph:
                 _lib.check(self._L.aoh_kv_advance(paged._h, 1, C.c_void_p(_lib.stream_handle())), "aoh_kv_advance")
         finally:
             paged.device_length = False
-        self._set_length(paged.kv_seq_len)  # capture does not execute: the device length is the host's again
+        self._follow()  # capture does not execute: the device length is the host's again
 
-    def _set_length(self, n: int) -> None:
+    def _follow(self) -> None:
+        """The device length is the host's, with pages for the steps from there."""
         from . import _lib
 
+        self._length = n = self.paged.kv_seq_len
+        self.paged.reserve(n + self._max_steps + 1)
         _lib.check(self._L.aoh_kv_set_length(self.paged._h, n, self._C.c_void_p(_lib.stream_handle())),
                    "aoh_kv_set_length")
 
@@ -302,7 +306,9 @@ class ModelDecodeGraph:
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
         """Decode one token per sequence (token_ids: (B,) or (B, 1)) and advance.
         With controls, token_ids counts as output before its logits are processed."""
+        if self.paged.kv_seq_len != self._length:
+            self._follow()
         self._inputs(token_ids)
         self.graph.replay()
-        self.paged.kv_seq_len += 1
+        self.paged.kv_seq_len = self._length = self._length + 1
         return self.logits

@@ -207,3 +207,36 @@ def test_sections_given_as_tensors_that_change():
         sections[1].fill_(32 - a)
         got, _ = rope_axes_qk(q, k, pos, inv, sections)
         check_rope(q, got, pos, inv, (a, 32 - a), False, None, 0, 1.0)
+
+
+def test_a_captured_step_follows_the_cache(cuda_device):
+    """One captured step for two prompts, and with eager steps between its own."""
+    from aoh_b200.hf import ModelDecodeGraph, patch_aoh_model
+    from tests.test_hf_gpu import _tiny
+    from tests.test_operators_hf_gpu import LABELS, _prompt, _run
+
+    model = _tiny("llama")
+    make_cache, _, _ = patch_aoh_model(model, LABELS, 16, 48)
+    first, second = _prompt(120, seed=1), _prompt(260, seed=2)
+    eager, cache = make_cache(max_context=512), make_cache(max_context=512)
+    cache.track_weights()
+    eager.track_weights()
+    _run(model, cache, first, [0, 110])
+    g = ModelDecodeGraph(model, cache, max_steps=16)
+    for t in range(110, 114):
+        g.step(first[:, t])
+    cache.reset()
+    for c in (cache, eager):
+        _run(model, c, second, [0, 200])
+    for t in range(200, 212):
+        want = _run(model, eager, second, [t, t + 1])[0]
+        got = (_run(model, cache, second, [t, t + 1])[0] if t % 4 == 3 else g.step(second[:, t])).float()
+        assert (got - want).abs().max() <= 0.05 * want.abs().max()
+    assert cache.get_seq_length() == 212 and cache.paged.device_status() == 0
+    for layer in range(2):
+        for head in range(2):
+            rows = range(212) if LABELS[layer][head] else range(164, 212)
+            for x, y in zip(*(c.paged.read_rows(layer, 0, head, rows) for c in (cache, eager))):
+                assert torch.equal(x, y)
+    # sums in key ranges planned for max_context: fp32 in another order, of values up to 4 * 212
+    assert ((cache.key_weights.rows - eager.key_weights.rows).abs() <= 4 * 212 * 2.0 ** -18).all()
