@@ -28,6 +28,11 @@
 // MUFU alone would take 1024 cycles an SM for a product that the tensor cores
 // do in 512.  Four warpgroups keep it fed, and one pair in eight goes to a
 // polynomial of the same accuracy on the FMA pipe.
+// A query row's maximum and sum reach the sums as one fp32 number, -(m + log2 l):
+// with m and 1 / l apart, as the few-rows kernels have them, an element would
+// take a product more.  Its rounding is half a step of a number of the scores'
+// size, as the score's own is: 1.4e-7 to 1.8e-7 from the exact weights (plain
+// fp32: 0.4e-7 to 1.1e-7).
 #include <type_traits>
 
 #include "common.cuh"

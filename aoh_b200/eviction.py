@@ -41,6 +41,8 @@ def key_weights(cache: AoHKVCache, layer_idx: int, q: torch.Tensor, *, past_len:
     contiguous and evenly spaced (a slice of a larger buffer); its first T columns
     are written, or with ``accumulate`` added to.  A cache in device-length mode
     takes single tokens and ``out`` of max_context columns or more.
+    q and the keys are finite: a NaN among them may make weights of its retrieval
+    head NaN or be left out of the sums.
     """
     if not 0 <= layer_idx < cache.num_layers:
         raise ValueError(f"layer_idx {layer_idx} out of range")
