@@ -240,3 +240,50 @@ def test_a_captured_step_follows_the_cache(cuda_device):
                 assert torch.equal(x, y)
     # sums in key ranges planned for max_context: fp32 in another order, of values up to 4 * 212
     assert ((cache.key_weights.rows - eager.key_weights.rows).abs() <= 4 * 212 * 2.0 ** -18).all()
+
+
+FIRST_CALLS = """
+import torch
+from aoh_b200 import AoHKVCache, key_weights, penalize_logits, rope_axes_qk, select_keys, evict
+def make(n, dt=torch.bfloat16):
+    return AoHKVCache([[1, 0]], 8, sink_size=16, recent_size=32, max_context=n, dtype=dt, reserve_all=True)
+def fill(c, n):
+    k = torch.randn((1, n, 2, 128), generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(c.dtype)
+    c.append_layer(0, k, k)
+    c.kv_seq_len = n
+    return c
+big, into = fill(make(20_000), 20_000), make(512)
+f32 = fill(make(300, torch.float32), 300)
+q = {c: torch.randn((1, c, 8, 128), device="cuda").bfloat16() for c in (1, 5, 40, 300)}
+k = torch.randn((1, 300, 2, 128), device="cuda").bfloat16()
+pos, inv = torch.arange(300, device="cuda").expand(1, 1, 300), torch.ones(64, device="cuda")
+x = torch.randn((3, 128_256), device="cuda")
+def calls():
+    out = [*rope_axes_qk(q[300], k, pos, inv, (64,))]
+    out.append(key_weights(big, 0, q[1], past_len=3999))
+    out += [key_weights(big, 0, q[c], past_len=20_000 - c) for c in (1, 5, 40, 300)]
+    out.append(key_weights(f32, 0, q[5].float(), past_len=295))
+    kept, w = select_keys(out[3].view(1, -1), 400, sink=16, recent=32)
+    evict(big, kept, into)
+    return out + [kept, w, into.pool, *penalize_logits(x, greedy=True), *penalize_logits(x[:, 1:], greedy=True)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    captured = calls()
+g.replay()
+torch.cuda.synchronize()
+captured = [t.clone() for t in captured]
+assert all(torch.equal(a, b) for a, b in zip(captured, calls()))
+print("alike")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured(cuda_device):
+    """No operator needs an eager call before: kernels are prepared within a capture as well."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parents[1])
+    assert r.returncode == 0 and "alike" in r.stdout, r.stderr[-2000:]
