@@ -142,7 +142,9 @@ def make_aoh_forward(layer_idx: int, num_q: int, num_kv: int, head_dim: int):
             # QK-norm (Qwen3) and RoPE in one kernel, straight into the layout the attention takes
             cos, sin = position_embeddings
             # one row of positions for the whole batch comes as (1, C, D)
-            cos, sin = (t.to(torch.bfloat16).expand(bsz, q_len, head_dim).contiguous() for t in (cos, sin))
+            if cos.shape[0] != bsz:
+                cos, sin = cos.expand(bsz, q_len, head_dim), sin.expand(bsz, q_len, head_dim)
+            cos, sin = cos.to(torch.bfloat16).contiguous(), sin.to(torch.bfloat16).contiguous()
             q, k = rope_qk(q.contiguous(), k.contiguous(), cos, sin, None if qn is None else qn.weight,
                            None if kn is None else kn.weight, getattr(qn, "variance_epsilon", 1e-6))
         else:
