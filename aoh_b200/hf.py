@@ -222,7 +222,8 @@ class ModelDecodeGraph:
     ``max_steps`` tokens are reserved up front.  ``step(token_ids)`` returns the
     step's logits (B, 1, vocab) -- a tensor the next step overwrites.  The graph
     follows the cache's ``kv_seq_len``: after other forwards, or after ``reset()``
-    and the next prompt, it goes on from there.
+    and the next prompt, it goes on from there.  Key weights are added up if the
+    cache was tracking them when the step was captured.
 
     ``controls``: keyword arguments of :func:`penalize_logits` (repetition,
     presence, frequency, bias, allowed, allowed_rows) whose tensors the caller
@@ -261,7 +262,7 @@ class ModelDecodeGraph:
             # append (an append at this position would already overwrite a
             # streaming head's ring slot whose row the first replay still attends)
             _lib.check(self._L.aoh_kv_set_decode_append(paged._h, 0), "aoh_kv_set_decode_append")
-            weights = cache.key_weights
+            self._weights = weights = cache.key_weights
             before = None if weights is None else weights.rows.clone()
             try:
                 with torch.no_grad():
@@ -308,6 +309,8 @@ class ModelDecodeGraph:
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
         """Decode one token per sequence (token_ids: (B,) or (B, 1)) and advance.
         With controls, token_ids counts as output before its logits are processed."""
+        if self.cache.key_weights is not self._weights:
+            raise RuntimeError("the captured step adds to other key weights: capture it after track_weights()")
         if self.paged.kv_seq_len != self._length:
             self._follow()
         self._inputs(token_ids)

@@ -242,6 +242,28 @@ def test_a_captured_step_follows_the_cache(cuda_device):
     assert ((cache.key_weights.rows - eager.key_weights.rows).abs() <= 4 * 212 * 2.0 ** -18).all()
 
 
+def test_a_captured_step_refuses_weights_that_it_does_not_add_to(cuda_device):
+    """Tracked from a later time on, the sums would lack the captured steps."""
+    from aoh_b200.hf import ModelDecodeGraph, patch_aoh_model
+    from tests.test_hf_gpu import _tiny
+    from tests.test_operators_hf_gpu import LABELS, _prompt, _run
+
+    model = _tiny("llama")
+    make_cache, _, _ = patch_aoh_model(model, LABELS, 16, 48)
+    cache, ids = make_cache(max_context=128), _prompt(70)
+    _run(model, cache, ids, [0, 64])
+    g = ModelDecodeGraph(model, cache, max_steps=8)
+    g.step(ids[:, 64])
+    cache.track_weights()
+    with pytest.raises(RuntimeError):
+        g.step(ids[:, 65])
+    assert cache.get_seq_length() == 65
+    g = ModelDecodeGraph(model, cache, max_steps=8)
+    g.step(ids[:, 65])
+    # the step's query gave its keys 1 for each of a group's 4 heads: 66 weights' roundings
+    assert ((cache.key_weights.rows.double().sum(1) - 4).abs() <= 4 * 70 * 2.0 ** -24 + 4e-5).all()
+
+
 FIRST_CALLS = """
 import torch
 from aoh_b200 import AoHKVCache, key_weights, penalize_logits, rope_axes_qk, select_keys, evict
